@@ -173,7 +173,7 @@ def _quantize(x):
     x = torch.nn.functional.pad(x.float(), (0, blocks * BLOCK - cols)).view(rows, blocks, BLOCK)
     top = x.abs().amax(2)
     half, e = torch.frexp(top)  # top = half * 2^e, half in [0.5, 1); 448 = 0.875 * 2^9
-    e = torch.where(top > 0, (e - 9 + (half > 0.875).int()).clamp(min=-126), 0).int()
+    e = torch.where(top > 0, (e - 9 + (half > 0.875).int()).clamp(min=-100), 0).int()
     values = (x * _power(-e)[..., None]).to(torch.float8_e4m3fn).view(rows, blocks * BLOCK).view(torch.uint8)
     exponents = torch.zeros(rows, -(-blocks // 4) * 4, dtype=torch.uint8, device=x.device)
     exponents[:, :blocks] = (e + 127).to(torch.uint8)
@@ -291,9 +291,9 @@ def _exact_rounded(x):
     for at in range(0, x.shape[1], BLOCK):
         v = x[:, at: at + BLOCK].double()
         top = v.abs().amax(1, keepdim=True)
-        scale = torch.exp2(torch.ceil(torch.log2(torch.where(top > 0, top, 448.0) / 448)).clamp(min=-126))
+        scale = torch.exp2(torch.ceil(torch.log2(torch.where(top > 0, top, 448.0) / 448)).clamp(min=-100))
         scale = torch.where(top > 448 * scale, 2 * scale, scale)  # whatever the logarithm was rounded to
-        scale = torch.where((top > 0) & (top <= 224 * scale) & (scale > 2.0**-126), scale / 2, scale)
+        scale = torch.where((top > 0) & (top <= 224 * scale) & (scale > 2.0**-100), scale / 2, scale)
         v = v / scale
         size = torch.where(v == 0, 1.0, v.abs())
         step = torch.exp2(torch.floor(torch.log2(size)).clamp(min=-6) - 3)
