@@ -184,6 +184,20 @@ SIGNATURES = {
     "gsx_hip_adc_step": (_st, [_vp, ctypes.POINTER(AdcParams), ctypes.c_uint64, ctypes.POINTER(GsRows), _i64,
                                ctypes.POINTER(GsRows), ctypes.POINTER(_i32), ctypes.POINTER(_i64), _vp]),
     "gsx_hip_gather_rows_kernel_launch": (_st, [_vp, _vp, _i64, _i64, _vp, _i64, _vp, _vp]),
+    "gsx_hip_lookup_forward": (_st, [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _f, _vp, _i32, _i64, _vp, _vp]),
+    "gsx_hip_lookup_backward_temp_bytes": (ctypes.c_size_t, [_i64, _i64, _i64]),
+    "gsx_hip_lookup_backward": (_st, [_vp, _i32, _i64, _vp, _i64, _i64, _f, _vp, _i64, _i64, _i32, _vp, _vp]),
+    "gsx_hip_blocks_quantize": (_st, [_vp, _i32, _i64, _i64, _i64, _i32, _vp, _i64, _vp, _i64, _vp]),
+    "gsx_hip_blocks_matmul_temp_bytes": (ctypes.c_size_t, [_i64, _i64, _i64]),
+    "gsx_hip_blocks_matmul": (_st, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _i32, _i64, _vp,
+                                    _vp]),
+    "gsx_hip_linear_temp_bytes": (ctypes.c_size_t, [_i64, _i64, _i64]),
+    "gsx_hip_linear_forward": (_st, [_vp, _i32, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _i32, _i64, _vp, _vp]),
+    "gsx_hip_distill_temp_bytes": (ctypes.c_size_t, [_i64, _i64]),
+    "gsx_hip_distill_forward": (_st, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _i32, _f, _vp, _vp, _vp, _vp, _i64, _f,
+                                      _vp, _vp]),
+    "gsx_hip_distill_backward": (_st, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _i32, _f, _vp, _vp, _vp, _f, _vp, _i64,
+                                       _vp]),
 }
 
 _LIB = None

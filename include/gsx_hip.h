@@ -261,7 +261,13 @@ gsx_hip_status gsx_hip_radix_sort_keys_u64(uint64_t* keys, uint64_t* keys_alt, i
  * (gsx/src/gsx-impl.h:302-458) that the CUDA backend implements in gsx-cuda/buffer.c and
  * reduce-kernels.cu; semantics of the CPU backend (gsx/src/gsx-cpu/core.c:874-2019). Pointers are
  * device pointers; nothing here synchronises except where stated. */
-enum { GSX_HIP_DTYPE_F32 = 0, GSX_HIP_DTYPE_U8 = 1, GSX_HIP_DTYPE_I32 = 2 };
+enum {
+    GSX_HIP_DTYPE_F32 = 0,
+    GSX_HIP_DTYPE_U8 = 1,
+    GSX_HIP_DTYPE_I32 = 2,
+    GSX_HIP_DTYPE_BF16 = 3, /* the label-field operators only, as F16 */
+    GSX_HIP_DTYPE_F16 = 4
+};
 enum {                                   /* gsx_impl_unary_op (gsx-impl.h:295-300) */
     GSX_HIP_UNARY_EXP = 0,
     GSX_HIP_UNARY_SIGMOID = 1,
@@ -463,6 +469,80 @@ gsx_hip_status gsx_hip_adc_step(gsx_hip_adc_context* context, const gsx_hip_adc_
 gsx_hip_status gsx_hip_gather_rows_kernel_launch(const void* src, void* dst, int64_t row_bytes, int64_t row_count,
                                                  const int32_t* src_indices, int64_t src_row_count,
                                                  int* out_has_out_of_range, hipStream_t stream);
+
+/* ---- label fields -------------------------------------------------------------------------------
+ * Operators of language models beside a Gaussian scene (no counterpart in the reference): each
+ * Gaussian or pixel holds the id of a code, the code's row is looked up, a head held in 8-bit blocks
+ * turns rows into logits, and a teacher's top logits train them. Row types are GSX_HIP_DTYPE_F32,
+ * BF16 or F16; strides count elements from row to row (>= the row's length, which lies
+ * contiguously); sums and softmax statistics are float32 and a result is rounded once, to nearest
+ * even. Pointers are aligned to their elements. Results do not depend on the order in which workgroups
+ * run: two calls on the same inputs give the same bits. `temp` is device memory of the size that the
+ * matching *_temp_bytes call gives (16-byte aligned; null where that is 0), used by work on `stream`
+ * until the call's work is done; its contents need no initial value. Nothing here synchronises or
+ * allocates, and every call may be captured into a graph. A call of no rows does nothing. */
+
+/* out[i, 0..width) = scale * table[ids[i], 0..width). An id outside [0, table_rows) gives a row of zeros; if it is
+ * not negative (a negative id stands for "no code"), *out_has_out_of_range (a device int, may be null) is set to 1. */
+gsx_hip_status gsx_hip_lookup_forward(const void* table, int32_t table_type, int64_t table_rows, int64_t table_stride,
+                                      const int32_t* ids, int64_t count, int64_t width, float scale, void* out,
+                                      int32_t out_type, int64_t out_stride, int* out_has_out_of_range,
+                                      hipStream_t stream);
+/* grad_table[v, :] = scale * sum of grad_out[i, :] over the i with ids[i] = v (ids outside the table are left out). Rows
+ * that no id names become 0; with accumulate != 0 the sums are added to what grad_table holds instead, and those rows
+ * stay as they are. grad_table is float32 with rows table_stride apart. count may be at most 2^32 - 1,
+ * table_rows 2^31 - 1. */
+size_t gsx_hip_lookup_backward_temp_bytes(int64_t count, int64_t table_rows, int64_t width);
+gsx_hip_status gsx_hip_lookup_backward(const void* grad_out, int32_t grad_type, int64_t grad_stride, const int32_t* ids,
+                                       int64_t count, int64_t width, float scale, float* grad_table, int64_t table_rows,
+                                       int64_t table_stride, int32_t accumulate, void* temp, hipStream_t stream);
+
+/* Matrices in 8-bit blocks. A row of `cols` values is cut into blocks of 128; a block holds E4M3 values (OCP: 4 exponent
+ * bits, 3 mantissa bits, largest 448) and one byte e + 127 for its scale 2^e, with e the least whole number >= -100 such that
+ * max |x| <= 448 * 2^e over the block's finite x (e = 0 where that maximum is 0). Each x * 2^-e is rounded to the nearest
+ * E4M3 value, ties to even; a non-finite x becomes NaN. Value rows are 16-byte aligned (stride a multiple of 16, >= cols),
+ * exponent rows 4-byte aligned (stride a multiple of 4, >= ceil(cols / 128)). Products are exact for e from -100 to 119. What lies between a row's last value and its
+ * stride is never used as a value; quantize writes zeros there up to the last block's end.
+ * transpose != 0 lays out the blocks of src^T (src_cols rows of src_rows values, blocks along src's rows). */
+gsx_hip_status gsx_hip_blocks_quantize(const void* src, int32_t src_type, int64_t src_rows, int64_t src_cols,
+                                       int64_t src_stride, int32_t transpose, uint8_t* values, int64_t values_stride,
+                                       uint8_t* exponents, int64_t exponents_stride, hipStream_t stream);
+/* out [m, n] = a b^T for block matrices a [m, k] and b [n, k]; m, n and k at most 2^31 - 1. */
+size_t gsx_hip_blocks_matmul_temp_bytes(int64_t m, int64_t n, int64_t k);
+gsx_hip_status gsx_hip_blocks_matmul(const uint8_t* a_values, int64_t a_values_stride, const uint8_t* a_exponents,
+                                     int64_t a_exponents_stride, const uint8_t* b_values, int64_t b_values_stride,
+                                     const uint8_t* b_exponents, int64_t b_exponents_stride, int64_t m, int64_t n,
+                                     int64_t k, void* out, int32_t out_type, int64_t out_stride, void* temp,
+                                     hipStream_t stream);
+/* out [m, n] = blocks(x) w^T: the rows of x [m, k] are quantised as above and multiplied with the block matrix w [n, k]. */
+size_t gsx_hip_linear_temp_bytes(int64_t m, int64_t n, int64_t k);
+gsx_hip_status gsx_hip_linear_forward(const void* x, int32_t x_type, int64_t x_stride, const uint8_t* w_values,
+                                      int64_t w_values_stride, const uint8_t* w_exponents, int64_t w_exponents_stride,
+                                      int64_t m, int64_t n, int64_t k, void* out, int32_t out_type, int64_t out_stride,
+                                      void* temp, hipStream_t stream);
+
+/* Distillation from a teacher's top logits. Row r of `logits` [rows, vocab] is the student's z; teacher_ids and teacher_logits
+ * [rows, top] (rows teacher_stride apart, top at most 1024) name the teacher's entries. An entry counts if its id lies in
+ * [0, vocab) and its logit is not -inf. With T the temperature (1e-6 to 1e6), p = softmax(t / T) over the entries that
+ * count, q = softmax(z / T) over the whole row and w = row_weight[r] (null: 1):
+ *   loss[r] = w T^2 sum_k p_k (log p_k - log q_{id_k}),   dz_j = c w T (q_j - sum of p_k over the entries with id_k = j)
+ * A row of weight 0 or without an entry that counts has loss 0 and gradient 0 whatever its logits are. A logit of -inf has
+ * q = 0. A row of nothing but -inf has no distribution: loss +inf (w > 0), gradient 0. NaN or +inf in a row's logits gives NaN.
+ * forward writes loss [rows], row_stats [rows][2] (max z and the sum of exp((z - max z) / T); for the backward) and, with
+ * c = grad_scale, the gradient (logits' type); each of the three may be null. backward writes the gradient with
+ * c = grad_scale * row_grad[r] (null: 1) from a forward's row_stats of the same logits and temperature. The gradient may not
+ * overlap the logits. */
+size_t gsx_hip_distill_temp_bytes(int64_t rows, int64_t vocab);
+gsx_hip_status gsx_hip_distill_forward(const void* logits, int32_t logits_type, int64_t logits_stride, int64_t rows,
+                                       int64_t vocab, const int32_t* teacher_ids, const float* teacher_logits,
+                                       int64_t teacher_stride, int32_t top, float temperature, const float* row_weight,
+                                       float* loss, float* row_stats, void* grad_logits, int64_t grad_stride,
+                                       float grad_scale, void* temp, hipStream_t stream);
+gsx_hip_status gsx_hip_distill_backward(const void* logits, int32_t logits_type, int64_t logits_stride, int64_t rows,
+                                        int64_t vocab, const int32_t* teacher_ids, const float* teacher_logits,
+                                        int64_t teacher_stride, int32_t top, float temperature, const float* row_weight,
+                                        const float* row_stats, const float* row_grad, float grad_scale,
+                                        void* grad_logits, int64_t grad_stride, hipStream_t stream);
 
 #ifdef __cplusplus
 }
