@@ -5,6 +5,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "common.hpp"
 #include "fields.hpp"
 
 namespace gsx_amd {
@@ -55,21 +56,51 @@ __global__ __launch_bounds__(kRowThreads) void lookup_kernel(const T* __restrict
     }
 }
 
-// One wave per table row and 64 columns: it reads all ids, 64 at a time, and adds the rows of its id in ascending order.
-template <typename T>
+// ---- gradient -----------------------------------------------------------------------------------------------------------
+//
+// Few ids: one wave per table row and 64 vectors of V columns reads all ids, 64 at a time, and adds the rows of its id.
+//
+// Many: the ids are sorted with their positions as values (ids outside the table as table_rows, behind all others), so each
+// table row owns a run of positions. Runs of up to kRunPart rows are summed by one group of lanes each; longer ones in parts of
+// kRunPart sorted positions, whose sums a last launch joins. Every sum has a fixed order, so results repeat bit for bit, and
+// the most frequent id's run is spread over as many workgroups as it has parts.
+
+constexpr int kRunPart = 128;
+
+template <typename T, int V>
+__device__ inline void add_row(float (&sum)[V], const T* __restrict__ p) {
+    const Vec<T, V> x = *reinterpret_cast<const Vec<T, V>*>(p);
+#pragma unroll
+    for (int k = 0; k < V; ++k) sum[k] += to_float(x.v[k]);
+}
+
+template <int V>
+__device__ inline void store_row(float* p, const float (&sum)[V], float scale, bool accumulate) {
+    Vec<float, V> y;
+#pragma unroll
+    for (int k = 0; k < V; ++k) y.v[k] = sum[k] * scale;
+    if (accumulate) {
+        const Vec<float, V> old = *reinterpret_cast<const Vec<float, V>*>(p);
+#pragma unroll
+        for (int k = 0; k < V; ++k) y.v[k] += old.v[k];
+    }
+    *reinterpret_cast<Vec<float, V>*>(p) = y;
+}
+
+template <typename T, int V>
 __global__ __launch_bounds__(kRowThreads) void lookup_scan_kernel(const T* __restrict__ grad, int64_t grad_stride,
                                                                   const int32_t* __restrict__ ids, int64_t count,
                                                                   float scale, float* __restrict__ out,
-                                                                  int64_t table_rows, int64_t out_stride, int64_t width,
+                                                                  int64_t table_rows, int64_t out_stride, int64_t vecs,
                                                                   int accumulate) {
     const int lane = threadIdx.x & 63;
-    const int64_t parts = (width + 63) / 64;
+    const int64_t parts = ceil_div(vecs, 64);
     const int64_t waves = table_rows * parts;
     for (int64_t w = (int64_t)blockIdx.x * (kRowThreads / 64) + threadIdx.x / 64; w < waves;
          w += (int64_t)gridDim.x * (kRowThreads / 64)) {
         const int64_t v = w / parts;
-        const int64_t col = w % parts * 64 + lane;
-        float sum = 0.0f;
+        const int64_t vec = w % parts * 64 + lane;
+        float sum[V] = {};
         bool any = false;
         for (int64_t at = 0; at < count; at += 64) {
             const int32_t id = at + lane < count ? ids[at + lane] : -1;
@@ -78,14 +109,168 @@ __global__ __launch_bounds__(kRowThreads) void lookup_scan_kernel(const T* __res
                 const int k = __builtin_ctzll(mine);
                 mine &= mine - 1;
                 any = true;
-                if (col < width) sum += to_float(grad[(at + k) * grad_stride + col]);
+                if (vec < vecs) add_row<T, V>(sum, grad + (at + k) * grad_stride + vec * V);
             }
         }
-        if (col < width) {
-            float* const p = out + v * out_stride + col;
-            if (accumulate == 0) *p = sum * scale;
-            else if (any) *p += sum * scale;
+        if (vec < vecs && (any || accumulate == 0)) store_row<V>(out + v * out_stride + vec * V, sum, scale, accumulate != 0);
+    }
+}
+
+template <typename KeyT>
+__global__ __launch_bounds__(kRowThreads) void lookup_keys_kernel(const int32_t* __restrict__ ids, int64_t count,
+                                                                  int32_t table_rows, KeyT* __restrict__ keys) {
+    for (int64_t i = (int64_t)blockIdx.x * kRowThreads + threadIdx.x; i < count; i += (int64_t)gridDim.x * kRowThreads) {
+        const int32_t id = ids[i];
+        keys[i] = (KeyT)(id >= 0 && id < table_rows ? id : table_rows);
+    }
+}
+
+// starts[v] = the number of sorted keys below v, for v in [0, table_rows].
+template <typename KeyT>
+__global__ __launch_bounds__(kRowThreads) void lookup_starts_kernel(const KeyT* __restrict__ keys, int64_t count,
+                                                                    int64_t table_rows, uint32_t* __restrict__ starts) {
+    for (int64_t v = (int64_t)blockIdx.x * kRowThreads + threadIdx.x; v <= table_rows;
+         v += (int64_t)gridDim.x * kRowThreads) {
+        int64_t lo = 0, hi = count;
+        while (lo < hi) {
+            const int64_t mid = (lo + hi) / 2;
+            if ((int64_t)keys[mid] < v) lo = mid + 1;
+            else hi = mid;
         }
+        starts[v] = (uint32_t)lo;
+    }
+}
+
+// Sum over sorted positions [begin, end), `step` apart from `begin` on, of the rows' vector at `col`.
+template <typename T, int V>
+__device__ inline void sum_run(float (&sum)[V], const T* __restrict__ grad, int64_t grad_stride,
+                               const uint32_t* __restrict__ order, uint32_t begin, uint32_t end, uint32_t step,
+                               int64_t col) {
+    constexpr int kAhead = 4;  // rows whose loads are in flight together
+    int64_t p = begin;
+    for (; p + (kAhead - 1) * (int64_t)step < end; p += kAhead * (int64_t)step) {
+        Vec<T, V> x[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            x[u] = *reinterpret_cast<const Vec<T, V>*>(grad + (int64_t)order[p + u * (int64_t)step] * grad_stride + col);
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+            for (int k = 0; k < V; ++k) sum[k] += to_float(x[u].v[k]);
+    }
+    for (; p < end; p += step) add_row<T, V>(sum, grad + (int64_t)order[p] * grad_stride + col);
+}
+
+// A group of `lanes` (a power of two, at most 64) lanes per table row, `tiles` times `lanes` vectors of it.
+template <typename T, int V>
+__global__ __launch_bounds__(kRowThreads) void lookup_runs_kernel(const T* __restrict__ grad, int64_t grad_stride,
+                                                                  const uint32_t* __restrict__ order,
+                                                                  const uint32_t* __restrict__ starts, float scale,
+                                                                  float* __restrict__ out, int64_t table_rows,
+                                                                  int64_t out_stride, int64_t vecs, int lanes, int tiles,
+                                                                  int accumulate) {
+    const int sub = threadIdx.x & (lanes - 1);
+    const int64_t parts = ceil_div(vecs, (int64_t)lanes * tiles);
+    const int64_t groups = table_rows * parts, per_block = kRowThreads / lanes;
+    for (int64_t g = (int64_t)blockIdx.x * per_block + threadIdx.x / lanes; g < groups; g += (int64_t)gridDim.x * per_block) {
+        const int64_t v = g / parts;
+        const uint32_t begin = starts[v], end = starts[v + 1];
+        if (end - begin > (uint32_t)kRunPart || (accumulate != 0 && begin == end)) continue;
+        const int64_t first = g % parts * lanes * tiles + sub;
+        for (int t = 0; t < tiles; ++t) {
+            const int64_t vec = first + (int64_t)t * lanes;
+            if (vec >= vecs) break;
+            float sum[V] = {};
+            sum_run<T, V>(sum, grad, grad_stride, order, begin, end, 1, vec * V);
+            store_row<V>(out + v * out_stride + vec * V, sum, scale, accumulate != 0);
+        }
+    }
+}
+
+// Sorted positions [c kRunPart, (c + 1) kRunPart) cross at most two long runs, that of the first key (its sum goes to slot 0)
+// and that of the last key if it is another one (slot 1). One wave per part and 64 vectors; fewer vectors leave 64 / lanes
+// groups, each of which takes every so manieth position.
+template <typename T, int V, typename KeyT>
+__global__ __launch_bounds__(kRowThreads) void lookup_parts_kernel(const T* __restrict__ grad, int64_t grad_stride,
+                                                                   const uint32_t* __restrict__ order,
+                                                                   const KeyT* __restrict__ keys,
+                                                                   const uint32_t* __restrict__ starts, int64_t count,
+                                                                   int64_t table_rows, int64_t vecs, int lanes,
+                                                                   float* __restrict__ partial) {
+    const int64_t tiles = ceil_div(vecs, lanes);
+    const int64_t waves = ceil_div(count, kRunPart) * tiles;
+    const int lane = threadIdx.x & 63;
+    for (int64_t w = (int64_t)blockIdx.x * (kRowThreads / 64) + threadIdx.x / 64; w < waves;
+         w += (int64_t)gridDim.x * (kRowThreads / 64)) {
+        const int64_t c = w / tiles;
+        const int64_t vec = w % tiles * lanes + (lane & (lanes - 1));
+        const int64_t first = c * kRunPart, last = min(first + kRunPart, count) - 1;
+        const int64_t k0 = keys[first], k1 = keys[last];
+#pragma unroll 1
+        for (int slot = 0; slot < 2; ++slot) {
+            const int64_t key = slot == 0 ? k0 : k1;
+            if (key >= table_rows || (slot == 1 && k1 == k0)) continue;
+            const uint32_t begin = starts[key], end = starts[key + 1];
+            if (end - begin <= (uint32_t)kRunPart) continue;
+            float sum[V] = {};
+            const uint32_t from = (uint32_t)max((int64_t)begin, first), to = (uint32_t)min((int64_t)end, last + 1);
+            if (vec < vecs)
+                sum_run<T, V>(sum, grad, grad_stride, order, from + lane / lanes, to, 64 / lanes, vec * V);
+            for (int off = lanes; off < 64; off <<= 1) {
+#pragma unroll
+                for (int k = 0; k < V; ++k) sum[k] += __shfl_xor(sum[k], off, 64);
+            }
+            if (vec < vecs && lane < lanes) {
+                Vec<float, V> y;
+#pragma unroll
+                for (int k = 0; k < V; ++k) y.v[k] = sum[k];
+                *reinterpret_cast<Vec<float, V>*>(partial + ((2 * c + slot) * vecs + vec) * V) = y;
+            }
+        }
+    }
+}
+
+// The long run that begins among the positions of part c (at most one does: the last key's): its parts' sums in a fixed order,
+// by the groups of a workgroup and then across them.
+template <int V, typename KeyT>
+__global__ __launch_bounds__(kRowThreads) void lookup_join_kernel(const KeyT* __restrict__ keys,
+                                                                  const uint32_t* __restrict__ starts, int64_t count,
+                                                                  int64_t table_rows, int64_t vecs, int lanes,
+                                                                  const float* __restrict__ partial, float scale,
+                                                                  float* __restrict__ out, int64_t out_stride,
+                                                                  int accumulate) {
+    __shared__ float s_sum[kRowThreads * V];
+    const int64_t tiles = ceil_div(vecs, lanes);
+    const int64_t blocks = ceil_div(count, kRunPart) * tiles;
+    for (int64_t b = blockIdx.x; b < blocks; b += gridDim.x) {
+        const int64_t c = b / tiles;
+        const int64_t first = c * kRunPart, last = min(first + kRunPart, count) - 1;
+        const int64_t key = keys[last];
+        if (key >= table_rows) continue;  // uniform, as the next
+        const int64_t begin = starts[key], end = starts[key + 1];
+        if (end - begin <= kRunPart || begin < first) continue;
+        const int64_t vec = b % tiles * lanes + (threadIdx.x & (lanes - 1));
+        const int groups = kRowThreads / lanes, group = threadIdx.x / lanes;
+        float sum[V] = {};
+        if (vec < vecs) {
+            for (int64_t p = c + group; p <= (end - 1) / kRunPart; p += groups) {
+                // a run that begins inside part c is that part's last key; in the later parts it is the first
+                const int slot = p == c && begin != first ? 1 : 0;
+                const Vec<float, V> x = *reinterpret_cast<const Vec<float, V>*>(partial + ((2 * p + slot) * vecs + vec) * V);
+#pragma unroll
+                for (int k = 0; k < V; ++k) sum[k] += x.v[k];
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < V; ++k) s_sum[threadIdx.x * V + k] = sum[k];
+        __syncthreads();
+        if (group == 0 && vec < vecs) {
+            for (int g = 1; g < groups; ++g)
+#pragma unroll
+                for (int k = 0; k < V; ++k) sum[k] += s_sum[(g * lanes + threadIdx.x) * V + k];
+            store_row<V>(out + key * out_stride + vec * V, sum, scale, accumulate != 0);
+        }
+        __syncthreads();
     }
 }
 
@@ -118,6 +303,85 @@ gsx_hip_status launch_lookup(const void* table, int64_t table_rows, int64_t tabl
                        dim3(kRowThreads), 0, stream, static_cast<const T*>(table), table_rows, table_stride, ids, count,
                        vecs, tile_rows, parts, tiles, scale, static_cast<O*>(out), out_stride, flag);
     return fields_launched("lookup launch");
+}
+
+// Up to this many ids the gradient takes the scan.
+constexpr int64_t kScanMost = 256;
+
+unsigned rows_grid(int64_t blocks) { return (unsigned)(blocks < kRowMostBlocks ? blocks : kRowMostBlocks); }
+
+// Workspace of the sorted gradient: byte offsets of its arrays.
+struct SortedIds {
+    static bool narrow(int64_t table_rows) { return table_rows <= UINT16_MAX; }
+    int64_t keys, keys_alt, keys_sorted, order_alt, order, sort, starts, partial, bytes;
+    SortedIds(int64_t count, int64_t table_rows, int64_t width) {
+        int64_t at = 0;
+        const auto take = [&](int64_t size) {
+            const int64_t here = at;
+            at += ceil_div(size, 256) * 256;
+            return here;
+        };
+        const int64_t key = narrow(table_rows) ? 2 : 4;
+        keys = take(count * key);
+        keys_alt = take(count * key);
+        keys_sorted = take(count * key);
+        order_alt = take(count * 4);
+        order = take(count * 4);
+        sort = take((int64_t)tile_sort_temp_bytes(count));
+        starts = take((table_rows + 1) * 4);
+        partial = take(ceil_div(count, kRunPart) * 2 * width * 4);
+        bytes = at;
+    }
+};
+
+// Columns a lane sums at once: four where both sides' rows allow vector accesses.
+int grad_vector(const void* grad, int32_t type, int64_t grad_stride, const float* out, int64_t out_stride, int64_t width) {
+    return width % 4 == 0 && grad_stride % 4 == 0 && out_stride % 4 == 0 && aligned_to(grad, 4 * type_bytes(type)) &&
+                   aligned_to(out, 16)
+               ? 4
+               : 1;
+}
+
+template <typename T, int V, typename KeyT>
+gsx_hip_status sorted_backward(const T* grad, int64_t grad_stride, const int32_t* ids, int64_t count, int64_t width,
+                               float scale, float* out, int64_t table_rows, int64_t out_stride, int accumulate, void* temp,
+                               hipStream_t stream) {
+    const SortedIds at(count, table_rows, width);
+    uint8_t* const base = static_cast<uint8_t*>(temp);
+    KeyT* const keys = reinterpret_cast<KeyT*>(base + at.keys);
+    KeyT* const sorted = reinterpret_cast<KeyT*>(base + at.keys_sorted);
+    uint32_t* const order = reinterpret_cast<uint32_t*>(base + at.order);
+    uint32_t* const starts = reinterpret_cast<uint32_t*>(base + at.starts);
+    float* const partial = reinterpret_cast<float*>(base + at.partial);
+    hipLaunchKernelGGL((lookup_keys_kernel<KeyT>), dim3(rows_grid(ceil_div(count, kRowThreads))), dim3(kRowThreads), 0,
+                       stream, ids, count, (int32_t)table_rows, keys);
+    int bits = 1;
+    while ((table_rows >> bits) != 0) ++bits;
+    const int passes = (bits + 7) / 8;
+    const int digit = (bits + passes - 1) / passes;
+    const gsx_hip_status st = tile_sort<KeyT>(keys, reinterpret_cast<KeyT*>(base + at.keys_alt), sorted,
+                                              reinterpret_cast<uint32_t*>(base + at.order_alt), order, count, bits, passes,
+                                              digit < 6 ? 6 : digit, base + at.sort, stream);
+    if (st != GSX_HIP_SUCCESS) return fields_fail(st, "lookup backward: sort");
+    hipLaunchKernelGGL((lookup_starts_kernel<KeyT>), dim3(rows_grid(ceil_div(table_rows + 1, kRowThreads))),
+                       dim3(kRowThreads), 0, stream, sorted, count, table_rows, starts);
+    const int64_t vecs = width / V;
+    int lanes = 1;
+    while (lanes < vecs && lanes < 64) lanes *= 2;
+    // a group takes up to eight times its lanes of a row where there are rows enough to fill the GPU
+    int tiles = 1;
+    while (tiles < 8 && tiles * lanes < vecs && table_rows * ceil_div(vecs, 2 * tiles * lanes) >= 16384) tiles *= 2;
+    const int64_t groups = table_rows * ceil_div(vecs, (int64_t)lanes * tiles);
+    hipLaunchKernelGGL((lookup_runs_kernel<T, V>), dim3(rows_grid(ceil_div(groups, kRowThreads / lanes))),
+                       dim3(kRowThreads), 0, stream, grad, grad_stride, order, starts, scale, out, table_rows, out_stride,
+                       vecs, lanes, tiles, accumulate);
+    const int64_t parts = ceil_div(count, kRunPart) * ceil_div(vecs, lanes);
+    hipLaunchKernelGGL((lookup_parts_kernel<T, V, KeyT>), dim3(rows_grid(ceil_div(parts, kRowThreads / 64))),
+                       dim3(kRowThreads), 0, stream, grad, grad_stride, order, sorted, starts, count, table_rows, vecs,
+                       lanes, partial);
+    hipLaunchKernelGGL((lookup_join_kernel<V, KeyT>), dim3(rows_grid(parts)), dim3(kRowThreads), 0, stream, sorted, starts,
+                       count, table_rows, vecs, lanes, partial, scale, out, out_stride, accumulate);
+    return fields_launched("lookup backward launch");
 }
 
 }  // namespace
@@ -158,10 +422,9 @@ gsx_hip_status gsx_hip_lookup_forward(const void* table, int32_t table_type, int
 }
 
 size_t gsx_hip_lookup_backward_temp_bytes(int64_t count, int64_t table_rows, int64_t width) {
-    (void)count;
-    (void)table_rows;
-    (void)width;
-    return 0;
+    if (count <= kScanMost || table_rows <= 0 || width <= 0 || count > (int64_t)UINT32_MAX || table_rows > INT32_MAX)
+        return 0;
+    return (size_t)SortedIds(count, table_rows, width).bytes;
 }
 
 gsx_hip_status gsx_hip_lookup_backward(const void* grad_out, int32_t grad_type, int64_t grad_stride, const int32_t* ids,
@@ -178,14 +441,32 @@ gsx_hip_status gsx_hip_lookup_backward(const void* grad_out, int32_t grad_type, 
         return fields_fail(GSX_HIP_ERROR_INVALID_ARGUMENT, "lookup backward: null pointer");
     if (!aligned_to(grad_out, type_bytes(grad_type)) || !aligned_to(grad_table, 4) || !aligned_to(ids, 4))
         return fields_fail(GSX_HIP_ERROR_INVALID_ARGUMENT, "lookup backward: pointers must be aligned to their elements");
-    (void)temp;
+    const int vector = grad_vector(grad_out, grad_type, grad_stride, grad_table, table_stride, width);
+    if (count <= kScanMost) {
+        return with_type(grad_type, [&](auto t) {
+            using T = decltype(t);
+            const int64_t blocks = ceil_div(table_rows * ceil_div(width / vector, 64), kRowThreads / 64);
+            hipLaunchKernelGGL((vector == 4 ? lookup_scan_kernel<T, 4> : lookup_scan_kernel<T, 1>), dim3(rows_grid(blocks)),
+                               dim3(kRowThreads), 0, stream, static_cast<const T*>(grad_out), grad_stride, ids, count,
+                               scale, grad_table, table_rows, table_stride, width / vector, accumulate);
+            return fields_launched("lookup backward launch");
+        });
+    }
+    if (temp == nullptr || !aligned_to(temp, 16))
+        return fields_fail(GSX_HIP_ERROR_INVALID_ARGUMENT, "lookup backward: the workspace must be non-null and 16-byte aligned");
     return with_type(grad_type, [&](auto t) {
         using T = decltype(t);
-        const int64_t blocks = ceil_div(table_rows * ceil_div(width, 64), kRowThreads / 64);
-        hipLaunchKernelGGL((lookup_scan_kernel<T>), dim3((unsigned)(blocks < kRowMostBlocks ? blocks : kRowMostBlocks)),
-                           dim3(kRowThreads), 0, stream, static_cast<const T*>(grad_out), grad_stride, ids, count, scale,
-                           grad_table, table_rows, table_stride, width, accumulate);
-        return fields_launched("lookup backward launch");
+        const T* grad = static_cast<const T*>(grad_out);
+        if (SortedIds::narrow(table_rows)) {
+            return vector == 4 ? sorted_backward<T, 4, uint16_t>(grad, grad_stride, ids, count, width, scale, grad_table,
+                                                                 table_rows, table_stride, accumulate, temp, stream)
+                               : sorted_backward<T, 1, uint16_t>(grad, grad_stride, ids, count, width, scale, grad_table,
+                                                                 table_rows, table_stride, accumulate, temp, stream);
+        }
+        return vector == 4 ? sorted_backward<T, 4, uint32_t>(grad, grad_stride, ids, count, width, scale, grad_table,
+                                                             table_rows, table_stride, accumulate, temp, stream)
+                           : sorted_backward<T, 1, uint32_t>(grad, grad_stride, ids, count, width, scale, grad_table,
+                                                             table_rows, table_stride, accumulate, temp, stream);
     });
 }
 
