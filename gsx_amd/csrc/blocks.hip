@@ -19,7 +19,6 @@ namespace gsx_amd {
 constexpr int kBlock = 128;
 constexpr int kLeastExponent = -100;  // the least E4M3 step is 2^-9: q * 2^e stays far above bfloat16's subnormals, which are cut
 constexpr int kQuantThreads = 256;
-constexpr int64_t kSumPart = 8192;  // k after which a running sum starts anew: a float sum of 100k terms is 2e-6 off, of parts 6e-7
 constexpr int64_t kBlocksMostGrid = 1 << 20;
 
 typedef int v8i __attribute__((ext_vector_type(8)));
@@ -129,11 +128,11 @@ struct BlockMatrix {
     int64_t values_stride, exponents_stride;
 };
 
-// 16 bytes of row r at column k; columns from `cols` on read as zero.
-__device__ inline v4i load_values(const BlockMatrix& x, int64_t r, int64_t k, int64_t cols) {
+// 16 bytes of a row at column k; columns from `cols` on read as zero.
+__device__ inline v4i load_values(const uint8_t* row, int64_t k, int64_t cols) {
     v4i v = {0, 0, 0, 0};
     if (k >= cols) return v;
-    v = *reinterpret_cast<const v4i*>(x.values + r * x.values_stride + k);
+    v = *reinterpret_cast<const v4i*>(row + k);
     const int64_t left = cols - k;
     if (left < 16) {
 #pragma unroll
@@ -143,6 +142,31 @@ __device__ inline v4i load_values(const BlockMatrix& x, int64_t r, int64_t k, in
         }
     }
     return v;
+}
+
+// Four elements at any element's address (the hardware takes wide accesses that are not aligned).
+template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) Quad {
+    T v[4];
+};
+
+// 4 TN consecutive columns from `col` on of a row of n.
+template <int TN, typename O>
+__device__ inline void store_columns(O* __restrict__ row, int64_t col, int64_t n, const v4f (&x)[TN]) {
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+        const int64_t c = col + 4 * j;
+        if (c + 4 <= n) {
+            Quad<O> q;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) q.v[i] = from_float<O>(x[j][i]);
+            *reinterpret_cast<Quad<O>*>(row + c) = q;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (c + i < n) row[c + i] = from_float<O>(x[j][i]);
+        }
+    }
 }
 
 // Eight E4M3 values (two words) times `scale`, exactly, in bfloat16.
@@ -157,40 +181,223 @@ __device__ inline v8bf to_bf16(int lo, int hi, float scale) {
 // 2^e from the byte e + 127.
 __device__ inline float block_scale(uint32_t byte) { return __builtin_bit_cast(float, byte << 23); }
 
-// One wave per 16 x 16 tile of c, operands straight from memory. Lane l of a matrix instruction holds row l % 16 of each
-// operand and eight of its k, and rows 4 (l / 16) .. + 3 of column l % 16 of the result. Which k a lane holds is the same for
-// both operands: of a block, lane l has the 32 from 32 (l / 16) on, eight for each of four instructions.
-template <typename O>
-__global__ __launch_bounds__(256) void product_tile_kernel(BlockMatrix a, BlockMatrix b, int64_t m, int64_t n, int64_t k,
-                                                           O* __restrict__ out, int64_t out_stride) {
-    const int lane = threadIdx.x & 63;
-    const int64_t tiles_n = ceil_div(n, 16), tiles = ceil_div(m, 16) * tiles_n;
-    for (int64_t tile = (int64_t)blockIdx.x * 4 + threadIdx.x / 64; tile < tiles; tile += (int64_t)gridDim.x * 4) {
-        const int64_t m0 = tile / tiles_n * 16, n0 = tile % tiles_n * 16;
-        const int64_t ra = min(m0 + (lane & 15), m - 1), rb = min(n0 + (lane & 15), n - 1);
-        v4f acc = {0.0f, 0.0f, 0.0f, 0.0f}, total = acc;
-        for (int64_t k0 = 0; k0 < k; k0 += kBlock) {
-            if (k0 % kSumPart == 0) {
-                total += acc;
-                acc = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-            }
-            const int64_t at = k0 + 32 * (lane / 16);
-            const v4i a0 = load_values(a, ra, at, k), a1 = load_values(a, ra, at + 16, k);
-            const v4i b0 = load_values(b, rb, at, k), b1 = load_values(b, rb, at + 16, k);
-            const float sa = block_scale(a.exponents[ra * a.exponents_stride + k0 / kBlock]);
-            const float sb = block_scale(b.exponents[rb * b.exponents_stride + k0 / kBlock]);
-            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(to_bf16(a0[0], a0[1], sa), to_bf16(b0[0], b0[1], sb), acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(to_bf16(a0[2], a0[3], sa), to_bf16(b0[2], b0[3], sb), acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(to_bf16(a1[0], a1[1], sa), to_bf16(b1[0], b1[1], sb), acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(to_bf16(a1[2], a1[3], sa), to_bf16(b1[2], b1[3], sb), acc, 0, 0, 0);
-        }
-        acc += total;
-        const int64_t col = n0 + (lane & 15);
+// ---- product ------------------------------------------------------------------------------------------------------------
+//
+// A workgroup of WM x WN waves forms a tile of c: BM rows (of a) by BN columns (rows of b), a wave TM x TN times 16 x 16 of it.
+// Blocks of 128 k of both operands' tiles lie in LDS, two at a time: while one is multiplied the next is on its way there,
+// straight from memory. A row is eight chunks of 16 bytes; chunk c lies at place c ^ swizzle(row), so that the lanes of one
+// read, which hold different rows' same chunk, meet different banks.
+//
+// The matrix instructions take b as their first operand: a lane then holds four consecutive columns of one row of c. Which
+// row of b a lane brings for instruction j is chosen so that its 4 TN columns are consecutive too, and leave in wide stores.
+
+typedef __attribute__((address_space(3))) void* LdsPtr;
+typedef const __attribute__((address_space(1))) void* GlobalPtr;
+
+// Row of b, within a wave's 16 TN, that index r of instruction j stands for.
+template <int TN>
+__device__ constexpr int column_of(int j, int r) {
+    return (r / 4) * (4 * TN) + 4 * j + r % 4;
+}
+
+// Places of the chunks: a's rows are read 16 in a row, b's as column_of orders them.
+__device__ inline int swizzle_a(int row) { return row & 7; }
+template <int TN>
+__device__ inline int swizzle_b(int row) {
+    return (row & 3) | ((row / (4 * TN)) & 1) << 2;
+}
+
+struct ProductTile {
+    int64_t m0, n0;
+    int64_t first, last;  // blocks of k
+    int64_t split;
+};
+
+// Tiles in bands of eight rows of tiles, so that workgroups that run together share operands in an L2; workgroup b runs on
+// XCD b % 8 and takes its share of the sequence in one piece.
+__device__ inline ProductTile product_tile(int64_t t, int64_t total, int64_t tiles_m, int64_t tiles_n, int bm, int bn,
+                                           int64_t blocks, int64_t splits) {
+    const int64_t per = (total + 7) / 8;
+    const int64_t whole = total / 8 * 8;
+    int64_t at = total % 8 == 0 ? (t % 8) * per + t / 8 : (t < whole ? (t % 8) * (total / 8) + t / 8 : t);
+    ProductTile r;
+    r.split = at % splits;
+    at /= splits;
+    const int64_t band = at / (8 * tiles_n), in_band = at % (8 * tiles_n);
+    const int64_t rows = min((int64_t)8, tiles_m - band * 8);
+    r.m0 = (band * 8 + in_band % rows) * bm;
+    r.n0 = in_band / rows * bn;
+    r.first = blocks * r.split / splits;
+    r.last = blocks * (r.split + 1) / splits;
+    return r;
+}
+
+// One block of k: `next`'s loads are begun (BASES: where a's and b's rows of that block start), then `now`, which they do not
+// touch, is multiplied. __restrict__ says so to the compiler, which otherwise waits for the loads before it reads LDS.
+template <int TM, int TN, int WM, int WN, int kLoads>
+__device__ __forceinline__ void product_step(const uint8_t* __restrict__ now, const uint32_t* __restrict__ exponents,
+                                             int shift, uint8_t* __restrict__ next, bool load, const uint8_t* a_next,
+                                             const uint8_t* b_next, const uint32_t (&offset)[kLoads], int lane, int wave,
+                                             v4f (&acc)[TM][TN]) {
+    constexpr int BM = 16 * TM * WM, kWaves = WM * WN;
+    if (load) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int64_t row = m0 + 4 * (lane / 16) + i;
-            if (row < m && col < n) out[row * out_stride + col] = from_float<O>(acc[i]);
+        for (int u = 0; u < kLoads; ++u) {
+            const uint8_t* const base = 8 * (u * kWaves + wave) < BM ? a_next : b_next;
+            __builtin_amdgcn_global_load_lds((GlobalPtr)(base + (uint64_t)offset[u] * 16),
+                                             (LdsPtr)(next + (u * kWaves + wave) * 1024), 16, 0, 0);
         }
+    }
+    const int wm = wave / WN, wn = wave % WN;
+    const uint8_t* const s_a = now;
+    const uint8_t* const s_b = now + BM * kBlock;
+    float scale_b[TN], scale_a[TM];
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+        scale_b[j] = block_scale((exponents[BM + wn * 16 * TN + column_of<TN>(j, lane & 15)] >> shift) & 255u);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) scale_a[i] = block_scale((exponents[wm * 16 * TM + i * 16 + (lane & 15)] >> shift) & 255u);
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        const int c = 2 * (lane / 16) + half;
+        v8bf vb[TN][2];
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+            const int row = wn * 16 * TN + column_of<TN>(j, lane & 15);
+            const v4i x = *reinterpret_cast<const v4i*>(s_b + row * kBlock + ((c ^ swizzle_b<TN>(row)) * 16));
+            vb[j][0] = to_bf16(x[0], x[1], scale_b[j]);
+            vb[j][1] = to_bf16(x[2], x[3], scale_b[j]);
+        }
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+            const int row = wm * 16 * TM + i * 16 + (lane & 15);
+            const v4i x = *reinterpret_cast<const v4i*>(s_a + row * kBlock + ((c ^ swizzle_a(row)) * 16));
+            const v8bf va0 = to_bf16(x[0], x[1], scale_a[i]), va1 = to_bf16(x[2], x[3], scale_a[i]);
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vb[j][0], va0, acc[i][j], 0, 0, 0);
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vb[j][1], va1, acc[i][j], 0, 0, 0);
+        }
+    }
+}
+
+template <typename O, int TM, int TN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void product_kernel(BlockMatrix a, BlockMatrix b, int64_t m, int64_t n, int64_t k,
+                                                               int64_t tiles_m, int64_t tiles_n, int64_t splits,
+                                                               O* __restrict__ out, int64_t out_stride,
+                                                               float* __restrict__ partial) {
+    constexpr int kThreads = 64 * WM * WN, BM = 16 * TM * WM, BN = 16 * TN * WN;
+    constexpr int kRows = BM + BN, kLoads = kRows * 8 / kThreads, kWaves = WM * WN;
+    static_assert(kRows * 8 % kThreads == 0 && BM % (8 * kWaves) == 0, "whole loads, each of one operand");
+    __shared__ __attribute__((aligned(1024))) uint8_t s_values[2][kRows * kBlock];
+    __shared__ uint32_t s_exponents[2][kRows];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int64_t blocks = ceil_div(k, kBlock), total = tiles_m * tiles_n * splits;
+    for (int64_t t = blockIdx.x; t < total; t += gridDim.x) {
+        const ProductTile tile = product_tile(t, total, tiles_m, tiles_n, BM, BN, blocks, splits);
+        // Load u of a wave: eight rows (lane / 8) from row 8 (u kWaves + wave) on, a's rows before b's. Rows past the last one
+        // repeat it; what they give is not stored. Offsets from the tile's first row are kept in units of 16 bytes.
+        const uint8_t* const a_tile = a.values + tile.m0 * a.values_stride;
+        const uint8_t* const b_tile = b.values + tile.n0 * b.values_stride;
+        const int most_a = (int)min(m - 1 - tile.m0, (int64_t)BM), most_b = (int)min(n - 1 - tile.n0, (int64_t)BN);
+        const uint32_t a_step = (uint32_t)(a.values_stride / 16), b_step = (uint32_t)(b.values_stride / 16);
+        uint32_t offset[kLoads];
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u) {
+            const int row = 8 * (u * kWaves + wave) + lane / 8;
+            offset[u] = row < BM ? min(row, most_a) * a_step + (uint32_t)((lane & 7) ^ swizzle_a(row))
+                                 : min(row - BM, most_b) * b_step + (uint32_t)((lane & 7) ^ swizzle_b<TN>(row - BM));
+        }
+        // a block through registers, with zeros past the last k: the first one, and a cut last one
+        const auto stage = [&](int64_t kb) {
+            const int64_t k0 = kb * kBlock;
+#pragma unroll 1
+            for (int u = wave; u < kRows / 8; u += kWaves) {
+                const int row = 8 * u + lane / 8;
+                const uint8_t* const p = row < BM ? a_tile + min(row, most_a) * a.values_stride
+                                                  : b_tile + min(row - BM, most_b) * b.values_stride;
+                const int chunk = (lane & 7) ^ (row < BM ? swizzle_a(row) : swizzle_b<TN>(row - BM));
+                *reinterpret_cast<v4i*>(s_values[kb & 1] + u * 1024 + lane * 16) = load_values(p, k0 + chunk * 16, k);
+            }
+        };
+        // four blocks' exponents of a row are one word; thread r brings row r's
+        const auto stage_exponents = [&](int64_t group) {
+#pragma unroll
+            for (int row = threadIdx.x; row < kRows; row += kThreads) {
+                const uint8_t* const p = row < BM ? a.exponents + (tile.m0 + min(row, most_a)) * a.exponents_stride
+                                                  : b.exponents + (tile.n0 + min(row - BM, most_b)) * b.exponents_stride;
+                s_exponents[group & 1][row] = reinterpret_cast<const uint32_t*>(p)[group];
+            }
+        };
+        v4f acc[TM][TN];
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        if (tile.first < tile.last) {
+            stage(tile.first);
+            stage_exponents(tile.first / 4);
+        }
+        for (int64_t kb = tile.first; kb < tile.last; ++kb) {
+            // This block is in LDS (the barrier does not wait for loads that go there), the one before it has been read.
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            const int64_t next = kb + 1;
+            const bool more = next < tile.last, whole = (next + 1) * kBlock <= k;
+            if (more && next % 4 == 0) stage_exponents(next / 4);
+            if (more && !whole) stage(next);
+            product_step<TM, TN, WM, WN, kLoads>(s_values[kb & 1], s_exponents[(kb / 4) & 1], (int)(kb % 4) * 8,
+                                                 s_values[next & 1], more && whole, a_tile + next * kBlock,
+                                                 b_tile + next * kBlock, offset, lane, wave, acc);
+        }
+        __syncthreads();  // the next tile's first block goes where this one's last was read
+        const int wm = wave / WN, wn = wave % WN;
+        const int64_t col = tile.n0 + wn * 16 * TN + (lane / 16) * (4 * TN);
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+            const int64_t row = tile.m0 + wm * 16 * TM + i * 16 + (lane & 15);
+            if (row >= m) continue;
+            if (splits == 1) {
+                store_columns<TN>(out + row * out_stride, col, n, acc[i]);
+            } else {
+                store_columns<TN>(partial + (tile.split * m + row) * n, col, n, acc[i]);
+            }
+        }
+    }
+}
+
+// out = the sum over splits of partial [splits][m][n], in their order: 16 groups of a workgroup take every 16th split of 16
+// vectors each, then the groups' sums are added.
+template <typename O>
+__global__ __launch_bounds__(256) void product_join_kernel(const float* __restrict__ partial, int64_t m, int64_t n,
+                                                           int64_t splits, O* __restrict__ out, int64_t out_stride) {
+    __shared__ v4f s_sum[256];
+    const int64_t size = m * n, vecs = ceil_div(size, 4);
+    const int group = threadIdx.x / 16;
+    for (int64_t b = blockIdx.x; b < ceil_div(vecs, 16); b += gridDim.x) {
+        const int64_t e = (b * 16 + (threadIdx.x & 15)) * 4;
+        v4f sum = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (e + 4 <= size) {
+#pragma unroll 4
+            for (int64_t s = group; s < splits; s += 16) {
+                const Quad<float> x = *reinterpret_cast<const Quad<float>*>(partial + s * size + e);
+                sum += v4f{x.v[0], x.v[1], x.v[2], x.v[3]};
+            }
+        } else {
+            for (int64_t s = group; s < splits; s += 16)
+                for (int i = 0; i < 4; ++i)
+                    if (e + i < size) sum[i] += partial[s * size + e + i];
+        }
+        s_sum[threadIdx.x] = sum;
+        __syncthreads();
+        if (group == 0) {
+            for (int g = 1; g < 16; ++g) sum += s_sum[g * 16 + threadIdx.x];
+            for (int i = 0; i < 4; ++i)
+                if (e + i < size) out[(e + i) / n * out_stride + (e + i) % n] = from_float<O>(sum[i]);
+        }
+        __syncthreads();
     }
 }
 
@@ -219,8 +426,40 @@ gsx_hip_status block_matrix_check(const void* values, const void* exponents, int
     return GSX_HIP_SUCCESS;
 }
 
+// 256 rows of a product's operand lie within 2^36 bytes (the kernel's offsets): value strides below 2^28.
+constexpr int64_t kMostSummands = (int64_t)1 << 27;
+constexpr int64_t kMostStride = (int64_t)1 << 28;
+
 bool product_sizes(int64_t m, int64_t n, int64_t k) {
-    return m >= 0 && n >= 0 && k >= 0 && m <= INT32_MAX && n <= INT32_MAX && k <= INT32_MAX;
+    return m >= 0 && n >= 0 && k >= 0 && m <= INT32_MAX && n <= INT32_MAX && k <= kMostSummands;
+}
+
+// Tiles and splits of a product by its sizes alone. Large tiles move the fewest bytes through LDS for a product; they are taken
+// where they fill the GPU's 256 CUs, smaller ones where they do not. What is still short of two workgroups a CU is split over k,
+// four blocks or more to a part.
+struct ProductPlan {
+    int bm, bn;
+    int64_t tiles_m, tiles_n, splits;
+    int64_t temp_bytes;
+};
+
+constexpr int64_t kSplitTarget = 512;
+constexpr int64_t kSplitMostBlocks = 512;  // blocks of k after which a float sum starts anew
+
+ProductPlan product_plan(int64_t m, int64_t n, int64_t k) {
+    ProductPlan p;
+    const auto tiles = [&](int64_t edge) { return ceil_div(m, edge) * ceil_div(n, edge); };
+    const int edge = tiles(256) >= 192 ? 256 : tiles(128) >= 256 || (m > 64 && n > 64) ? 128 : 64;
+    p.bm = p.bn = edge;
+    p.tiles_m = ceil_div(m, edge);
+    p.tiles_n = ceil_div(n, edge);
+    const int64_t blocks = ceil_div(k, kBlock), count = p.tiles_m * p.tiles_n;
+    int64_t splits = count >= kSplitTarget / 2 ? 1 : ceil_div(kSplitTarget, count);
+    if (splits > blocks / 4) splits = blocks / 4;
+    if (splits < ceil_div(blocks, kSplitMostBlocks)) splits = ceil_div(blocks, kSplitMostBlocks);
+    p.splits = splits < 1 ? 1 : splits;
+    p.temp_bytes = p.splits > 1 ? p.splits * m * n * 4 : 0;
+    return p;
 }
 
 // The quantised rows of gsx_hip_linear_forward in its workspace, rounded up for what follows them.
@@ -263,10 +502,7 @@ gsx_hip_status gsx_hip_blocks_quantize(const void* src, int32_t src_type, int64_
 }
 
 size_t gsx_hip_blocks_matmul_temp_bytes(int64_t m, int64_t n, int64_t k) {
-    (void)m;
-    (void)n;
-    (void)k;
-    return 0;
+    return product_sizes(m, n, k) && m > 0 && n > 0 ? (size_t)product_plan(m, n, k).temp_bytes : 0;
 }
 
 gsx_hip_status gsx_hip_blocks_matmul(const uint8_t* a_values, int64_t a_values_stride, const uint8_t* a_exponents,
@@ -276,7 +512,9 @@ gsx_hip_status gsx_hip_blocks_matmul(const uint8_t* a_values, int64_t a_values_s
                                      hipStream_t stream) {
     if (!known_type(out_type)) return fields_fail(GSX_HIP_ERROR_NOT_SUPPORTED, "blocks: the product is f32, bf16 or f16");
     if (!product_sizes(m, n, k))
-        return fields_fail(GSX_HIP_ERROR_OUT_OF_RANGE, "blocks: a product's sizes must lie between 0 and 2^31 - 1");
+        return fields_fail(GSX_HIP_ERROR_OUT_OF_RANGE, "blocks: a product has at most 2^31 - 1 rows and columns and 2^27 summands");
+    if (a_values_stride >= kMostStride || b_values_stride >= kMostStride)
+        return fields_fail(GSX_HIP_ERROR_OUT_OF_RANGE, "blocks: a product's value rows lie less than 2^28 bytes apart");
     gsx_hip_status st = block_matrix_check(a_values, a_exponents, m, k, a_values_stride, a_exponents_stride);
     if (st != GSX_HIP_SUCCESS) return st;
     st = block_matrix_check(b_values, b_exponents, n, k, b_values_stride, b_exponents_stride);
@@ -286,13 +524,30 @@ gsx_hip_status gsx_hip_blocks_matmul(const uint8_t* a_values, int64_t a_values_s
     if (m == 0 || n == 0) return GSX_HIP_SUCCESS;
     if (out == nullptr || !aligned_to(out, type_bytes(out_type)))
         return fields_fail(GSX_HIP_ERROR_INVALID_ARGUMENT, "blocks: the product must be non-null and aligned to its elements");
-    (void)temp;
+    const ProductPlan plan = product_plan(m, n, k);
+    if (plan.temp_bytes > 0 && (temp == nullptr || !aligned_to(temp, 16)))
+        return fields_fail(GSX_HIP_ERROR_INVALID_ARGUMENT, "blocks: the workspace must be non-null and 16-byte aligned");
     const BlockMatrix a = {a_values, a_exponents, a_values_stride, a_exponents_stride};
     const BlockMatrix b = {b_values, b_exponents, b_values_stride, b_exponents_stride};
+    const unsigned grid = blocks_grid(plan.tiles_m * plan.tiles_n * plan.splits);
+    float* const partial = static_cast<float*>(temp);
     return with_type(out_type, [&](auto t) {
         using O = decltype(t);
-        hipLaunchKernelGGL((product_tile_kernel<O>), dim3(blocks_grid(ceil_div(ceil_div(m, 16) * ceil_div(n, 16), 4))),
-                           dim3(256), 0, stream, a, b, m, n, k, static_cast<O*>(out), out_stride);
+        O* const to = static_cast<O*>(out);
+        if (plan.bm == 256) {
+            hipLaunchKernelGGL((product_kernel<O, 8, 4, 2, 4>), dim3(grid), dim3(512), 0, stream, a, b, m, n, k, plan.tiles_m,
+                               plan.tiles_n, plan.splits, to, out_stride, partial);
+        } else if (plan.bm == 128) {
+            hipLaunchKernelGGL((product_kernel<O, 4, 4, 2, 2>), dim3(grid), dim3(256), 0, stream, a, b, m, n, k, plan.tiles_m,
+                               plan.tiles_n, plan.splits, to, out_stride, partial);
+        } else {
+            hipLaunchKernelGGL((product_kernel<O, 2, 2, 2, 2>), dim3(grid), dim3(256), 0, stream, a, b, m, n, k, plan.tiles_m,
+                               plan.tiles_n, plan.splits, to, out_stride, partial);
+        }
+        if (plan.splits > 1) {
+            hipLaunchKernelGGL((product_join_kernel<O>), dim3(blocks_grid(ceil_div(ceil_div(m * n, 4), 16))), dim3(256), 0,
+                               stream, partial, m, n, plan.splits, to, out_stride);
+        }
         return fields_launched("blocks matmul launch");
     });
 }
@@ -307,7 +562,7 @@ gsx_hip_status gsx_hip_linear_forward(const void* x, int32_t x_type, int64_t x_s
                                       int64_t m, int64_t n, int64_t k, void* out, int32_t out_type, int64_t out_stride,
                                       void* temp, hipStream_t stream) {
     if (!product_sizes(m, n, k))
-        return fields_fail(GSX_HIP_ERROR_OUT_OF_RANGE, "linear: sizes must lie between 0 and 2^31 - 1");
+        return fields_fail(GSX_HIP_ERROR_OUT_OF_RANGE, "linear: at most 2^31 - 1 rows and columns and 2^27 summands");
     if (m > 0 && k > 0 && temp == nullptr) return fields_fail(GSX_HIP_ERROR_INVALID_ARGUMENT, "linear: null workspace");
     const int64_t blocks = ceil_div(k, kBlock);
     uint8_t* const values = static_cast<uint8_t*>(temp);

@@ -507,7 +507,8 @@ gsx_hip_status gsx_hip_lookup_backward(const void* grad_out, int32_t grad_type, 
 gsx_hip_status gsx_hip_blocks_quantize(const void* src, int32_t src_type, int64_t src_rows, int64_t src_cols,
                                        int64_t src_stride, int32_t transpose, uint8_t* values, int64_t values_stride,
                                        uint8_t* exponents, int64_t exponents_stride, hipStream_t stream);
-/* out [m, n] = a b^T for block matrices a [m, k] and b [n, k]; m, n and k at most 2^31 - 1. */
+/* out [m, n] = a b^T for block matrices a [m, k] and b [n, k]; m and n at most 2^31 - 1, k at most 2^27, value strides below
+ * 2^28. */
 size_t gsx_hip_blocks_matmul_temp_bytes(int64_t m, int64_t n, int64_t k);
 gsx_hip_status gsx_hip_blocks_matmul(const uint8_t* a_values, int64_t a_values_stride, const uint8_t* a_exponents,
                                      int64_t a_exponents_stride, const uint8_t* b_values, int64_t b_values_stride,
