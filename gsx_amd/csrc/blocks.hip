@@ -19,6 +19,7 @@ namespace gsx_amd {
 constexpr int kBlock = 128;
 constexpr int kLeastExponent = -100;  // the least E4M3 step is 2^-9: q * 2^e stays far above bfloat16's subnormals, which are cut
 constexpr int kQuantThreads = 256;
+constexpr int kQuantUnroll = 4;
 constexpr int64_t kBlocksMostGrid = 1 << 20;
 
 typedef int v8i __attribute__((ext_vector_type(8)));
@@ -48,7 +49,29 @@ __device__ inline uint32_t pack_e4m3(const float* x, int e) {
     return (uint32_t)out;
 }
 
-// 16 lanes per block of 128, eight values a lane: src row r, columns [128 kb, 128 kb + 128).
+// Four and eight elements at any element's address (the hardware takes wide accesses that are not aligned).
+template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) Quad {
+    T v[4];
+};
+template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) Octet {
+    T v[8];
+};
+
+// Largest finite magnitude (its bits) among a lane's eight values.
+__device__ inline uint32_t largest(const float (&x)[8]) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const uint32_t bits = __builtin_bit_cast(uint32_t, x[k]) & 0x7fffffffu;
+        if (finite_bits(bits)) top = max(top, bits);
+    }
+    return top;
+}
+
+// 16 lanes per block of 128, eight values a lane, kQuantUnroll blocks of one row a group: src row r, columns [128 kb, 128 kb +
+// 128). The whole blocks' loads are wide (at any element's alignment) and issued together.
 template <typename T>
 __global__ __launch_bounds__(kQuantThreads) void quantize_rows_kernel(const T* __restrict__ src, int64_t src_stride,
                                                                       int64_t rows, int64_t cols, int64_t blocks,
@@ -56,31 +79,45 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_rows_kernel(const T* _
                                                                       int64_t values_stride,
                                                                       uint8_t* __restrict__ exponents,
                                                                       int64_t exponents_stride) {
-    const int64_t total = rows * blocks;
+    const int64_t spans = ceil_div(blocks, kQuantUnroll), total = rows * spans;
     const int sub = threadIdx.x & 15;
     for (int64_t b = (int64_t)blockIdx.x * (kQuantThreads / 16) + threadIdx.x / 16; b < total;
          b += (int64_t)gridDim.x * (kQuantThreads / 16)) {
-        const int64_t r = b / blocks, kb = b % blocks;
-        const int64_t col = kb * kBlock + sub * 8;
-        float x[8];
-        uint32_t top = 0;
+        const int64_t r = b / spans, kb0 = b % spans * kQuantUnroll;
+        const T* const row = src + r * src_stride;
+        float x[kQuantUnroll][8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            x[k] = col + k < cols ? to_float(src[r * src_stride + col + k]) : 0.0f;
-            const uint32_t bits = __builtin_bit_cast(uint32_t, x[k]) & 0x7fffffffu;
-            if (finite_bits(bits)) top = max(top, bits);
+        for (int u = 0; u < kQuantUnroll; ++u) {
+            const int64_t col = (kb0 + u) * kBlock + sub * 8;
+            if (col + 8 <= cols) {
+                const Octet<T> v = *reinterpret_cast<const Octet<T>*>(row + col);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[u][k] = to_float(v.v[k]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[u][k] = col + k < cols ? to_float(row[col + k]) : 0.0f;
+            }
         }
 #pragma unroll
-        for (int off = 8; off > 0; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off, 16));
-        const int e = block_exponent(top);
-        uint8_t* const to = values + r * values_stride + col;
-        if (col < values_stride) *reinterpret_cast<uint2*>(to) = make_uint2(pack_e4m3(x, e), pack_e4m3(x + 4, e));
-        if (sub == 0) exponents[r * exponents_stride + kb] = (uint8_t)(e + 127);
+        for (int u = 0; u < kQuantUnroll; ++u) {
+            uint32_t top = largest(x[u]);
+#pragma unroll
+            for (int off = 8; off > 0; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off, 16));
+            if (kb0 + u >= blocks) continue;
+            const int e = block_exponent(top);
+            const int64_t col = (kb0 + u) * kBlock + sub * 8;
+            if (col < values_stride)
+                *reinterpret_cast<uint2*>(values + r * values_stride + col) =
+                    make_uint2(pack_e4m3(x[u], e), pack_e4m3(x[u] + 4, e));
+            if (sub == 0) exponents[r * exponents_stride + kb0 + u] = (uint8_t)(e + 127);
+        }
     }
 }
 
 // Blocks of src^T: output row c is src column c, its blocks lie along src's rows. A workgroup takes 128 src rows (one block)
-// of 64 columns through LDS.
+// of 64 columns; thread t reads 4 columns (t % 16) of the eight rows from 8 (t / 16) on, and the columns'
+// maxima and the values are exchanged through LDS. The values' bytes lie there as [column][row], a column 136 bytes (34 banks)
+// apart, and leave 16 bytes a lane.
 template <typename T>
 __global__ __launch_bounds__(kQuantThreads) void quantize_columns_kernel(const T* __restrict__ src, int64_t src_stride,
                                                                          int64_t src_rows, int64_t src_cols,
@@ -88,37 +125,61 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_columns_kernel(const T
                                                                          int64_t values_stride,
                                                                          uint8_t* __restrict__ exponents,
                                                                          int64_t exponents_stride) {
-    __shared__ float s_x[kBlock][65];
-    const int64_t tiles = ceil_div(src_cols, 64) * blocks;
+    constexpr int kPitch = 136;
+    __shared__ uint32_t s_top[4][64];
+    __shared__ __attribute__((aligned(16))) uint8_t s_q[64 * kPitch];
+    const int64_t strips = ceil_div(src_cols, 64), tiles = strips * blocks;
+    const int quad = threadIdx.x & 15, r0 = threadIdx.x / 16 * 8, wave = threadIdx.x / 64;
     for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-        const int64_t kb = tile % blocks, c0 = tile / blocks * 64;
-        for (int i = threadIdx.x; i < kBlock * 64; i += kQuantThreads) {
-            const int64_t r = kb * kBlock + i / 64, c = c0 + i % 64;
-            s_x[i / 64][i % 64] = r < src_rows && c < src_cols ? to_float(src[r * src_stride + c]) : 0.0f;
+        const int64_t kb = tile / strips, c0 = tile % strips * 64;
+        const int64_t col = c0 + quad * 4;
+        float x[8][4];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int64_t r = kb * kBlock + r0 + i;
+            const T* const p = src + r * src_stride + col;
+            if (r < src_rows && col + 4 <= src_cols) {
+                const Quad<T> v = *reinterpret_cast<const Quad<T>*>(p);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[i][k] = to_float(v.v[k]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[i][k] = r < src_rows && col + k < src_cols ? to_float(p[k]) : 0.0f;
+            }
         }
-        __syncthreads();
-        const int sub = threadIdx.x & 15;
-        for (int c = threadIdx.x / 16; c < 64; c += kQuantThreads / 16) {
-            float x[8];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
             uint32_t top = 0;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                x[k] = s_x[sub * 8 + k][c];
-                const uint32_t bits = __builtin_bit_cast(uint32_t, x[k]) & 0x7fffffffu;
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t bits = __builtin_bit_cast(uint32_t, x[i][k]) & 0x7fffffffu;
                 if (finite_bits(bits)) top = max(top, bits);
             }
-#pragma unroll
-            for (int off = 8; off > 0; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off, 16));
-            const int e = block_exponent(top);
-            const int64_t col = kb * kBlock + sub * 8;
-            if (c0 + c < src_cols) {
-                if (col < values_stride)
-                    *reinterpret_cast<uint2*>(values + (c0 + c) * values_stride + col) =
-                        make_uint2(pack_e4m3(x, e), pack_e4m3(x + 4, e));
-                if (sub == 0) exponents[(c0 + c) * exponents_stride + kb] = (uint8_t)(e + 127);
-            }
+            top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
+            top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+            if ((threadIdx.x & 63) < 16) s_top[wave][quad * 4 + k] = top;
         }
         __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int c = quad * 4 + k;
+            const uint32_t top = max(max(s_top[0][c], s_top[1][c]), max(s_top[2][c], s_top[3][c]));
+            const int e = block_exponent(top);
+            const float y[8] = {x[0][k], x[1][k], x[2][k], x[3][k], x[4][k], x[5][k], x[6][k], x[7][k]};
+            *reinterpret_cast<uint2*>(s_q + c * kPitch + r0) = make_uint2(pack_e4m3(y, e), pack_e4m3(y + 4, e));
+            if (threadIdx.x < 16 && c0 + c < src_cols)
+                exponents[(c0 + c) * exponents_stride + kb] = (uint8_t)(e + 127);
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < 64 * 8; i += kQuantThreads) {
+            const int c = i / 8, at = i % 8 * 16;
+            if (c0 + c >= src_cols || kb * kBlock + at >= values_stride) continue;
+            const uint2 lo = *reinterpret_cast<const uint2*>(s_q + c * kPitch + at);
+            const uint2 hi = *reinterpret_cast<const uint2*>(s_q + c * kPitch + at + 8);
+            *reinterpret_cast<uint4*>(values + (c0 + c) * values_stride + kb * kBlock + at) =
+                make_uint4(lo.x, lo.y, hi.x, hi.y);
+        }
+        __syncthreads();  // s_q and s_top are written again
     }
 }
 
@@ -143,12 +204,6 @@ __device__ inline v4i load_values(const uint8_t* row, int64_t k, int64_t cols) {
     }
     return v;
 }
-
-// Four elements at any element's address (the hardware takes wide accesses that are not aligned).
-template <typename T>
-struct __attribute__((packed, aligned(sizeof(T)))) Quad {
-    T v[4];
-};
 
 // 4 TN consecutive columns from `col` on of a row of n.
 template <int TN, typename O>
@@ -493,7 +548,7 @@ gsx_hip_status gsx_hip_blocks_quantize(const void* src, int32_t src_type, int64_
                                dim3(kQuantThreads), 0, stream, static_cast<const T*>(src), src_stride, src_rows, src_cols,
                                blocks, values, values_stride, exponents, exponents_stride);
         } else {
-            hipLaunchKernelGGL((quantize_rows_kernel<T>), dim3(blocks_grid(ceil_div(rows * blocks, kQuantThreads / 16))),
+            hipLaunchKernelGGL((quantize_rows_kernel<T>), dim3(blocks_grid(ceil_div(rows * ceil_div(blocks, kQuantUnroll), kQuantThreads / 16))),
                                dim3(kQuantThreads), 0, stream, static_cast<const T*>(src), src_stride, rows, cols, blocks,
                                values, values_stride, exponents, exponents_stride);
         }
