@@ -14,63 +14,12 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
-#include "fields.hpp"
+#include "blocks.hpp"
 
 namespace gsx_amd {
 
-constexpr int kBlock = 128;
-constexpr int kLeastExponent = -100;  // the least E4M3 step is 2^-9: q * 2^e stays far above bfloat16's subnormals, which are cut
 constexpr int kQuantThreads = 256;
 constexpr int kQuantUnroll = 4;
-constexpr int64_t kBlocksMostGrid = 1 << 20;
-
-typedef int v8i __attribute__((ext_vector_type(8)));
-typedef int v4i __attribute__((ext_vector_type(4)));
-typedef float v4f __attribute__((ext_vector_type(4)));
-typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
-typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
-
-__device__ inline bool finite_bits(uint32_t bits) { return (bits & 0x7f800000u) != 0x7f800000u; }
-
-// Exponent of a block whose largest finite magnitude has the float bits `top` (sign cleared): 448 = 1.75 * 2^8.
-__device__ inline int block_exponent(uint32_t top) {
-    if (top == 0) return 0;
-    const int e = (int)(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
-    return max(e, kLeastExponent);
-}
-
-// Four E4M3 bytes of x * 2^-e. |x| <= 448 * 2^e, so no finite value rounds past 448.
-__device__ inline uint32_t pack_e4m3(const float* x, int e) {
-    const float scale = __builtin_bit_cast(float, (uint32_t)(127 - e) << 23);
-    int out = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * scale, x[1] * scale, 0, false);
-    out = __builtin_amdgcn_cvt_pk_fp8_f32(x[2] * scale, x[3] * scale, out, true);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        if (!finite_bits(__builtin_bit_cast(uint32_t, x[k]))) out |= 0x7f << (8 * k);
-    }
-    return (uint32_t)out;
-}
-
-// Four and eight elements at any element's address (the hardware takes wide accesses that are not aligned).
-template <typename T>
-struct __attribute__((packed, aligned(sizeof(T)))) Quad {
-    T v[4];
-};
-template <typename T>
-struct __attribute__((packed, aligned(sizeof(T)))) Octet {
-    T v[8];
-};
-
-// Largest finite magnitude (its bits) among a lane's eight values.
-__device__ inline uint32_t largest(const float (&x)[8]) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        const uint32_t bits = __builtin_bit_cast(uint32_t, x[k]) & 0x7fffffffu;
-        if (finite_bits(bits)) top = max(top, bits);
-    }
-    return top;
-}
 
 // 16 lanes per block of 128, eight values a lane, kQuantUnroll blocks of one row a group: src row r, columns [128 kb, 128 kb +
 // 128). The whole blocks' loads are wide (at any element's alignment) and issued together.
@@ -185,59 +134,6 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_columns_kernel(const T
     }
 }
 
-struct BlockMatrix {
-    const uint8_t* values;
-    const uint8_t* exponents;
-    int64_t values_stride, exponents_stride;
-};
-
-// 16 bytes of a row at column k; columns from `cols` on read as zero.
-__device__ inline v4i load_values(const uint8_t* row, int64_t k, int64_t cols) {
-    v4i v = {0, 0, 0, 0};
-    if (k >= cols) return v;
-    v = *reinterpret_cast<const v4i*>(row + k);
-    const int64_t left = cols - k;
-    if (left < 16) {
-#pragma unroll
-        for (int d = 0; d < 4; ++d) {
-            const int64_t bytes = left - 4 * d;
-            if (bytes < 4) v[d] = bytes <= 0 ? 0 : v[d] & (int)((1u << (8 * bytes)) - 1u);
-        }
-    }
-    return v;
-}
-
-// 4 TN consecutive columns from `col` on of a row of n.
-template <int TN, typename O>
-__device__ inline void store_columns(O* __restrict__ row, int64_t col, int64_t n, const v4f (&x)[TN]) {
-#pragma unroll
-    for (int j = 0; j < TN; ++j) {
-        const int64_t c = col + 4 * j;
-        if (c + 4 <= n) {
-            Quad<O> q;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) q.v[i] = from_float<O>(x[j][i]);
-            *reinterpret_cast<Quad<O>*>(row + c) = q;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (c + i < n) row[c + i] = from_float<O>(x[j][i]);
-        }
-    }
-}
-
-// Eight E4M3 values (two words) times `scale`, exactly, in bfloat16.
-__device__ inline v8bf to_bf16(int lo, int hi, float scale) {
-    const v2bf a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)lo, scale, false);
-    const v2bf b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)lo, scale, true);
-    const v2bf c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)hi, scale, false);
-    const v2bf d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)hi, scale, true);
-    return v8bf{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
-
-// 2^e from the byte e + 127.
-__device__ inline float block_scale(uint32_t byte) { return __builtin_bit_cast(float, byte << 23); }
-
 // ---- product ------------------------------------------------------------------------------------------------------------
 //
 // A workgroup of WM x WN waves forms a tile of c: BM rows (of a) by BN columns (rows of b), a wave TM x TN times 16 x 16 of it.
@@ -247,22 +143,6 @@ __device__ inline float block_scale(uint32_t byte) { return __builtin_bit_cast(f
 //
 // The matrix instructions take b as their first operand: a lane then holds four consecutive columns of one row of c. Which
 // row of b a lane brings for instruction j is chosen so that its 4 TN columns are consecutive too, and leave in wide stores.
-
-typedef __attribute__((address_space(3))) void* LdsPtr;
-typedef const __attribute__((address_space(1))) void* GlobalPtr;
-
-// Row of b, within a wave's 16 TN, that index r of instruction j stands for.
-template <int TN>
-__device__ constexpr int column_of(int j, int r) {
-    return (r / 4) * (4 * TN) + 4 * j + r % 4;
-}
-
-// Places of the chunks: a's rows are read 16 in a row, b's as column_of orders them.
-__device__ inline int swizzle_a(int row) { return row & 7; }
-template <int TN>
-__device__ inline int swizzle_b(int row) {
-    return (row & 3) | ((row / (4 * TN)) & 1) << 2;
-}
 
 struct ProductTile {
     int64_t m0, n0;
@@ -488,11 +368,9 @@ __global__ __launch_bounds__(256) void product_join_kernel(const float* __restri
 
 using namespace gsx_amd;
 
-namespace {
+namespace gsx_amd {
 
-unsigned blocks_grid(int64_t wanted) { return (unsigned)(wanted < kBlocksMostGrid ? wanted : kBlocksMostGrid); }
-
-bool block_matrix_fits(int64_t rows, int64_t cols, int64_t values_stride, int64_t exponents_stride) {
+static bool block_matrix_fits(int64_t rows, int64_t cols, int64_t values_stride, int64_t exponents_stride) {
     return rows >= 0 && cols >= 0 && cols <= INT64_MAX - 256 && rows_fit(rows, values_stride, cols) &&
            rows_fit(rows, exponents_stride, ceil_div(cols, kBlock)) && values_stride % 16 == 0 && exponents_stride % 4 == 0;
 }
@@ -510,12 +388,16 @@ gsx_hip_status block_matrix_check(const void* values, const void* exponents, int
 }
 
 // 256 rows of a product's operand lie within 2^36 bytes (the kernel's offsets): value strides below 2^28.
-constexpr int64_t kMostSummands = (int64_t)1 << 27;
-constexpr int64_t kMostStride = (int64_t)1 << 28;
+static constexpr int64_t kMostSummands = (int64_t)1 << 27;
+static constexpr int64_t kMostStride = (int64_t)1 << 28;
 
 bool product_sizes(int64_t m, int64_t n, int64_t k) {
     return m >= 0 && n >= 0 && k >= 0 && m <= INT32_MAX && n <= INT32_MAX && k <= kMostSummands;
 }
+
+}  // namespace gsx_amd
+
+namespace {
 
 // Tiles and splits of a product by its sizes alone. Large tiles move the fewest bytes through LDS for a product; they are taken
 // where they fill the GPU's 256 CUs, smaller ones where they do not. What is still short of two workgroups a CU is split over k,
@@ -546,12 +428,6 @@ ProductPlan product_plan(int64_t m, int64_t n, int64_t k) {
     p.splits = splits < 1 ? 1 : splits;
     p.temp_bytes = p.splits > 1 ? p.splits * m * n * 4 : 0;
     return p;
-}
-
-// The quantised rows of gsx_hip_linear_forward in its workspace, rounded up for what follows them.
-int64_t linear_rows_bytes(int64_t m, int64_t k) {
-    const int64_t blocks = ceil_div(k, kBlock);
-    return ceil_div(m * (blocks * kBlock + ceil_div(blocks, 4) * 4), 256) * 256;
 }
 
 }  // namespace
@@ -642,29 +518,6 @@ gsx_hip_status gsx_hip_blocks_matmul(const uint8_t* a_values, int64_t a_values_s
         }
         return fields_launched("blocks matmul launch");
     });
-}
-
-size_t gsx_hip_linear_temp_bytes(int64_t m, int64_t n, int64_t k) {
-    if (!product_sizes(m, n, k)) return 0;
-    return (size_t)linear_rows_bytes(m, k) + gsx_hip_blocks_matmul_temp_bytes(m, n, k);
-}
-
-gsx_hip_status gsx_hip_linear_forward(const void* x, int32_t x_type, int64_t x_stride, const uint8_t* w_values,
-                                      int64_t w_values_stride, const uint8_t* w_exponents, int64_t w_exponents_stride,
-                                      int64_t m, int64_t n, int64_t k, void* out, int32_t out_type, int64_t out_stride,
-                                      void* temp, hipStream_t stream) {
-    if (!product_sizes(m, n, k))
-        return fields_fail(GSX_HIP_ERROR_OUT_OF_RANGE, "linear: at most 2^31 - 1 rows and columns and 2^27 summands");
-    if (m > 0 && k > 0 && temp == nullptr) return fields_fail(GSX_HIP_ERROR_INVALID_ARGUMENT, "linear: null workspace");
-    const int64_t blocks = ceil_div(k, kBlock);
-    uint8_t* const values = static_cast<uint8_t*>(temp);
-    uint8_t* const exponents = values + m * blocks * kBlock;
-    uint8_t* const rest = values + linear_rows_bytes(m, k);
-    const gsx_hip_status st = gsx_hip_blocks_quantize(x, x_type, m, k, x_stride, 0, values, blocks * kBlock, exponents,
-                                                      ceil_div(blocks, 4) * 4, stream);
-    if (st != GSX_HIP_SUCCESS) return st;
-    return gsx_hip_blocks_matmul(values, blocks * kBlock, exponents, ceil_div(blocks, 4) * 4, w_values, w_values_stride,
-                                 w_exponents, w_exponents_stride, m, n, k, out, out_type, out_stride, rest, stream);
 }
 
 }  // extern "C"

@@ -1,0 +1,435 @@
+// linear.hip - rows times a weight held in 8-bit blocks, the rows quantised on the way.
+//
+//   out[i, :] = sum over k of blocks(x)[i, k] w[:, k]        (blocks(x), w: see blocks.hip)
+//
+// Three ways by the sizes: few rows read the weight once and split k over a workgroup's waves; many rows and few columns
+// quantise each row's block in the registers of the wave that multiplies it, so x is read once and nothing is written but the
+// result; everything else quantises x into the workspace and takes the tiled product.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "blocks.hpp"
+#include "common.hpp"
+
+namespace gsx_amd {
+
+// Of a block's 128 k, a lane group g = lane / 16 holds 16 from 16 g on and 16 from 64 + 16 g on: one load of the four groups
+// reads 64 bytes of each weight row in a piece.
+__device__ inline int64_t piece_k(int64_t k0, int half, int lane) { return k0 + 64 * half + 16 * (lane / 16); }
+
+// A lane's 32 elements of block k0 of a row as they lie in memory, zeros past the last column.
+template <typename T>
+struct RawBlock {
+    uint32_t w[4][2 * sizeof(T)];
+};
+
+template <typename T>
+__device__ inline float element_of(const RawBlock<T>& x, int i) {
+    const uint32_t* const w = x.w[i / 8];
+    if constexpr (sizeof(T) == 4) {
+        return __builtin_bit_cast(float, w[i % 8]);
+    } else if constexpr (__is_same(T, __bf16)) {
+        const uint32_t word = w[i % 8 / 2];
+        return __builtin_bit_cast(float, i & 1 ? word & 0xffff0000u : word << 16);
+    } else {
+        const uint32_t word = w[i % 8 / 2];
+        return to_float(__builtin_bit_cast(T, (uint16_t)(i & 1 ? word >> 16 : word)));
+    }
+}
+
+template <typename T>
+__device__ inline void load_block(const T* __restrict__ row, int64_t k0, int64_t cols, int lane, RawBlock<T>& x) {
+    struct __attribute__((packed, aligned(sizeof(T)))) Words {  // at any element's address
+        uint32_t w[2 * sizeof(T)];
+    };
+#pragma unroll
+    for (int o = 0; o < 4; ++o) {
+        const int64_t at = piece_k(k0, o / 2, lane) + 8 * (o & 1);
+        Words v = {};
+        if (at + 8 <= cols) {
+            v = *reinterpret_cast<const Words*>(row + at);
+        } else if (at < cols) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (at + i >= cols) continue;
+                if constexpr (sizeof(T) == 4) v.w[i] = __builtin_bit_cast(uint32_t, row[at + i]);
+                else v.w[i / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, row[at + i]) << (16 * (i & 1));
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < (int)(2 * sizeof(T)); ++i) x.w[o][i] = v.w[i];
+    }
+}
+
+// The values that a row's block stands for, from the 32 that each of its four lanes holds; y[o] are those of w[o].
+template <typename T>
+__device__ inline void quantize_block(const RawBlock<T>& raw, v8bf (&y)[4]) {
+    float x[32];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+        x[i] = element_of(raw, i);
+        top = max(top, __builtin_bit_cast(uint32_t, x[i]) & 0x7fffffffu);
+    }
+    const bool special = __builtin_amdgcn_ballot_w64(!finite_bits(top)) != 0;
+    if (special) {  // rare: infinities and NaN do not count for the scale
+        top = 0;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            const uint32_t bits = __builtin_bit_cast(uint32_t, x[i]) & 0x7fffffffu;
+            if (finite_bits(bits)) top = max(top, bits);
+        }
+    }
+    top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+    const int e = block_exponent(top);
+    const float scale = block_scale((uint32_t)(e + 127));
+    int q[8];
+    if (special) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q[i] = (int)pack_e4m3(x + 4 * i, e);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q[i] = (int)pack_finite(x + 4 * i, e);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = to_bf16(q[2 * i], q[2 * i + 1], scale);
+}
+
+// ---- few rows -------------------------------------------------------------------------------------------------------------
+//
+// A workgroup of up to 8 waves forms 16 J columns of out for up to 16 rows; wave w takes blocks w, w + waves, ... of k, so
+// that together they read whole stretches of the weight's rows, and the waves' sums are joined through LDS. The rows of x
+// are quantised into LDS first, `span` blocks of k at a time (all of them where they fit), while the weight's first block is
+// on its way.
+constexpr int kFewRows = 16;
+constexpr int kFewWaves = 8;
+constexpr int kFewBytes = 16384;  // of quantised rows in LDS
+
+template <int J>
+struct WeightBlock {
+    v4i v[J][2];
+    uint32_t exponent[J];
+};
+
+template <int J>
+__device__ inline void load_weight(const BlockMatrix& w, const int64_t (&row)[J], int64_t kb, int64_t k, int lane,
+                                   WeightBlock<J>& b) {
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        const uint8_t* const p = w.values + row[j] * w.values_stride;
+        if ((kb + 1) * kBlock <= k) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+                b.v[j][half] = *reinterpret_cast<const v4i*>(p + piece_k(kb * kBlock, half, lane));
+        } else {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) b.v[j][half] = load_values(p, piece_k(kb * kBlock, half, lane), k);
+        }
+        b.exponent[j] = w.exponents[row[j] * w.exponents_stride + kb];
+    }
+}
+
+template <typename T, typename O, int J>
+__global__ __launch_bounds__(64 * kFewWaves, 4) void linear_few_kernel(const T* __restrict__ x, int64_t x_stride, BlockMatrix w,
+                                                                    int m, int64_t n, int64_t k, int span,
+                                                                    O* __restrict__ out, int64_t out_stride) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t s_few[];
+    v4f(*const s_acc)[J][64] = reinterpret_cast<v4f(*)[J][64]>(s_few);  // one for each wave
+    uint8_t* const s_x = s_few + sizeof(v4f) * 64 * J * (blockDim.x / 64);  // [block][row][128], chunk c at place c ^ row % 8
+    uint8_t* const s_e = s_x + (int64_t)span * m * kBlock;
+    const int lane = threadIdx.x & 63, waves = blockDim.x / 64;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int64_t blocks = ceil_div(k, kBlock), tiles = ceil_div(n, 16 * J);
+    const int x_row = min(lane & 15, m - 1);
+    for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
+        const int64_t n0 = t * 16 * J;
+        int64_t row[J];
+#pragma unroll
+        for (int j = 0; j < J; ++j) row[j] = min(n0 + column_of<J>(j, lane & 15), n - 1);
+        v4f acc[J];
+#pragma unroll
+        for (int j = 0; j < J; ++j) acc[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        WeightBlock<J> next;
+        for (int64_t kb0 = 0; kb0 < blocks; kb0 += span) {
+            const int64_t end = min(kb0 + span, blocks);
+            if (kb0 + wave < end) load_weight<J>(w, row, kb0 + wave, k, lane, next);
+            if (blocks > span || t == blockIdx.x) {
+                __syncthreads();
+                const int sub = threadIdx.x & 15;
+                for (int i = threadIdx.x / 16; i < (int)(end - kb0) * m; i += blockDim.x / 16) {
+                    const int64_t kb = kb0 + i / m;
+                    const int r = i % m;
+                    const int64_t col = kb * kBlock + sub * 8;
+                    float v[8];
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) v[c] = col + c < k ? to_float(x[r * x_stride + col + c]) : 0.0f;
+                    uint32_t top = largest(v);
+#pragma unroll
+                    for (int off = 8; off > 0; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off, 16));
+                    const int e = block_exponent(top);
+                    *reinterpret_cast<uint2*>(s_x + i * kBlock + ((sub / 2) ^ (r & 7)) * 16 + (sub & 1) * 8) =
+                        make_uint2(pack_e4m3(v, e), pack_e4m3(v + 4, e));
+                    if (sub == 0) s_e[i] = (uint8_t)(e + 127);
+                }
+                __syncthreads();
+            }
+            for (int64_t kb = kb0 + wave; kb < end; kb += waves) {
+                const WeightBlock<J> now = next;
+                if (kb + waves < end) load_weight<J>(w, row, kb + waves, k, lane, next);
+                const int at = (int)(kb - kb0) * m + x_row;
+                const float x_scale = block_scale(s_e[at]);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const v4i q = *reinterpret_cast<const v4i*>(s_x + at * kBlock + ((4 * half + lane / 16) ^ (x_row & 7)) * 16);
+                    const v8bf x0 = to_bf16(q[0], q[1], x_scale), x1 = to_bf16(q[2], q[3], x_scale);
+#pragma unroll
+                    for (int j = 0; j < J; ++j) {
+                        const float scale = block_scale(now.exponent[j]);
+                        const v4i u = now.v[j][half];
+                        acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(to_bf16(u[0], u[1], scale), x0, acc[j], 0, 0, 0);
+                        acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(to_bf16(u[2], u[3], scale), x1, acc[j], 0, 0, 0);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < J; ++j) s_acc[wave][j][lane] = acc[j];
+        __syncthreads();
+        if (wave == 0) {
+            for (int v = 1; v < waves; ++v)
+#pragma unroll
+                for (int j = 0; j < J; ++j) acc[j] += s_acc[v][j][lane];
+            if ((lane & 15) < m) store_columns<J>(out + (lane & 15) * out_stride, n0 + (lane / 16) * (4 * J), n, acc);
+        }
+        __syncthreads();
+    }
+}
+
+// ---- few columns ----------------------------------------------------------------------------------------------------------
+//
+// A wave takes 16 R rows and all (up to 16 TN) columns; x is read once, straight into registers, a block ahead. The weight lies
+// in LDS for the workgroup's four waves, all of it where it fits (kHeadBytes) and is then read once for all the tiles of a
+// workgroup, else a block of 128 k at a time; each wave converts it. The result passes through LDS, 16 rows of a wave at a
+// time, and leaves in whole stretches of its rows.
+constexpr int kHeadThreads = 256;
+constexpr int kHeadBytes = 49152;
+template <int TN>
+constexpr int kHeadRows = TN > 4 ? 16 : 32;  // of a wave: more hide less of the loads' time for want of registers
+template <typename O, int TN>
+constexpr int kHeadPitch = 16 * TN * (int)sizeof(O) + 16;
+template <int TN>
+constexpr int kHeadResident = kHeadBytes / (16 * TN * kBlock);  // blocks of k that fit
+
+template <typename T, typename O, int TN>
+__global__ __launch_bounds__(kHeadThreads, 2) void linear_head_kernel(const T* __restrict__ x, int64_t x_stride,
+                                                                      BlockMatrix w, int64_t m, int64_t n, int64_t k,
+                                                                      int slots, O* __restrict__ out, int64_t out_stride) {
+    constexpr int R = kHeadRows<TN> / 16, kRows = 16 * TN, kWaves = kHeadThreads / 64;
+    constexpr int kOct = 8;  // columns a lane stores at once
+    extern __shared__ __attribute__((aligned(16))) uint8_t s_head[];  // slots for blocks of the weight, their exponents
+    uint8_t* const s_w = s_head;
+    uint8_t* const s_e = s_head + slots * kRows * kBlock;
+    __shared__ __attribute__((aligned(16))) uint8_t s_out[kWaves][16 * kHeadPitch<O, TN>];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x / 64;
+    const int64_t blocks = ceil_div(k, kBlock), tiles = ceil_div(m, kHeadRows<TN> * kWaves);
+    const bool resident = blocks <= slots;
+    const auto stage = [&](int64_t kb, int slot) {
+        for (int i = threadIdx.x; i < kRows * 8; i += kHeadThreads) {
+            const int row = i / 8, chunk = i % 8;
+            const int64_t source = min((int64_t)row, n - 1);
+            *reinterpret_cast<v4i*>(s_w + (slot * kRows + row) * kBlock + ((chunk ^ swizzle_b<TN>(row)) * 16)) =
+                load_values(w.values + source * w.values_stride, kb * kBlock + chunk * 16, k);
+            if (chunk == 0) s_e[slot * kRows + row] = w.exponents[source * w.exponents_stride + kb];
+        }
+    };
+    RawBlock<T> next[R];
+    const auto load = [&](int64_t tile, int64_t kb) {
+        const int64_t m0 = (tile * kWaves + wave) * kHeadRows<TN>;
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            load_block<T>(x + min(m0 + r * 16 + (lane & 15), m - 1) * x_stride, kb * kBlock, k, lane, next[r]);
+    };
+    if ((int64_t)blockIdx.x < tiles && blocks > 0) load(blockIdx.x, 0);
+    if (resident) {
+        for (int64_t kb = 0; kb < blocks; ++kb) stage(kb, (int)kb);
+        __syncthreads();
+    }
+    // lanes of a stretch of 8 columns, a power of two, and the rows that 64 lanes cover
+    int across = 1;
+    while (across * kOct < n) across *= 2;
+    for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
+        const int64_t m0 = (t * kWaves + wave) * kHeadRows<TN>;
+        v4f acc[R][TN];
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[r][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int64_t kb = 0; kb < blocks; ++kb) {
+            int slot = (int)kb;
+            if (!resident) {
+                slot = 0;
+                __syncthreads();
+                stage(kb, 0);
+                __syncthreads();
+            }
+            v8bf vx[R][4];
+#pragma unroll
+            for (int r = 0; r < R; ++r) quantize_block<T>(next[r], vx[r]);
+            if (kb + 1 < blocks) load(t, kb + 1);
+            else if (t + gridDim.x < tiles) load(t + gridDim.x, 0);
+            const uint8_t* const values = s_w + slot * kRows * kBlock;
+#pragma unroll
+            for (int j = 0; j < TN; ++j) {
+                const int row = column_of<TN>(j, lane & 15);
+                const float scale = block_scale(s_e[slot * kRows + row]);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const v4i q = *reinterpret_cast<const v4i*>(
+                        values + row * kBlock + (((4 * half + lane / 16) ^ swizzle_b<TN>(row)) * 16));
+                    const v8bf w0 = to_bf16(q[0], q[1], scale), w1 = to_bf16(q[2], q[3], scale);
+#pragma unroll
+                    for (int r = 0; r < R; ++r) {
+                        acc[r][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w0, vx[r][2 * half], acc[r][j], 0, 0, 0);
+                        acc[r][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w1, vx[r][2 * half + 1], acc[r][j], 0, 0, 0);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            uint8_t* const mine = s_out[wave];
+            wave_lds_sync();
+#pragma unroll
+            for (int j = 0; j < TN; ++j) {
+                Vec<O, 4> q;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) q.v[i] = from_float<O>(acc[r][j][i]);
+                *reinterpret_cast<Vec<O, 4>*>(mine + (lane & 15) * kHeadPitch<O, TN> +
+                                              ((lane / 16) * 4 * TN + 4 * j) * sizeof(O)) = q;
+            }
+            wave_lds_sync();
+            const int col = lane % across * kOct;
+            for (int i = lane / across; i < 16; i += 64 / across) {
+                const int64_t row = m0 + r * 16 + i;
+                if (row >= m || col >= n) continue;
+                const O* const from = reinterpret_cast<const O*>(mine + i * kHeadPitch<O, TN>) + col;
+                O* const to = out + row * out_stride + col;
+                if (col + kOct <= n) {
+                    *reinterpret_cast<Octet<O>*>(to) = *reinterpret_cast<const Octet<O>*>(from);
+                } else {
+                    for (int c = 0; c < n - col; ++c) to[c] = from[c];
+                }
+            }
+        }
+    }
+}
+
+}  // namespace gsx_amd
+
+using namespace gsx_amd;
+
+namespace {
+
+constexpr int64_t kHeadMostColumns = 256;
+
+enum class LinearWay { kFew, kHead, kTiles };
+
+LinearWay linear_way(int64_t m, int64_t n, int64_t k) {
+    if (m <= kFewRows) return LinearWay::kFew;
+    if (n <= kHeadMostColumns && (m >= 16384 || k <= 512)) return LinearWay::kHead;
+    return LinearWay::kTiles;
+}
+
+// The quantised rows in the workspace, rounded up for what follows them.
+int64_t linear_rows_bytes(int64_t m, int64_t k) {
+    const int64_t blocks = ceil_div(k, kBlock);
+    return ceil_div(m * (blocks * kBlock + ceil_div(blocks, 4) * 4), 256) * 256;
+}
+
+template <typename T, typename O, int TN>
+void launch_head(const T* x, int64_t x_stride, const BlockMatrix& w, int64_t m, int64_t n, int64_t k, O* out,
+                 int64_t out_stride, hipStream_t stream) {
+    // as many workgroups as run at once: registers and LDS leave four a CU at most
+    const int64_t tiles = ceil_div(m, kHeadRows<TN> * (kHeadThreads / 64)), blocks = ceil_div(k, kBlock);
+    const int slots = blocks <= kHeadResident<TN> ? (int)(blocks > 0 ? blocks : 1) : 1;
+    const int lds = slots * 16 * TN * (kBlock + 1);
+    hipLaunchKernelGGL((linear_head_kernel<T, O, TN>), dim3((unsigned)(tiles < 1024 ? tiles : 1024)), dim3(kHeadThreads),
+                       (unsigned)lds, stream, x, x_stride, w, m, n, k, slots, out, out_stride);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t gsx_hip_linear_temp_bytes(int64_t m, int64_t n, int64_t k) {
+    if (!product_sizes(m, n, k) || linear_way(m, n, k) != LinearWay::kTiles) return 0;
+    return (size_t)linear_rows_bytes(m, k) + gsx_hip_blocks_matmul_temp_bytes(m, n, k);
+}
+
+gsx_hip_status gsx_hip_linear_forward(const void* x, int32_t x_type, int64_t x_stride, const uint8_t* w_values,
+                                      int64_t w_values_stride, const uint8_t* w_exponents, int64_t w_exponents_stride,
+                                      int64_t m, int64_t n, int64_t k, void* out, int32_t out_type, int64_t out_stride,
+                                      void* temp, hipStream_t stream) {
+    if (!known_type(x_type) || !known_type(out_type))
+        return fields_fail(GSX_HIP_ERROR_NOT_SUPPORTED, "linear: rows are f32, bf16 or f16");
+    if (!product_sizes(m, n, k))
+        return fields_fail(GSX_HIP_ERROR_OUT_OF_RANGE, "linear: at most 2^31 - 1 rows and columns and 2^27 summands");
+    if (!rows_fit(m, x_stride, k) || !rows_fit(m, out_stride, n))
+        return fields_fail(GSX_HIP_ERROR_INVALID_ARGUMENT, "linear: strides must be at least the rows' lengths");
+    const gsx_hip_status wrong = block_matrix_check(w_values, w_exponents, n, k, w_values_stride, w_exponents_stride);
+    if (wrong != GSX_HIP_SUCCESS) return wrong;
+    if (m == 0 || n == 0) return GSX_HIP_SUCCESS;
+    if (out == nullptr || (k > 0 && x == nullptr) || !aligned_to(out, type_bytes(out_type)) ||
+        !aligned_to(x, type_bytes(x_type)))
+        return fields_fail(GSX_HIP_ERROR_INVALID_ARGUMENT, "linear: rows must be non-null and aligned to their elements");
+    const LinearWay way = linear_way(m, n, k);
+    if (way == LinearWay::kTiles) {
+        if (k > 0 && (temp == nullptr || !aligned_to(temp, 16)))
+            return fields_fail(GSX_HIP_ERROR_INVALID_ARGUMENT, "linear: the workspace must be non-null and 16-byte aligned");
+        const int64_t blocks = ceil_div(k, kBlock), words = ceil_div(blocks, 4) * 4;
+        uint8_t* const values = static_cast<uint8_t*>(temp);
+        uint8_t* const exponents = values + m * blocks * kBlock;
+        const gsx_hip_status st = gsx_hip_blocks_quantize(x, x_type, m, k, x_stride, 0, values, blocks * kBlock, exponents,
+                                                          words, stream);
+        if (st != GSX_HIP_SUCCESS) return st;
+        return gsx_hip_blocks_matmul(values, blocks * kBlock, exponents, words, w_values, w_values_stride, w_exponents,
+                                     w_exponents_stride, m, n, k, out, out_type, out_stride,
+                                     values + linear_rows_bytes(m, k), stream);
+    }
+    const BlockMatrix w = {w_values, w_exponents, w_values_stride, w_exponents_stride};
+    return with_type(x_type, [&](auto tx) {
+        return with_type(out_type, [&](auto to) {
+            using T = decltype(tx);
+            using O = decltype(to);
+            const T* const from = static_cast<const T*>(x);
+            O* const result = static_cast<O*>(out);
+            if (way == LinearWay::kFew) {
+                // waves enough for the GPU: 32 columns a workgroup where that leaves 1024 of them, else 16, and up to 8
+                // waves over k
+                const int64_t blocks = ceil_div(k, kBlock), strips = ceil_div(n, 16);
+                const int j = strips >= 2048 ? 2 : 1;
+                int64_t waves = 4;
+                while (waves < kFewWaves && waves < blocks && ceil_div(strips, j) * waves < 4096) waves *= 2;
+                const int64_t groups = ceil_div(strips, j);
+                int64_t span = kFewBytes / kBlock / m;
+                if (span > blocks) span = blocks;
+                const int64_t lds = waves * j * 1024 + span * m * (kBlock + 1);
+                hipLaunchKernelGGL((j == 2 ? linear_few_kernel<T, O, 2> : linear_few_kernel<T, O, 1>),
+                                   dim3((unsigned)(groups < 1024 ? groups : 1024)), dim3((unsigned)waves * 64),
+                                   (unsigned)lds, stream, from, x_stride, w, (int)m, n, k, (int)span, result, out_stride);
+            } else if (n <= 64) {
+                launch_head<T, O, 4>(from, x_stride, w, m, n, k, result, out_stride, stream);
+            } else if (n <= 128) {
+                launch_head<T, O, 8>(from, x_stride, w, m, n, k, result, out_stride, stream);
+            } else if (n <= 192) {
+                launch_head<T, O, 12>(from, x_stride, w, m, n, k, result, out_stride, stream);
+            } else {
+                launch_head<T, O, 16>(from, x_stride, w, m, n, k, result, out_stride, stream);
+            }
+            return fields_launched("linear launch");
+        });
+    });
+}
+
+}  // extern "C"

@@ -332,5 +332,10 @@ def test_blocks_refusals_of_the_c_interface():
     good = (p, 16, p, 4, p, 16, p, 4)
     for m, n, k, stride in ((-1, 1, 16, 1), (2**31, 1, 16, 1), (1, 1, 2**31, 1), (1, 2, 16, 1)):
         assert lib.gsx_hip_blocks_matmul(*good, m, n, k, p, 0, stride, None, None) < 0
-    assert lib.gsx_hip_linear_forward(p, 0, 16, p, 16, p, 4, 1, 1, 16, p, 0, 1, None, None) == _lib.ERROR_INVALID_ARGUMENT
+    # a call that needs a workspace (some sizes need none), refused before anything runs
+    y = torch.zeros(1024 * 1024, device="cuda").data_ptr()
+    assert lib.gsx_hip_linear_temp_bytes(300, 300, 1024) > 0
+    assert lib.gsx_hip_linear_forward(y, 0, 1024, y, 1024, y, 8, 300, 300, 1024, y, 0, 300, None,
+                                      None) == _lib.ERROR_INVALID_ARGUMENT
+    assert lib.gsx_hip_linear_forward(p, 0, 15, p, 16, p, 4, 1, 1, 16, p, 0, 1, None, None) == _lib.ERROR_INVALID_ARGUMENT
     assert lib.gsx_hip_linear_temp_bytes(-1, 4, 4) == 0
