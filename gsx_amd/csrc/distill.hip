@@ -8,11 +8,17 @@
 #include <math.h>
 #include <stdint.h>
 
+#include "common.hpp"
 #include "fields.hpp"
 
 namespace gsx_amd {
 
-constexpr int kDistillThreads = 256;
+// Maximum m of a set of logits and sum s of exp((z - m) / T), joined over disjoint sets. m = -inf: nothing above -inf (s = 0). A
+// NaN or +inf among the logits leaves a NaN in s: (z - m) / T is one.
+struct MaxSum {
+    float m, s;
+};
+
 constexpr int kDistillMostTop = 1024;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -22,18 +28,16 @@ struct DistillArgs {
     const float* teacher;
     int32_t top;
     float temperature;
-    float scale2;            // log2(e) / temperature
-    const float* row_weight; // may be null: 1
-    const float* row_grad;   // may be null: 1
+    float scale2;             // log2(e) / temperature
+    const float* row_weight;  // may be null: 1
+    const float* row_grad;    // may be null: 1
     float grad_scale;
-    float* loss;
-    float* stats;
-};
-
-// Maximum m of a set of logits and sum s of exp((z - m) / T), joined over disjoint sets. m = -inf: nothing yet (s = 0). A NaN
-// or +inf among the logits leaves a NaN in s.
-struct MaxSum {
-    float m, s;
+    float* loss;              // may be null
+    float* stats;             // may be null where it is written
+    int32_t from_stats;       // read them instead of forming them
+    int64_t first_row;        // of a launch over a part of the rows
+    int64_t slice, slices;    // logits of a workgroup where a row has several, and how many
+    MaxSum* partial;
 };
 
 __device__ inline float exp2_scaled(float x, float m, float scale2) { return __builtin_amdgcn_exp2f((x - m) * scale2); }
@@ -46,151 +50,352 @@ __device__ inline MaxSum join(MaxSum a, MaxSum b, float scale2) {
     return r;
 }
 
-__device__ inline MaxSum wave_join(MaxSum a, float scale2) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-        MaxSum b;
-        b.m = __shfl_xor(a.m, off, 64);
-        b.s = __shfl_xor(a.s, off, 64);
-        a = join(a, b, scale2);
-    }
-    return a;
+// A group of kGroup threads works on one row: a wave of its own, or the whole workgroup.
+template <int kGroup>
+__device__ inline void group_sync() {
+    if constexpr (kGroup == 64) wave_lds_sync();
+    else __syncthreads();
 }
 
-// The teacher's side of one row in LDS, by the whole workgroup: s_id (-1: not valid) and s_p (p_k); true if there is a valid
-// entry. log p_k = (t_k - m) / T - log_sum. Ends with a barrier.
-template <int kThreads>
-__device__ inline bool teacher_row(const DistillArgs& a, int64_t row, int32_t* s_id, float* s_p, float* s_wave,
-                                   float& t_max, float& log_sum) {
+// Sum and maximum over a group; s_wave holds a float for each of the group's waves. NaN does not pass max_of_group (fmaxf).
+template <int kGroup>
+__device__ inline float sum_of_group(float v, float* s_wave) {
+    v = wave_sum(v);
+    if constexpr (kGroup == 64) return v;
+    const int wave = threadIdx.x / 64;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) s_wave[wave] = v;
+    __syncthreads();
+    v = s_wave[0];
+#pragma unroll
+    for (int w = 1; w < kGroup / 64; ++w) v += s_wave[w];
+    return v;
+}
+
+template <int kGroup>
+__device__ inline float max_of_group(float v, float* s_wave) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
+    if constexpr (kGroup == 64) return v;
+    const int wave = threadIdx.x / 64;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) s_wave[wave] = v;
+    __syncthreads();
+    v = s_wave[0];
+#pragma unroll
+    for (int w = 1; w < kGroup / 64; ++w) v = fmaxf(v, s_wave[w]);
+    return v;
+}
+
+// The teacher's side of one row: in LDS for each entry its id (-1: does not count), its p and the student's logit there.
+struct Teacher {
+    int32_t* id;
+    float* p;
+    float* z;
+    float max, log_sum;  // log p_k = (t_k - max) / T - log_sum
+    bool any;            // an entry counts
+};
+
+// Loads what teacher_finish needs; between the two the caller may load its part of the row.
+template <typename T, int kGroup>
+__device__ inline void teacher_load(const DistillArgs& a, const T* __restrict__ z, int64_t row, int tid, Teacher& r) {
     const int32_t* ids = a.ids + row * a.teacher_stride;
     const float* t = a.teacher + row * a.teacher_stride;
-    float m = -INFINITY;
-    bool nan = false;
-    for (int k = threadIdx.x; k < a.top; k += kThreads) {
+    for (int k = tid; k < a.top; k += kGroup) {
         const int32_t id = ids[k];
         const float x = t[k];
-        const bool valid = id >= 0 && id < a.vocab && !(x == -INFINITY);
-        s_id[k] = valid ? id : -1;
-        s_p[k] = x;
-        if (valid) {
-            m = fmaxf(m, x);
-            nan |= x != x;
-        }
+        const bool counts = id >= 0 && id < a.vocab && !(x == -INFINITY);
+        r.id[k] = counts ? id : -1;
+        r.p[k] = x;
+        r.z[k] = counts ? to_float(z[id]) : 0.0f;
     }
-    if (nan) m = NAN;
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-        const float o = __shfl_xor(m, off, 64);
-        m = m != m || o != o ? NAN : fmaxf(m, o);
-    }
-    if ((threadIdx.x & 63) == 0) s_wave[threadIdx.x / 64] = m;
-    __syncthreads();
-    m = s_wave[0];
-    for (int w = 1; w < kThreads / 64; ++w) m = m != m || s_wave[w] != s_wave[w] ? NAN : fmaxf(m, s_wave[w]);
-    t_max = m;
-    const bool any = !(m == -INFINITY);
-    const float inv_t = 1.0f / a.temperature;
-    float sum = 0.0f;
-    for (int k = threadIdx.x; k < a.top; k += kThreads) {
-        const float e = s_id[k] >= 0 ? expf((s_p[k] - m) * inv_t) : 0.0f;
-        s_p[k] = e;
-        sum += e;
-    }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
-    __syncthreads();  // s_wave has been read
-    if ((threadIdx.x & 63) == 0) s_wave[threadIdx.x / 64] = sum;
-    __syncthreads();
-    sum = 0.0f;
-    for (int w = 0; w < kThreads / 64; ++w) sum += s_wave[w];
-    log_sum = logf(sum);
-    for (int k = threadIdx.x; k < a.top; k += kThreads) s_p[k] = any ? s_p[k] / sum : 0.0f;
-    __syncthreads();
-    return any;
 }
 
-// sum_k p_k (log p_k - log q_{id_k}) of one row by the whole workgroup (every thread returns it).
-template <typename T, int kThreads>
-__device__ inline float cross_terms(const DistillArgs& a, const T* z, int64_t row, const int32_t* s_id, const float* s_p,
-                                    float* s_wave, float t_max, float log_sum, MaxSum q) {
+template <int kGroup>
+__device__ inline void teacher_finish(const DistillArgs& a, int tid, float* s_wave, Teacher& r) {
+    float m = -INFINITY, any = 0.0f;
+    for (int k = tid; k < a.top; k += kGroup) {
+        if (r.id[k] < 0) continue;
+        m = fmaxf(m, r.p[k]);
+        any = 1.0f;
+    }
+    m = max_of_group<kGroup>(m, s_wave);
+    const float inv_t = 1.0f / a.temperature;
+    float sum = 0.0f;
+    for (int k = tid; k < a.top; k += kGroup) {
+        const float e = r.id[k] >= 0 ? expf((r.p[k] - m) * inv_t) : 0.0f;  // NaN stays NaN, in the sum too
+        r.p[k] = e;
+        sum += e;
+    }
+    r.any = max_of_group<kGroup>(any, s_wave) != 0.0f;
+    sum = sum_of_group<kGroup>(sum, s_wave);
+    r.max = m;
+    r.log_sum = logf(sum);
+    for (int k = tid; k < a.top; k += kGroup) r.p[k] = r.any ? r.p[k] / sum : 0.0f;
+    group_sync<kGroup>();
+}
+
+// sum_k p_k (log p_k - log q_{id_k}) by the group (every thread returns it).
+template <int kGroup>
+__device__ inline float cross_terms(const DistillArgs& a, int64_t row, int tid, const Teacher& r, float* s_wave, MaxSum q) {
     const float* t = a.teacher + row * a.teacher_stride;
     const float inv_t = 1.0f / a.temperature;
     const float log_s = logf(q.s);
     float sum = 0.0f;
-    for (int k = threadIdx.x; k < a.top; k += kThreads) {
-        if (s_id[k] < 0 || s_p[k] == 0.0f) continue;
-        const float log_p = (t[k] - t_max) * inv_t - log_sum;
-        const float x = to_float(z[s_id[k]]);
+    for (int k = tid; k < a.top; k += kGroup) {
+        if (r.id[k] < 0 || r.p[k] == 0.0f) continue;
+        const float log_p = (t[k] - r.max) * inv_t - r.log_sum;
+        const float x = r.z[k];
         const float log_q = x == -INFINITY && !(q.s != q.s) ? -INFINITY : (x - q.m) * inv_t - log_s;
-        sum += s_p[k] * (log_p - log_q);
+        sum += r.p[k] * (log_p - log_q);
     }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) s_wave[threadIdx.x / 64] = sum;
-    __syncthreads();
-    sum = 0.0f;
-    for (int w = 0; w < kThreads / 64; ++w) sum += s_wave[w];
-    return sum;
+    return sum_of_group<kGroup>(sum, s_wave);
 }
 
-// Gradient of a row by the whole workgroup: every logit's q_j first, then the teacher's entries again with all their p_k.
-template <typename T, int kThreads>
-__device__ inline void write_grad(const DistillArgs& a, const T* z, T* g, const int32_t* s_id, const float* s_p, MaxSum q,
-                                  bool live, float c) {
-    const float base = q.m == -INFINITY ? 0.0f : q.m;
-    if (!live || q.s == 0.0f) {
-        for (int64_t j = threadIdx.x; j < a.vocab; j += kThreads) g[j] = from_float<T>(0.0f);
-        return;
-    }
-    const float cq = c / q.s;
-    for (int64_t j = threadIdx.x; j < a.vocab; j += kThreads)
-        g[j] = from_float<T>(cq * exp2_scaled(to_float(z[j]), base, a.scale2));
-    __syncthreads();  // orders these stores before the entries' below
-    for (int k = threadIdx.x; k < a.top; k += kThreads) {
-        const int32_t id = s_id[k];
-        if (id < 0) continue;
-        float p = 0.0f;
-        for (int o = 0; o < a.top; ++o) p += s_id[o] == id ? s_p[o] : 0.0f;
-        g[id] = from_float<T>(cq * exp2_scaled(to_float(z[id]), base, a.scale2) - c * p);
+// The gradient of logit z with softmax numerator and denominator from q: base = q.m, cq = c / q.s.
+__device__ inline float q_term(float z, float base, float cq, float scale2) { return cq * exp2_scaled(z, base, scale2); }
+
+// The teacher's entries with ids in [from, to) again, with all their p: after the group's stores of c q_j. c = 0 and a row
+// without a distribution need none.
+template <typename T, int kGroup>
+__device__ inline void patch_entries(const DistillArgs& a, T* __restrict__ g, int64_t from, int64_t to, int tid,
+                                     const Teacher& r, float base, float cq, float c) {
+    for (int k = tid; k < a.top; k += kGroup) {
+        const int32_t id = r.id[k];
+        if (id < from || id >= to || id < 0) continue;
+        float p = 0.0f;  // an id that is named twice has both
+        for (int o = 0; o < a.top; ++o) p += r.id[o] == id ? r.p[o] : 0.0f;
+        g[id] = from_float<T>(q_term(r.z[k], base, cq, a.scale2) - c * p);
     }
 }
 
-// One workgroup per row: maximum and sum in one pass over the logits, then (grad) a second pass.
+// 16 bytes of logits at any element's address.
 template <typename T>
-__global__ __launch_bounds__(kDistillThreads) void distill_row_kernel(DistillArgs a, const T* __restrict__ logits,
-                                                                      T* __restrict__ grad, int from_stats) {
-    __shared__ int32_t s_id[kDistillMostTop];
-    __shared__ float s_p[kDistillMostTop];
-    __shared__ float s_wave[2 * kDistillThreads / 64];
-    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        const T* z = logits + row * a.logits_stride;
-        float t_max, log_sum;
-        const bool any = teacher_row<kDistillThreads>(a, row, s_id, s_p, s_wave, t_max, log_sum);
+struct Words {
+    static constexpr int kElements = 16 / (int)sizeof(T);
+    uint32_t w[4];
+};
+template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) LooseWords {
+    uint32_t w[4];
+};
+
+template <typename T>
+__device__ inline float element_of(const Words<T>& x, int i) {
+    if constexpr (sizeof(T) == 4) {
+        return __builtin_bit_cast(float, x.w[i]);
+    } else if constexpr (__is_same(T, __bf16)) {
+        return __builtin_bit_cast(float, i & 1 ? x.w[i / 2] & 0xffff0000u : x.w[i / 2] << 16);
+    } else {
+        return to_float(__builtin_bit_cast(T, (uint16_t)(i & 1 ? x.w[i / 2] >> 16 : x.w[i / 2])));
+    }
+}
+
+// Keeps the compiler from holding what it unpacked or computed from x beside x itself until the next use: registers are what
+// bounds the rows that fit.
+template <typename T>
+__device__ inline void repack(Words<T>& x) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(x.w[i]));
+}
+
+template <typename T>
+__device__ inline uint32_t element_bits(float x) {
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(uint32_t, x);
+    else return __builtin_bit_cast(uint16_t, from_float<T>(x));
+}
+
+// Vector v of a row, -inf in all its elements where there is none (v >= vecs). The elements behind a row's last whole vector
+// (fewer than a vector) are taken one a thread, see tail_of.
+template <typename T>
+__device__ inline Words<T> load_words(const T* __restrict__ z, int64_t v, int64_t vecs) {
+    constexpr uint32_t kNone = sizeof(T) == 4 ? 0xff800000u : __is_same(T, __bf16) ? 0xff80ff80u : 0xfc00fc00u;
+    Words<T> x = {{kNone, kNone, kNone, kNone}};
+    if (v < vecs) {
+        const LooseWords<T> y = *reinterpret_cast<const LooseWords<T>*>(z + v * Words<T>::kElements);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x.w[i] = y.w[i];
+    }
+    return x;
+}
+
+template <typename T>
+__device__ inline void store_words(T* __restrict__ g, int64_t v, int64_t vecs, const float (&y)[Words<T>::kElements]) {
+    if (v >= vecs) return;
+    LooseWords<T> x;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x.w[i] = element_bits<T>(y[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x.w[i] = element_bits<T>(y[2 * i]) | element_bits<T>(y[2 * i + 1]) << 16;
+    }
+    *reinterpret_cast<LooseWords<T>*>(g + v * Words<T>::kElements) = x;
+}
+
+// Place of a thread's element behind the last whole vector of a row of `length`; -1: it has none.
+template <typename T>
+__device__ inline int64_t tail_of(int64_t length, int tid) {
+    const int64_t at = length / Words<T>::kElements * Words<T>::kElements + tid;
+    return at < length ? at : -1;
+}
+
+// Rows that fit the registers of a group: kGroup threads hold kVecs times 16 bytes each. The logits are read once; maximum, sum
+// and gradient come from registers.
+template <typename T, int kGroup, int kVecs>
+__global__ __launch_bounds__(kGroup < 256 ? 256 : kGroup) void distill_held_kernel(DistillArgs a, const T* __restrict__ logits,
+                                                                                   T* __restrict__ grad) {
+    constexpr int kGroups = kGroup < 256 ? 256 / kGroup : 1;  // rows of a workgroup
+    constexpr int kElements = Words<T>::kElements;
+    extern __shared__ uint8_t s_distill[];
+    __shared__ float s_wave[16];
+    const int group = kGroups == 1 ? 0 : threadIdx.x / kGroup, tid = kGroups == 1 ? threadIdx.x : threadIdx.x % kGroup;
+    Teacher r;
+    r.id = reinterpret_cast<int32_t*>(s_distill) + group * 3 * a.top;
+    r.p = reinterpret_cast<float*>(r.id + a.top);
+    r.z = r.p + a.top;
+    const int64_t vecs = a.vocab / kElements, tail = tail_of<T>(a.vocab, tid);
+    for (int64_t row = (int64_t)blockIdx.x * kGroups + group; row < a.rows; row += (int64_t)gridDim.x * kGroups) {
+        const T* const z = logits + row * a.logits_stride;
         const float w = a.row_weight != nullptr ? a.row_weight[row] : 1.0f;
-        const bool live = any && w != 0.0f;
-        MaxSum q = {-INFINITY, 0.0f};
-        if (from_stats != 0) {
+        Words<T> x[kVecs];
+        group_sync<kGroup>();  // the row before has been patched
+#pragma unroll
+        for (int u = 0; u < kVecs; ++u) x[u] = load_words<T>(z, (int64_t)u * kGroup + tid, vecs);
+        const float last = tail >= 0 ? to_float(z[tail]) : -INFINITY;
+        teacher_load<T, kGroup>(a, z, row, tid, r);
+        MaxSum q;
+        if (a.from_stats != 0) {
             q.m = a.stats[2 * row];
             q.s = a.stats[2 * row + 1];
         } else {
-            for (int64_t j = threadIdx.x; j < a.vocab; j += kDistillThreads) {
-                MaxSum one = {to_float(z[j]), 1.0f};
-                if (one.m == -INFINITY) one.s = 0.0f;
-                if (one.m != one.m) one = {-INFINITY, NAN};
-                q = join(q, one, a.scale2);
+            float m = last == last ? last : -INFINITY;
+#pragma unroll
+            for (int u = 0; u < kVecs; ++u)
+#pragma unroll
+                for (int i = 0; i < kElements; ++i) m = fmaxf(m, element_of(x[u], i));
+            q.m = max_of_group<kGroup>(m, s_wave);
+            const float base = q.m == -INFINITY ? 0.0f : q.m;
+            float s = exp2_scaled(last, base, a.scale2);
+#pragma unroll
+            for (int u = 0; u < kVecs; ++u) {
+                repack(x[u]);
+#pragma unroll
+                for (int i = 0; i < kElements; ++i) s += exp2_scaled(element_of(x[u], i), base, a.scale2);
             }
-            q = wave_join(q, a.scale2);
-            __syncthreads();
-            if ((threadIdx.x & 63) == 0) {
-                s_wave[2 * (threadIdx.x / 64)] = q.m;
-                s_wave[2 * (threadIdx.x / 64) + 1] = q.s;
+            q.s = sum_of_group<kGroup>(s, s_wave);
+        }
+        teacher_finish<kGroup>(a, tid, s_wave, r);
+        const bool live = r.any && w != 0.0f;
+        if (a.from_stats == 0) {
+            const float terms = cross_terms<kGroup>(a, row, tid, r, s_wave, q);
+            if (tid == 0) {
+                if (a.loss != nullptr) a.loss[row] = live ? w * a.temperature * a.temperature * terms : 0.0f;
+                if (a.stats != nullptr) {
+                    a.stats[2 * row] = q.m;
+                    a.stats[2 * row + 1] = q.s;
+                }
             }
-            __syncthreads();
-            q = {s_wave[0], s_wave[1]};
-            for (int i = 1; i < kDistillThreads / 64; ++i) q = join(q, {s_wave[2 * i], s_wave[2 * i + 1]}, a.scale2);
-            __syncthreads();
-            const float terms = cross_terms<T, kDistillThreads>(a, z, row, s_id, s_p, s_wave, t_max, log_sum, q);
+        }
+        if (grad == nullptr) continue;
+        T* const g = grad + row * a.grad_stride;
+        const bool some = live && q.s != 0.0f;
+        const float c = (a.row_grad != nullptr ? a.row_grad[row] : 1.0f) * a.grad_scale * w * a.temperature;
+        const float cq = some ? c / q.s : 0.0f, base = q.m == -INFINITY ? 0.0f : q.m;
+#pragma unroll
+        for (int u = 0; u < kVecs; ++u) {
+            float y[kElements];
+            repack(x[u]);
+#pragma unroll
+            for (int i = 0; i < kElements; ++i)
+                y[i] = some ? q_term(element_of(x[u], i), base, cq, a.scale2) : 0.0f;
+            store_words<T>(g, (int64_t)u * kGroup + tid, vecs, y);
+        }
+        if (tail >= 0) g[tail] = from_float<T>(some ? q_term(last, base, cq, a.scale2) : 0.0f);
+        if (some) {
+            group_sync<kGroup>();  // orders those stores before the entries'
+            patch_entries<T, kGroup>(a, g, 0, a.vocab, tid, r, base, cq, c);
+        }
+    }
+}
+
+// Longer rows, and few of them: a row is cut into slices of a workgroup each. This launch leaves every slice's maximum and sum,
+constexpr int kSliceThreads = 256;
+
+template <typename T>
+__global__ __launch_bounds__(kSliceThreads) void distill_slices_kernel(DistillArgs a, const T* __restrict__ logits) {
+    __shared__ float s_wave[kSliceThreads / 64];
+    constexpr int kElements = Words<T>::kElements, kAhead = 4;
+    const int64_t total = a.rows * a.slices;
+    for (int64_t b = blockIdx.x; b < total; b += gridDim.x) {
+        const int64_t row = a.first_row + b / a.slices, from = b % a.slices * a.slice;
+        const int64_t to = min(from + a.slice, a.vocab);
+        const T* const z = logits + row * a.logits_stride + from;
+        const int64_t vecs = (to - from) / kElements, tail = tail_of<T>(to - from, threadIdx.x);
+        MaxSum q = {-INFINITY, 0.0f};
+        if (tail >= 0) {
+            const float last = to_float(z[tail]);
+            q.m = last == last ? last : -INFINITY;
+            q.s = exp2_scaled(last, q.m == -INFINITY ? 0.0f : q.m, a.scale2);
+        }
+        for (int64_t v = threadIdx.x; v < vecs; v += kSliceThreads * kAhead) {
+            Words<T> x[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) x[u] = load_words<T>(z, v + u * kSliceThreads, vecs);
+            float m = q.m;
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+                for (int i = 0; i < kElements; ++i) m = fmaxf(m, element_of(x[u], i));
+            const float base = m == -INFINITY ? 0.0f : m;
+            float s = q.s * exp2_scaled(q.m, base, a.scale2);
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+                for (int i = 0; i < kElements; ++i) s += exp2_scaled(element_of(x[u], i), base, a.scale2);
+            q = {m, s};
+        }
+        const float m = max_of_group<kSliceThreads>(q.m, s_wave);
+        const float base = m == -INFINITY ? 0.0f : m;
+        const float s = sum_of_group<kSliceThreads>(q.s * exp2_scaled(q.m, base, a.scale2), s_wave);
+        if (threadIdx.x == 0) a.partial[b] = {m, s};
+    }
+}
+
+// and this one joins them (every workgroup of a row does), writes the loss (the first slice's) and the gradient.
+template <typename T>
+__global__ __launch_bounds__(kSliceThreads) void distill_finish_kernel(DistillArgs a, const T* __restrict__ logits,
+                                                                       T* __restrict__ grad, int64_t slices_run) {
+    extern __shared__ uint8_t s_distill[];
+    __shared__ float s_wave[kSliceThreads / 64];
+    constexpr int kElements = Words<T>::kElements, kAhead = 4;
+    Teacher r;
+    r.id = reinterpret_cast<int32_t*>(s_distill);
+    r.p = reinterpret_cast<float*>(r.id + a.top);
+    r.z = r.p + a.top;
+    const int64_t total = a.rows * slices_run;
+    for (int64_t b = blockIdx.x; b < total; b += gridDim.x) {
+        const int64_t local = b / slices_run, row = a.first_row + local, from = b % slices_run * a.slice;
+        const int64_t to = min(from + a.slice, a.vocab);
+        const T* const z = logits + row * a.logits_stride;
+        const float w = a.row_weight != nullptr ? a.row_weight[row] : 1.0f;
+        __syncthreads();  // the slice before has been patched
+        teacher_load<T, kSliceThreads>(a, z, row, threadIdx.x, r);
+        MaxSum q = {-INFINITY, 0.0f};
+        if (a.from_stats != 0) {
+            q.m = a.stats[2 * row];
+            q.s = a.stats[2 * row + 1];
+        } else {
+            for (int64_t i = threadIdx.x; i < a.slices; i += kSliceThreads) q = join(q, a.partial[local * a.slices + i], a.scale2);
+            const float m = max_of_group<kSliceThreads>(q.m, s_wave);
+            const float base = m == -INFINITY ? 0.0f : m;
+            q.s = sum_of_group<kSliceThreads>(q.s * exp2_scaled(q.m, base, a.scale2), s_wave);
+            q.m = m;
+        }
+        teacher_finish<kSliceThreads>(a, threadIdx.x, s_wave, r);
+        const bool live = r.any && w != 0.0f;
+        if (a.from_stats == 0 && from == 0) {
+            const float terms = cross_terms<kSliceThreads>(a, row, threadIdx.x, r, s_wave, q);
             if (threadIdx.x == 0) {
                 if (a.loss != nullptr) a.loss[row] = live ? w * a.temperature * a.temperature * terms : 0.0f;
                 if (a.stats != nullptr) {
@@ -199,11 +404,29 @@ __global__ __launch_bounds__(kDistillThreads) void distill_row_kernel(DistillArg
                 }
             }
         }
-        if (grad != nullptr) {
-            const float c = (a.row_grad != nullptr ? a.row_grad[row] : 1.0f) * a.grad_scale * w * a.temperature;
-            write_grad<T, kDistillThreads>(a, z, grad + row * a.grad_stride, s_id, s_p, q, live, c);
+        if (grad == nullptr) continue;
+        T* const g = grad + row * a.grad_stride;
+        const bool some = live && q.s != 0.0f;
+        const float c = (a.row_grad != nullptr ? a.row_grad[row] : 1.0f) * a.grad_scale * w * a.temperature;
+        const float cq = some ? c / q.s : 0.0f, base = q.m == -INFINITY ? 0.0f : q.m;
+        const int64_t vecs = (to - from) / kElements, tail = tail_of<T>(to - from, threadIdx.x);
+        for (int64_t v = threadIdx.x; v < vecs; v += kSliceThreads * kAhead) {
+            Words<T> x[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) x[u] = load_words<T>(z + from, v + u * kSliceThreads, vecs);
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                float y[kElements];
+#pragma unroll
+                for (int i = 0; i < kElements; ++i) y[i] = some ? q_term(element_of(x[u], i), base, cq, a.scale2) : 0.0f;
+                store_words<T>(g + from, v + u * kSliceThreads, vecs, y);
+            }
         }
-        __syncthreads();
+        if (tail >= 0) g[from + tail] = from_float<T>(some ? q_term(to_float(z[from + tail]), base, cq, a.scale2) : 0.0f);
+        if (some) {
+            __syncthreads();  // orders those stores before the entries'
+            patch_entries<T, kSliceThreads>(a, g, from, to, threadIdx.x, r, base, cq, c);
+        }
     }
 }
 
@@ -233,14 +456,86 @@ gsx_hip_status distill_check(const DistillArgs& a, const void* logits, int32_t t
     return GSX_HIP_SUCCESS;
 }
 
-gsx_hip_status distill_launch(const DistillArgs& a, const void* logits, int32_t type, void* grad, int from_stats,
+// A row is held by a wave (up to 4 KB), by 256 threads (32 KB) or by 1024 (256 KB), where there are rows enough for the GPU's 256
+// CUs; else, and beyond, it is cut into slices of 16 KB or more, so that some 1024 workgroups share the logits.
+struct DistillPlan {
+    int group, vecs;        // group = 0: slices
+    int64_t slice, slices;  // logits of a slice
+    int64_t batch;          // rows of a pair of launches: what they read twice stays in the 256 MB cache between
+};
+
+DistillPlan distill_plan(int64_t rows, int64_t vocab, int64_t bytes) {
+    DistillPlan p = {};
+    const int64_t vecs = vocab * bytes / 16;  // the few elements behind the last whole vector are held besides
+    if (vecs <= 64 * 4) p.group = 64;
+    else if (vecs <= 256 * 8) p.group = 256;
+    else if (vecs <= 1024 * 16 && rows >= 192) p.group = 1024;
+    if (p.group != 0) {
+        p.vecs = vecs > 0 ? (int)ceil_div(vecs, p.group) : 1;
+        p.batch = rows;
+        return p;
+    }
+    const int64_t least = 16384 / bytes;
+    int64_t slices = ceil_div(1024, rows);
+    if (slices > vocab / least) slices = vocab / least;
+    if (slices < 1) slices = 1;
+    p.slice = ceil_div(ceil_div(vocab, slices), 2048) * 2048;
+    p.slices = ceil_div(vocab, p.slice);
+    p.batch = rows;
+    if (p.batch > ceil_div((int64_t)128 << 20, vocab * bytes)) p.batch = ceil_div((int64_t)128 << 20, vocab * bytes);
+    return p;
+}
+
+template <typename T, int kGroup, int kVecs>
+gsx_hip_status launch_held(const DistillArgs& a, const T* logits, T* grad, hipStream_t stream) {
+    const int per = kGroup < 256 ? 256 / kGroup : 1;
+    const int64_t blocks = ceil_div(a.rows, per);
+    hipLaunchKernelGGL((distill_held_kernel<T, kGroup, kVecs>), dim3((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20)),
+                       dim3(kGroup < 256 ? 256 : kGroup), (unsigned)(per * 12 * a.top), stream, a, logits, grad);
+    return fields_launched("distill launch");
+}
+
+template <typename T>
+gsx_hip_status launch_distill(const DistillPlan& p, DistillArgs a, const T* logits, T* grad, void* temp,
                               hipStream_t stream) {
+    if (p.group == 64) {
+        if (p.vecs <= 1) return launch_held<T, 64, 1>(a, logits, grad, stream);
+        if (p.vecs <= 2) return launch_held<T, 64, 2>(a, logits, grad, stream);
+        return launch_held<T, 64, 4>(a, logits, grad, stream);
+    }
+    if (p.group == 256) {
+        if (p.vecs <= 2) return launch_held<T, 256, 2>(a, logits, grad, stream);
+        if (p.vecs <= 4) return launch_held<T, 256, 4>(a, logits, grad, stream);
+        return launch_held<T, 256, 8>(a, logits, grad, stream);
+    }
+    if (p.group == 1024) {
+        if (p.vecs <= 4) return launch_held<T, 1024, 4>(a, logits, grad, stream);
+        if (p.vecs <= 6) return launch_held<T, 1024, 6>(a, logits, grad, stream);
+        if (p.vecs <= 8) return launch_held<T, 1024, 8>(a, logits, grad, stream);
+        if (p.vecs <= 12) return launch_held<T, 1024, 12>(a, logits, grad, stream);
+        return launch_held<T, 1024, 16>(a, logits, grad, stream);
+    }
+    const int64_t rows = a.rows;
+    a.slice = p.slice;
+    a.slices = p.slices;
+    a.partial = static_cast<MaxSum*>(temp);
+    const int64_t run = grad != nullptr ? p.slices : 1;
+    const auto grid = [](int64_t blocks) { return dim3((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20)); };
+    for (a.first_row = 0; a.first_row < rows; a.first_row += p.batch) {
+        a.rows = rows - a.first_row < p.batch ? rows - a.first_row : p.batch;
+        if (a.from_stats == 0)
+            hipLaunchKernelGGL((distill_slices_kernel<T>), grid(a.rows * p.slices), dim3(kSliceThreads), 0, stream, a, logits);
+        hipLaunchKernelGGL((distill_finish_kernel<T>), grid(a.rows * run), dim3(kSliceThreads), (unsigned)(12 * a.top), stream,
+                           a, logits, grad, run);
+    }
+    return fields_launched("distill launch");
+}
+
+gsx_hip_status distill_launch(const DistillPlan& p, const DistillArgs& a, const void* logits, int32_t type, void* grad,
+                              void* temp, hipStream_t stream) {
     return with_type(type, [&](auto t) {
         using T = decltype(t);
-        hipLaunchKernelGGL((distill_row_kernel<T>), dim3((unsigned)(a.rows < (1 << 20) ? a.rows : (1 << 20))),
-                           dim3(kDistillThreads), 0, stream, a, static_cast<const T*>(logits), static_cast<T*>(grad),
-                           from_stats);
-        return fields_launched("distill launch");
+        return launch_distill<T>(p, a, static_cast<const T*>(logits), static_cast<T*>(grad), temp, stream);
     });
 }
 
@@ -265,9 +560,14 @@ DistillArgs distill_args(int64_t logits_stride, int64_t rows, int64_t vocab, con
 extern "C" {
 
 size_t gsx_hip_distill_temp_bytes(int64_t rows, int64_t vocab) {
-    (void)rows;
-    (void)vocab;
-    return 0;
+    if (rows <= 0 || vocab <= 0 || vocab > INT32_MAX) return 0;
+    int64_t most = 0;  // whatever the logits' type is
+    for (int64_t bytes = 2; bytes <= 4; bytes += 2) {
+        const DistillPlan p = distill_plan(rows, vocab, bytes);
+        const int64_t need = p.group != 0 ? 0 : p.batch * p.slices * (int64_t)sizeof(MaxSum);
+        if (need > most) most = need;
+    }
+    return (size_t)most;
 }
 
 gsx_hip_status gsx_hip_distill_forward(const void* logits, int32_t logits_type, int64_t logits_stride, int64_t rows,
@@ -283,8 +583,10 @@ gsx_hip_status gsx_hip_distill_forward(const void* logits, int32_t logits_type, 
     a.stats = row_stats;
     const gsx_hip_status st = distill_check(a, logits, logits_type, grad_logits);
     if (st != GSX_HIP_SUCCESS || rows == 0) return st;
-    (void)temp;
-    return distill_launch(a, logits, logits_type, grad_logits, 0, stream);
+    const DistillPlan p = distill_plan(rows, vocab, type_bytes(logits_type));
+    if (p.group == 0 && (temp == nullptr || !aligned_to(temp, 16)))
+        return fields_fail(GSX_HIP_ERROR_INVALID_ARGUMENT, "distill: the workspace must be non-null and 16-byte aligned");
+    return distill_launch(p, a, logits, logits_type, grad_logits, temp, stream);
 }
 
 gsx_hip_status gsx_hip_distill_backward(const void* logits, int32_t logits_type, int64_t logits_stride, int64_t rows,
@@ -302,7 +604,9 @@ gsx_hip_status gsx_hip_distill_backward(const void* logits, int32_t logits_type,
     if (st != GSX_HIP_SUCCESS || rows == 0) return st;
     if (row_stats == nullptr || grad_logits == nullptr)
         return fields_fail(GSX_HIP_ERROR_INVALID_ARGUMENT, "distill backward: null pointer");
-    return distill_launch(a, logits, logits_type, grad_logits, 1, stream);
+    a.from_stats = 1;
+    return distill_launch(distill_plan(rows, vocab, type_bytes(logits_type)), a, logits, logits_type, grad_logits, nullptr,
+                          stream);
 }
 
 }  // extern "C"
