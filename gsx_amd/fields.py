@@ -35,15 +35,17 @@ def _type(dtype) -> int:
 
 def _rows(t: torch.Tensor, what: str, dtype=None, shape=None):
     """(address, stride) of a matrix with contiguous rows."""
-    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+    if t.get_device() != _device():
         raise GsxHipError(f"{what} must live on the current HIP device")
     if dtype is not None and t.dtype != dtype:
         raise GsxHipError(f"{what} must be {dtype}, not {t.dtype}")
-    if t.dim() != 2 or (shape is not None and tuple(t.shape) != shape):
-        raise GsxHipError(f"{what} must be a matrix{'' if shape is None else f' of shape {shape}'}, not {tuple(t.shape)}")
-    rows, cols = t.shape
-    stride = t.stride(0) if rows > 1 and cols > 0 else cols
-    if (cols > 1 and t.stride(1) != 1) or stride < cols:
+    size = t.shape
+    if len(size) != 2 or (shape is not None and size != shape):
+        raise GsxHipError(f"{what} must be a matrix{'' if shape is None else f' of shape {shape}'}, not {tuple(size)}")
+    rows, cols = size
+    step, inner = t.stride()
+    stride = step if rows > 1 and cols > 0 else cols
+    if (cols > 1 and inner != 1) or stride < cols:
         raise GsxHipError(f"{what} must have contiguous rows that do not overlap")
     return t.data_ptr(), stride
 
@@ -51,17 +53,23 @@ def _rows(t: torch.Tensor, what: str, dtype=None, shape=None):
 def _vector(t: torch.Tensor | None, what: str, dtype, count: int):
     if t is None:
         return None
-    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+    if t.get_device() != _device():
         raise GsxHipError(f"{what} must live on the current HIP device")
-    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != count or not t.is_contiguous():
+    if t.dtype != dtype or t.shape != (count,) or not t.is_contiguous():
         raise GsxHipError(f"{what} must be {count} contiguous {dtype} values")
     return t.data_ptr()
+
+
+_device = torch.cuda.current_device
+# the current stream's handle without a Stream object around it: a quarter of a small call's time
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 def _run(stream, call):
     """call(stream handle) with what it allocates belonging to the stream that it runs on."""
     if stream is None:
-        return call(torch.cuda.current_stream().cuda_stream)
+        return call(_current_stream(_device()))
     with torch.cuda.stream(stream):
         return call(stream.cuda_stream)
 
