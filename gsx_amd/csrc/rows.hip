@@ -161,28 +161,47 @@ __device__ inline void sum_run(float (&sum)[V], const T* __restrict__ grad, int6
     for (; p < end; p += step) add_row<T, V>(sum, grad + (int64_t)order[p] * grad_stride + col);
 }
 
-// A group of `lanes` (a power of two, at most 64) lanes per table row, `tiles` times `lanes` vectors of it.
-template <typename T, int V>
+// A group of `lanes` (a power of two, at most 64) lanes per table row and kTiles times `lanes` vectors of it. The loads of kAhead
+// rows in all tiles are issued together; past the run's end the last row is loaded again and not added.
+template <typename T, int V, int kTiles>
 __global__ __launch_bounds__(kRowThreads) void lookup_runs_kernel(const T* __restrict__ grad, int64_t grad_stride,
                                                                   const uint32_t* __restrict__ order,
                                                                   const uint32_t* __restrict__ starts, float scale,
                                                                   float* __restrict__ out, int64_t table_rows,
-                                                                  int64_t out_stride, int64_t vecs, int lanes, int tiles,
+                                                                  int64_t out_stride, int64_t vecs, int lanes,
                                                                   int accumulate) {
+    constexpr int kAhead = 8 / kTiles;
     const int sub = threadIdx.x & (lanes - 1);
-    const int64_t parts = ceil_div(vecs, (int64_t)lanes * tiles);
+    const int64_t parts = ceil_div(vecs, (int64_t)lanes * kTiles);
     const int64_t groups = table_rows * parts, per_block = kRowThreads / lanes;
     for (int64_t g = (int64_t)blockIdx.x * per_block + threadIdx.x / lanes; g < groups; g += (int64_t)gridDim.x * per_block) {
         const int64_t v = g / parts;
         const uint32_t begin = starts[v], end = starts[v + 1];
         if (end - begin > (uint32_t)kRunPart || (accumulate != 0 && begin == end)) continue;
-        const int64_t first = g % parts * lanes * tiles + sub;
-        for (int t = 0; t < tiles; ++t) {
-            const int64_t vec = first + (int64_t)t * lanes;
-            if (vec >= vecs) break;
-            float sum[V] = {};
-            sum_run<T, V>(sum, grad, grad_stride, order, begin, end, 1, vec * V);
-            store_row<V>(out + v * out_stride + vec * V, sum, scale, accumulate != 0);
+        const int64_t first = g % parts * lanes * kTiles + sub;
+        float sum[kTiles][V] = {};
+        for (int64_t p = begin; p < end; p += kAhead) {
+            Vec<T, V> x[kAhead][kTiles];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const T* const row = grad + (int64_t)order[min(p + u, (int64_t)end - 1)] * grad_stride;
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t)
+                    x[u][t] = *reinterpret_cast<const Vec<T, V>*>(row + min(first + t * lanes, vecs - 1) * V);
+            }
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                if (p + u >= end) continue;
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                    for (int k = 0; k < V; ++k) sum[t][k] += to_float(x[u][t].v[k]);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+            const int64_t vec = first + t * lanes;
+            if (vec < vecs) store_row<V>(out + v * out_stride + vec * V, sum[t], scale, accumulate != 0);
         }
     }
 }
@@ -368,13 +387,11 @@ gsx_hip_status sorted_backward(const T* grad, int64_t grad_stride, const int32_t
     const int64_t vecs = width / V;
     int lanes = 1;
     while (lanes < vecs && lanes < 64) lanes *= 2;
-    // a group takes up to eight times its lanes of a row where there are rows enough to fill the GPU
-    int tiles = 1;
-    while (tiles < 8 && tiles * lanes < vecs && table_rows * ceil_div(vecs, 2 * tiles * lanes) >= 16384) tiles *= 2;
-    const int64_t groups = table_rows * ceil_div(vecs, (int64_t)lanes * tiles);
-    hipLaunchKernelGGL((lookup_runs_kernel<T, V>), dim3(rows_grid(ceil_div(groups, kRowThreads / lanes))),
-                       dim3(kRowThreads), 0, stream, grad, grad_stride, order, starts, scale, out, table_rows, out_stride,
-                       vecs, lanes, tiles, accumulate);
+    // a wave takes 256 vectors of a row where the rows are that long, else its lanes share rows
+    const int64_t groups = table_rows * ceil_div(vecs, vecs > 64 ? 256 : lanes);
+    hipLaunchKernelGGL((vecs > 64 ? lookup_runs_kernel<T, V, 4> : lookup_runs_kernel<T, V, 1>),
+                       dim3(rows_grid(ceil_div(groups, kRowThreads / lanes))), dim3(kRowThreads), 0, stream, grad,
+                       grad_stride, order, starts, scale, out, table_rows, out_stride, vecs, lanes, accumulate);
     const int64_t parts = ceil_div(count, kRunPart) * ceil_div(vecs, lanes);
     hipLaunchKernelGGL((lookup_parts_kernel<T, V, KeyT>), dim3(rows_grid(ceil_div(parts, kRowThreads / 64))),
                        dim3(kRowThreads), 0, stream, grad, grad_stride, order, sorted, starts, count, table_rows, vecs,
