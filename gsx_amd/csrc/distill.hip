@@ -58,9 +58,19 @@ __device__ inline void group_sync() {
 }
 
 // Sum and maximum over a group; s_wave holds a float for each of the group's waves. NaN does not pass max_of_group (fmaxf).
+__device__ inline float wave_reduce_max(float v) {  // lane moves as in wave_reduce_sum; NaN is passed over
+    v = fmaxf(v, dpp_move<0xb1, 0xf>(v));
+    v = fmaxf(v, dpp_move<0x4e, 0xf>(v));
+    v = fmaxf(v, dpp_move<0x141, 0xf>(v));
+    v = fmaxf(v, dpp_move<0x140, 0xf>(v));
+    v = fmaxf(v, dpp_move<0x142, 0xa>(v));  // lanes that get nothing here do not reach lane 63
+    v = fmaxf(v, dpp_move<0x143, 0xc>(v));
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
+
 template <int kGroup>
 __device__ inline float sum_of_group(float v, float* s_wave) {
-    v = wave_sum(v);
+    v = wave_reduce_sum(v);
     if constexpr (kGroup == 64) return v;
     const int wave = threadIdx.x / 64;
     __syncthreads();
@@ -74,8 +84,7 @@ __device__ inline float sum_of_group(float v, float* s_wave) {
 
 template <int kGroup>
 __device__ inline float max_of_group(float v, float* s_wave) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
+    v = wave_reduce_max(v);
     if constexpr (kGroup == 64) return v;
     const int wave = threadIdx.x / 64;
     __syncthreads();
@@ -87,11 +96,15 @@ __device__ inline float max_of_group(float v, float* s_wave) {
     return v;
 }
 
-// The teacher's side of one row: in LDS for each entry its id (-1: does not count), its p and the student's logit there.
+// The teacher's side of one row: in LDS for each entry its id (-1: does not count), its logit, its p and the student's logit
+// there.
 struct Teacher {
     int32_t* id;
+    float* t;
     float* p;
     float* z;
+    uint16_t* slot;      // of a wave's row: an entry that names each logit
+    bool unique;         // no id is known to be named twice
     float max, log_sum;  // log p_k = (t_k - max) / T - log_sum
     bool any;            // an entry counts
 };
@@ -106,24 +119,24 @@ __device__ inline void teacher_load(const DistillArgs& a, const T* __restrict__ 
         const float x = t[k];
         const bool counts = id >= 0 && id < a.vocab && !(x == -INFINITY);
         r.id[k] = counts ? id : -1;
-        r.p[k] = x;
+        r.t[k] = x;
         r.z[k] = counts ? to_float(z[id]) : 0.0f;
     }
 }
 
 template <int kGroup>
-__device__ inline void teacher_finish(const DistillArgs& a, int tid, float* s_wave, Teacher& r) {
+__device__ inline void teacher_finish(const DistillArgs& a, int tid, float* s_wave, Teacher& r, bool want_unique) {
     float m = -INFINITY, any = 0.0f;
     for (int k = tid; k < a.top; k += kGroup) {
         if (r.id[k] < 0) continue;
-        m = fmaxf(m, r.p[k]);
+        m = fmaxf(m, r.t[k]);
         any = 1.0f;
     }
     m = max_of_group<kGroup>(m, s_wave);
     const float inv_t = 1.0f / a.temperature;
     float sum = 0.0f;
     for (int k = tid; k < a.top; k += kGroup) {
-        const float e = r.id[k] >= 0 ? expf((r.p[k] - m) * inv_t) : 0.0f;  // NaN stays NaN, in the sum too
+        const float e = r.id[k] >= 0 ? expf((r.t[k] - m) * inv_t) : 0.0f;  // NaN stays NaN, in the sum too
         r.p[k] = e;
         sum += e;
     }
@@ -132,19 +145,29 @@ __device__ inline void teacher_finish(const DistillArgs& a, int tid, float* s_wa
     r.max = m;
     r.log_sum = logf(sum);
     for (int k = tid; k < a.top; k += kGroup) r.p[k] = r.any ? r.p[k] / sum : 0.0f;
+    r.unique = false;
+    if constexpr (kGroup == 64) {  // whoever wrote a slot last finds itself there; an id named twice leaves somebody else
+        if (want_unique) {
+            for (int k = tid; k < a.top; k += kGroup)
+                if (r.id[k] >= 0) r.slot[r.id[k]] = (uint16_t)k;
+            group_sync<kGroup>();
+            bool twice = false;
+            for (int k = tid; k < a.top; k += kGroup) twice |= r.id[k] >= 0 && r.slot[r.id[k]] != (uint16_t)k;
+            r.unique = wave_none(twice);
+        }
+    }
     group_sync<kGroup>();
 }
 
 // sum_k p_k (log p_k - log q_{id_k}) by the group (every thread returns it).
 template <int kGroup>
-__device__ inline float cross_terms(const DistillArgs& a, int64_t row, int tid, const Teacher& r, float* s_wave, MaxSum q) {
-    const float* t = a.teacher + row * a.teacher_stride;
+__device__ inline float cross_terms(const DistillArgs& a, int tid, const Teacher& r, float* s_wave, MaxSum q) {
     const float inv_t = 1.0f / a.temperature;
     const float log_s = logf(q.s);
     float sum = 0.0f;
     for (int k = tid; k < a.top; k += kGroup) {
         if (r.id[k] < 0 || r.p[k] == 0.0f) continue;
-        const float log_p = (t[k] - r.max) * inv_t - r.log_sum;
+        const float log_p = (r.t[k] - r.max) * inv_t - r.log_sum;
         const float x = r.z[k];
         const float log_q = x == -INFINITY && !(q.s != q.s) ? -INFINITY : (x - q.m) * inv_t - log_s;
         sum += r.p[k] * (log_p - log_q);
@@ -163,8 +186,11 @@ __device__ inline void patch_entries(const DistillArgs& a, T* __restrict__ g, in
     for (int k = tid; k < a.top; k += kGroup) {
         const int32_t id = r.id[k];
         if (id < from || id >= to || id < 0) continue;
-        float p = 0.0f;  // an id that is named twice has both
-        for (int o = 0; o < a.top; ++o) p += r.id[o] == id ? r.p[o] : 0.0f;
+        float p = r.p[k];
+        if (!r.unique) {  // an id that is named twice has both
+            p = 0.0f;
+            for (int o = 0; o < a.top; ++o) p += r.id[o] == id ? r.p[o] : 0.0f;
+        }
         g[id] = from_float<T>(q_term(r.z[k], base, cq, a.scale2) - c * p);
     }
 }
@@ -205,14 +231,13 @@ __device__ inline uint32_t element_bits(float x) {
     else return __builtin_bit_cast(uint16_t, from_float<T>(x));
 }
 
-// Vector v of a row, -inf in all its elements where there is none (v >= vecs). The elements behind a row's last whole vector
-// (fewer than a vector) are taken one a thread, see tail_of.
+// Vector v of a row, -inf in all its elements where there is none (v >= vecs).
 template <typename T>
-__device__ inline Words<T> load_words(const T* __restrict__ z, int64_t v, int64_t vecs) {
+__device__ inline Words<T> load_words(const T* __restrict__ z, int v, int vecs) {
     constexpr uint32_t kNone = sizeof(T) == 4 ? 0xff800000u : __is_same(T, __bf16) ? 0xff80ff80u : 0xfc00fc00u;
     Words<T> x = {{kNone, kNone, kNone, kNone}};
     if (v < vecs) {
-        const LooseWords<T> y = *reinterpret_cast<const LooseWords<T>*>(z + v * Words<T>::kElements);
+        const LooseWords<T> y = *reinterpret_cast<const LooseWords<T>*>(z + (uint32_t)v * Words<T>::kElements);
 #pragma unroll
         for (int i = 0; i < 4; ++i) x.w[i] = y.w[i];
     }
@@ -220,7 +245,7 @@ __device__ inline Words<T> load_words(const T* __restrict__ z, int64_t v, int64_
 }
 
 template <typename T>
-__device__ inline void store_words(T* __restrict__ g, int64_t v, int64_t vecs, const float (&y)[Words<T>::kElements]) {
+__device__ inline void store_words(T* __restrict__ g, int v, int vecs, const float (&y)[Words<T>::kElements]) {
     if (v >= vecs) return;
     LooseWords<T> x;
     if constexpr (sizeof(T) == 4) {
@@ -230,14 +255,30 @@ __device__ inline void store_words(T* __restrict__ g, int64_t v, int64_t vecs, c
 #pragma unroll
         for (int i = 0; i < 4; ++i) x.w[i] = element_bits<T>(y[2 * i]) | element_bits<T>(y[2 * i + 1]) << 16;
     }
-    *reinterpret_cast<LooseWords<T>*>(g + v * Words<T>::kElements) = x;
+    typedef uint32_t Loose2 __attribute__((ext_vector_type(4), aligned(2)));
+    typedef uint32_t Loose4 __attribute__((ext_vector_type(4), aligned(4)));
+    const Loose4 y4 = {x.w[0], x.w[1], x.w[2], x.w[3]};
+    if constexpr (sizeof(T) == 4) __builtin_nontemporal_store(y4, reinterpret_cast<Loose4*>(g + (uint32_t)v * Words<T>::kElements));
+    else __builtin_nontemporal_store(y4, reinterpret_cast<Loose2*>(g + (uint32_t)v * Words<T>::kElements));
 }
 
-// Place of a thread's element behind the last whole vector of a row of `length`; -1: it has none.
+// A stretch of `length` logits at z: `lead` elements up to the first address that is a multiple of 16, then `vecs` vectors, then
+// fewer than a vector. What is before and behind the vectors is taken one a thread (fewer than 16 threads): `loose` is a
+// thread's element or -1. Vectors that are not aligned cost a fifth (rows of 65537 bf16: 271 against 237 us).
+struct Stretch {
+    int lead, vecs;
+    int64_t loose;
+};
+
 template <typename T>
-__device__ inline int64_t tail_of(int64_t length, int tid) {
-    const int64_t at = length / Words<T>::kElements * Words<T>::kElements + tid;
-    return at < length ? at : -1;
+__device__ inline Stretch stretch_of(const T* z, int64_t length, int tid) {
+    constexpr int kElements = Words<T>::kElements;
+    Stretch s;
+    s.lead = (int)min((int64_t)((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15) / (int64_t)sizeof(T), length);
+    s.vecs = (int)((length - s.lead) / kElements);
+    const int64_t behind = s.lead + (int64_t)s.vecs * kElements + (tid - s.lead);
+    s.loose = tid < s.lead ? tid : behind < length ? behind : -1;
+    return s;
 }
 
 // Rows that fit the registers of a group: kGroup threads hold kVecs times 16 bytes each. The logits are read once; maximum, sum
@@ -251,18 +292,20 @@ __global__ __launch_bounds__(kGroup < 256 ? 256 : kGroup) void distill_held_kern
     __shared__ float s_wave[16];
     const int group = kGroups == 1 ? 0 : threadIdx.x / kGroup, tid = kGroups == 1 ? threadIdx.x : threadIdx.x % kGroup;
     Teacher r;
-    r.id = reinterpret_cast<int32_t*>(s_distill) + group * 3 * a.top;
-    r.p = reinterpret_cast<float*>(r.id + a.top);
+    r.id = reinterpret_cast<int32_t*>(s_distill) + group * 4 * a.top;
+    r.t = reinterpret_cast<float*>(r.id + a.top);
+    r.p = r.t + a.top;
     r.z = r.p + a.top;
-    const int64_t vecs = a.vocab / kElements, tail = tail_of<T>(a.vocab, tid);
+    r.slot = reinterpret_cast<uint16_t*>(s_distill + kGroups * 16 * a.top) + group * a.vocab;  // a wave's row only
     for (int64_t row = (int64_t)blockIdx.x * kGroups + group; row < a.rows; row += (int64_t)gridDim.x * kGroups) {
         const T* const z = logits + row * a.logits_stride;
         const float w = a.row_weight != nullptr ? a.row_weight[row] : 1.0f;
+        const Stretch st = stretch_of<T>(z, a.vocab, tid);
         Words<T> x[kVecs];
         group_sync<kGroup>();  // the row before has been patched
 #pragma unroll
-        for (int u = 0; u < kVecs; ++u) x[u] = load_words<T>(z, (int64_t)u * kGroup + tid, vecs);
-        const float last = tail >= 0 ? to_float(z[tail]) : -INFINITY;
+        for (int u = 0; u < kVecs; ++u) x[u] = load_words<T>(z + st.lead + u * kGroup * kElements, tid, st.vecs - u * kGroup);
+        const float last = st.loose >= 0 ? to_float(z[st.loose]) : -INFINITY;
         teacher_load<T, kGroup>(a, z, row, tid, r);
         MaxSum q;
         if (a.from_stats != 0) {
@@ -285,10 +328,10 @@ __global__ __launch_bounds__(kGroup < 256 ? 256 : kGroup) void distill_held_kern
             }
             q.s = sum_of_group<kGroup>(s, s_wave);
         }
-        teacher_finish<kGroup>(a, tid, s_wave, r);
+        teacher_finish<kGroup>(a, tid, s_wave, r, grad != nullptr);
         const bool live = r.any && w != 0.0f;
         if (a.from_stats == 0) {
-            const float terms = cross_terms<kGroup>(a, row, tid, r, s_wave, q);
+            const float terms = cross_terms<kGroup>(a, tid, r, s_wave, q);
             if (tid == 0) {
                 if (a.loss != nullptr) a.loss[row] = live ? w * a.temperature * a.temperature * terms : 0.0f;
                 if (a.stats != nullptr) {
@@ -309,9 +352,9 @@ __global__ __launch_bounds__(kGroup < 256 ? 256 : kGroup) void distill_held_kern
 #pragma unroll
             for (int i = 0; i < kElements; ++i)
                 y[i] = some ? q_term(element_of(x[u], i), base, cq, a.scale2) : 0.0f;
-            store_words<T>(g, (int64_t)u * kGroup + tid, vecs, y);
+            store_words<T>(g + st.lead + u * kGroup * kElements, tid, st.vecs - u * kGroup, y);
         }
-        if (tail >= 0) g[tail] = from_float<T>(some ? q_term(last, base, cq, a.scale2) : 0.0f);
+        if (st.loose >= 0) g[st.loose] = from_float<T>(some ? q_term(last, base, cq, a.scale2) : 0.0f);
         if (some) {
             group_sync<kGroup>();  // orders those stores before the entries'
             patch_entries<T, kGroup>(a, g, 0, a.vocab, tid, r, base, cq, c);
@@ -331,17 +374,17 @@ __global__ __launch_bounds__(kSliceThreads) void distill_slices_kernel(DistillAr
         const int64_t row = a.first_row + b / a.slices, from = b % a.slices * a.slice;
         const int64_t to = min(from + a.slice, a.vocab);
         const T* const z = logits + row * a.logits_stride + from;
-        const int64_t vecs = (to - from) / kElements, tail = tail_of<T>(to - from, threadIdx.x);
+        const Stretch st = stretch_of<T>(z, to - from, threadIdx.x);
         MaxSum q = {-INFINITY, 0.0f};
-        if (tail >= 0) {
-            const float last = to_float(z[tail]);
+        if (st.loose >= 0) {
+            const float last = to_float(z[st.loose]);
             q.m = last == last ? last : -INFINITY;
             q.s = exp2_scaled(last, q.m == -INFINITY ? 0.0f : q.m, a.scale2);
         }
-        for (int64_t v = threadIdx.x; v < vecs; v += kSliceThreads * kAhead) {
+        for (int v = threadIdx.x; v < st.vecs; v += kSliceThreads * kAhead) {
             Words<T> x[kAhead];
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u) x[u] = load_words<T>(z, v + u * kSliceThreads, vecs);
+            for (int u = 0; u < kAhead; ++u) x[u] = load_words<T>(z + st.lead, v + u * kSliceThreads, st.vecs);
             float m = q.m;
 #pragma unroll
             for (int u = 0; u < kAhead; ++u)
@@ -371,8 +414,10 @@ __global__ __launch_bounds__(kSliceThreads) void distill_finish_kernel(DistillAr
     constexpr int kElements = Words<T>::kElements, kAhead = 4;
     Teacher r;
     r.id = reinterpret_cast<int32_t*>(s_distill);
-    r.p = reinterpret_cast<float*>(r.id + a.top);
+    r.t = reinterpret_cast<float*>(r.id + a.top);
+    r.p = r.t + a.top;
     r.z = r.p + a.top;
+    r.slot = nullptr;
     const int64_t total = a.rows * slices_run;
     for (int64_t b = blockIdx.x; b < total; b += gridDim.x) {
         const int64_t local = b / slices_run, row = a.first_row + local, from = b % slices_run * a.slice;
@@ -381,6 +426,16 @@ __global__ __launch_bounds__(kSliceThreads) void distill_finish_kernel(DistillAr
         const float w = a.row_weight != nullptr ? a.row_weight[row] : 1.0f;
         __syncthreads();  // the slice before has been patched
         teacher_load<T, kSliceThreads>(a, z, row, threadIdx.x, r);
+        // the slice's first vectors are on their way while the sums are joined
+        const Stretch st = stretch_of<T>(z + from, to - from, threadIdx.x);
+        Words<T> x[kAhead];
+        float last = -INFINITY;
+        if (grad != nullptr) {
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u)
+                x[u] = load_words<T>(z + from + st.lead, threadIdx.x + u * kSliceThreads, st.vecs);
+            if (st.loose >= 0) last = to_float(z[from + st.loose]);
+        }
         MaxSum q = {-INFINITY, 0.0f};
         if (a.from_stats != 0) {
             q.m = a.stats[2 * row];
@@ -392,10 +447,10 @@ __global__ __launch_bounds__(kSliceThreads) void distill_finish_kernel(DistillAr
             q.s = sum_of_group<kSliceThreads>(q.s * exp2_scaled(q.m, base, a.scale2), s_wave);
             q.m = m;
         }
-        teacher_finish<kSliceThreads>(a, threadIdx.x, s_wave, r);
+        teacher_finish<kSliceThreads>(a, threadIdx.x, s_wave, r, false);
         const bool live = r.any && w != 0.0f;
         if (a.from_stats == 0 && from == 0) {
-            const float terms = cross_terms<kSliceThreads>(a, row, threadIdx.x, r, s_wave, q);
+            const float terms = cross_terms<kSliceThreads>(a, threadIdx.x, r, s_wave, q);
             if (threadIdx.x == 0) {
                 if (a.loss != nullptr) a.loss[row] = live ? w * a.temperature * a.temperature * terms : 0.0f;
                 if (a.stats != nullptr) {
@@ -409,20 +464,20 @@ __global__ __launch_bounds__(kSliceThreads) void distill_finish_kernel(DistillAr
         const bool some = live && q.s != 0.0f;
         const float c = (a.row_grad != nullptr ? a.row_grad[row] : 1.0f) * a.grad_scale * w * a.temperature;
         const float cq = some ? c / q.s : 0.0f, base = q.m == -INFINITY ? 0.0f : q.m;
-        const int64_t vecs = (to - from) / kElements, tail = tail_of<T>(to - from, threadIdx.x);
-        for (int64_t v = threadIdx.x; v < vecs; v += kSliceThreads * kAhead) {
-            Words<T> x[kAhead];
+        for (int v = threadIdx.x; v < st.vecs; v += kSliceThreads * kAhead) {
+            if (v != (int)threadIdx.x) {
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u) x[u] = load_words<T>(z + from, v + u * kSliceThreads, vecs);
+                for (int u = 0; u < kAhead; ++u) x[u] = load_words<T>(z + from + st.lead, v + u * kSliceThreads, st.vecs);
+            }
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
                 float y[kElements];
 #pragma unroll
                 for (int i = 0; i < kElements; ++i) y[i] = some ? q_term(element_of(x[u], i), base, cq, a.scale2) : 0.0f;
-                store_words<T>(g + from, v + u * kSliceThreads, vecs, y);
+                store_words<T>(g + from + st.lead, v + u * kSliceThreads, st.vecs, y);
             }
         }
-        if (tail >= 0) g[from + tail] = from_float<T>(some ? q_term(to_float(z[from + tail]), base, cq, a.scale2) : 0.0f);
+        if (st.loose >= 0) g[from + st.loose] = from_float<T>(some ? q_term(last, base, cq, a.scale2) : 0.0f);
         if (some) {
             __syncthreads();  // orders those stores before the entries'
             patch_entries<T, kSliceThreads>(a, g, from, to, threadIdx.x, r, base, cq, c);
@@ -456,8 +511,10 @@ gsx_hip_status distill_check(const DistillArgs& a, const void* logits, int32_t t
     return GSX_HIP_SUCCESS;
 }
 
-// A row is held by a wave (up to 4 KB), by 256 threads (32 KB) or by 1024 (256 KB), where there are rows enough for the GPU's 256
-// CUs; else, and beyond, it is cut into slices of 16 KB or more, so that some 1024 workgroups share the logits.
+// A row is held by a wave (up to 4 KB), by 256 threads (64 KB), 512 (128 KB) or 1024 (256 KB): the smallest group that holds it in
+// 16 vectors a thread, so that two or more rows share a CU and one loads while another is computed (65536 logits of bf16: 512
+// threads take 227 us for 4096 rows, 1024 with half the vectors each 289). Above 32 KB only where there are rows enough for the GPU's 256 CUs; else, and beyond, a row is cut
+// into slices of 16 KB or more, so that some 2048 workgroups share the logits.
 struct DistillPlan {
     int group, vecs;        // group = 0: slices
     int64_t slice, slices;  // logits of a slice
@@ -468,7 +525,8 @@ DistillPlan distill_plan(int64_t rows, int64_t vocab, int64_t bytes) {
     DistillPlan p = {};
     const int64_t vecs = vocab * bytes / 16;  // the few elements behind the last whole vector are held besides
     if (vecs <= 64 * 4) p.group = 64;
-    else if (vecs <= 256 * 8) p.group = 256;
+    else if (vecs <= 256 * 8 || (vecs <= 256 * 16 && rows >= 192)) p.group = 256;
+    else if (vecs <= 512 * 16 && rows >= 192) p.group = 512;
     else if (vecs <= 1024 * 16 && rows >= 192) p.group = 1024;
     if (p.group != 0) {
         p.vecs = vecs > 0 ? (int)ceil_div(vecs, p.group) : 1;
@@ -476,13 +534,13 @@ DistillPlan distill_plan(int64_t rows, int64_t vocab, int64_t bytes) {
         return p;
     }
     const int64_t least = 16384 / bytes;
-    int64_t slices = ceil_div(1024, rows);
+    p.batch = ceil_div((int64_t)128 << 20, vocab * bytes);
+    if (p.batch > rows) p.batch = rows;
+    int64_t slices = ceil_div(2048, p.batch);
     if (slices > vocab / least) slices = vocab / least;
     if (slices < 1) slices = 1;
     p.slice = ceil_div(ceil_div(vocab, slices), 2048) * 2048;
     p.slices = ceil_div(vocab, p.slice);
-    p.batch = rows;
-    if (p.batch > ceil_div((int64_t)128 << 20, vocab * bytes)) p.batch = ceil_div((int64_t)128 << 20, vocab * bytes);
     return p;
 }
 
@@ -491,7 +549,7 @@ gsx_hip_status launch_held(const DistillArgs& a, const T* logits, T* grad, hipSt
     const int per = kGroup < 256 ? 256 / kGroup : 1;
     const int64_t blocks = ceil_div(a.rows, per);
     hipLaunchKernelGGL((distill_held_kernel<T, kGroup, kVecs>), dim3((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20)),
-                       dim3(kGroup < 256 ? 256 : kGroup), (unsigned)(per * 12 * a.top), stream, a, logits, grad);
+                       dim3(kGroup < 256 ? 256 : kGroup), (unsigned)(per * 16 * a.top + (kGroup == 64 ? per * 2 * a.vocab : 0)), stream, a, logits, grad);
     return fields_launched("distill launch");
 }
 
@@ -506,12 +564,15 @@ gsx_hip_status launch_distill(const DistillPlan& p, DistillArgs a, const T* logi
     if (p.group == 256) {
         if (p.vecs <= 2) return launch_held<T, 256, 2>(a, logits, grad, stream);
         if (p.vecs <= 4) return launch_held<T, 256, 4>(a, logits, grad, stream);
-        return launch_held<T, 256, 8>(a, logits, grad, stream);
+        if (p.vecs <= 8) return launch_held<T, 256, 8>(a, logits, grad, stream);
+        if (p.vecs <= 12) return launch_held<T, 256, 12>(a, logits, grad, stream);
+        return launch_held<T, 256, 16>(a, logits, grad, stream);
+    }
+    if (p.group == 512) {
+        if (p.vecs <= 12) return launch_held<T, 512, 12>(a, logits, grad, stream);
+        return launch_held<T, 512, 16>(a, logits, grad, stream);
     }
     if (p.group == 1024) {
-        if (p.vecs <= 4) return launch_held<T, 1024, 4>(a, logits, grad, stream);
-        if (p.vecs <= 6) return launch_held<T, 1024, 6>(a, logits, grad, stream);
-        if (p.vecs <= 8) return launch_held<T, 1024, 8>(a, logits, grad, stream);
         if (p.vecs <= 12) return launch_held<T, 1024, 12>(a, logits, grad, stream);
         return launch_held<T, 1024, 16>(a, logits, grad, stream);
     }
@@ -525,7 +586,7 @@ gsx_hip_status launch_distill(const DistillPlan& p, DistillArgs a, const T* logi
         a.rows = rows - a.first_row < p.batch ? rows - a.first_row : p.batch;
         if (a.from_stats == 0)
             hipLaunchKernelGGL((distill_slices_kernel<T>), grid(a.rows * p.slices), dim3(kSliceThreads), 0, stream, a, logits);
-        hipLaunchKernelGGL((distill_finish_kernel<T>), grid(a.rows * run), dim3(kSliceThreads), (unsigned)(12 * a.top), stream,
+        hipLaunchKernelGGL((distill_finish_kernel<T>), grid(a.rows * run), dim3(kSliceThreads), (unsigned)(16 * a.top), stream,
                            a, logits, grad, run);
     }
     return fields_launched("distill launch");

@@ -51,7 +51,10 @@ __global__ __launch_bounds__(kRowThreads) void lookup_kernel(const T* __restrict
             Vec<O, V> y;
 #pragma unroll
             for (int k = 0; k < V; ++k) y.v[k] = from_float<O>(fits ? to_float(x[u].v[k]) * scale : 0.0f);
-            *reinterpret_cast<Vec<O, V>*>(out + row[u] * out_stride + col[u]) = y;
+            if constexpr (V * sizeof(O) == 16) {
+                typedef float v4 __attribute__((ext_vector_type(4)));
+                __builtin_nontemporal_store(__builtin_bit_cast(v4, y), reinterpret_cast<v4*>(out + row[u] * out_stride + col[u]));
+            } else *reinterpret_cast<Vec<O, V>*>(out + row[u] * out_stride + col[u]) = y;
         }
     }
 }
@@ -84,7 +87,10 @@ __device__ inline void store_row(float* p, const float (&sum)[V], float scale, b
 #pragma unroll
         for (int k = 0; k < V; ++k) y.v[k] += old.v[k];
     }
-    *reinterpret_cast<Vec<float, V>*>(p) = y;
+    if constexpr (V == 4) {
+        typedef float v4 __attribute__((ext_vector_type(4)));
+        __builtin_nontemporal_store(v4{y.v[0], y.v[1], y.v[2], y.v[3]}, reinterpret_cast<v4*>(p));
+    } else *reinterpret_cast<Vec<float, V>*>(p) = y;
 }
 
 template <typename T, int V>
