@@ -138,8 +138,8 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_columns_kernel(const T
 //
 // A workgroup of WM x WN waves forms a tile of c: BM rows (of a) by BN columns (rows of b), a wave TM x TN times 16 x 16 of it.
 // Blocks of 128 k of both operands' tiles lie in LDS, two at a time: while one is multiplied the next is on its way there,
-// straight from memory. A row is eight chunks of 16 bytes; chunk c lies at place c ^ swizzle(row), so that the lanes of one
-// read, which hold different rows' same chunk, meet different banks.
+// straight from memory. A row is eight chunks of 16 bytes; chunk c lies at place c ^ swizzle(row), and a lane of group g = lane /
+// 16 reads chunks g and g + 4: no two lanes of a read meet in a bank (with chunks 2 g and 2 g + 1 each read takes twice as long).
 //
 // The matrix instructions take b as their first operand: a lane then holds four consecutive columns of one row of c. Which
 // row of b a lane brings for instruction j is chosen so that its 4 TN columns are consecutive too, and leave in wide stores.
@@ -195,8 +195,8 @@ __device__ __forceinline__ void product_step(const uint8_t* __restrict__ now, co
         for (int j = 0; j < TN; ++j) {
             const int row = wn * 16 * TN + column_of<TN>(j, lane & 15);
             scale_b[j] = (int)(exponents[BM + row] >> shift);
-            const v4i lo = *reinterpret_cast<const v4i*>(s_b + row * kBlock + ((2 * (lane / 16)) ^ swizzle_b<TN>(row)) * 16);
-            const v4i hi = *reinterpret_cast<const v4i*>(s_b + row * kBlock + ((2 * (lane / 16) + 1) ^ swizzle_b<TN>(row)) * 16);
+            const v4i lo = *reinterpret_cast<const v4i*>(s_b + row * kBlock + ((lane / 16) ^ swizzle_b<TN>(row)) * 16);
+            const v4i hi = *reinterpret_cast<const v4i*>(s_b + row * kBlock + ((lane / 16 + 4) ^ swizzle_b<TN>(row)) * 16);
             vb[j] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
         }
 #pragma unroll
@@ -204,8 +204,8 @@ __device__ __forceinline__ void product_step(const uint8_t* __restrict__ now, co
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
             const int row = wm * 16 * TM + i * 16 + (lane & 15);
-            const v4i lo = *reinterpret_cast<const v4i*>(s_a + row * kBlock + ((2 * (lane / 16)) ^ swizzle_a(row)) * 16);
-            const v4i hi = *reinterpret_cast<const v4i*>(s_a + row * kBlock + ((2 * (lane / 16) + 1) ^ swizzle_a(row)) * 16);
+            const v4i lo = *reinterpret_cast<const v4i*>(s_a + row * kBlock + ((lane / 16) ^ swizzle_a(row)) * 16);
+            const v4i hi = *reinterpret_cast<const v4i*>(s_a + row * kBlock + ((lane / 16 + 4) ^ swizzle_a(row)) * 16);
             const v8i va = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
             for (int j = 0; j < TN; ++j)
@@ -222,7 +222,7 @@ __device__ __forceinline__ void product_step(const uint8_t* __restrict__ now, co
     for (int i = 0; i < TM; ++i) scale_a[i] = block_scale((exponents[wm * 16 * TM + i * 16 + (lane & 15)] >> shift) & 255u);
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-        const int c = 2 * (lane / 16) + half;
+        const int c = lane / 16 + 4 * half;
         v8bf vb[TN][2];
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
