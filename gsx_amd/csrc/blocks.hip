@@ -388,11 +388,17 @@ gsx_hip_status block_matrix_check(const void* values, const void* exponents, int
 }
 
 // 256 rows of a product's operand lie within 2^36 bytes (the kernel's offsets): value strides below 2^28.
-static constexpr int64_t kMostSummands = (int64_t)1 << 27;
 static constexpr int64_t kMostStride = (int64_t)1 << 28;
 
 bool product_sizes(int64_t m, int64_t n, int64_t k) {
     return m >= 0 && n >= 0 && k >= 0 && m <= INT32_MAX && n <= INT32_MAX && k <= kMostSummands;
+}
+
+gsx_hip_status join_products(const float* partial, int64_t m, int64_t n, int64_t splits, float* out, int64_t out_stride,
+                             hipStream_t stream) {
+    hipLaunchKernelGGL((product_join_kernel<float>), dim3(blocks_grid(ceil_div(ceil_div(m * n, 4), 16))), dim3(256), 0, stream,
+                       partial, m, n, splits, out, out_stride);
+    return fields_launched("product join launch");
 }
 
 }  // namespace gsx_amd

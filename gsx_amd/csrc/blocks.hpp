@@ -134,7 +134,11 @@ __device__ inline int swizzle_b(int row) {
     return (row & 3) | ((row / (4 * TN)) & 1) << 2;
 }
 
+constexpr int64_t kMostSummands = (int64_t)1 << 27;
 bool product_sizes(int64_t m, int64_t n, int64_t k);
+// out [m, n] = the sum of partial [splits][m][n] over the splits, in a fixed order.
+gsx_hip_status join_products(const float* partial, int64_t m, int64_t n, int64_t splits, float* out, int64_t out_stride,
+                             hipStream_t stream);
 gsx_hip_status block_matrix_check(const void* values, const void* exponents, int64_t rows, int64_t cols,
                                   int64_t values_stride, int64_t exponents_stride);
 

@@ -325,6 +325,197 @@ __global__ __launch_bounds__(kHeadThreads, 2) void linear_head_kernel(const T* _
     }
 }
 
+// ---- gradient of the weight, narrow layers ----------------------------------------------------------------------------------
+//
+//   gw[i, j] = sum over rows r of blocks(dy^T)[i, r] blocks(x^T)[j, r]
+//
+// A workgroup takes a stretch of blocks of 128 rows. Of each it reads dy and x once, finds the columns' maxima, quantises the
+// columns into LDS (a column's 128 values in a row of kWeightPitch bytes, so that a read of 16 columns meets 16 different
+// banks) and multiplies them, 2 x 4 waves with NT x KT tiles of 16 x 16 each; the next block's rows are on their way meanwhile.
+// The stretches' sums are joined by another launch. Memory bounds it: quantised copies of dy^T and x^T, written and read
+// again, would double what it moves.
+constexpr int kWeightThreads = 512;
+constexpr int kWeightPitch = 144;
+constexpr int kWeightPatches = 3;  // of 8 rows by 4 columns a thread holds: up to 96 quads of columns
+constexpr int64_t kWeightMostColumns = 4 * 96 - 6;
+
+// Four elements of a row as they lie in memory.
+template <typename T>
+struct RawQuad {
+    uint32_t w[sizeof(T)];
+};
+
+template <typename T>
+__device__ inline float element_of(const RawQuad<T>& x, int i) {
+    if constexpr (sizeof(T) == 4) {
+        return __builtin_bit_cast(float, x.w[i]);
+    } else if constexpr (__is_same(T, __bf16)) {
+        return __builtin_bit_cast(float, i & 1 ? x.w[i / 2] & 0xffff0000u : x.w[i / 2] << 16);
+    } else {
+        return to_float(__builtin_bit_cast(T, (uint16_t)(i & 1 ? x.w[i / 2] >> 16 : x.w[i / 2])));
+    }
+}
+
+template <typename T>
+__device__ inline RawQuad<T> load_quad(const T* __restrict__ p) {
+    struct __attribute__((packed, aligned(sizeof(T)))) Words {  // at any element's address
+        uint32_t w[sizeof(T)];
+    };
+    RawQuad<T> x;
+    const Words v = *reinterpret_cast<const Words*>(p);
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T); ++i) x.w[i] = v.w[i];
+    return x;
+}
+
+// Without its first `back` elements, zeros behind the others.
+template <typename T>
+__device__ inline RawQuad<T> shift_quad(RawQuad<T> x, int back) {
+    if constexpr (sizeof(T) == 4) {
+        for (; back > 0; --back) {
+            x.w[0] = x.w[1];
+            x.w[1] = x.w[2];
+            x.w[2] = x.w[3];
+            x.w[3] = 0;
+        }
+    } else {
+        const uint64_t v = ((uint64_t)x.w[1] << 32 | x.w[0]) >> (16 * back);
+        x.w[0] = (uint32_t)v;
+        x.w[1] = (uint32_t)(v >> 32);
+    }
+    return x;
+}
+
+template <typename T, int NT, int KT>
+__global__ __launch_bounds__(kWeightThreads) void linear_weight_kernel(const T* __restrict__ x, int64_t x_stride,
+                                                                       const T* __restrict__ dy, int64_t dy_stride,
+                                                                       int64_t m, int n, int k,
+                                                                       float* __restrict__ partial) {
+    constexpr int kN = 32 * NT, kK = 64 * KT;
+    __shared__ __attribute__((aligned(16))) uint8_t s_q[(kN + kK) * kWeightPitch];
+    __shared__ uint32_t s_top[kN + kK];
+    __shared__ uint8_t s_e[kN + kK];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x / 64, wn = wave / 4, wk = wave % 4;
+    const int64_t blocks = ceil_div(m, kBlock);
+    const int64_t first = blocks * blockIdx.x / gridDim.x, last = blocks * (blockIdx.x + 1) / gridDim.x;
+    // patch u of a thread: 8 rows from r0 on of the quad of columns at `column` of LDS (dy's columns before x's). A last quad that
+    // is cut is read from `back` columns further left, so that no read leaves its row.
+    const int dy_quads = (n + 3) / 4, quads = dy_quads + (k + 3) / 4;
+    int r0[kWeightPatches], column[kWeightPatches], back[kWeightPatches];
+    bool some[kWeightPatches];
+    const T* from[kWeightPatches];
+    int64_t stride[kWeightPatches];
+#pragma unroll
+    for (int u = 0; u < kWeightPatches; ++u) {
+        const int p = threadIdx.x + u * kWeightThreads, q = p % quads;
+        const bool is_dy = q < dy_quads;
+        const int c = (is_dy ? q : q - dy_quads) * 4;
+        r0[u] = p / quads * 8;
+        column[u] = is_dy ? c : kN + c;
+        some[u] = r0[u] < kBlock;
+        back[u] = max(0, c + 4 - (is_dy ? n : k));
+        from[u] = (is_dy ? dy : x) + (c - back[u]);
+        stride[u] = is_dy ? dy_stride : x_stride;
+    }
+    RawQuad<T> raw[kWeightPatches][8];
+    const auto load = [&](int64_t block) {
+#pragma unroll
+        for (int u = 0; u < kWeightPatches; ++u)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int64_t row = block * kBlock + r0[u] + i;
+                raw[u][i] = {};
+                if (some[u] && row < m) raw[u][i] = load_quad<T>(from[u] + row * stride[u]);
+            }
+    };
+    v4f acc[NT][KT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < KT; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    if (first < last) load(first);
+    for (int64_t block = first; block < last; ++block) {
+        for (int i = threadIdx.x; i < kN + kK; i += kWeightThreads) s_top[i] = 0;
+        __syncthreads();  // and the block before has been multiplied
+#pragma unroll
+        for (int u = 0; u < kWeightPatches; ++u) {
+            if (!some[u]) continue;
+            if (back[u] != 0) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) raw[u][i] = shift_quad<T>(raw[u][i], back[u]);
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                uint32_t top = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint32_t bits = __builtin_bit_cast(uint32_t, element_of(raw[u][i], c)) & 0x7fffffffu;
+                    if (finite_bits(bits)) top = max(top, bits);
+                }
+                atomicMax(&s_top[column[u] + c], top);
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < kWeightPatches; ++u) {
+            if (!some[u]) continue;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)  // unpacked anew: not held beside the words since the maxima were taken
+#pragma unroll
+                for (int w = 0; w < (int)sizeof(T); ++w) asm volatile("" : "+v"(raw[u][i].w[w]));
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int e = block_exponent(s_top[column[u] + c]);
+                float v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = element_of(raw[u][i], c);
+                *reinterpret_cast<uint2*>(s_q + (column[u] + c) * kWeightPitch + r0[u]) =
+                    make_uint2(pack_e4m3(v, e), pack_e4m3(v + 4, e));
+                if (r0[u] == 0) s_e[column[u] + c] = (uint8_t)(e + 127);
+            }
+        }
+        __syncthreads();
+        if (block + 1 < last) load(block + 1);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int at = (lane / 16) * 16 + 64 * half;
+            v8bf vx[KT][2];
+#pragma unroll
+            for (int j = 0; j < KT; ++j) {
+                const int c = kN + (wk * KT + j) * 16 + (lane & 15);
+                const v4i q = *reinterpret_cast<const v4i*>(s_q + c * kWeightPitch + at);
+                const float scale = block_scale(s_e[c]);
+                vx[j][0] = to_bf16(q[0], q[1], scale);
+                vx[j][1] = to_bf16(q[2], q[3], scale);
+            }
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                const int c = (wn * NT + i) * 16 + (lane & 15);
+                const v4i q = *reinterpret_cast<const v4i*>(s_q + c * kWeightPitch + at);
+                const float scale = block_scale(s_e[c]);
+                const v8bf y0 = to_bf16(q[0], q[1], scale), y1 = to_bf16(q[2], q[3], scale);
+#pragma unroll
+                for (int j = 0; j < KT; ++j) {
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vx[j][0], y0, acc[i][j], 0, 0, 0);
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vx[j][1], y1, acc[i][j], 0, 0, 0);
+                }
+            }
+        }
+    }
+    // the result's rows are columns of dy (lane % 16), its columns four of x a lane
+    float* const to = partial + (int64_t)blockIdx.x * n * k;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+        const int row = (wn * NT + i) * 16 + (lane & 15);
+        if (row >= n) continue;
+#pragma unroll
+        for (int j = 0; j < KT; ++j) {
+            const v4f one[1] = {acc[i][j]};
+            store_columns<1>(to + (int64_t)row * k, (wk * KT + j) * 16 + (lane / 16) * 4, k, one);
+        }
+    }
+}
+
 }  // namespace gsx_amd
 
 using namespace gsx_amd;
@@ -357,6 +548,33 @@ void launch_head(const T* x, int64_t x_stride, const BlockMatrix& w, int64_t m, 
     hipLaunchKernelGGL((linear_head_kernel<T, O, TN>), dim3((unsigned)(tiles < 1024 ? tiles : 1024)), dim3(kHeadThreads),
                        (unsigned)lds, stream, x, x_stride, w, m, n, k, slots, out, out_stride);
 }
+
+// Stretches of rows that the weight's gradient of a narrow layer is split into; 0: the layer is not narrow, or too short for its
+// partial sums to be few beside what is read.
+int64_t weight_stretches(int64_t m, int64_t n, int64_t k) {
+    if (n < 4 || k < 4 || n + k > kWeightMostColumns || n > (k <= 128 ? 256 : 128) || k > 256 || m < 8192) return 0;
+    const int64_t blocks = ceil_div(m, kBlock);
+    return blocks < 256 ? blocks : 256;
+}
+
+struct WeightBlocks {  // workspace of the general way: byte offsets
+    int64_t blocks, words, dy_values, dy_exponents, x_values, x_exponents, rest;
+    WeightBlocks(int64_t m, int64_t n, int64_t k) {
+        blocks = ceil_div(m, kBlock);
+        words = ceil_div(blocks, 4) * 4;
+        int64_t at = 0;
+        const auto take = [&](int64_t size) {
+            const int64_t here = at;
+            at += ceil_div(size, 256) * 256;
+            return here;
+        };
+        dy_values = take(n * blocks * kBlock);
+        dy_exponents = take(n * words);
+        x_values = take(k * blocks * kBlock);
+        x_exponents = take(k * words);
+        rest = at;
+    }
+};
 
 }  // namespace
 
@@ -429,6 +647,61 @@ gsx_hip_status gsx_hip_linear_forward(const void* x, int32_t x_type, int64_t x_s
             }
             return fields_launched("linear launch");
         });
+    });
+}
+
+size_t gsx_hip_linear_backward_weight_temp_bytes(int64_t m, int64_t n, int64_t k) {
+    if (!product_sizes(m, n, k) || m > kMostSummands || n == 0 || k == 0) return 0;
+    const int64_t stretches = weight_stretches(m, n, k);
+    if (stretches > 0) return (size_t)(stretches * n * k * 4);
+    return (size_t)WeightBlocks(m, n, k).rest + gsx_hip_blocks_matmul_temp_bytes(n, k, m);
+}
+
+gsx_hip_status gsx_hip_linear_backward_weight(const void* x, int32_t x_type, int64_t x_stride, const void* grad_out,
+                                              int32_t grad_type, int64_t grad_stride, int64_t m, int64_t n, int64_t k,
+                                              float* grad_weight, int64_t weight_stride, void* temp, hipStream_t stream) {
+    if (!known_type(x_type) || !known_type(grad_type))
+        return fields_fail(GSX_HIP_ERROR_NOT_SUPPORTED, "linear backward: rows are f32, bf16 or f16");
+    if (!product_sizes(m, n, k) || m > kMostSummands)
+        return fields_fail(GSX_HIP_ERROR_OUT_OF_RANGE, "linear backward: at most 2^27 rows, 2^31 - 1 and 2^27 columns");
+    if (!rows_fit(m, x_stride, k) || !rows_fit(m, grad_stride, n) || !rows_fit(n, weight_stride, k))
+        return fields_fail(GSX_HIP_ERROR_INVALID_ARGUMENT, "linear backward: strides must be at least the rows' lengths");
+    if (n == 0 || k == 0) return GSX_HIP_SUCCESS;
+    if (grad_weight == nullptr || !aligned_to(grad_weight, 4) ||
+        (m > 0 && (x == nullptr || grad_out == nullptr || temp == nullptr)) || !aligned_to(x, type_bytes(x_type)) ||
+        !aligned_to(grad_out, type_bytes(grad_type)) || !aligned_to(temp, 16))
+        return fields_fail(GSX_HIP_ERROR_INVALID_ARGUMENT,
+                           "linear backward: rows and workspace must be non-null and aligned to their elements");
+    const int64_t stretches = x_type == grad_type ? weight_stretches(m, n, k) : 0;
+    if (stretches == 0) {
+        const WeightBlocks at(m, n, k);
+        uint8_t* const base = static_cast<uint8_t*>(temp);
+        gsx_hip_status st = gsx_hip_blocks_quantize(grad_out, grad_type, m, n, grad_stride, 1, base + at.dy_values,
+                                                    at.blocks * kBlock, base + at.dy_exponents, at.words, stream);
+        if (st != GSX_HIP_SUCCESS) return st;
+        st = gsx_hip_blocks_quantize(x, x_type, m, k, x_stride, 1, base + at.x_values, at.blocks * kBlock,
+                                     base + at.x_exponents, at.words, stream);
+        if (st != GSX_HIP_SUCCESS) return st;
+        return gsx_hip_blocks_matmul(base + at.dy_values, at.blocks * kBlock, base + at.dy_exponents, at.words,
+                                     base + at.x_values, at.blocks * kBlock, base + at.x_exponents, at.words, n, k, m,
+                                     grad_weight, GSX_HIP_DTYPE_F32, weight_stride, base + at.rest, stream);
+    }
+    return with_type(x_type, [&](auto t) {
+        using T = decltype(t);
+        float* const partial = static_cast<float*>(temp);
+        const auto go = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3((unsigned)stretches), dim3(kWeightThreads), 0, stream, static_cast<const T*>(x),
+                               x_stride, static_cast<const T*>(grad_out), grad_stride, m, (int)n, (int)k, partial);
+        };
+        if (k <= 128) {
+            if (n <= 128) go(linear_weight_kernel<T, 4, 2>);
+            else if (n <= 192) go(linear_weight_kernel<T, 6, 2>);
+            else go(linear_weight_kernel<T, 8, 2>);
+        } else {
+            go(linear_weight_kernel<T, 4, 4>);
+        }
+        const gsx_hip_status st = fields_launched("linear backward launch");
+        return st != GSX_HIP_SUCCESS ? st : join_products(partial, n, k, stretches, grad_weight, weight_stride, stream);
     });
 }
 

@@ -220,18 +220,32 @@ def linear(x: torch.Tensor, weight: Blocks, out_dtype=None, out: torch.Tensor | 
     return _run(stream, call)
 
 
-def linear_backward(x: torch.Tensor, grad_out: torch.Tensor, weight_t: Blocks, stream=None):
+def linear_backward(x: torch.Tensor, grad_out: torch.Tensor, weight_t: Blocks, grad_weight: torch.Tensor | None = None,
+                    stream=None):
     """Gradients of linear(x, weight) for the upstream grad_out [m, n]: (grad_x in grad_out's type, grad_weight float32).
 
     weight_t holds the transposed weight [k, n] in blocks. grad_x = blocks(grad_out) weight_t^T and
     grad_weight = blocks(grad_out^T) blocks(x^T)^T: every operand is quantised along the axis that is summed over."""
-    if grad_out.dim() != 2 or x.dim() != 2 or x.shape[0] != grad_out.shape[0]:
-        raise GsxHipError("x and grad_out must be matrices with the same number of rows")
-    if weight_t.cols != grad_out.shape[1] or weight_t.rows != x.shape[1]:
-        raise GsxHipError(f"weight_t must be [{x.shape[1]}, {grad_out.shape[1]}], not [{weight_t.rows}, {weight_t.cols}]")
+    lib = _lib.load(require_device=False)
+    base, stride = _rows(x, "x")
+    grad_base, grad_stride = _rows(grad_out, "grad_out")
+    m, k = x.shape
+    n = grad_out.shape[1]
+    if grad_out.shape[0] != m:
+        raise GsxHipError("x and grad_out must have the same number of rows")
+    if weight_t.cols != n or weight_t.rows != k:
+        raise GsxHipError(f"weight_t must be [{k}, {n}], not [{weight_t.rows}, {weight_t.cols}]")
     grad_x = linear(grad_out, weight_t, stream=stream)
-    grad_weight = matmul(quantize(grad_out, True, stream), quantize(x, True, stream), stream=stream)
-    return grad_x, grad_weight
+
+    def call(handle):
+        result = torch.empty((n, k), dtype=torch.float32, device=x.device) if grad_weight is None else grad_weight
+        to, to_stride = _rows(result, "grad_weight", torch.float32, (n, k))
+        temp = _temp(lib.gsx_hip_linear_backward_weight_temp_bytes(m, n, k))
+        check(lib.gsx_hip_linear_backward_weight(base, _type(x.dtype), stride, grad_base, _type(grad_out.dtype), grad_stride,
+                                                 m, n, k, to, to_stride, _address(temp), handle), "linear backward")
+        return result
+
+    return grad_x, _run(stream, call)
 
 
 def _teacher(logits, teacher_ids, teacher_logits, row_weight):

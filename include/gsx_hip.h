@@ -522,6 +522,14 @@ gsx_hip_status gsx_hip_linear_forward(const void* x, int32_t x_type, int64_t x_s
                                       int64_t m, int64_t n, int64_t k, void* out, int32_t out_type, int64_t out_stride,
                                       void* temp, hipStream_t stream);
 
+/* Gradient of linear_forward's weight for the upstream grad_out [m, n]: grad_weight [n, k] (float32) = blocks(grad_out^T)
+ * blocks(x^T)^T, both quantised along the m rows that are summed over (at most 2^27). (The gradient of x is linear_forward of
+ * grad_out with the transposed weight's blocks.) */
+size_t gsx_hip_linear_backward_weight_temp_bytes(int64_t m, int64_t n, int64_t k);
+gsx_hip_status gsx_hip_linear_backward_weight(const void* x, int32_t x_type, int64_t x_stride, const void* grad_out,
+                                              int32_t grad_type, int64_t grad_stride, int64_t m, int64_t n, int64_t k,
+                                              float* grad_weight, int64_t weight_stride, void* temp, hipStream_t stream);
+
 /* Distillation from a teacher's top logits. Row r of `logits` [rows, vocab] is the student's z; teacher_ids and teacher_logits
  * [rows, top] (rows teacher_stride apart, top at most 1024) name the teacher's entries. An entry counts if its id lies in
  * [0, vocab) and its logit is not -inf. With T the temperature (1e-6 to 1e6), p = softmax(t / T) over the entries that

@@ -221,6 +221,40 @@ def test_linear_backward(m, n, k, kind):
         assert (np.abs(got.double().cpu().numpy() - want) <= bound).all()
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("m,n,k", [(8192, 1, 1), (8193, 130, 127), (9000, 150, 128), (20001, 33, 257), (8200, 256, 120),
+                                   (12345, 61, 200), (40000, 200, 60), (8191, 150, 128)])
+def test_weight_gradient_of_narrow_layers(m, n, k, kind):
+    """Many rows and few columns, with odd strides: sums of m terms in parts."""
+    from gsx_amd import fields
+    g = torch.Generator("cuda").manual_seed(m)
+    x = torch.randn(m, k + 3, device="cuda", generator=g).to(DTYPES[kind])[:, 1: k + 1]
+    dy = torch.randn(m, n + 1, device="cuda", generator=g).to(DTYPES[kind])[:, 1:]
+    x[m // 2], dy[3, 0] = 0, 300.0
+    wt = fields.quantize(torch.randn(n, k, device="cuda", generator=g), transpose=True)
+    print(f"[case] weight gradient {m} x {n} x {k} {kind}", flush=True)
+    base = torch.full((n, k + 2), 7.0, device="cuda")
+    _, dw = fields.linear_backward(x, dy, wt, grad_weight=base[:, 1: k + 1])
+    p, q = (_values(*_want_blocks(s.double().cpu().numpy().T), m) for s in (dy, x))
+    want, size = p @ q.T, np.abs(p) @ np.abs(q).T
+    # a part's sum of at most m terms and a join: see test_matmul
+    assert (np.abs(dw.double().cpu().numpy() - want) <= size * (m + 8) * 2.0**-23 + np.abs(want) * 2.0**-24).all()
+    assert np.linalg.norm(dw.double().cpu().numpy() - want) <= 2e-6 * np.linalg.norm(want) + 2.0**-23 * np.linalg.norm(size) / 16
+    assert (base[:, 0] == 7).all() and (base[:, -1] == 7).all()
+    again = fields.linear_backward(x, dy, wt)[1]
+    assert torch.equal(again, dw)
+
+
+def test_weight_gradient_keeps_non_finite_columns_apart():
+    from gsx_amd import fields
+    x, dy = torch.randn(9000, 20, device="cuda"), torch.randn(9000, 30, device="cuda")
+    x[17, 3], dy[8999, 7] = float("inf"), float("nan")
+    _, dw = fields.linear_backward(x, dy, fields.quantize(torch.randn(30, 20, device="cuda"), transpose=True))
+    bad = torch.zeros(30, 20, dtype=torch.bool, device="cuda")
+    bad[:, 3], bad[7] = True, True
+    assert torch.equal(torch.isnan(dw), bad)
+
+
 def test_linear_gradient_against_differences():
     """With operands that 8 bits hold exactly the product is bilinear, so central differences of it are exact."""
     from gsx_amd import fields
