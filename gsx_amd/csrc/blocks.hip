@@ -36,31 +36,26 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_rows_kernel(const T* _
          b += (int64_t)gridDim.x * (kQuantThreads / 16)) {
         const int64_t r = b / spans, kb0 = b % spans * kQuantUnroll;
         const T* const row = src + r * src_stride;
-        float x[kQuantUnroll][8];
+        Raw<T, 8> x[kQuantUnroll][1];
 #pragma unroll
         for (int u = 0; u < kQuantUnroll; ++u) {
             const int64_t col = (kb0 + u) * kBlock + sub * 8;
-            if (col + 8 <= cols) {
-                const Octet<T> v = *reinterpret_cast<const Octet<T>*>(row + col);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) x[u][k] = to_float(v.v[k]);
-            } else {
-#pragma unroll
-                for (int k = 0; k < 8; ++k) x[u][k] = col + k < cols ? to_float(row[col + k]) : 0.0f;
-            }
+            x[u][0] = load_raw<T, 8>(row, col, cols);
         }
 #pragma unroll
         for (int u = 0; u < kQuantUnroll; ++u) {
-            uint32_t top = largest(x[u]);
+            bool special;
+            uint32_t top = largest_raw<T, 8, 1>(x[u], special);
 #pragma unroll
             for (int off = 8; off > 0; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off, 16));
             if (kb0 + u >= blocks) continue;
-            const int e = block_exponent(top);
+            const uint32_t e = (uint32_t)(block_exponent(top) + 127);
+            const float scale = block_scale(e);
             const int64_t col = (kb0 + u) * kBlock + sub * 8;
             if (col < values_stride)
                 *reinterpret_cast<uint2*>(values + r * values_stride + col) =
-                    make_uint2(pack_e4m3(x[u], e), pack_e4m3(x[u] + 4, e));
-            if (sub == 0) exponents[r * exponents_stride + kb0 + u] = (uint8_t)(e + 127);
+                    make_uint2(pack_raw<T, 8>(x[u][0], 0, scale, special), pack_raw<T, 8>(x[u][0], 4, scale, special));
+            if (sub == 0) exponents[r * exponents_stride + kb0 + u] = (uint8_t)e;
         }
     }
 }
@@ -84,42 +79,28 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_columns_kernel(const T
     for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
         const int64_t kb = tile / strips, c0 = tile % strips * 64;
         const int64_t col = c0 + quad * 4;
-        float x[8][4];
+        Raw<T, 4> x[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int64_t r = kb * kBlock + r0 + i;
-            const T* const p = src + r * src_stride + col;
-            if (r < src_rows && col + 4 <= src_cols) {
-                const Quad<T> v = *reinterpret_cast<const Quad<T>*>(p);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) x[i][k] = to_float(v.v[k]);
-            } else {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) x[i][k] = r < src_rows && col + k < src_cols ? to_float(p[k]) : 0.0f;
-            }
+            x[i] = load_raw<T, 4>(src + r * src_stride, col, r < src_rows ? src_cols : 0);
         }
+        uint32_t top[4];
+        const bool special = patch_tops<T>(x, top);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            uint32_t top = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const uint32_t bits = __builtin_bit_cast(uint32_t, x[i][k]) & 0x7fffffffu;
-                if (finite_bits(bits)) top = max(top, bits);
-            }
-            top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
-            top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
-            if ((threadIdx.x & 63) < 16) s_top[wave][quad * 4 + k] = top;
+            top[k] = max(top[k], (uint32_t)__shfl_xor((int)top[k], 16, 64));
+            top[k] = max(top[k], (uint32_t)__shfl_xor((int)top[k], 32, 64));
+            if ((threadIdx.x & 63) < 16) s_top[wave][quad * 4 + k] = top[k];
         }
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const int c = quad * 4 + k;
-            const uint32_t top = max(max(s_top[0][c], s_top[1][c]), max(s_top[2][c], s_top[3][c]));
-            const int e = block_exponent(top);
-            const float y[8] = {x[0][k], x[1][k], x[2][k], x[3][k], x[4][k], x[5][k], x[6][k], x[7][k]};
-            *reinterpret_cast<uint2*>(s_q + c * kPitch + r0) = make_uint2(pack_e4m3(y, e), pack_e4m3(y + 4, e));
-            if (threadIdx.x < 16 && c0 + c < src_cols)
-                exponents[(c0 + c) * exponents_stride + kb] = (uint8_t)(e + 127);
+            const uint32_t most = max(max(s_top[0][c], s_top[1][c]), max(s_top[2][c], s_top[3][c]));
+            const uint32_t e = (uint32_t)(block_exponent(most) + 127);
+            *reinterpret_cast<uint2*>(s_q + c * kPitch + r0) = patch_column<T>(x, k, block_scale(e), special);
+            if (threadIdx.x < 16 && c0 + c < src_cols) exponents[(c0 + c) * exponents_stride + kb] = (uint8_t)e;
         }
         __syncthreads();
         for (int i = threadIdx.x; i < 64 * 8; i += kQuantThreads) {

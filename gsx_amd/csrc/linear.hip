@@ -17,83 +17,46 @@ namespace gsx_amd {
 // reads 64 bytes of each weight row in a piece.
 __device__ inline int64_t piece_k(int64_t k0, int half, int lane) { return k0 + 64 * half + 16 * (lane / 16); }
 
-// A lane's 32 elements of block k0 of a row as they lie in memory, zeros past the last column.
+// A lane's 32 elements of block k0 of a row. In a block that is cut, what lies past the last column is put right only when the
+// block is used (cut_block): nothing waits for a load that is issued ahead.
 template <typename T>
 struct RawBlock {
-    uint32_t w[4][2 * sizeof(T)];
+    Raw<T, 8> v[4];
 };
 
 template <typename T>
-__device__ inline float element_of(const RawBlock<T>& x, int i) {
-    const uint32_t* const w = x.w[i / 8];
-    if constexpr (sizeof(T) == 4) {
-        return __builtin_bit_cast(float, w[i % 8]);
-    } else if constexpr (__is_same(T, __bf16)) {
-        const uint32_t word = w[i % 8 / 2];
-        return __builtin_bit_cast(float, i & 1 ? word & 0xffff0000u : word << 16);
+__device__ inline void load_block(const T* __restrict__ row, int64_t k0, int64_t cols, int lane, RawBlock<T>& x) {
+    if (cols >= 8) {
+#pragma unroll
+        for (int o = 0; o < 4; ++o)
+            x.v[o] = load_raw<T, 8>(row + min(piece_k(k0, o / 2, lane) + 8 * (o & 1), cols - 8));
     } else {
-        const uint32_t word = w[i % 8 / 2];
-        return to_float(__builtin_bit_cast(T, (uint16_t)(i & 1 ? word >> 16 : word)));
+#pragma unroll
+        for (int o = 0; o < 4; ++o) x.v[o] = load_raw<T, 8>(row, piece_k(k0, o / 2, lane) + 8 * (o & 1), cols);
     }
 }
 
 template <typename T>
-__device__ inline void load_block(const T* __restrict__ row, int64_t k0, int64_t cols, int lane, RawBlock<T>& x) {
-    struct __attribute__((packed, aligned(sizeof(T)))) Words {  // at any element's address
-        uint32_t w[2 * sizeof(T)];
-    };
+__device__ inline void cut_block(int64_t k0, int64_t cols, int lane, RawBlock<T>& x) {
+    if (k0 + kBlock <= cols || cols < 8) return;
 #pragma unroll
     for (int o = 0; o < 4; ++o) {
-        const int64_t at = piece_k(k0, o / 2, lane) + 8 * (o & 1);
-        Words v = {};
-        if (at + 8 <= cols) {
-            v = *reinterpret_cast<const Words*>(row + at);
-        } else if (at < cols) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (at + i >= cols) continue;
-                if constexpr (sizeof(T) == 4) v.w[i] = __builtin_bit_cast(uint32_t, row[at + i]);
-                else v.w[i / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, row[at + i]) << (16 * (i & 1));
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < (int)(2 * sizeof(T)); ++i) x.w[o][i] = v.w[i];
+        const int64_t over = piece_k(k0, o / 2, lane) + 8 * (o & 1) + 8 - cols;
+        if (over > 0) x.v[o] = over < 8 ? shift_raw<T, 8>(x.v[o], (int)over) : Raw<T, 8>{};
     }
 }
 
-// The values that a row's block stands for, from the 32 that each of its four lanes holds; y[o] are those of w[o].
+// The values that a row's block stands for, from the 32 that each of its four lanes holds; y[o] are those of v[o].
 template <typename T>
 __device__ inline void quantize_block(const RawBlock<T>& raw, v8bf (&y)[4]) {
-    float x[32];
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-        x[i] = element_of(raw, i);
-        top = max(top, __builtin_bit_cast(uint32_t, x[i]) & 0x7fffffffu);
-    }
-    const bool special = __builtin_amdgcn_ballot_w64(!finite_bits(top)) != 0;
-    if (special) {  // rare: infinities and NaN do not count for the scale
-        top = 0;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            const uint32_t bits = __builtin_bit_cast(uint32_t, x[i]) & 0x7fffffffu;
-            if (finite_bits(bits)) top = max(top, bits);
-        }
-    }
+    bool special;
+    uint32_t top = largest_raw<T, 8, 4>(raw.v, special);
     top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
     top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
-    const int e = block_exponent(top);
-    const float scale = block_scale((uint32_t)(e + 127));
-    int q[8];
-    if (special) {
+    const float scale = block_scale((uint32_t)(block_exponent(top) + 127));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] = (int)pack_e4m3(x + 4 * i, e);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] = (int)pack_finite(x + 4 * i, e);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = to_bf16(q[2 * i], q[2 * i + 1], scale);
+    for (int o = 0; o < 4; ++o)
+        y[o] = to_bf16((int)pack_raw<T, 8>(raw.v[o], 0, scale, special), (int)pack_raw<T, 8>(raw.v[o], 4, scale, special), scale);
 }
 
 // ---- few rows -------------------------------------------------------------------------------------------------------------
@@ -161,16 +124,16 @@ __global__ __launch_bounds__(64 * kFewWaves, 4) void linear_few_kernel(const T* 
                     const int64_t kb = kb0 + i / m;
                     const int r = i % m;
                     const int64_t col = kb * kBlock + sub * 8;
-                    float v[8];
-#pragma unroll
-                    for (int c = 0; c < 8; ++c) v[c] = col + c < k ? to_float(x[r * x_stride + col + c]) : 0.0f;
-                    uint32_t top = largest(v);
+                    const Raw<T, 8> v[1] = {load_raw<T, 8>(x + r * x_stride, col, k)};
+                    bool special;
+                    uint32_t top = largest_raw<T, 8, 1>(v, special);
 #pragma unroll
                     for (int off = 8; off > 0; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off, 16));
-                    const int e = block_exponent(top);
+                    const uint32_t e = (uint32_t)(block_exponent(top) + 127);
+                    const float scale = block_scale(e);
                     *reinterpret_cast<uint2*>(s_x + i * kBlock + ((sub / 2) ^ (r & 7)) * 16 + (sub & 1) * 8) =
-                        make_uint2(pack_e4m3(v, e), pack_e4m3(v + 4, e));
-                    if (sub == 0) s_e[i] = (uint8_t)(e + 127);
+                        make_uint2(pack_raw<T, 8>(v[0], 0, scale, special), pack_raw<T, 8>(v[0], 4, scale, special));
+                    if (sub == 0) s_e[i] = (uint8_t)e;
                 }
                 __syncthreads();
             }
@@ -275,7 +238,10 @@ __global__ __launch_bounds__(kHeadThreads, 2) void linear_head_kernel(const T* _
             }
             v8bf vx[R][4];
 #pragma unroll
-            for (int r = 0; r < R; ++r) quantize_block<T>(next[r], vx[r]);
+            for (int r = 0; r < R; ++r) {
+                cut_block<T>(kb * kBlock, k, lane, next[r]);
+                quantize_block<T>(next[r], vx[r]);
+            }
             if (kb + 1 < blocks) load(t, kb + 1);
             else if (t + gridDim.x < tiles) load(t + gridDim.x, 0);
             const uint8_t* const values = s_w + slot * kRows * kBlock;
@@ -339,53 +305,6 @@ constexpr int kWeightPitch = 144;
 constexpr int kWeightPatches = 3;  // of 8 rows by 4 columns a thread holds: up to 96 quads of columns
 constexpr int64_t kWeightMostColumns = 4 * 96 - 6;
 
-// Four elements of a row as they lie in memory.
-template <typename T>
-struct RawQuad {
-    uint32_t w[sizeof(T)];
-};
-
-template <typename T>
-__device__ inline float element_of(const RawQuad<T>& x, int i) {
-    if constexpr (sizeof(T) == 4) {
-        return __builtin_bit_cast(float, x.w[i]);
-    } else if constexpr (__is_same(T, __bf16)) {
-        return __builtin_bit_cast(float, i & 1 ? x.w[i / 2] & 0xffff0000u : x.w[i / 2] << 16);
-    } else {
-        return to_float(__builtin_bit_cast(T, (uint16_t)(i & 1 ? x.w[i / 2] >> 16 : x.w[i / 2])));
-    }
-}
-
-template <typename T>
-__device__ inline RawQuad<T> load_quad(const T* __restrict__ p) {
-    struct __attribute__((packed, aligned(sizeof(T)))) Words {  // at any element's address
-        uint32_t w[sizeof(T)];
-    };
-    RawQuad<T> x;
-    const Words v = *reinterpret_cast<const Words*>(p);
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T); ++i) x.w[i] = v.w[i];
-    return x;
-}
-
-// Without its first `back` elements, zeros behind the others.
-template <typename T>
-__device__ inline RawQuad<T> shift_quad(RawQuad<T> x, int back) {
-    if constexpr (sizeof(T) == 4) {
-        for (; back > 0; --back) {
-            x.w[0] = x.w[1];
-            x.w[1] = x.w[2];
-            x.w[2] = x.w[3];
-            x.w[3] = 0;
-        }
-    } else {
-        const uint64_t v = ((uint64_t)x.w[1] << 32 | x.w[0]) >> (16 * back);
-        x.w[0] = (uint32_t)v;
-        x.w[1] = (uint32_t)(v >> 32);
-    }
-    return x;
-}
-
 template <typename T, int NT, int KT>
 __global__ __launch_bounds__(kWeightThreads) void linear_weight_kernel(const T* __restrict__ x, int64_t x_stride,
                                                                        const T* __restrict__ dy, int64_t dy_stride,
@@ -417,7 +336,7 @@ __global__ __launch_bounds__(kWeightThreads) void linear_weight_kernel(const T* 
         from[u] = (is_dy ? dy : x) + (c - back[u]);
         stride[u] = is_dy ? dy_stride : x_stride;
     }
-    RawQuad<T> raw[kWeightPatches][8];
+    Raw<T, 4> raw[kWeightPatches][8];
     const auto load = [&](int64_t block) {
 #pragma unroll
         for (int u = 0; u < kWeightPatches; ++u)
@@ -425,7 +344,7 @@ __global__ __launch_bounds__(kWeightThreads) void linear_weight_kernel(const T* 
             for (int i = 0; i < 8; ++i) {
                 const int64_t row = block * kBlock + r0[u] + i;
                 raw[u][i] = {};
-                if (some[u] && row < m) raw[u][i] = load_quad<T>(from[u] + row * stride[u]);
+                if (some[u] && row < m) raw[u][i] = load_raw<T, 4>(from[u] + row * stride[u]);
             }
     };
     v4f acc[NT][KT];
@@ -437,41 +356,29 @@ __global__ __launch_bounds__(kWeightThreads) void linear_weight_kernel(const T* 
     for (int64_t block = first; block < last; ++block) {
         for (int i = threadIdx.x; i < kN + kK; i += kWeightThreads) s_top[i] = 0;
         __syncthreads();  // and the block before has been multiplied
+        bool special[kWeightPatches];
 #pragma unroll
         for (int u = 0; u < kWeightPatches; ++u) {
             if (!some[u]) continue;
             if (back[u] != 0) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) raw[u][i] = shift_quad<T>(raw[u][i], back[u]);
+                for (int i = 0; i < 8; ++i) raw[u][i] = shift_raw<T, 4>(raw[u][i], back[u]);
             }
+            uint32_t top[4];
+            special[u] = patch_tops<T>(raw[u], top);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint32_t top = 0;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const uint32_t bits = __builtin_bit_cast(uint32_t, element_of(raw[u][i], c)) & 0x7fffffffu;
-                    if (finite_bits(bits)) top = max(top, bits);
-                }
-                atomicMax(&s_top[column[u] + c], top);
-            }
+            for (int c = 0; c < 4; ++c) atomicMax(&s_top[column[u] + c], top[c]);
         }
         __syncthreads();
 #pragma unroll
         for (int u = 0; u < kWeightPatches; ++u) {
             if (!some[u]) continue;
 #pragma unroll
-            for (int i = 0; i < 8; ++i)  // unpacked anew: not held beside the words since the maxima were taken
-#pragma unroll
-                for (int w = 0; w < (int)sizeof(T); ++w) asm volatile("" : "+v"(raw[u][i].w[w]));
-#pragma unroll
             for (int c = 0; c < 4; ++c) {
-                const int e = block_exponent(s_top[column[u] + c]);
-                float v[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = element_of(raw[u][i], c);
+                const uint32_t e = (uint32_t)(block_exponent(s_top[column[u] + c]) + 127);
                 *reinterpret_cast<uint2*>(s_q + (column[u] + c) * kWeightPitch + r0[u]) =
-                    make_uint2(pack_e4m3(v, e), pack_e4m3(v + 4, e));
-                if (r0[u] == 0) s_e[column[u] + c] = (uint8_t)(e + 127);
+                    patch_column<T>(raw[u], c, block_scale(e), special[u]);
+                if (r0[u] == 0) s_e[column[u] + c] = (uint8_t)e;
             }
         }
         __syncthreads();
