@@ -278,13 +278,16 @@ __global__ __launch_bounds__(kHeadThreads, 2) void linear_head_kernel(const T* _
             const int col = lane % across * kOct;
             for (int i = lane / across; i < 16; i += 64 / across) {
                 const int64_t row = m0 + r * 16 + i;
-                if (row >= m || col >= n) continue;
-                const O* const from = reinterpret_cast<const O*>(mine + i * kHeadPitch<O, TN>) + col;
-                O* const to = out + row * out_stride + col;
-                if (col + kOct <= n) {
-                    *reinterpret_cast<Octet<O>*>(to) = *reinterpret_cast<const Octet<O>*>(from);
-                } else {
-                    for (int c = 0; c < n - col; ++c) to[c] = from[c];
+                if (row < m && col + kOct <= n)
+                    *reinterpret_cast<Octet<O>*>(out + row * out_stride + col) =
+                        *reinterpret_cast<const Octet<O>*>(mine + i * kHeadPitch<O, TN> + col * sizeof(O));
+            }
+            if (n % kOct != 0) {  // the last columns of eight rows at a time, one a lane
+                const int64_t last = n / kOct * kOct + lane % kOct;
+                for (int i = lane / kOct; i < 16; i += 64 / kOct) {
+                    const int64_t row = m0 + r * 16 + i;
+                    if (row < m && last < n)
+                        out[row * out_stride + last] = reinterpret_cast<const O*>(mine + i * kHeadPitch<O, TN>)[last];
                 }
             }
         }
