@@ -386,16 +386,16 @@ gsx_hip_status join_products(const float* partial, int64_t m, int64_t n, int64_t
 
 namespace {
 
-// Tiles and splits of a product by its sizes alone. Large tiles move the fewest bytes through LDS for a product; they are taken
-// where they fill the GPU's 256 CUs, smaller ones where they do not. What is still short of two workgroups a CU is split over k,
-// four blocks or more to a part.
+// Tiles and splits of a product by its sizes alone. Tiles of 256 and 192 run one to a CU, of 128 two; the edge is the one whose
+// whole rounds of tiles cover the product with the least work, the larger one where two do (4001 x 2050 x 4100: 272 us for both
+// gradients with 231 tiles of 192, 544 tiles of 128 need two rounds and NNN). What fills less than
+// half a round is split over k, four blocks or more to a part.
 struct ProductPlan {
-    int bm, bn;
+    int edge;
     int64_t tiles_m, tiles_n, splits;
     int64_t temp_bytes;
 };
 
-constexpr int64_t kSplitTarget = 512;
 // Products of at least this many summands with a 16-bit result go through the 8-bit instructions: below, memory bounds them and
 // nothing is gained; 8192^3 takes 515 us instead of 850.
 constexpr int64_t kEightLeast = 1024;
@@ -403,13 +403,18 @@ constexpr int64_t kSplitMostBlocks = 512;  // blocks of k after which a float su
 
 ProductPlan product_plan(int64_t m, int64_t n, int64_t k) {
     ProductPlan p;
-    const auto tiles = [&](int64_t edge) { return ceil_div(m, edge) * ceil_div(n, edge); };
-    const int edge = tiles(256) >= 192 ? 256 : tiles(128) >= 256 || (m > 64 && n > 64) ? 128 : 64;
-    p.bm = p.bn = edge;
-    p.tiles_m = ceil_div(m, edge);
-    p.tiles_n = ceil_div(n, edge);
+    const auto cost = [&](int64_t edge, int64_t slots) {
+        return ceil_div(ceil_div(m, edge) * ceil_div(n, edge), slots) * (slots / 256) * edge * edge;
+    };
+    p.edge = 256;
+    if (cost(192, 256) < cost(256, 256)) p.edge = 192;
+    if (cost(128, 512) < cost(p.edge, 256)) p.edge = 128;
+    if (m <= 64 || n <= 64) p.edge = 64;
+    p.tiles_m = ceil_div(m, p.edge);
+    p.tiles_n = ceil_div(n, p.edge);
     const int64_t blocks = ceil_div(k, kBlock), count = p.tiles_m * p.tiles_n;
-    int64_t splits = count >= kSplitTarget / 2 ? 1 : ceil_div(kSplitTarget, count);
+    const int64_t slots = p.edge >= 192 ? 256 : 512;
+    int64_t splits = count >= slots / 2 ? 1 : slots / count;  // one round of workgroups
     if (splits > blocks / 4) splits = blocks / 4;
     if (splits < ceil_div(blocks, kSplitMostBlocks)) splits = ceil_div(blocks, kSplitMostBlocks);
     p.splits = splits < 1 ? 1 : splits;
@@ -489,14 +494,16 @@ gsx_hip_status gsx_hip_blocks_matmul(const uint8_t* a_values, int64_t a_values_s
         };
         if constexpr (sizeof(O) == 2) {
             if (k >= kEightLeast) {
-                if (plan.bm == 256) go(product_kernel<O, 8, 4, 2, 4, true>, 512);
-                else if (plan.bm == 128) go(product_kernel<O, 4, 4, 2, 2, true>, 256);
+                if (plan.edge == 256) go(product_kernel<O, 8, 4, 2, 4, true>, 512);
+                else if (plan.edge == 192) go(product_kernel<O, 6, 3, 2, 4, true>, 512);
+                else if (plan.edge == 128) go(product_kernel<O, 4, 4, 2, 2, true>, 256);
                 else go(product_kernel<O, 2, 2, 2, 2, true>, 256);
             }
         }
         if (sizeof(O) == 4 || k < kEightLeast) {
-            if (plan.bm == 256) go(product_kernel<O, 8, 4, 2, 4, false>, 512);
-            else if (plan.bm == 128) go(product_kernel<O, 4, 4, 2, 2, false>, 256);
+            if (plan.edge == 256) go(product_kernel<O, 8, 4, 2, 4, false>, 512);
+            else if (plan.edge == 192) go(product_kernel<O, 6, 3, 2, 4, false>, 512);
+            else if (plan.edge == 128) go(product_kernel<O, 4, 4, 2, 2, false>, 256);
             else go(product_kernel<O, 2, 2, 2, 2, false>, 256);
         }
         if (plan.splits > 1) {
