@@ -193,7 +193,7 @@ SIGNATURES = {
                                     _vp]),
     "gsx_hip_linear_temp_bytes": (ctypes.c_size_t, [_i64, _i64, _i64]),
     "gsx_hip_linear_forward": (_st, [_vp, _i32, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _i32, _i64, _vp, _vp]),
-    "gsx_hip_linear_backward_weight_temp_bytes": (ctypes.c_size_t, [_i64, _i64, _i64]),
+    "gsx_hip_linear_backward_weight_temp_bytes": (ctypes.c_size_t, [_i32, _i32, _i64, _i64, _i64]),
     "gsx_hip_linear_backward_weight": (_st, [_vp, _i32, _i64, _vp, _i32, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _vp]),
     "gsx_hip_distill_temp_bytes": (ctypes.c_size_t, [_i64, _i64]),
     "gsx_hip_distill_forward": (_st, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _i32, _f, _vp, _vp, _vp, _vp, _i64, _f,

@@ -464,7 +464,8 @@ void launch_head(const T* x, int64_t x_stride, const BlockMatrix& w, int64_t m, 
 
 // Stretches of rows that the weight's gradient of a narrow layer is split into; 0: the layer is not narrow, or too short for its
 // partial sums to be few beside what is read.
-int64_t weight_stretches(int64_t m, int64_t n, int64_t k) {
+int64_t weight_stretches(int32_t x_type, int32_t grad_type, int64_t m, int64_t n, int64_t k) {
+    if (x_type != grad_type) return 0;  // the kernel is built for rows of one type
     if (n < 4 || k < 4 || n + k > kWeightMostColumns || n > (k <= 128 ? 256 : 128) || k > 256 || m < 8192) return 0;
     const int64_t blocks = ceil_div(m, kBlock);
     return blocks < 256 ? blocks : 256;
@@ -563,9 +564,9 @@ gsx_hip_status gsx_hip_linear_forward(const void* x, int32_t x_type, int64_t x_s
     });
 }
 
-size_t gsx_hip_linear_backward_weight_temp_bytes(int64_t m, int64_t n, int64_t k) {
+size_t gsx_hip_linear_backward_weight_temp_bytes(int32_t x_type, int32_t grad_type, int64_t m, int64_t n, int64_t k) {
     if (!product_sizes(m, n, k) || m > kMostSummands || n == 0 || k == 0) return 0;
-    const int64_t stretches = weight_stretches(m, n, k);
+    const int64_t stretches = weight_stretches(x_type, grad_type, m, n, k);
     if (stretches > 0) return (size_t)(stretches * n * k * 4);
     return (size_t)WeightBlocks(m, n, k).rest + gsx_hip_blocks_matmul_temp_bytes(n, k, m);
 }
@@ -585,7 +586,7 @@ gsx_hip_status gsx_hip_linear_backward_weight(const void* x, int32_t x_type, int
         !aligned_to(grad_out, type_bytes(grad_type)) || !aligned_to(temp, 16))
         return fields_fail(GSX_HIP_ERROR_INVALID_ARGUMENT,
                            "linear backward: rows and workspace must be non-null and aligned to their elements");
-    const int64_t stretches = x_type == grad_type ? weight_stretches(m, n, k) : 0;
+    const int64_t stretches = weight_stretches(x_type, grad_type, m, n, k);
     if (stretches == 0) {
         const WeightBlocks at(m, n, k);
         uint8_t* const base = static_cast<uint8_t*>(temp);

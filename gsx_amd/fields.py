@@ -229,6 +229,7 @@ def linear_backward(x: torch.Tensor, grad_out: torch.Tensor, weight_t: Blocks, g
     lib = _lib.load(require_device=False)
     base, stride = _rows(x, "x")
     grad_base, grad_stride = _rows(grad_out, "grad_out")
+    x_type, grad_type = _type(x.dtype), _type(grad_out.dtype)
     m, k = x.shape
     n = grad_out.shape[1]
     if grad_out.shape[0] != m:
@@ -240,9 +241,9 @@ def linear_backward(x: torch.Tensor, grad_out: torch.Tensor, weight_t: Blocks, g
     def call(handle):
         result = torch.empty((n, k), dtype=torch.float32, device=x.device) if grad_weight is None else grad_weight
         to, to_stride = _rows(result, "grad_weight", torch.float32, (n, k))
-        temp = _temp(lib.gsx_hip_linear_backward_weight_temp_bytes(m, n, k))
-        check(lib.gsx_hip_linear_backward_weight(base, _type(x.dtype), stride, grad_base, _type(grad_out.dtype), grad_stride,
-                                                 m, n, k, to, to_stride, _address(temp), handle), "linear backward")
+        temp = _temp(lib.gsx_hip_linear_backward_weight_temp_bytes(x_type, grad_type, m, n, k))
+        check(lib.gsx_hip_linear_backward_weight(base, x_type, stride, grad_base, grad_type, grad_stride, m, n, k, to,
+                                                 to_stride, _address(temp), handle), "linear backward")
         return result
 
     return grad_x, _run(stream, call)

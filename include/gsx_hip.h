@@ -525,7 +525,7 @@ gsx_hip_status gsx_hip_linear_forward(const void* x, int32_t x_type, int64_t x_s
 /* Gradient of linear_forward's weight for the upstream grad_out [m, n]: grad_weight [n, k] (float32) = blocks(grad_out^T)
  * blocks(x^T)^T, both quantised along the m rows that are summed over (at most 2^27). (The gradient of x is linear_forward of
  * grad_out with the transposed weight's blocks.) */
-size_t gsx_hip_linear_backward_weight_temp_bytes(int64_t m, int64_t n, int64_t k);
+size_t gsx_hip_linear_backward_weight_temp_bytes(int32_t x_type, int32_t grad_type, int64_t m, int64_t n, int64_t k);
 gsx_hip_status gsx_hip_linear_backward_weight(const void* x, int32_t x_type, int64_t x_stride, const void* grad_out,
                                               int32_t grad_type, int64_t grad_stride, int64_t m, int64_t n, int64_t k,
                                               float* grad_weight, int64_t weight_stride, void* temp, hipStream_t stream);

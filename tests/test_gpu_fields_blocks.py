@@ -245,6 +245,24 @@ def test_weight_gradient_of_narrow_layers(m, n, k, kind):
     assert torch.equal(again, dw)
 
 
+def test_weight_gradient_of_narrow_layers_with_two_types():
+    """Rows and gradients of different types take the way of wide layers, whose workspace is larger."""
+    from gsx_amd import _lib, fields
+    m, n, k = 8200, 40, 24
+    lib = _lib.load()
+    codes = {"f32": fields._type(torch.float32), "bf16": fields._type(torch.bfloat16)}
+    mixed = lib.gsx_hip_linear_backward_weight_temp_bytes(codes["bf16"], codes["f32"], m, n, k)
+    assert mixed >= (n + k) * (m + m // 128)
+    x = torch.randn(m, k, device="cuda").bfloat16()
+    dy = torch.randn(m, n, device="cuda")
+    wt = fields.quantize(torch.randn(n, k, device="cuda"), transpose=True)
+    print(f"[case] weight gradient {m} x {n} x {k} of two types", flush=True)
+    _, dw = fields.linear_backward(x, dy, wt)
+    p, q = (_values(*_want_blocks(s.double().cpu().numpy().T), m) for s in (dy, x))
+    want, size = p @ q.T, np.abs(p) @ np.abs(q).T
+    assert (np.abs(dw.double().cpu().numpy() - want) <= size * (m + 8) * 2.0**-23 + np.abs(want) * 2.0**-24).all()
+
+
 def test_weight_gradient_keeps_non_finite_columns_apart():
     from gsx_amd import fields
     x, dy = torch.randn(9000, 20, device="cuda"), torch.randn(9000, 30, device="cuda")
