@@ -357,6 +357,9 @@ __global__ __launch_bounds__(kWeightThreads) void linear_weight_kernel(const T* 
         for (int j = 0; j < KT; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     if (first < last) load(first);
     for (int64_t block = first; block < last; ++block) {
+        // what follows from these is worked out anew for each block: kept, it takes the registers of the rows
+#pragma unroll
+        for (int u = 0; u < kWeightPatches; ++u) asm volatile("" : "+v"(column[u]), "+v"(r0[u]));
         for (int i = threadIdx.x; i < kN + kK; i += kWeightThreads) s_top[i] = 0;
         __syncthreads();  // and the block before has been multiplied
         bool special[kWeightPatches];
