@@ -282,7 +282,7 @@ __device__ inline Stretch stretch_of(const T* z, int64_t length, int tid) {
 }
 
 // Rows that fit the registers of a group: kGroup threads hold kVecs times 16 bytes each. The logits are read once; maximum, sum
-// and gradient come from registers.
+// and gradient come from registers. Memory bounds long rows: 4096 of 65537 bf16, 1.07 GB in 233 us, 4.6 TB/s, a copy's rate.
 template <typename T, int kGroup, int kVecs>
 __global__ __launch_bounds__(kGroup < 256 ? 256 : kGroup) void distill_held_kernel(DistillArgs a, const T* __restrict__ logits,
                                                                                    T* __restrict__ grad) {
@@ -405,7 +405,8 @@ __global__ __launch_bounds__(kSliceThreads) void distill_slices_kernel(DistillAr
     }
 }
 
-// and this one joins them (every workgroup of a row does), writes the loss (the first slice's) and the gradient.
+// and this one joins them (every workgroup of a row does), writes the loss (the first slice's) and the gradient. One row of 131072
+// float32: 3 and 9 us, chains of barriers and loads rather than bytes.
 template <typename T>
 __global__ __launch_bounds__(kSliceThreads) void distill_finish_kernel(DistillArgs a, const T* __restrict__ logits,
                                                                        T* __restrict__ grad, int64_t slices_run) {
@@ -512,9 +513,9 @@ gsx_hip_status distill_check(const DistillArgs& a, const void* logits, int32_t t
 }
 
 // A row is held by a wave (up to 4 KB), by 256 threads (64 KB), 512 (128 KB) or 1024 (256 KB): the smallest group that holds it in
-// 16 vectors a thread, so that two or more rows share a CU and one loads while another is computed (65536 logits of bf16: 512
-// threads take 227 us for 4096 rows, 1024 with half the vectors each 289). Above 32 KB only where there are rows enough for the GPU's 256 CUs; else, and beyond, a row is cut
-// into slices of 16 KB or more, so that some 2048 workgroups share the logits.
+// 16 vectors a thread, so that two or more rows share a CU and one loads while another is computed (4096 rows of 65536 bf16:
+// 512 threads 227 us, 1024 with half the vectors each 289). Above 32 KB only where there are rows enough for the GPU's 256 CUs;
+// else, and beyond, a row is cut into slices of 16 KB or more, so that some 2048 workgroups share the logits.
 struct DistillPlan {
     int group, vecs;        // group = 0: slices
     int64_t slice, slices;  // logits of a slice

@@ -64,7 +64,7 @@ __device__ inline void quantize_block(const RawBlock<T>& raw, v8bf (&y)[4]) {
 // A workgroup of up to 8 waves forms 16 J columns of out for up to 16 rows; wave w takes blocks w, w + waves, ... of k, so
 // that together they read whole stretches of the weight's rows, and the waves' sums are joined through LDS. The rows of x
 // are quantised into LDS first, `span` blocks of k at a time (all of them where they fit), while the weight's first block is
-// on its way.
+// on its way. Reading the weight bounds it: one row, 32768 x 4096, 135 MB in 28.6 us (4.7 TB/s).
 constexpr int kFewRows = 16;
 constexpr int kFewWaves = 8;
 constexpr int kFewBytes = 32768;  // of quantised rows in LDS
@@ -174,7 +174,8 @@ __global__ __launch_bounds__(64 * kFewWaves, 4) void linear_few_kernel(const T* 
 // A wave takes 16 R rows and all (up to 16 TN) columns; x is read once, straight into registers, a block ahead. The weight lies
 // in LDS for the workgroup's four waves, all of it where it fits (kHeadBytes) and is then read once for all the tiles of a
 // workgroup, else a block of 128 k at a time; each wave converts it. The result passes through LDS, 16 rows of a wave at a
-// time, and leaves in whole stretches of its rows.
+// time, and leaves in whole stretches of its rows. 307200 x 128 to 150 columns: 53 us for 171 MB, 3.2 TB/s; quantising and
+// converting in two waves a SIMD is about as long as the memory's time and only partly hides in it.
 constexpr int kHeadThreads = 256;
 constexpr int kHeadBytes = 49152;
 template <int TN>
@@ -301,8 +302,10 @@ __global__ __launch_bounds__(kHeadThreads, 2) void linear_head_kernel(const T* _
 // A workgroup takes a stretch of blocks of 128 rows. Of each it reads dy and x once, finds the columns' maxima, quantises the
 // columns into LDS (a column's 128 values in a row of kWeightPitch bytes, so that a read of 16 columns meets 16 different
 // banks) and multiplies them, 2 x 4 waves with NT x KT tiles of 16 x 16 each; the next block's rows are on their way meanwhile.
-// The stretches' sums are joined by another launch. Memory bounds it: quantised copies of dy^T and x^T, written and read
-// again, would double what it moves.
+// The stretches' sums are joined by another launch. Quantised copies of dy^T and x^T, written and read again, would double what
+// is moved. 307200 x 150 x 128 of bf16: 69 us for 171 MB, 2.5 TB/s. Registers leave one workgroup
+// a CU, whose phases (maxima, quantising, products) stand between barriers: with a second block's rows on their way it is no
+// faster; with 16 waves 4% for 16-bit types, whose float32 form spills.
 constexpr int kWeightThreads = 512;
 constexpr int kWeightPitch = 144;
 constexpr int kWeightPatches = 3;  // of 8 rows by 4 columns a thread holds: up to 96 quads of columns
