@@ -2,7 +2,8 @@
 
 The compute lives in libgsx_hip.so (hand-written HIP kernels behind the C ABI declared in
 include/gsx_hip.h). This package holds the ctypes binding (_lib), a host-side mirror of gsx's
-renderer / loss / optimizer interface (backend) and the seeded benchmark scenes (scenes).
+renderer / loss / optimizer interface (backend), the seeded benchmark scenes (scenes), the operators of
+label fields (fields) and a training step that uses them (label_field).
 """
 import os
 
