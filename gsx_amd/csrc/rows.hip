@@ -5,6 +5,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "common.hpp"
 #include "fields.hpp"
 
@@ -15,16 +17,32 @@ constexpr int kRowUnroll = 4;
 constexpr int kRowTile = kRowThreads * kRowUnroll;  // vectors of V elements a workgroup copies at a time
 constexpr int64_t kRowMostBlocks = 1 << 20;
 
+// V elements at any element's address: rows of odd widths and strides move in wide vectors too (150000 x 385 looked up: 54 us, one
+// element at a time 105).
+template <typename T, int V>
+struct __attribute__((packed, aligned(sizeof(T)))) Span {
+    T v[V];
+};
+
 // What these kernels write is much, written once and read by a later launch: it passes the caches by and leaves what is read in
 // them (1M rows of 64 looked up: 44 us against 60; the gradient of 65536 x 2048: 104 against 158).
 template <typename O, int V>
-__device__ inline void store_past_caches(O* p, const Vec<O, V>& y) {
+__device__ inline void store_past_caches(O* p, const Span<O, V>& y) {
     if constexpr (V * sizeof(O) == 16) {
-        typedef float v4 __attribute__((ext_vector_type(4)));
-        __builtin_nontemporal_store(__builtin_bit_cast(v4, y), reinterpret_cast<v4*>(p));
+        typedef uint32_t Words4 __attribute__((ext_vector_type(4), aligned(4)));
+        typedef uint32_t Words2 __attribute__((ext_vector_type(4), aligned(2)));
+        using Words = std::conditional_t<sizeof(O) == 4, Words4, Words2>;
+        __builtin_nontemporal_store(__builtin_bit_cast(Words, y), reinterpret_cast<Words*>(p));
     } else {
-        *reinterpret_cast<Vec<O, V>*>(p) = y;
+        *reinterpret_cast<Span<O, V>*>(p) = y;
     }
+}
+
+// Column at which vector `vec` of a row begins. A last vector that would end behind the row is moved back into it: its first
+// columns are the vector's before too, and both form the same values for them.
+template <int V>
+__device__ inline int64_t column_at(int64_t vec, int64_t width) {
+    return min(vec * V, width - V);
 }
 
 // A tile is `tile_rows` whole rows of `vecs` vectors, or (vecs > kRowTile) a part of one row. Every id, then every row vector
@@ -33,9 +51,10 @@ __device__ inline void store_past_caches(O* p, const Vec<O, V>& y) {
 template <typename T, typename O, int V>
 __global__ __launch_bounds__(kRowThreads) void lookup_kernel(const T* __restrict__ table, int64_t table_rows,
                                                              int64_t table_stride, const int32_t* __restrict__ ids,
-                                                             int64_t count, int64_t vecs, int tile_rows, int64_t parts,
+                                                             int64_t count, int64_t width, int tile_rows, int64_t parts,
                                                              int64_t tiles, float scale, O* __restrict__ out,
                                                              int64_t out_stride, int* __restrict__ out_of_range) {
+    const int64_t vecs = ceil_div(width, V);
     for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
         const int64_t row0 = tile / parts * tile_rows;
         const int64_t col0 = tile % parts * kRowTile;
@@ -43,25 +62,25 @@ __global__ __launch_bounds__(kRowThreads) void lookup_kernel(const T* __restrict
         const uint32_t work = (uint32_t)min((int64_t)tile_rows, count - row0) * cols;
         int32_t id[kRowUnroll];
         int64_t row[kRowUnroll], col[kRowUnroll];
-        Vec<T, V> x[kRowUnroll];
+        Span<T, V> x[kRowUnroll];
 #pragma unroll
         for (int u = 0; u < kRowUnroll; ++u) {
             const uint32_t e = threadIdx.x + u * kRowThreads;
             row[u] = row0 + e / cols;
-            col[u] = (col0 + e % cols) * V;
+            col[u] = column_at<V>(col0 + e % cols, width);
             id[u] = e < work ? ids[row[u]] : -1;
         }
 #pragma unroll
         for (int u = 0; u < kRowUnroll; ++u) {
             if (id[u] >= 0 && id[u] < table_rows)
-                x[u] = *reinterpret_cast<const Vec<T, V>*>(table + (int64_t)id[u] * table_stride + col[u]);
+                x[u] = *reinterpret_cast<const Span<T, V>*>(table + (int64_t)id[u] * table_stride + col[u]);
         }
 #pragma unroll
         for (int u = 0; u < kRowUnroll; ++u) {
             if (threadIdx.x + u * kRowThreads >= work) continue;
             const bool fits = id[u] >= 0 && id[u] < table_rows;
             if (id[u] >= table_rows && out_of_range != nullptr) *out_of_range = 1;
-            Vec<O, V> y;
+            Span<O, V> y;
 #pragma unroll
             for (int k = 0; k < V; ++k) y.v[k] = from_float<O>(fits ? to_float(x[u].v[k]) * scale : 0.0f);
             store_past_caches<O, V>(out + row[u] * out_stride + col[u], y);
@@ -71,8 +90,9 @@ __global__ __launch_bounds__(kRowThreads) void lookup_kernel(const T* __restrict
 
 // ---- gradient -----------------------------------------------------------------------------------------------------------
 //
-// Few ids: one wave per table row and 64 vectors of V columns reads all ids, 64 at a time, and adds the rows of its id (77 ids,
-// 1001 rows of 385: 3.6 us, near a launch's least).
+// Few ids: one wave per table row and some vectors of V columns reads all ids, 64 at a time, and adds the rows of its id (77 ids,
+// 1001 rows of 385: 3.6 us, near a launch's least). It hardly reads, so its stores stay in the caches as far as they fit (4 ids,
+// 56074 rows of 900: 27 us against 47, 100000 of 1024: 72 either way).
 //
 // Many: the ids are sorted with their positions as values (ids outside the table as table_rows, behind all others), so each
 // table row owns a run of positions. Runs of up to kRunPart rows are summed by one group of lanes each; longer ones in parts of
@@ -84,67 +104,100 @@ __global__ __launch_bounds__(kRowThreads) void lookup_kernel(const T* __restrict
 constexpr int kRunPart = 128;
 
 template <typename T, int V>
-__device__ inline void add_row(float (&sum)[V], const T* __restrict__ p) {
-    const Vec<T, V> x = *reinterpret_cast<const Vec<T, V>*>(p);
+__device__ inline void add_span(float (&sum)[V], const Span<T, V>& x) {
 #pragma unroll
     for (int k = 0; k < V; ++k) sum[k] += to_float(x.v[k]);
 }
 
-template <int V>
-__device__ inline void store_row(float* p, const float (&sum)[V], float scale, bool accumulate) {
-    Vec<float, V> y;
+// Vector `vec` of a row of the result, past the caches or not.
+template <int V, bool kPast>
+__device__ inline void store_row(float* row, int64_t vec, int64_t width, const float (&sum)[V], float scale, bool accumulate) {
+    const int64_t col = column_at<V>(vec, width);
+    float* const p = row + col;
+    if (accumulate && col != vec * V) {  // the vector before adds to the columns they share
+        for (int k = (int)(vec * V - col); k < V; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (i == k) p[k] += sum[i] * scale;
+        return;
+    }
+    Span<float, V> y;
 #pragma unroll
     for (int k = 0; k < V; ++k) y.v[k] = sum[k] * scale;
     if (accumulate) {
-        const Vec<float, V> old = *reinterpret_cast<const Vec<float, V>*>(p);
+        const Span<float, V> old = *reinterpret_cast<const Span<float, V>*>(p);
 #pragma unroll
         for (int k = 0; k < V; ++k) y.v[k] += old.v[k];
     }
-    store_past_caches<float, V>(p, y);
+    if constexpr (kPast) store_past_caches<float, V>(p, y);
+    else *reinterpret_cast<Span<float, V>*>(p) = y;
 }
 
-template <typename T, int V>
+// kTiles times 64 vectors of a row a wave, or (kSplit > 1) 64 vectors a workgroup, whose waves take every kSplit-th 64 ids each.
+template <typename T, int V, int kTiles, int kSplit>
 __global__ __launch_bounds__(kRowThreads) void lookup_scan_kernel(const T* __restrict__ grad, int64_t grad_stride,
                                                                   const int32_t* __restrict__ ids, int64_t count,
                                                                   float scale, float* __restrict__ out,
-                                                                  int64_t table_rows, int64_t out_stride, int64_t vecs,
+                                                                  int64_t table_rows, int64_t out_stride, int64_t width,
                                                                   int accumulate) {
-    const int lane = threadIdx.x & 63;
-    const int64_t parts = ceil_div(vecs, 64);
-    const int64_t waves = table_rows * parts;
-    for (int64_t w = (int64_t)blockIdx.x * (kRowThreads / 64) + threadIdx.x / 64; w < waves;
-         w += (int64_t)gridDim.x * (kRowThreads / 64)) {
+    static_assert(kSplit == 1 || (kSplit == kRowThreads / 64 && kTiles == 1), "a workgroup's waves share one row");
+    constexpr int kAhead = 8 / kTiles;  // rows whose loads are in flight together
+    __shared__ float s_sum[kSplit][kSplit > 1 ? 64 * V : 1];
+    __shared__ int s_any;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x / 64;
+    const int64_t vecs = ceil_div(width, V), parts = ceil_div(vecs, 64 * kTiles);
+    const int64_t works = table_rows * parts, per_block = kRowThreads / 64 / kSplit;
+    for (int64_t w = blockIdx.x * per_block + (kSplit > 1 ? 0 : wave); w < works; w += gridDim.x * per_block) {
         const int64_t v = w / parts;
-        const int64_t vec = w % parts * 64 + lane;
-        float sum[V] = {};
+        const int64_t first = w % parts * 64 * kTiles + lane;
+        float sum[kTiles][V] = {};
         bool any = false;
-        for (int64_t at = 0; at < count; at += 64) {
+        if constexpr (kSplit > 1) {
+            if (threadIdx.x == 0) s_any = 0;
+            __syncthreads();
+        }
+        for (int64_t at = kSplit > 1 ? 64 * wave : 0; at < count; at += 64 * kSplit) {
             const int32_t id = at + lane < count ? ids[at + lane] : -1;
             uint64_t mine = __builtin_amdgcn_ballot_w64(id == v);
-            while (mine != 0) {  // the rows of four ids at a time
+            while (mine != 0) {
                 any = true;
-                int64_t row[4];
-                bool some[4];
+                Span<T, V> x[kAhead][kTiles];
+                bool some[kAhead];
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
+                for (int u = 0; u < kAhead; ++u) {
                     some[u] = mine != 0;
-                    row[u] = at + (some[u] ? __builtin_ctzll(mine) : 0);
+                    if (!some[u]) continue;
+                    const T* const row = grad + (at + __builtin_ctzll(mine)) * grad_stride;
                     mine &= mine - 1;
+#pragma unroll
+                    for (int t = 0; t < kTiles; ++t)
+                        x[u][t] = *reinterpret_cast<const Span<T, V>*>(row + column_at<V>(min(first + 64 * t, vecs - 1), width));
                 }
-                if (vec < vecs) {
-                    Vec<T, V> x[4];
 #pragma unroll
-                    for (int u = 0; u < 4; ++u)
-                        if (some[u]) x[u] = *reinterpret_cast<const Vec<T, V>*>(grad + row[u] * grad_stride + vec * V);
+                for (int u = 0; u < kAhead; ++u)
+                    if (some[u])
 #pragma unroll
-                    for (int u = 0; u < 4; ++u)
-                        if (some[u])
-#pragma unroll
-                            for (int k = 0; k < V; ++k) sum[k] += to_float(x[u].v[k]);
-                }
+                        for (int t = 0; t < kTiles; ++t) add_span<T, V>(sum[t], x[u][t]);
             }
         }
-        if (vec < vecs && (any || accumulate == 0)) store_row<V>(out + v * out_stride + vec * V, sum, scale, accumulate != 0);
+        if constexpr (kSplit > 1) {
+            if (any && lane == 0) s_any = 1;
+#pragma unroll
+            for (int k = 0; k < V; ++k) s_sum[wave][k * 64 + lane] = sum[0][k];
+            __syncthreads();
+            any = s_any != 0;
+            if (wave == 0)
+                for (int i = 1; i < kSplit; ++i)
+#pragma unroll
+                    for (int k = 0; k < V; ++k) sum[0][k] += s_sum[i][k * 64 + lane];
+            __syncthreads();
+            if (wave != 0) continue;
+        }
+        if (!any && accumulate != 0) continue;
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+            if (first + 64 * t < vecs)
+                store_row<V, false>(out + v * out_stride, first + 64 * t, width, sum[t], scale, accumulate != 0);
     }
 }
 
@@ -181,16 +234,15 @@ __device__ inline void sum_run(float (&sum)[V], const T* __restrict__ grad, int6
     constexpr int kAhead = 4;  // rows whose loads are in flight together
     int64_t p = begin;
     for (; p + (kAhead - 1) * (int64_t)step < end; p += kAhead * (int64_t)step) {
-        Vec<T, V> x[kAhead];
+        Span<T, V> x[kAhead];
 #pragma unroll
         for (int u = 0; u < kAhead; ++u)
-            x[u] = *reinterpret_cast<const Vec<T, V>*>(grad + (int64_t)order[p + u * (int64_t)step] * grad_stride + col);
+            x[u] = *reinterpret_cast<const Span<T, V>*>(grad + (int64_t)order[p + u * (int64_t)step] * grad_stride + col);
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u)
-#pragma unroll
-            for (int k = 0; k < V; ++k) sum[k] += to_float(x[u].v[k]);
+        for (int u = 0; u < kAhead; ++u) add_span<T, V>(sum, x[u]);
     }
-    for (; p < end; p += step) add_row<T, V>(sum, grad + (int64_t)order[p] * grad_stride + col);
+    for (; p < end; p += step)
+        add_span<T, V>(sum, *reinterpret_cast<const Span<T, V>*>(grad + (int64_t)order[p] * grad_stride + col));
 }
 
 // A group of `lanes` (a power of two, at most 64) lanes per table row and kTiles times `lanes` vectors of it. The loads of kAhead
@@ -198,9 +250,10 @@ __device__ inline void sum_run(float (&sum)[V], const T* __restrict__ grad, int6
 template <typename T, int V, int kTiles>
 __device__ inline void sum_short_runs(const T* __restrict__ grad, int64_t grad_stride, const uint32_t* __restrict__ order,
                                       const uint32_t* __restrict__ starts, float scale, float* __restrict__ out,
-                                      int64_t table_rows, int64_t out_stride, int64_t vecs, int lanes, int accumulate,
+                                      int64_t table_rows, int64_t out_stride, int64_t width, int lanes, int accumulate,
                                       int64_t block, int64_t blocks) {
     constexpr int kAhead = 8 / kTiles;
+    const int64_t vecs = ceil_div(width, V);
     const int sub = threadIdx.x & (lanes - 1);
     const int64_t parts = ceil_div(vecs, (int64_t)lanes * kTiles);
     const int64_t groups = table_rows * parts, per_block = kRowThreads / lanes;
@@ -211,27 +264,27 @@ __device__ inline void sum_short_runs(const T* __restrict__ grad, int64_t grad_s
         const int64_t first = g % parts * lanes * kTiles + sub;
         float sum[kTiles][V] = {};
         for (int64_t p = begin; p < end; p += kAhead) {
-            Vec<T, V> x[kAhead][kTiles];
+            Span<T, V> x[kAhead][kTiles];
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
                 const T* const row = grad + (int64_t)order[min(p + u, (int64_t)end - 1)] * grad_stride;
 #pragma unroll
                 for (int t = 0; t < kTiles; ++t)
-                    x[u][t] = *reinterpret_cast<const Vec<T, V>*>(row + min(first + t * lanes, vecs - 1) * V);
+                    x[u][t] = *reinterpret_cast<const Span<T, V>*>(row + column_at<V>(min(first + t * lanes, vecs - 1), width));
             }
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
-                if (p + u >= end) continue;
+                const bool some = p + u < end;  // a zero is added where there is no row: a sum is never -0
 #pragma unroll
                 for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-                    for (int k = 0; k < V; ++k) sum[t][k] += to_float(x[u][t].v[k]);
+                    for (int k = 0; k < V; ++k) sum[t][k] += some ? to_float(x[u][t].v[k]) : 0.0f;
             }
         }
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) {
             const int64_t vec = first + t * lanes;
-            if (vec < vecs) store_row<V>(out + v * out_stride + vec * V, sum[t], scale, accumulate != 0);
+            if (vec < vecs) store_row<V, true>(out + v * out_stride, vec, width, sum[t], scale, accumulate != 0);
         }
     }
 }
@@ -242,8 +295,9 @@ __device__ inline void sum_short_runs(const T* __restrict__ grad, int64_t grad_s
 template <typename T, int V, typename KeyT>
 __device__ inline void sum_long_parts(const T* __restrict__ grad, int64_t grad_stride, const uint32_t* __restrict__ order,
                                       const KeyT* __restrict__ keys, const uint32_t* __restrict__ starts, int64_t count,
-                                      int64_t table_rows, int64_t vecs, int lanes, float* __restrict__ partial, int64_t block,
+                                      int64_t table_rows, int64_t width, int lanes, float* __restrict__ partial, int64_t block,
                                       int64_t blocks) {
+    const int64_t vecs = ceil_div(width, V);
     const int64_t tiles = ceil_div(vecs, lanes);
     const int64_t waves = ceil_div(count, kRunPart) * tiles;
     const int lane = threadIdx.x & 63;
@@ -262,7 +316,7 @@ __device__ inline void sum_long_parts(const T* __restrict__ grad, int64_t grad_s
             float sum[V] = {};
             const uint32_t from = (uint32_t)max((int64_t)begin, first), to = (uint32_t)min((int64_t)end, last + 1);
             if (vec < vecs)
-                sum_run<T, V>(sum, grad, grad_stride, order, from + lane / lanes, to, 64 / lanes, vec * V);
+                sum_run<T, V>(sum, grad, grad_stride, order, from + lane / lanes, to, 64 / lanes, column_at<V>(vec, width));
             for (int off = lanes; off < 64; off <<= 1) {
 #pragma unroll
                 for (int k = 0; k < V; ++k) sum[k] += __shfl_xor(sum[k], off, 64);
@@ -284,14 +338,14 @@ __global__ __launch_bounds__(kRowThreads) void lookup_runs_kernel(const T* __res
                                                                   const KeyT* __restrict__ keys,
                                                                   const uint32_t* __restrict__ starts, int64_t count,
                                                                   float scale, float* __restrict__ out, int64_t table_rows,
-                                                                  int64_t out_stride, int64_t vecs, int lanes,
+                                                                  int64_t out_stride, int64_t width, int lanes,
                                                                   int accumulate, float* __restrict__ partial,
                                                                   int64_t part_blocks) {
     if ((int64_t)blockIdx.x < part_blocks) {
-        sum_long_parts<T, V, KeyT>(grad, grad_stride, order, keys, starts, count, table_rows, vecs, lanes, partial, blockIdx.x,
+        sum_long_parts<T, V, KeyT>(grad, grad_stride, order, keys, starts, count, table_rows, width, lanes, partial, blockIdx.x,
                                    part_blocks);
     } else {
-        sum_short_runs<T, V, kTiles>(grad, grad_stride, order, starts, scale, out, table_rows, out_stride, vecs, lanes,
+        sum_short_runs<T, V, kTiles>(grad, grad_stride, order, starts, scale, out, table_rows, out_stride, width, lanes,
                                      accumulate, blockIdx.x - part_blocks, gridDim.x - part_blocks);
     }
 }
@@ -301,11 +355,12 @@ __global__ __launch_bounds__(kRowThreads) void lookup_runs_kernel(const T* __res
 template <int V, typename KeyT>
 __global__ __launch_bounds__(kRowThreads) void lookup_join_kernel(const KeyT* __restrict__ keys,
                                                                   const uint32_t* __restrict__ starts, int64_t count,
-                                                                  int64_t table_rows, int64_t vecs, int lanes,
+                                                                  int64_t table_rows, int64_t width, int lanes,
                                                                   const float* __restrict__ partial, float scale,
                                                                   float* __restrict__ out, int64_t out_stride,
                                                                   int accumulate) {
     __shared__ float s_sum[kRowThreads * V];
+    const int64_t vecs = ceil_div(width, V);
     const int64_t tiles = ceil_div(vecs, lanes);
     const int64_t blocks = ceil_div(count, kRunPart) * tiles;
     for (int64_t b = blockIdx.x; b < blocks; b += gridDim.x) {
@@ -345,7 +400,7 @@ __global__ __launch_bounds__(kRowThreads) void lookup_join_kernel(const KeyT* __
             for (int g = 1; g < groups; ++g)
 #pragma unroll
                 for (int k = 0; k < V; ++k) sum[k] += s_sum[(g * lanes + threadIdx.x) * V + k];
-            store_row<V>(out + key * out_stride + vec * V, sum, scale, accumulate != 0);
+            store_row<V, true>(out + key * out_stride, vec, width, sum, scale, accumulate != 0);
         }
         __syncthreads();
     }
@@ -357,38 +412,28 @@ using namespace gsx_amd;
 
 namespace {
 
-// Elements a thread moves at once: 16 bytes of the wider type where bases, strides and width allow it, else half of that, ...
-int lookup_vector(const void* a, int32_t a_type, int64_t a_stride, const void* b, int32_t b_type, int64_t b_stride,
-                  int64_t width) {
-    const int64_t ab = type_bytes(a_type), bb = type_bytes(b_type);
-    for (int64_t v = 16 / (ab > bb ? ab : bb); v > 1; v /= 2) {
-        if (width % v == 0 && a_stride % v == 0 && b_stride % v == 0 && aligned_to(a, v * ab) && aligned_to(b, v * bb))
-            return (int)v;
-    }
-    return 1;
-}
-
 template <typename T, typename O, int V>
 gsx_hip_status launch_lookup(const void* table, int64_t table_rows, int64_t table_stride, const int32_t* ids,
                              int64_t count, int64_t width, float scale, void* out, int64_t out_stride, int* flag,
                              hipStream_t stream) {
-    const int64_t vecs = width / V;
+    const int64_t vecs = ceil_div(width, V);
     const int tile_rows = vecs >= kRowTile ? 1 : (int)(kRowTile / vecs);
     const int64_t parts = ceil_div(vecs, kRowTile);
     const int64_t tiles = ceil_div(count, tile_rows) * parts;
     hipLaunchKernelGGL((lookup_kernel<T, O, V>), dim3((unsigned)(tiles < kRowMostBlocks ? tiles : kRowMostBlocks)),
                        dim3(kRowThreads), 0, stream, static_cast<const T*>(table), table_rows, table_stride, ids, count,
-                       vecs, tile_rows, parts, tiles, scale, static_cast<O*>(out), out_stride, flag);
+                       width, tile_rows, parts, tiles, scale, static_cast<O*>(out), out_stride, flag);
     return fields_launched("lookup launch");
 }
 
-// Few ids take the scan: one launch instead of ten, but every wave reads every id. Up to 2048 ids on 1000 rows 10 to 13 us against
-// 30 to 36; on 65536 rows of 64, 1024 ids 30 us against 38, 2048 ids 48 against 39; on 65536 rows of 2048, 256 ids 96 against
-// 126, 512 ids 139 against 127.
+// Few ids take the scan: one launch instead of ten, but every wave reads every id. More than 256 are shared by a workgroup's waves
+// (2048 ids on 1000 rows 11 us against 36 by sorting, all of them on one row 35) while there are no more than some 16 000
+// waves' rows (2048 ids on 16384 rows of 64 23 us against 35, on 65536 80
+// against 42).
+constexpr int64_t kScanSplit = 256;  // ids above which a workgroup's waves share them
+constexpr int64_t kScanLong = 8192;  // waves that fill the GPU: from there on a wave takes 256 vectors of a row
 bool takes_scan(int64_t count, int64_t table_rows, int64_t width) {
-    if (count <= 256) return true;
-    const int64_t waves = table_rows * ceil_div(width, 256);
-    return count <= 2048 && waves <= 1500000 / ceil_div(count, 64);
+    return count <= kScanSplit || (count <= 2048 && table_rows * ceil_div(width, 256) <= 16384);
 }
 
 unsigned rows_grid(int64_t blocks) { return (unsigned)(blocks < kRowMostBlocks ? blocks : kRowMostBlocks); }
@@ -412,18 +457,10 @@ struct SortedIds {
         order = take(count * 4);
         sort = take((int64_t)tile_sort_temp_bytes(count));
         starts = take((table_rows + 1) * 4);
-        partial = take(ceil_div(count, kRunPart) * 2 * width * 4);
+        partial = take(ceil_div(count, kRunPart) * 2 * ceil_div(width, 4) * 16);
         bytes = at;
     }
 };
-
-// Columns a lane sums at once: four where both sides' rows allow vector accesses.
-int grad_vector(const void* grad, int32_t type, int64_t grad_stride, const float* out, int64_t out_stride, int64_t width) {
-    return width % 4 == 0 && grad_stride % 4 == 0 && out_stride % 4 == 0 && aligned_to(grad, 4 * type_bytes(type)) &&
-                   aligned_to(out, 16)
-               ? 4
-               : 1;
-}
 
 template <typename T, int V, typename KeyT>
 gsx_hip_status sorted_backward(const T* grad, int64_t grad_stride, const int32_t* ids, int64_t count, int64_t width,
@@ -448,7 +485,7 @@ gsx_hip_status sorted_backward(const T* grad, int64_t grad_stride, const int32_t
     if (st != GSX_HIP_SUCCESS) return fields_fail(st, "lookup backward: sort");
     hipLaunchKernelGGL((lookup_starts_kernel<KeyT>), dim3(rows_grid(ceil_div(table_rows + 1, kRowThreads))),
                        dim3(kRowThreads), 0, stream, sorted, count, table_rows, starts);
-    const int64_t vecs = width / V;
+    const int64_t vecs = ceil_div(width, V);
     int lanes = 1;
     while (lanes < vecs && lanes < 64) lanes *= 2;
     // a wave takes 256 vectors of a row where the rows are that long, else its lanes share rows
@@ -456,11 +493,19 @@ gsx_hip_status sorted_backward(const T* grad, int64_t grad_stride, const int32_t
     const int64_t parts = ceil_div(count, kRunPart) * ceil_div(vecs, lanes);
     const unsigned part_blocks = rows_grid(ceil_div(parts, kRowThreads / 64));
     const unsigned run_blocks = rows_grid(ceil_div(groups, kRowThreads / lanes));
-    hipLaunchKernelGGL((vecs > 64 ? lookup_runs_kernel<T, V, 4, KeyT> : lookup_runs_kernel<T, V, 1, KeyT>),
-                       dim3(part_blocks + run_blocks), dim3(kRowThreads), 0, stream, grad, grad_stride, order, sorted, starts,
-                       count, scale, out, table_rows, out_stride, vecs, lanes, accumulate, partial, (int64_t)part_blocks);
+    const auto runs = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(part_blocks + run_blocks), dim3(kRowThreads), 0, stream, grad, grad_stride, order,
+                           sorted, starts, count, scale, out, table_rows, out_stride, width, lanes, accumulate, partial,
+                           (int64_t)part_blocks);
+    };
+    if constexpr (V > 1) {
+        if (vecs > 64) runs(lookup_runs_kernel<T, V, 4, KeyT>);
+        else runs(lookup_runs_kernel<T, V, 1, KeyT>);
+    } else {
+        runs(lookup_runs_kernel<T, V, 1, KeyT>);  // rows of up to three columns
+    }
     hipLaunchKernelGGL((lookup_join_kernel<V, KeyT>), dim3(rows_grid(parts)), dim3(kRowThreads), 0, stream, sorted, starts,
-                       count, table_rows, vecs, lanes, partial, scale, out, out_stride, accumulate);
+                       count, table_rows, width, lanes, partial, scale, out, out_stride, accumulate);
     return fields_launched("lookup backward launch");
 }
 
@@ -481,7 +526,6 @@ gsx_hip_status gsx_hip_lookup_forward(const void* table, int32_t table_type, int
         return fields_fail(GSX_HIP_ERROR_INVALID_ARGUMENT, "lookup: null pointer");
     if (!aligned_to(table, type_bytes(table_type)) || !aligned_to(out, type_bytes(out_type)) || !aligned_to(ids, 4))
         return fields_fail(GSX_HIP_ERROR_INVALID_ARGUMENT, "lookup: pointers must be aligned to their elements");
-    const int v = lookup_vector(table, table_type, table_stride, out, out_type, out_stride, width);
     return with_type(table_type, [&](auto t) {
         return with_type(out_type, [&](auto o) {
             using T = decltype(t);
@@ -491,11 +535,12 @@ gsx_hip_status gsx_hip_lookup_forward(const void* table, int32_t table_type, int
                 return launch(table, table_rows, table_stride, ids, count, width, scale, out, out_stride,
                               out_has_out_of_range, stream);
             };
+            // as many elements a thread as 16 bytes of the wider type hold, fewer in rows shorter than that
             if constexpr (kMost >= 8) {
-                if (v == 8) return go(launch_lookup<T, O, 8>);
+                if (width >= 8) return go(launch_lookup<T, O, 8>);
             }
-            if (v == 4) return go(launch_lookup<T, O, 4>);
-            if (v == 2) return go(launch_lookup<T, O, 2>);
+            if (width >= 4) return go(launch_lookup<T, O, 4>);
+            if (width >= 2) return go(launch_lookup<T, O, 2>);
             return go(launch_lookup<T, O, 1>);
         });
     });
@@ -522,14 +567,23 @@ gsx_hip_status gsx_hip_lookup_backward(const void* grad_out, int32_t grad_type, 
         return fields_fail(GSX_HIP_ERROR_INVALID_ARGUMENT, "lookup backward: null pointer");
     if (!aligned_to(grad_out, type_bytes(grad_type)) || !aligned_to(grad_table, 4) || !aligned_to(ids, 4))
         return fields_fail(GSX_HIP_ERROR_INVALID_ARGUMENT, "lookup backward: pointers must be aligned to their elements");
-    const int vector = grad_vector(grad_out, grad_type, grad_stride, grad_table, table_stride, width);
+    const bool wide = width >= 4;  // columns a lane sums at once: four, or one of short rows
     if (takes_scan(count, table_rows, width)) {
         return with_type(grad_type, [&](auto t) {
             using T = decltype(t);
-            const int64_t blocks = ceil_div(table_rows * ceil_div(width / vector, 64), kRowThreads / 64);
-            hipLaunchKernelGGL((vector == 4 ? lookup_scan_kernel<T, 4> : lookup_scan_kernel<T, 1>), dim3(rows_grid(blocks)),
-                               dim3(kRowThreads), 0, stream, static_cast<const T*>(grad_out), grad_stride, ids, count,
-                               scale, grad_table, table_rows, table_stride, width / vector, accumulate);
+            const int64_t vecs = ceil_div(width, wide ? 4 : 1);
+            const auto go = [&](auto kernel, int64_t blocks) {
+                hipLaunchKernelGGL(kernel, dim3(rows_grid(blocks)), dim3(kRowThreads), 0, stream,
+                                   static_cast<const T*>(grad_out), grad_stride, ids, count, scale, grad_table, table_rows,
+                                   table_stride, width, accumulate);
+            };
+            const int64_t waves = table_rows * ceil_div(vecs, 64), long_waves = table_rows * ceil_div(vecs, 256);
+            if (count > kScanSplit)
+                go(wide ? lookup_scan_kernel<T, 4, 1, 4> : lookup_scan_kernel<T, 1, 1, 4>, waves);
+            else if (vecs > 64 && long_waves >= kScanLong)
+                go(lookup_scan_kernel<T, 4, 4, 1>, ceil_div(long_waves, 4));
+            else
+                go(wide ? lookup_scan_kernel<T, 4, 1, 1> : lookup_scan_kernel<T, 1, 1, 1>, ceil_div(waves, 4));
             return fields_launched("lookup backward launch");
         });
     }
@@ -539,12 +593,12 @@ gsx_hip_status gsx_hip_lookup_backward(const void* grad_out, int32_t grad_type, 
         using T = decltype(t);
         const T* grad = static_cast<const T*>(grad_out);
         if (SortedIds::narrow(table_rows)) {
-            return vector == 4 ? sorted_backward<T, 4, uint16_t>(grad, grad_stride, ids, count, width, scale, grad_table,
+            return wide ? sorted_backward<T, 4, uint16_t>(grad, grad_stride, ids, count, width, scale, grad_table,
                                                                  table_rows, table_stride, accumulate, temp, stream)
                                : sorted_backward<T, 1, uint16_t>(grad, grad_stride, ids, count, width, scale, grad_table,
                                                                  table_rows, table_stride, accumulate, temp, stream);
         }
-        return vector == 4 ? sorted_backward<T, 4, uint32_t>(grad, grad_stride, ids, count, width, scale, grad_table,
+        return wide ? sorted_backward<T, 4, uint32_t>(grad, grad_stride, ids, count, width, scale, grad_table,
                                                              table_rows, table_stride, accumulate, temp, stream)
                            : sorted_backward<T, 1, uint32_t>(grad, grad_stride, ids, count, width, scale, grad_table,
                                                              table_rows, table_stride, accumulate, temp, stream);

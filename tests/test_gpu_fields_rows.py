@@ -212,3 +212,31 @@ def test_lookup_on_another_stream():
     grad = fields.lookup_backward(got, ids, 1000, stream=s)
     s.synchronize()
     assert torch.equal(got, want) and torch.equal(grad, grad_want)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("count,rows,width", [(1, 3, 5), (200, 50, 7), (200, 20000, 259), (700, 300, 6), (2048, 1, 257),
+                                              (3000, 40, 9), (9000, 3, 259), (9000, 3, 2)])
+def test_gradient_of_odd_widths_is_added_to_a_table(count, rows, width, kind):
+    """The last vector of a row of an odd width overlaps the one before: their common columns are added once. A sum of c terms in
+    float32 is within (c + 3) 2^-24 of the sum of its terms' magnitudes, the table's value among them."""
+    from gsx_amd import fields
+    g = torch.Generator("cuda").manual_seed(count + width)
+    dtype = {"f32": torch.float32, "bf16": torch.bfloat16}[kind]
+    grad = torch.randn(count, width + 1, device="cuda", generator=g).to(dtype)[:, 1:]
+    ids = torch.randint(-1, rows, (count,), device="cuda", generator=g, dtype=torch.int32)
+    base = torch.randn(rows, width + 3, device="cuda", generator=g)
+    before = base.clone()
+    print(f"[case] gradient of {count} ids added to {rows} x {width} {kind}", flush=True)
+    fields.lookup_backward(grad, ids, rows, 0.5, grad_table=base[:, 2: width + 2], accumulate=True)
+    i, x = ids.cpu().numpy(), grad.double().cpu().numpy()
+    want, size = (np.zeros((rows, width)) for _ in range(2))
+    for v in np.unique(i[i >= 0]):
+        want[v], size[v] = 0.5 * x[i == v].sum(0), 0.5 * np.abs(x[i == v]).sum(0)
+    old = before[:, 2: width + 2].double().cpu().numpy()
+    got = base[:, 2: width + 2].double().cpu().numpy()
+    assert (np.abs(got - (old + want)) <= (count + 3) * 2.0**-24 * (size + np.abs(old))).all()
+    outside = [0, 1, width + 2]
+    assert torch.equal(base[:, outside], before[:, outside])
+    plain = fields.lookup_backward(grad, ids, rows, 0.5)
+    assert (np.abs(plain.double().cpu().numpy() - want) <= (count + 3) * 2.0**-24 * size).all()
