@@ -123,7 +123,7 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_columns_kernel(const T
 // straight from memory. A row is eight chunks of 16 bytes; chunk c lies at place c ^ swizzle(row), and a lane of group g = lane /
 // 16 reads chunks g and g + 4: no two lanes of a read meet in a bank (with chunks 2 g and 2 g + 1 each read takes twice as long).
 //
-// 8192^3 with a 16-bit result: 500 us, 2.2 PFLOP/s of the 3.2 that a library's 8-bit product reaches; float32: 970 us, 1.1 of
+// 8192^3 with a 16-bit result: 480 us, 2.3 PFLOP/s of the 3.2 that a library's 8-bit product reaches; float32: 1000 us, 1.1 of
 // bfloat16's 1.6. A workgroup's LDS leaves one to a CU, two waves a SIMD: half of the time the matrix instructions wait, for LDS
 // reads, conversions (float32) and the barrier between blocks.
 //
@@ -155,6 +155,18 @@ __device__ inline ProductTile product_tile(int64_t t, int64_t total, int64_t til
     return r;
 }
 
+// Begins a wave's loads of a whole block, which go straight to LDS.
+template <int kLoads, int BM, int kWaves>
+__device__ __forceinline__ void load_block(uint8_t* __restrict__ to, const uint8_t* a_from, const uint8_t* b_from,
+                                           const uint32_t (&offset)[kLoads], int wave) {
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+        const uint8_t* const base = 8 * (u * kWaves + wave) < BM ? a_from : b_from;
+        __builtin_amdgcn_global_load_lds((GlobalPtr)(base + (uint64_t)offset[u] * 16),
+                                         (LdsPtr)(to + (u * kWaves + wave) * 1024), 16, 0, 0);
+    }
+}
+
 // One block of k: `next`'s loads are begun (BASES: where a's and b's rows of that block start), then `now`, which they do not
 // touch, is multiplied. __restrict__ says so to the compiler, which otherwise waits for the loads before it reads LDS.
 template <int TM, int TN, int WM, int WN, bool kEight, int kLoads>
@@ -163,14 +175,7 @@ __device__ __forceinline__ void product_step(const uint8_t* __restrict__ now, co
                                              const uint8_t* b_next, const uint32_t (&offset)[kLoads], int lane, int wave,
                                              v4f (&acc)[TM][TN]) {
     constexpr int BM = 16 * TM * WM, kWaves = WM * WN;
-    if (load) {
-#pragma unroll
-        for (int u = 0; u < kLoads; ++u) {
-            const uint8_t* const base = 8 * (u * kWaves + wave) < BM ? a_next : b_next;
-            __builtin_amdgcn_global_load_lds((GlobalPtr)(base + (uint64_t)offset[u] * 16),
-                                             (LdsPtr)(next + (u * kWaves + wave) * 1024), 16, 0, 0);
-        }
-    }
+    if (load) load_block<kLoads, BM, kWaves>(next, a_next, b_next, offset, wave);
     const int wm = wave / WN, wn = wave % WN;
     const uint8_t* const s_a = now;
     const uint8_t* const s_b = now + BM * kBlock;
@@ -239,6 +244,8 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(BlockMatrix a, Bl
                                                                float* __restrict__ partial) {
     constexpr int kThreads = 64 * WM * WN, BM = 16 * TM * WM, BN = 16 * TN * WN;
     constexpr int kRows = BM + BN, kLoads = kRows * 8 / kThreads, kWaves = WM * WN;
+    constexpr int kStaged = kLoads % 4 == 0 ? 4 : 2;
+    static_assert(kLoads % kStaged == 0, "whole groups of loads");
     static_assert(kRows * 8 % kThreads == 0 && BM % (8 * kWaves) == 0, "whole loads, each of one operand");
     __shared__ __attribute__((aligned(1024))) uint8_t s_values[2][kRows * kBlock];
     __shared__ uint32_t s_exponents[2][kRows];
@@ -259,16 +266,23 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(BlockMatrix a, Bl
             offset[u] = row < BM ? min(row, most_a) * a_step + (uint32_t)((lane & 7) ^ swizzle_a(row))
                                  : min(row - BM, most_b) * b_step + (uint32_t)((lane & 7) ^ swizzle_b<TN>(row - BM));
         }
-        // a block through registers, with zeros past the last k: the first one, and a cut last one
+        // a cut block, the last one: through registers, four loads at a time, with zeros past the last k
         const auto stage = [&](int64_t kb) {
             const int64_t k0 = kb * kBlock;
 #pragma unroll 1
-            for (int u = wave; u < kRows / 8; u += kWaves) {
-                const int row = 8 * u + lane / 8;
-                const uint8_t* const p = row < BM ? a_tile + min(row, most_a) * a.values_stride
-                                                  : b_tile + min(row - BM, most_b) * b.values_stride;
-                const int chunk = (lane & 7) ^ (row < BM ? swizzle_a(row) : swizzle_b<TN>(row - BM));
-                *reinterpret_cast<v4i*>(s_values[kb & 1] + u * 1024 + lane * 16) = load_values(p, k0 + chunk * 16, k);
+            for (int u0 = 0; u0 < kLoads; u0 += kStaged) {
+                v4i x[kStaged];
+#pragma unroll
+                for (int u = 0; u < kStaged; ++u) {
+                    const int row = 8 * ((u0 + u) * kWaves + wave) + lane / 8;
+                    const uint8_t* const p = row < BM ? a_tile + min(row, most_a) * a.values_stride
+                                                      : b_tile + min(row - BM, most_b) * b.values_stride;
+                    const int chunk = (lane & 7) ^ (row < BM ? swizzle_a(row) : swizzle_b<TN>(row - BM));
+                    x[u] = load_values(p, k0 + chunk * 16, k);
+                }
+#pragma unroll
+                for (int u = 0; u < kStaged; ++u)
+                    *reinterpret_cast<v4i*>(s_values[kb & 1] + ((u0 + u) * kWaves + wave) * 1024 + lane * 16) = x[u];
             }
         };
         // four blocks' exponents of a row are one word; thread r brings row r's
@@ -286,7 +300,11 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(BlockMatrix a, Bl
 #pragma unroll
             for (int j = 0; j < TN; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
         if (tile.first < tile.last) {
-            stage(tile.first);
+            if ((tile.first + 1) * kBlock <= k)
+                load_block<kLoads, BM, kWaves>(s_values[tile.first & 1], a_tile + tile.first * kBlock,
+                                               b_tile + tile.first * kBlock, offset, wave);
+            else
+                stage(tile.first);
             stage_exponents(tile.first / 4);
         }
         for (int64_t kb = tile.first; kb < tile.last; ++kb) {
@@ -392,7 +410,7 @@ gsx_hip_status join_products(const float* partial, int64_t m, int64_t n, int64_t
 namespace {
 
 // Tiles and splits of a product by its sizes alone. Tiles of 256 and 192 run one to a CU, of 128 two; the edge is the one whose
-// whole rounds of tiles cover the product with the least work, the larger one where two do (gradients of 4001 x 4100 x 2050: 217
+// whole rounds of tiles cover the product with the least work, the larger one where two do (gradients of 4001 x 4100 x 2050: 205
 // us with 231 and 242 tiles of 192, 282 with tiles of 128, 544 and 561 for 512 places). What fills less than half a round is
 // split over k, four blocks or more to a part.
 struct ProductPlan {
@@ -402,7 +420,7 @@ struct ProductPlan {
 };
 
 // Products of at least this many summands with a 16-bit result go through the 8-bit instructions: below, memory bounds them and
-// nothing is gained; 8192^3 takes 500 us instead of 970.
+// nothing is gained; 8192^3 takes 480 us instead of 1000.
 constexpr int64_t kEightLeast = 1024;
 constexpr int64_t kSplitMostBlocks = 512;  // blocks of k after which a float sum starts anew
 

@@ -262,18 +262,15 @@ struct BlockMatrix {
     int64_t values_stride, exponents_stride;
 };
 
-// 16 bytes of a row at column k; columns from `cols` on read as zero.
+// 16 bytes of a row at column k (a multiple of 16); columns from `cols` on read as zero. No branches, so that several loads may be
+// in flight.
 __device__ inline v4i load_values(const uint8_t* row, int64_t k, int64_t cols) {
-    v4i v = {0, 0, 0, 0};
-    if (k >= cols) return v;
-    v = *reinterpret_cast<const v4i*>(row + k);
-    const int64_t left = cols - k;
-    if (left < 16) {
+    v4i v = *reinterpret_cast<const v4i*>(row + min(k, (cols - 1) & ~(int64_t)15));
+    const int left = (int)max(min(cols - k, (int64_t)16), (int64_t)0);
 #pragma unroll
-        for (int d = 0; d < 4; ++d) {
-            const int64_t bytes = left - 4 * d;
-            if (bytes < 4) v[d] = bytes <= 0 ? 0 : v[d] & (int)((1u << (8 * bytes)) - 1u);
-        }
+    for (int d = 0; d < 4; ++d) {
+        const int bits = max(min(8 * (left - 4 * d), 32), 0);
+        v[d] &= (int)(0xffffffffull >> (32 - bits));
     }
     return v;
 }
