@@ -275,21 +275,25 @@ __device__ inline v4i load_values(const uint8_t* row, int64_t k, int64_t cols) {
     return v;
 }
 
-// 4 TN consecutive columns from `col` on of a row of n.
+// 4 TN consecutive columns from `col` on of a row of n, 16 bytes at a time where TN allows it.
 template <int TN, typename O>
 __device__ inline void store_columns(O* __restrict__ row, int64_t col, int64_t n, const v4f (&x)[TN]) {
+    constexpr int kQuads = sizeof(O) == 2 && TN % 2 == 0 ? 2 : 1, kCols = 4 * kQuads;
+    struct __attribute__((packed, aligned(sizeof(O)))) Piece {
+        O v[kCols];
+    };
 #pragma unroll
-    for (int j = 0; j < TN; ++j) {
+    for (int j = 0; j < TN; j += kQuads) {
         const int64_t c = col + 4 * j;
-        if (c + 4 <= n) {
-            Quad<O> q;
+        if (c + kCols <= n) {
+            Piece q;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) q.v[i] = from_float<O>(x[j][i]);
-            *reinterpret_cast<Quad<O>*>(row + c) = q;
+            for (int i = 0; i < kCols; ++i) q.v[i] = from_float<O>(x[j + i / 4][i % 4]);
+            *reinterpret_cast<Piece*>(row + c) = q;
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (c + i < n) row[c + i] = from_float<O>(x[j][i]);
+            for (int i = 0; i < kCols; ++i)
+                if (c + i < n) row[c + i] = from_float<O>(x[j + i / 4][i % 4]);
         }
     }
 }
