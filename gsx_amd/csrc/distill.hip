@@ -50,10 +50,10 @@ __device__ inline MaxSum join(MaxSum a, MaxSum b, float scale2) {
     return r;
 }
 
-// A group of kGroup threads works on one row: a wave of its own, or the whole workgroup.
+// A group of kGroup threads works on one row: 16 lanes of a wave, a wave of its own, or the whole workgroup.
 template <int kGroup>
 __device__ inline void group_sync() {
-    if constexpr (kGroup == 64) wave_lds_sync();
+    if constexpr (kGroup <= 64) wave_lds_sync();
     else __syncthreads();
 }
 
@@ -70,6 +70,12 @@ __device__ inline float wave_reduce_max(float v) {  // lane moves as in wave_red
 
 template <int kGroup>
 __device__ inline float sum_of_group(float v, float* s_wave) {
+    if constexpr (kGroup == 16) {
+        v += dpp_move<0xb1, 0xf>(v);
+        v += dpp_move<0x4e, 0xf>(v);
+        v += dpp_move<0x141, 0xf>(v);
+        return v + dpp_move<0x140, 0xf>(v);
+    }
     v = wave_reduce_sum(v);
     if constexpr (kGroup == 64) return v;
     const int wave = threadIdx.x / 64;
@@ -84,6 +90,12 @@ __device__ inline float sum_of_group(float v, float* s_wave) {
 
 template <int kGroup>
 __device__ inline float max_of_group(float v, float* s_wave) {
+    if constexpr (kGroup == 16) {
+        v = fmaxf(v, dpp_move<0xb1, 0xf>(v));
+        v = fmaxf(v, dpp_move<0x4e, 0xf>(v));
+        v = fmaxf(v, dpp_move<0x141, 0xf>(v));
+        return fmaxf(v, dpp_move<0x140, 0xf>(v));
+    }
     v = wave_reduce_max(v);
     if constexpr (kGroup == 64) return v;
     const int wave = threadIdx.x / 64;
@@ -103,7 +115,7 @@ struct Teacher {
     float* t;
     float* p;
     float* z;
-    uint16_t* slot;      // of a wave's row: an entry that names each logit
+    uint16_t* slot;      // of a row of a wave or less: an entry that names each logit
     bool unique;         // no id is known to be named twice
     float max, log_sum;  // log p_k = (t_k - max) / T - log_sum
     bool any;            // an entry counts
@@ -146,14 +158,15 @@ __device__ inline void teacher_finish(const DistillArgs& a, int tid, float* s_wa
     r.log_sum = logf(sum);
     for (int k = tid; k < a.top; k += kGroup) r.p[k] = r.any ? r.p[k] / sum : 0.0f;
     r.unique = false;
-    if constexpr (kGroup == 64) {  // whoever wrote a slot last finds itself there; an id named twice leaves somebody else
+    if constexpr (kGroup <= 64) {  // whoever wrote a slot last finds itself there; an id named twice leaves somebody else
         if (want_unique) {
             for (int k = tid; k < a.top; k += kGroup)
                 if (r.id[k] >= 0) r.slot[r.id[k]] = (uint16_t)k;
             group_sync<kGroup>();
             bool twice = false;
             for (int k = tid; k < a.top; k += kGroup) twice |= r.id[k] >= 0 && r.slot[r.id[k]] != (uint16_t)k;
-            r.unique = wave_none(twice);
+            if constexpr (kGroup == 64) r.unique = wave_none(twice);
+            else r.unique = (__builtin_amdgcn_ballot_w64(twice) >> (threadIdx.x & 48) & 0xffffu) == 0;
         }
     }
     group_sync<kGroup>();
@@ -282,7 +295,7 @@ __device__ inline Stretch stretch_of(const T* z, int64_t length, int tid) {
 }
 
 // Rows that fit the registers of a group: kGroup threads hold kVecs times 16 bytes each. The logits are read once; maximum, sum
-// and gradient come from registers. Memory bounds long rows: 4096 of 65537 bf16, 1.07 GB in 233 us, 4.6 TB/s, a copy's rate.
+// and gradient come from registers. Instructions bound short rows (307200 of 150 bf16: 88 us, 2.3 TB/s), memory bounds long rows: 4096 of 65537 bf16, 1.07 GB in 233 us, 4.6 TB/s, a copy's rate.
 template <typename T, int kGroup, int kVecs>
 __global__ __launch_bounds__(kGroup < 256 ? 256 : kGroup) void distill_held_kernel(DistillArgs a, const T* __restrict__ logits,
                                                                                    T* __restrict__ grad) {
@@ -296,7 +309,7 @@ __global__ __launch_bounds__(kGroup < 256 ? 256 : kGroup) void distill_held_kern
     r.t = reinterpret_cast<float*>(r.id + a.top);
     r.p = r.t + a.top;
     r.z = r.p + a.top;
-    r.slot = reinterpret_cast<uint16_t*>(s_distill + kGroups * 16 * a.top) + group * a.vocab;  // a wave's row only
+    r.slot = reinterpret_cast<uint16_t*>(s_distill + kGroups * 16 * a.top) + group * a.vocab;
     for (int64_t row = (int64_t)blockIdx.x * kGroups + group; row < a.rows; row += (int64_t)gridDim.x * kGroups) {
         const T* const z = logits + row * a.logits_stride;
         const float w = a.row_weight != nullptr ? a.row_weight[row] : 1.0f;
@@ -512,20 +525,23 @@ gsx_hip_status distill_check(const DistillArgs& a, const void* logits, int32_t t
     return GSX_HIP_SUCCESS;
 }
 
-// A row is held by a wave (up to 4 KB), by 256 threads (64 KB), 512 (128 KB) or 1024 (256 KB): the smallest group that holds it in
-// 16 vectors a thread, so that two or more rows share a CU and one loads while another is computed (4096 rows of 65536 bf16:
-// 512 threads 227 us, 1024 with half the vectors each 289). Above 32 KB only where there are rows enough for the GPU's 256 CUs;
-// else, and beyond, a row is cut into slices of 16 KB or more, so that some 2048 workgroups share the logits.
+// A row is held by 16 lanes of a wave (up to 1 KB, and 1792 bytes of LDS), by a wave (4 KB), by 256 threads (64 KB), 512 (128 KB)
+// or 1024 (256 KB): the smallest group that holds it in 16 vectors a thread, so that two or more rows share a CU and one loads
+// while another is computed. 307200 rows of 150 bf16 with 8 entries: 16 lanes 88 us, a wave 233; 100000 of 512 with 64 entries,
+// 2 KB of LDS: 97 and 91. 4096 rows of 65536 bf16: 512 threads 227 us, 1024 with half the vectors each 289. Above 32 KB only
+// where there are rows enough for the GPU's 256 CUs; else, and beyond, a row is cut into slices of 16 KB or more, so that some
+// 2048 workgroups share the logits.
 struct DistillPlan {
     int group, vecs;        // group = 0: slices
     int64_t slice, slices;  // logits of a slice
     int64_t batch;          // rows of a pair of launches: what they read twice stays in the 256 MB cache between
 };
 
-DistillPlan distill_plan(int64_t rows, int64_t vocab, int64_t bytes) {
+DistillPlan distill_plan(int64_t rows, int64_t vocab, int64_t bytes, int64_t top) {
     DistillPlan p = {};
     const int64_t vecs = vocab * bytes / 16;  // the few elements behind the last whole vector are held besides
-    if (vecs <= 64 * 4) p.group = 64;
+    if (vecs <= 16 * 4 && 16 * top + 2 * vocab <= 1792) p.group = 16;
+    else if (vecs <= 64 * 4) p.group = 64;
     else if (vecs <= 256 * 8 || (vecs <= 256 * 16 && rows >= 192)) p.group = 256;
     else if (vecs <= 512 * 16 && rows >= 192) p.group = 512;
     else if (vecs <= 1024 * 16 && rows >= 192) p.group = 1024;
@@ -550,13 +566,19 @@ gsx_hip_status launch_held(const DistillArgs& a, const T* logits, T* grad, hipSt
     const int per = kGroup < 256 ? 256 / kGroup : 1;
     const int64_t blocks = ceil_div(a.rows, per);
     hipLaunchKernelGGL((distill_held_kernel<T, kGroup, kVecs>), dim3((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20)),
-                       dim3(kGroup < 256 ? 256 : kGroup), (unsigned)(per * 16 * a.top + (kGroup == 64 ? per * 2 * a.vocab : 0)), stream, a, logits, grad);
+                       dim3(kGroup < 256 ? 256 : kGroup), (unsigned)(per * (16 * a.top + (kGroup <= 64 ? 2 * a.vocab : 0))),
+                       stream, a, logits, grad);
     return fields_launched("distill launch");
 }
 
 template <typename T>
 gsx_hip_status launch_distill(const DistillPlan& p, DistillArgs a, const T* logits, T* grad, void* temp,
                               hipStream_t stream) {
+    if (p.group == 16) {
+        if (p.vecs <= 1) return launch_held<T, 16, 1>(a, logits, grad, stream);
+        if (p.vecs <= 2) return launch_held<T, 16, 2>(a, logits, grad, stream);
+        return launch_held<T, 16, 4>(a, logits, grad, stream);
+    }
     if (p.group == 64) {
         if (p.vecs <= 1) return launch_held<T, 64, 1>(a, logits, grad, stream);
         if (p.vecs <= 2) return launch_held<T, 64, 2>(a, logits, grad, stream);
@@ -625,7 +647,7 @@ size_t gsx_hip_distill_temp_bytes(int64_t rows, int64_t vocab) {
     if (rows <= 0 || vocab <= 0 || vocab > INT32_MAX) return 0;
     int64_t most = 0;  // whatever the logits' type is
     for (int64_t bytes = 2; bytes <= 4; bytes += 2) {
-        const DistillPlan p = distill_plan(rows, vocab, bytes);
+        const DistillPlan p = distill_plan(rows, vocab, bytes, 1);
         const int64_t need = p.group != 0 ? 0 : p.batch * p.slices * (int64_t)sizeof(MaxSum);
         if (need > most) most = need;
     }
@@ -645,7 +667,7 @@ gsx_hip_status gsx_hip_distill_forward(const void* logits, int32_t logits_type, 
     a.stats = row_stats;
     const gsx_hip_status st = distill_check(a, logits, logits_type, grad_logits);
     if (st != GSX_HIP_SUCCESS || rows == 0) return st;
-    const DistillPlan p = distill_plan(rows, vocab, type_bytes(logits_type));
+    const DistillPlan p = distill_plan(rows, vocab, type_bytes(logits_type), top);
     if (p.group == 0 && (temp == nullptr || !aligned_to(temp, 16)))
         return fields_fail(GSX_HIP_ERROR_INVALID_ARGUMENT, "distill: the workspace must be non-null and 16-byte aligned");
     return distill_launch(p, a, logits, logits_type, grad_logits, temp, stream);
@@ -667,7 +689,7 @@ gsx_hip_status gsx_hip_distill_backward(const void* logits, int32_t logits_type,
     if (row_stats == nullptr || grad_logits == nullptr)
         return fields_fail(GSX_HIP_ERROR_INVALID_ARGUMENT, "distill backward: null pointer");
     a.from_stats = 1;
-    return distill_launch(distill_plan(rows, vocab, type_bytes(logits_type)), a, logits, logits_type, grad_logits, nullptr,
+    return distill_launch(distill_plan(rows, vocab, type_bytes(logits_type), top), a, logits, logits_type, grad_logits, nullptr,
                           stream);
 }
 

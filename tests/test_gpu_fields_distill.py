@@ -269,3 +269,20 @@ def test_distill_refusals():
                 lambda: fields.distill_backward(z, stats, i, t, grad=z)):
         with pytest.raises(GsxHipError):
             bad()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,vocab,top", [(37, 512, 16), (37, 513, 16), (37, 400, 62), (37, 400, 63), (37, 256, 80), (37, 300, 150),
+                                            (50, 3, 2), (1, 33, 1)])
+def test_rows_that_share_a_wave(rows, vocab, top, kind):
+    """About the sizes up to which 16 lanes hold a row, four rows a wave: masks, repeated entries and NaN stay in their row."""
+    z, ids, t = _make(rows, vocab, top, kind, vocab + top, pad=1)
+    weight = np.ones(rows, np.float32)
+    if rows > 1:
+        ids[0] = -1
+        ids[1] = ids[1, 0]
+        ids[2, -1] = ids[2, 0]
+        weight[3] = 0
+        z[3] = float("nan")
+        z[5, : vocab // 2] = -float("inf")
+    _check(z, ids, t, 2.0, weight, pad=1)
