@@ -335,36 +335,50 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(BlockMatrix a, Bl
     }
 }
 
-// out = the sum over splits of partial [splits][m][n], in their order: 16 groups of a workgroup take every 16th split of 16
-// vectors each, then the groups' sums are added.
-template <typename O>
+// out = the sum over splits of partial [splits][m][n], in their order: kGroups groups of a workgroup take every kGroups-th split
+// of 256 / kGroups vectors each, then the groups' sums are added.
+template <typename O, int kGroups>
 __global__ __launch_bounds__(256) void product_join_kernel(const float* __restrict__ partial, int64_t m, int64_t n,
                                                            int64_t splits, O* __restrict__ out, int64_t out_stride) {
-    __shared__ v4f s_sum[256];
+    constexpr int kVecs = 256 / kGroups;
+    __shared__ v4f s_sum[kGroups > 1 ? 256 : 1];
     const int64_t size = m * n, vecs = ceil_div(size, 4);
-    const int group = threadIdx.x / 16;
-    for (int64_t b = blockIdx.x; b < ceil_div(vecs, 16); b += gridDim.x) {
-        const int64_t e = (b * 16 + (threadIdx.x & 15)) * 4;
+    const int group = threadIdx.x / kVecs;
+    for (int64_t b = blockIdx.x; b < ceil_div(vecs, kVecs); b += gridDim.x) {
+        const int64_t e = (b * kVecs + threadIdx.x % kVecs) * 4;
         v4f sum = {0.0f, 0.0f, 0.0f, 0.0f};
         if (e + 4 <= size) {
 #pragma unroll 4
-            for (int64_t s = group; s < splits; s += 16) {
+            for (int64_t s = group; s < splits; s += kGroups) {
                 const Quad<float> x = *reinterpret_cast<const Quad<float>*>(partial + s * size + e);
                 sum += v4f{x.v[0], x.v[1], x.v[2], x.v[3]};
             }
         } else {
-            for (int64_t s = group; s < splits; s += 16)
+            for (int64_t s = group; s < splits; s += kGroups)
                 for (int i = 0; i < 4; ++i)
                     if (e + i < size) sum[i] += partial[s * size + e + i];
         }
-        s_sum[threadIdx.x] = sum;
-        __syncthreads();
-        if (group == 0) {
-            for (int g = 1; g < 16; ++g) sum += s_sum[g * 16 + threadIdx.x];
-            for (int i = 0; i < 4; ++i)
-                if (e + i < size) out[(e + i) / n * out_stride + (e + i) % n] = from_float<O>(sum[i]);
+        if constexpr (kGroups > 1) {
+            s_sum[threadIdx.x] = sum;
+            __syncthreads();
+            if (group == 0)
+                for (int g = 1; g < kGroups; ++g) sum += s_sum[g * kVecs + threadIdx.x];
+            __syncthreads();
         }
-        __syncthreads();
+        if (group != 0 || e >= size) continue;
+        int64_t row = size <= UINT32_MAX ? (uint32_t)e / (uint32_t)n : e / n, col = e - row * n;
+        if (col + 4 <= n) {
+            const v4f one[1] = {sum};
+            store_columns<1>(out + row * out_stride, col, n, one);
+            continue;
+        }
+        for (int i = 0; i < 4 && e + i < size; ++i) {
+            out[row * out_stride + col] = from_float<O>(sum[i]);
+            if (++col == n) {
+                col = 0;
+                ++row;
+            }
+        }
     }
 }
 
@@ -398,10 +412,22 @@ bool product_sizes(int64_t m, int64_t n, int64_t k) {
     return m >= 0 && n >= 0 && k >= 0 && m <= INT32_MAX && n <= INT32_MAX && k <= kMostSummands;
 }
 
+// Groups enough that no thread adds many splits, no more than there are (799 x 3734 in two parts: one group 9 us, sixteen 43).
+template <typename O>
+static void launch_join(const float* partial, int64_t m, int64_t n, int64_t splits, O* out, int64_t out_stride,
+                        hipStream_t stream) {
+    const auto go = [&](auto kernel, int64_t groups) {
+        hipLaunchKernelGGL(kernel, dim3(blocks_grid(ceil_div(ceil_div(m * n, 4), 256 / groups))), dim3(256), 0, stream, partial, m,
+                           n, splits, out, out_stride);
+    };
+    if (splits >= 32) go(product_join_kernel<O, 16>, 16);
+    else if (splits >= 8) go(product_join_kernel<O, 4>, 4);
+    else go(product_join_kernel<O, 1>, 1);
+}
+
 gsx_hip_status join_products(const float* partial, int64_t m, int64_t n, int64_t splits, float* out, int64_t out_stride,
                              hipStream_t stream) {
-    hipLaunchKernelGGL((product_join_kernel<float>), dim3(blocks_grid(ceil_div(ceil_div(m * n, 4), 16))), dim3(256), 0, stream,
-                       partial, m, n, splits, out, out_stride);
+    launch_join(partial, m, n, splits, out, out_stride, stream);
     return fields_launched("product join launch");
 }
 
@@ -529,10 +555,7 @@ gsx_hip_status gsx_hip_blocks_matmul(const uint8_t* a_values, int64_t a_values_s
             else if (plan.edge == 128) go(product_kernel<O, 4, 4, 2, 2, false>, 256);
             else go(product_kernel<O, 2, 2, 2, 2, false>, 256);
         }
-        if (plan.splits > 1) {
-            hipLaunchKernelGGL((product_join_kernel<O>), dim3(blocks_grid(ceil_div(ceil_div(m * n, 4), 16))), dim3(256), 0,
-                               stream, partial, m, n, plan.splits, to, out_stride);
-        }
+        if (plan.splits > 1) launch_join(partial, m, n, plan.splits, to, out_stride, stream);
         return fields_launched("blocks matmul launch");
     });
 }
