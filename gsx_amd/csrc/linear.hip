@@ -8,6 +8,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "blocks.hpp"
 #include "common.hpp"
 
@@ -174,8 +176,8 @@ __global__ __launch_bounds__(64 * kFewWaves, 4) void linear_few_kernel(const T* 
 // A wave takes 16 R rows and all (up to 16 TN) columns; x is read once, straight into registers, a block ahead. The weight lies
 // in LDS for the workgroup's four waves, all of it where it fits (kHeadBytes) and is then read once for all the tiles of a
 // workgroup, else a block of 128 k at a time; each wave converts it. The result passes through LDS, 16 rows of a wave at a
-// time, and leaves in whole stretches of its rows. 307200 x 128 to 150 columns: 53 us for 171 MB, 3.2 TB/s; quantising and
-// converting in two waves a SIMD is about as long as the memory's time and only partly hides in it.
+// time, and leaves in whole stretches of its rows. 307200 x 128 to 150 columns: 46 us for 171 MB, 3.7 TB/s; quantising and
+// converting in two or three waves a SIMD is about as long as the memory's time and only partly hides in it.
 constexpr int kHeadThreads = 256;
 constexpr int kHeadBytes = 49152;
 template <int TN>
@@ -439,6 +441,7 @@ using namespace gsx_amd;
 namespace {
 
 constexpr int64_t kHeadMostColumns = 256;
+constexpr int kHeadMostBlocks = 3;
 
 enum class LinearWay { kFew, kHead, kTiles };
 
@@ -447,7 +450,7 @@ enum class LinearWay { kFew, kHead, kTiles };
 // us against 37, 384 39 against 42, 768 75 against 68).
 LinearWay linear_way(int64_t m, int64_t n, int64_t k) {
     if (m <= kFewRows && (m <= 2 || m * ceil_div(k, kBlock) * kBlock <= kFewBytes)) return LinearWay::kFew;
-    if (n <= kHeadMostColumns && k <= 3 * kBlock) return LinearWay::kHead;
+    if (n <= kHeadMostColumns && k <= kHeadMostBlocks * kBlock) return LinearWay::kHead;
     return LinearWay::kTiles;
 }
 
@@ -460,11 +463,21 @@ int64_t linear_rows_bytes(int64_t m, int64_t k) {
 template <typename T, typename O, int TN>
 void launch_head(const T* x, int64_t x_stride, const BlockMatrix& w, int64_t m, int64_t n, int64_t k, O* out,
                  int64_t out_stride, hipStream_t stream) {
-    // as many workgroups as run at once: registers and LDS leave four a CU at most
+    // as many workgroups as run at once, so that all take the same share (307200 x 128 to 150 columns: 768 of them 48 us, 512 or
+    // 1024 53); registers and LDS decide how many a CU takes, which is asked once for each kernel and number of slots
     const int64_t tiles = ceil_div(m, kHeadRows<TN> * (kHeadThreads / 64)), blocks = ceil_div(k, kBlock);
     const int slots = blocks <= kHeadResident<TN> ? (int)(blocks > 0 ? blocks : 1) : 1;
     const int lds = slots * 16 * TN * (kBlock + 1);
-    hipLaunchKernelGGL((linear_head_kernel<T, O, TN>), dim3((unsigned)(tiles < 1024 ? tiles : 1024)), dim3(kHeadThreads),
+    static std::atomic<int> a_cu[kHeadMostBlocks + 1];
+    int each = a_cu[slots].load(std::memory_order_relaxed);
+    if (each == 0) {
+        if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&each, linear_head_kernel<T, O, TN>, kHeadThreads, lds) != hipSuccess ||
+            each < 1)
+            each = 1;
+        a_cu[slots].store(each, std::memory_order_relaxed);
+    }
+    const int64_t most = (int64_t)each * 256;
+    hipLaunchKernelGGL((linear_head_kernel<T, O, TN>), dim3((unsigned)(tiles < most ? tiles : most)), dim3(kHeadThreads),
                        (unsigned)lds, stream, x, x_stride, w, m, n, k, slots, out, out_stride);
 }
 
