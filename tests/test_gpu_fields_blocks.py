@@ -263,6 +263,24 @@ def test_weight_gradient_of_narrow_layers_with_two_types():
     assert (np.abs(dw.double().cpu().numpy() - want) <= size * (m + 8) * 2.0**-23 + np.abs(want) * 2.0**-24).all()
 
 
+@pytest.mark.parametrize("m,n,k", [(33000, 40, 768), (33000, 64, 700), (33000, 40, 769), (33000, 200, 128), (33000, 200, 256),
+                                   (500, 200, 256), (500, 200, 300), (500, 60, 500)])
+def test_linear_about_the_ways_sizes(m, n, k):
+    """linear() is quantize() and matmul() on either side of the sizes at which the way changes: both are sums of the same k products in
+    float32, each within k 2^-24 of the sum of their magnitudes, rounded once more."""
+    from gsx_amd import fields
+    g = torch.Generator("cuda").manual_seed(m + n + k)
+    x = torch.randn(m, k, device="cuda", generator=g)
+    w = fields.quantize(torch.randn(n, k, device="cuda", generator=g))
+    print(f"[case] linear {m} x {n} x {k}", flush=True)
+    got, q = fields.linear(x, w), fields.quantize(x)
+    size = q.float().abs() @ w.float().abs().T
+    assert ((got - fields.matmul(q, w)).abs() <= size * (2 * k + 8) * 2.0**-24).all()
+    rows = torch.tensor([0, m // 2, m - 1], device="cuda")
+    want = q.float()[rows].double() @ w.float().double().T
+    assert ((got[rows] - want).abs() <= size[rows] * (k + 8) * 2.0**-24).all()
+
+
 def test_weight_gradient_keeps_non_finite_columns_apart():
     from gsx_amd import fields
     x, dy = torch.randn(9000, 20, device="cuda"), torch.randn(9000, 30, device="cuda")
