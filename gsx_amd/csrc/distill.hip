@@ -295,7 +295,8 @@ __device__ inline Stretch stretch_of(const T* z, int64_t length, int tid) {
 }
 
 // Rows that fit the registers of a group: kGroup threads hold kVecs times 16 bytes each. The logits are read once; maximum, sum
-// and gradient come from registers. Instructions bound short rows (307200 of 150 bf16: 88 us, 2.3 TB/s), memory bounds long rows: 4096 of 65537 bf16, 1.07 GB in 233 us, 4.6 TB/s, a copy's rate.
+// and gradient come from registers. Instructions bound short rows (307200 of 150 bf16: 88 us, 2.3 TB/s), memory bounds long ones
+// (4096 of 65537 bf16: 1.07 GB in 233 us, 4.6 TB/s, a copy's rate).
 template <typename T, int kGroup, int kVecs>
 __global__ __launch_bounds__(kGroup < 256 ? 256 : kGroup) void distill_held_kernel(DistillArgs a, const T* __restrict__ logits,
                                                                                    T* __restrict__ grad) {

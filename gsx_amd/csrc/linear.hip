@@ -446,8 +446,8 @@ constexpr int kHeadMostBlocks = 6;
 enum class LinearWay { kFew, kHead, kTiles };
 
 // Few rows while the quantised rows fit a workgroup's LDS (k = n = 8192: 1 row 18 us against 24 through the tiled product, 4
-// rows 21 against 24.5, 8 rows, which do not fit, 28 against 24.5). Few columns up to some blocks of k: three (65536 x 150 x 384: 37
-// us either way, 512 47 against 44); up to 64 columns leave room for the weight's six in LDS, which pays with many rows
+// rows 21 against 24.5, 8 rows, which do not fit, 28 against 24.5). Few columns up to some blocks of k: three (65536 x 150 x 384:
+// 37 us either way, 512 47 against 44); up to 64 columns leave room for the weight's six in LDS, which pays with many rows
 // (40 columns, k = 768: 307200 rows 135 us against 186, 8000 rows 27 against 20); more than 192 columns one, two with few rows
 // (250 columns, k = 256: 307200 rows 154 us against 127, 2000 rows 17 against 19).
 LinearWay linear_way(int64_t m, int64_t n, int64_t k) {
