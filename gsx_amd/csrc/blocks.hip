@@ -6,11 +6,10 @@
 // The scale being a power of two, x * 2^-e is exact, and so is q * 2^e in bfloat16.
 // Product of a [m, k] and b [n, k]: c[m, n] = sum over k of (qa 2^ea) (qb 2^eb), sums in float32.
 //
-// float32 results are formed by the bfloat16 matrix instructions on converted operands, which keep every bit of a float32 sum.
-// The 8-bit instructions, which take E4M3 operands and their scales as they are and run at twice the rate, align groups of
-// eight products to the largest of them and keep 13 bits below it: over blocks of normally distributed values a result is
-// 1.5e-5 off, against 1e-8 with bfloat16 operands. They form long products (kEightLeast) whose result is rounded to 16 bits
-// anyway, at least 30 times as coarsely.
+// Products go through the bfloat16 matrix instructions on converted operands, which keep every bit of a float32 sum, whatever the
+// result's type. The 8-bit instructions, which take E4M3 operands and their scales as they are and run at twice the rate, align
+// groups of eight products to the largest of them and keep 13 bits below it: +-256 * 256 beside products of 1 leave nothing of
+// the latter, and no rounding of a result covers that.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -123,9 +122,8 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_columns_kernel(const T
 // straight from memory. A row is eight chunks of 16 bytes; chunk c lies at place c ^ swizzle(row), and a lane of group g = lane /
 // 16 reads chunks g and g + 4: no two lanes of a read meet in a bank (with chunks 2 g and 2 g + 1 each read takes twice as long).
 //
-// 8192^3 with a 16-bit result: 480 us, 2.3 PFLOP/s of the 3.2 that a library's 8-bit product reaches; float32: 1000 us, 1.1 of
-// bfloat16's 1.6. A workgroup's LDS leaves one to a CU, two waves a SIMD: half of the time the matrix instructions wait, for LDS
-// reads, conversions (float32) and the barrier between blocks.
+// 8192^3 with a 16-bit result: 865 us, 1.3 PFLOP/s of the 1.6 that a library's bfloat16 product reaches. A workgroup's LDS leaves
+// one to a CU, two waves a SIMD, and every wave converts what it reads.
 //
 // The matrix instructions take b as their first operand: a lane then holds four consecutive columns of one row of c. Which
 // row of b a lane brings for instruction j is chosen so that its 4 TN columns are consecutive too, and leave in wide stores.
@@ -169,7 +167,7 @@ __device__ __forceinline__ void load_block(uint8_t* __restrict__ to, const uint8
 
 // One block of k: `next`'s loads are begun (BASES: where a's and b's rows of that block start), then `now`, which they do not
 // touch, is multiplied. __restrict__ says so to the compiler, which otherwise waits for the loads before it reads LDS.
-template <int TM, int TN, int WM, int WN, bool kEight, int kLoads>
+template <int TM, int TN, int WM, int WN, int kLoads>
 __device__ __forceinline__ void product_step(const uint8_t* __restrict__ now, const uint32_t* __restrict__ exponents,
                                              int shift, uint8_t* __restrict__ next, bool load, const uint8_t* a_next,
                                              const uint8_t* b_next, const uint32_t (&offset)[kLoads], int lane, int wave,
@@ -179,32 +177,6 @@ __device__ __forceinline__ void product_step(const uint8_t* __restrict__ now, co
     const int wm = wave / WN, wn = wave % WN;
     const uint8_t* const s_a = now;
     const uint8_t* const s_b = now + BM * kBlock;
-    if constexpr (kEight) {
-        v8i vb[TN];
-        int scale_b[TN], scale_a[TM];  // the byte of this block lowest
-#pragma unroll
-        for (int j = 0; j < TN; ++j) {
-            const int row = wn * 16 * TN + column_of<TN>(j, lane & 15);
-            scale_b[j] = (int)(exponents[BM + row] >> shift);
-            const v4i lo = *reinterpret_cast<const v4i*>(s_b + row * kBlock + ((lane / 16) ^ swizzle_b<TN>(row)) * 16);
-            const v4i hi = *reinterpret_cast<const v4i*>(s_b + row * kBlock + ((lane / 16 + 4) ^ swizzle_b<TN>(row)) * 16);
-            vb[j] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-        }
-#pragma unroll
-        for (int i = 0; i < TM; ++i) scale_a[i] = (int)(exponents[wm * 16 * TM + i * 16 + (lane & 15)] >> shift);
-#pragma unroll
-        for (int i = 0; i < TM; ++i) {
-            const int row = wm * 16 * TM + i * 16 + (lane & 15);
-            const v4i lo = *reinterpret_cast<const v4i*>(s_a + row * kBlock + ((lane / 16) ^ swizzle_a(row)) * 16);
-            const v4i hi = *reinterpret_cast<const v4i*>(s_a + row * kBlock + ((lane / 16 + 4) ^ swizzle_a(row)) * 16);
-            const v8i va = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-            for (int j = 0; j < TN; ++j)
-                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(vb[j], va, acc[i][j], 0, 0, 0, scale_b[j], 0,
-                                                                             scale_a[i]);
-        }
-        return;
-    }
     float scale_b[TN], scale_a[TM];
 #pragma unroll
     for (int j = 0; j < TN; ++j)
@@ -237,7 +209,7 @@ __device__ __forceinline__ void product_step(const uint8_t* __restrict__ now, co
     }
 }
 
-template <typename O, int TM, int TN, int WM, int WN, bool kEight>
+template <typename O, int TM, int TN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void product_kernel(BlockMatrix a, BlockMatrix b, int64_t m, int64_t n, int64_t k,
                                                                int64_t tiles_m, int64_t tiles_n, int64_t splits,
                                                                O* __restrict__ out, int64_t out_stride,
@@ -315,7 +287,7 @@ __global__ __launch_bounds__(64 * WM * WN) void product_kernel(BlockMatrix a, Bl
             const bool more = next < tile.last, whole = (next + 1) * kBlock <= k;
             if (more && next % 4 == 0) stage_exponents(next / 4);
             if (more && !whole) stage(next);
-            product_step<TM, TN, WM, WN, kEight, kLoads>(s_values[kb & 1], s_exponents[(kb / 4) & 1], (int)(kb % 4) * 8,
+            product_step<TM, TN, WM, WN, kLoads>(s_values[kb & 1], s_exponents[(kb / 4) & 1], (int)(kb % 4) * 8,
                                                  s_values[next & 1], more && whole, a_tile + next * kBlock,
                                                  b_tile + next * kBlock, offset, lane, wave, acc);
         }
@@ -445,9 +417,6 @@ struct ProductPlan {
     int64_t temp_bytes;
 };
 
-// Products of at least this many summands with a 16-bit result go through the 8-bit instructions: below, memory bounds them and
-// nothing is gained; 8192^3 takes 480 us instead of 1000.
-constexpr int64_t kEightLeast = 1024;
 constexpr int64_t kSplitMostBlocks = 512;  // blocks of k after which a float sum starts anew
 
 ProductPlan product_plan(int64_t m, int64_t n, int64_t k) {
@@ -541,20 +510,10 @@ gsx_hip_status gsx_hip_blocks_matmul(const uint8_t* a_values, int64_t a_values_s
             hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), 0, stream, a, b, m, n, k, plan.tiles_m, plan.tiles_n,
                                plan.splits, to, out_stride, partial);
         };
-        if constexpr (sizeof(O) == 2) {
-            if (k >= kEightLeast) {
-                if (plan.edge == 256) go(product_kernel<O, 8, 4, 2, 4, true>, 512);
-                else if (plan.edge == 192) go(product_kernel<O, 6, 3, 2, 4, true>, 512);
-                else if (plan.edge == 128) go(product_kernel<O, 4, 4, 2, 2, true>, 256);
-                else go(product_kernel<O, 2, 2, 2, 2, true>, 256);
-            }
-        }
-        if (sizeof(O) == 4 || k < kEightLeast) {
-            if (plan.edge == 256) go(product_kernel<O, 8, 4, 2, 4, false>, 512);
-            else if (plan.edge == 192) go(product_kernel<O, 6, 3, 2, 4, false>, 512);
-            else if (plan.edge == 128) go(product_kernel<O, 4, 4, 2, 2, false>, 256);
-            else go(product_kernel<O, 2, 2, 2, 2, false>, 256);
-        }
+        if (plan.edge == 256) go(product_kernel<O, 8, 4, 2, 4>, 512);
+        else if (plan.edge == 192) go(product_kernel<O, 6, 3, 2, 4>, 512);
+        else if (plan.edge == 128) go(product_kernel<O, 4, 4, 2, 2>, 256);
+        else go(product_kernel<O, 2, 2, 2, 2>, 256);
         if (plan.splits > 1) launch_join(partial, m, n, plan.splits, to, out_stride, stream);
         return fields_launched("blocks matmul launch");
     });
