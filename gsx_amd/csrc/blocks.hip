@@ -417,7 +417,6 @@ struct ProductPlan {
     int64_t temp_bytes;
 };
 
-constexpr int64_t kSplitMostBlocks = 512;  // blocks of k after which a float sum starts anew
 
 ProductPlan product_plan(int64_t m, int64_t n, int64_t k) {
     ProductPlan p;
@@ -434,7 +433,7 @@ ProductPlan product_plan(int64_t m, int64_t n, int64_t k) {
     const int64_t slots = p.edge >= 192 ? 256 : 512;
     int64_t splits = count >= slots / 2 ? 1 : slots / count;  // one round of workgroups
     if (splits > blocks / 4) splits = blocks / 4;
-    if (splits < ceil_div(blocks, kSplitMostBlocks)) splits = ceil_div(blocks, kSplitMostBlocks);
+    if (splits < ceil_div(blocks, kSumMostBlocks)) splits = ceil_div(blocks, kSumMostBlocks);
     p.splits = splits < 1 ? 1 : splits;
     p.temp_bytes = p.splits > 1 ? p.splits * m * n * 4 : 0;
     return p;

@@ -8,6 +8,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "blocks.hpp"
@@ -69,6 +70,7 @@ __device__ inline void quantize_block(const RawBlock<T>& raw, v8bf (&y)[4]) {
 // on its way. Reading the weight bounds it: one row, 32768 x 4096, 135 MB in 28.6 us (4.7 TB/s).
 constexpr int kFewRows = 16;
 constexpr int kFewWaves = 8;
+constexpr int kFewLeastWaves = 4;
 constexpr int kFewBytes = 32768;  // of quantised rows in LDS
 
 template <int J>
@@ -445,13 +447,16 @@ constexpr int kHeadMostBlocks = 6;
 
 enum class LinearWay { kFew, kHead, kTiles };
 
-// Few rows while the quantised rows fit a workgroup's LDS (k = n = 8192: 1 row 18 us against 24 through the tiled product, 4
-// rows 21 against 24.5, 8 rows, which do not fit, 28 against 24.5). Few columns up to some blocks of k: three (65536 x 150 x 384:
-// 37 us either way, 512 47 against 44); up to 64 columns leave room for the weight's six in LDS, which pays with many rows
-// (40 columns, k = 768: 307200 rows 135 us against 186, 8000 rows 27 against 20); more than 192 columns one, two with few rows
-// (250 columns, k = 256: 307200 rows 154 us against 127, 2000 rows 17 against 19).
+// Few rows while the quantised rows fit a workgroup's LDS (k = n = 8192: 1 row 18 us against 24 through the tiled product, 4 rows 21
+// against 24.5, 8 rows, which do not fit, 28 against 24.5) and no wave's sum is longer than kSumMostBlocks (one row, k = 300000:
+// 64 columns 204 us and 1024 257 in longer sums, 19 and 96 through the tiled product). Few columns up to some blocks of k: three
+// (65536 x 150 x 384: 37 us either way, 512 47 against 44); up to 64 columns leave room for the weight's six in
+// LDS, which pays with many rows (40 columns, k = 768: 307200 rows 135 us against 186, 8000 rows 27 against 20); more than 192
+// columns one, two with few rows (250 columns, k = 256: 307200 rows 154 us against 127, 2000 rows 17 against 19).
 LinearWay linear_way(int64_t m, int64_t n, int64_t k) {
-    if (m <= kFewRows && (m <= 2 || m * ceil_div(k, kBlock) * kBlock <= kFewBytes)) return LinearWay::kFew;
+    const int64_t blocks = ceil_div(k, kBlock);
+    if (m <= kFewRows && (m <= 2 || m * blocks * kBlock <= kFewBytes) && blocks <= kFewLeastWaves * kSumMostBlocks)
+        return LinearWay::kFew;
     const bool many = m >= 32768;
     const int most = n <= 64 ? (many ? kHeadMostBlocks : 3) : n <= 192 ? 3 : many ? 1 : 2;
     return n <= kHeadMostColumns && k <= most * kBlock ? LinearWay::kHead : LinearWay::kTiles;
@@ -490,7 +495,7 @@ int64_t weight_stretches(int32_t x_type, int32_t grad_type, int64_t m, int64_t n
     if (x_type != grad_type) return 0;  // the kernel is built for rows of one type
     if (n < 4 || k < 4 || n + k > kWeightMostColumns || n > (k <= 128 ? 256 : 128) || k > 256 || m < 8192) return 0;
     const int64_t blocks = ceil_div(m, kBlock);
-    return blocks < 256 ? blocks : 256;
+    return blocks < 256 ? blocks : std::max<int64_t>(256, ceil_div(blocks, kSumMostBlocks));
 }
 
 struct WeightBlocks {  // workspace of the general way: byte offsets
@@ -563,7 +568,7 @@ gsx_hip_status gsx_hip_linear_forward(const void* x, int32_t x_type, int64_t x_s
                 // waves over k
                 const int64_t blocks = ceil_div(k, kBlock), strips = ceil_div(n, 16);
                 const int j = strips >= 2048 ? 2 : 1;
-                int64_t waves = 4;
+                int64_t waves = kFewLeastWaves;
                 while (waves < kFewWaves && waves < blocks && ceil_div(strips, j) * waves < 4096) waves *= 2;
                 const int64_t groups = ceil_div(strips, j);
                 int64_t span = kFewBytes / kBlock / m;
