@@ -469,8 +469,8 @@ int64_t linear_rows_bytes(int64_t m, int64_t k) {
 }
 
 template <typename T, typename O, int TN>
-void launch_head(const T* x, int64_t x_stride, const BlockMatrix& w, int64_t m, int64_t n, int64_t k, O* out,
-                 int64_t out_stride, hipStream_t stream) {
+gsx_hip_status launch_head(const T* x, int64_t x_stride, const BlockMatrix& w, int64_t m, int64_t n, int64_t k, O* out,
+                           int64_t out_stride, hipStream_t stream) {
     // as many workgroups as run at once, so that all take the same share (307200 x 128 to 150 columns: 768 of them 48 us, 512 or
     // 1024 53); registers and LDS decide how many a CU takes, which is asked once for each kernel and number of slots
     const int64_t tiles = ceil_div(m, kHeadRows<TN> * (kHeadThreads / 64)), blocks = ceil_div(k, kBlock);
@@ -479,14 +479,18 @@ void launch_head(const T* x, int64_t x_stride, const BlockMatrix& w, int64_t m, 
     static std::atomic<int> a_cu[kHeadMostBlocks + 1];
     int each = a_cu[slots].load(std::memory_order_relaxed);
     if (each == 0) {
-        if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&each, linear_head_kernel<T, O, TN>, kHeadThreads, lds) != hipSuccess ||
-            each < 1)
-            each = 1;
+        const hipError_t e =
+            hipOccupancyMaxActiveBlocksPerMultiprocessor(&each, linear_head_kernel<T, O, TN>, kHeadThreads, lds);
+        if (e != hipSuccess || each < 1) {
+            (void)hipGetLastError();  // it is returned here
+            return fields_fail(e != hipSuccess ? (gsx_hip_status)e : GSX_HIP_ERROR_INVALID_STATE, "linear: workgroups of a CU");
+        }
         a_cu[slots].store(each, std::memory_order_relaxed);
     }
     const int64_t most = (int64_t)each * 256;
     hipLaunchKernelGGL((linear_head_kernel<T, O, TN>), dim3((unsigned)(tiles < most ? tiles : most)), dim3(kHeadThreads),
                        (unsigned)lds, stream, x, x_stride, w, m, n, k, slots, out, out_stride);
+    return fields_launched("linear launch");
 }
 
 // Stretches of rows that the weight's gradient of a narrow layer is split into; 0: the layer is not narrow, or too short for its
@@ -577,16 +581,12 @@ gsx_hip_status gsx_hip_linear_forward(const void* x, int32_t x_type, int64_t x_s
                 hipLaunchKernelGGL((j == 2 ? linear_few_kernel<T, O, 2> : linear_few_kernel<T, O, 1>),
                                    dim3((unsigned)(groups < 1024 ? groups : 1024)), dim3((unsigned)waves * 64),
                                    (unsigned)lds, stream, from, x_stride, w, (int)m, n, k, (int)span, result, out_stride);
-            } else if (n <= 64) {
-                launch_head<T, O, 4>(from, x_stride, w, m, n, k, result, out_stride, stream);
-            } else if (n <= 128) {
-                launch_head<T, O, 8>(from, x_stride, w, m, n, k, result, out_stride, stream);
-            } else if (n <= 192) {
-                launch_head<T, O, 12>(from, x_stride, w, m, n, k, result, out_stride, stream);
-            } else {
-                launch_head<T, O, 16>(from, x_stride, w, m, n, k, result, out_stride, stream);
+                return fields_launched("linear launch");
             }
-            return fields_launched("linear launch");
+            if (n <= 64) return launch_head<T, O, 4>(from, x_stride, w, m, n, k, result, out_stride, stream);
+            if (n <= 128) return launch_head<T, O, 8>(from, x_stride, w, m, n, k, result, out_stride, stream);
+            if (n <= 192) return launch_head<T, O, 12>(from, x_stride, w, m, n, k, result, out_stride, stream);
+            return launch_head<T, O, 16>(from, x_stride, w, m, n, k, result, out_stride, stream);
         });
     });
 }

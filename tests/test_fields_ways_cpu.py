@@ -92,3 +92,21 @@ for rows, vocab, top, name in {DISTILLS!r}:
                                            None), "distill")
     assert fake.fake_launches_of(name) == before + (2 if b"finish" in name else 1), (rows, vocab, top)
 """)
+
+
+def test_a_refused_occupancy_query_ends_the_call_and_is_not_kept(host):
+    """A narrow layer asks how many workgroups a CU takes. If HIP refuses, nothing is launched, the caller gets HIP's error, no error
+    is left for later calls, and the next call asks again."""
+    host("""
+def linear():
+    return lib.gsx_hip_linear_forward(P, 0, 128, P, 128, P, 4, 307200, 150, 128, P, 0, 150, None, None)
+
+fake.fake_set_each_cu(-1)
+assert linear() == 1  # HIP's code for an invalid value
+assert fake.fake_launches_of(b"linear_head") == 0
+assert fake.hipGetLastError() == 0
+assert b"linear" in lib.gsx_hip_last_error_message()
+fake.fake_set_each_cu(3)
+_lib.check(linear(), "linear")
+assert fake.fake_launches_of(b"linear_head") == 1 and fake.fake_threads_of(b"linear_head") == 3 * 256 * 256
+""")
