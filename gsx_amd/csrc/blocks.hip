@@ -377,9 +377,6 @@ gsx_hip_status block_matrix_check(const void* values, const void* exponents, int
     return GSX_HIP_SUCCESS;
 }
 
-// 256 rows of a product's operand lie within 2^36 bytes (the kernel's offsets): value strides below 2^28.
-static constexpr int64_t kMostStride = (int64_t)1 << 28;
-
 bool product_sizes(int64_t m, int64_t n, int64_t k) {
     return m >= 0 && n >= 0 && k >= 0 && m <= INT32_MAX && n <= INT32_MAX && k <= kMostSummands;
 }

@@ -324,6 +324,8 @@ __device__ inline int swizzle_b(int row) {
 
 constexpr int64_t kMostSummands = (int64_t)1 << 27;
 constexpr int64_t kSumMostBlocks = 512;  // blocks of k after which a float sum starts anew, whatever way a product takes
+// 256 rows of a product's operand lie within 2^36 bytes (the kernel's offsets): value strides below 2^28.
+constexpr int64_t kMostStride = (int64_t)1 << 28;
 bool product_sizes(int64_t m, int64_t n, int64_t k);
 // out [m, n] = the sum of partial [splits][m][n] over the splits, in a fixed order.
 gsx_hip_status join_products(const float* partial, int64_t m, int64_t n, int64_t splits, float* out, int64_t out_stride,

@@ -550,6 +550,8 @@ gsx_hip_status gsx_hip_linear_forward(const void* x, int32_t x_type, int64_t x_s
     if (way == LinearWay::kTiles) {
         if (k > 0 && (temp == nullptr || !aligned_to(temp, 16)))
             return fields_fail(GSX_HIP_ERROR_INVALID_ARGUMENT, "linear: the workspace must be non-null and 16-byte aligned");
+        if (w_values_stride >= kMostStride)
+            return fields_fail(GSX_HIP_ERROR_OUT_OF_RANGE, "linear: a wide layer's value rows lie less than 2^28 bytes apart");
         const int64_t blocks = ceil_div(k, kBlock), words = ceil_div(blocks, 4) * 4;
         uint8_t* const values = static_cast<uint8_t*>(temp);
         uint8_t* const exponents = values + m * blocks * kBlock;

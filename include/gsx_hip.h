@@ -515,7 +515,8 @@ gsx_hip_status gsx_hip_blocks_matmul(const uint8_t* a_values, int64_t a_values_s
                                      const uint8_t* b_exponents, int64_t b_exponents_stride, int64_t m, int64_t n,
                                      int64_t k, void* out, int32_t out_type, int64_t out_stride, void* temp,
                                      hipStream_t stream);
-/* out [m, n] = blocks(x) w^T: the rows of x [m, k] are quantised as above and multiplied with the block matrix w [n, k]. */
+/* out [m, n] = blocks(x) w^T: the rows of x [m, k] are quantised as above and multiplied with the block matrix w [n, k].
+ * Where that takes a workspace, w's value stride is below 2^28. */
 size_t gsx_hip_linear_temp_bytes(int64_t m, int64_t n, int64_t k);
 gsx_hip_status gsx_hip_linear_forward(const void* x, int32_t x_type, int64_t x_stride, const uint8_t* w_values,
                                       int64_t w_values_stride, const uint8_t* w_exponents, int64_t w_exponents_stride,

@@ -110,3 +110,15 @@ fake.fake_set_each_cu(3)
 _lib.check(linear(), "linear")
 assert fake.fake_launches_of(b"linear_head") == 1 and fake.fake_threads_of(b"linear_head") == 3 * 256 * 256
 """)
+
+
+def test_a_weight_whose_rows_lie_too_far_apart_is_refused_before_anything_runs(host):
+    """The tiled product takes value rows less than 2^28 bytes apart; other ways of a linear layer have no such limit."""
+    host("""
+far = 1 << 28
+assert lib.gsx_hip_linear_forward(P, 0, 1024, P, far, P, 8, 300, 300, 1024, P, 0, 300, P, None) == -3
+assert b"2^28" in lib.gsx_hip_last_error_message()
+assert fake.fake_launches() == 0
+_lib.check(lib.gsx_hip_linear_forward(P, 0, 1024, P, far - 16, P, 8, 300, 300, 1024, P, 0, 300, P, None), "linear")
+_lib.check(lib.gsx_hip_linear_forward(P, 0, 1024, P, far, P, 8, 1, 300, 1024, P, 0, 300, None, None), "linear")
+""")
