@@ -1,4 +1,4 @@
-// fields.hpp - what the label-field kernels (rows.hip, blocks.hip, distill.hip) share: element types, vectors of them,
+// fields.hpp - what the label-field kernels (rows.hip, blocks.hip, linear.hip, distill.hip) share: element types, vectors of them,
 // and the host's checks.
 #pragma once
 

@@ -308,7 +308,8 @@ __global__ __launch_bounds__(kHeadThreads, 2) void linear_head_kernel(const T* _
 // banks) and multiplies them, 2 x 4 waves with NT x KT tiles of 16 x 16 each; the next block's rows are on their way meanwhile.
 // The stretches' sums are joined by another launch. Quantised copies of dy^T and x^T, written and read again, would double what
 // is moved. 307200 x 150 x 128 of bf16: 69 us for 171 MB, 2.5 TB/s. Registers leave one workgroup
-// a CU, whose phases (maxima, quantising, products) stand between barriers: with a second block's rows on their way it is no
+// a CU, whose phases (maxima, quantising, products) stand between barriers (the waves wait for 44% of their time, the vector units are
+// busy for 33%, the matrix units for 8%): with a second block's rows on their way it is no
 // faster; with 16 waves 4% for 16-bit types, whose float32 form spills.
 constexpr int kWeightThreads = 512;
 constexpr int kWeightPitch = 144;

@@ -501,8 +501,9 @@ gsx_hip_status gsx_hip_lookup_backward(const void* grad_out, int32_t grad_type, 
  * bits, 3 mantissa bits, largest 448) and one byte e + 127 for its scale 2^e, with e the least whole number >= -100 such that
  * max |x| <= 448 * 2^e over the block's finite x (e = 0 where that maximum is 0). Each x * 2^-e is rounded to the nearest
  * E4M3 value, ties to even; a non-finite x becomes NaN. Value rows are 16-byte aligned (stride a multiple of 16, >= cols),
- * exponent rows 4-byte aligned (stride a multiple of 4, >= ceil(cols / 128)). Products are exact for e from -100 to 119. What lies between a row's last value and its
- * stride is never used as a value; quantize writes zeros there up to the last block's end.
+ * exponent rows 4-byte aligned (stride a multiple of 4, >= ceil(cols / 128)). Products take values exactly for e from -100 to 119.
+ * A row's last 16 bytes of values and 4 of exponents are read whole, but what lies between its last value and its stride is
+ * never used as a value; quantize writes zeros there up to the last block's end.
  * transpose != 0 lays out the blocks of src^T (src_cols rows of src_rows values, blocks along src's rows). */
 gsx_hip_status gsx_hip_blocks_quantize(const void* src, int32_t src_type, int64_t src_rows, int64_t src_cols,
                                        int64_t src_stride, int32_t transpose, uint8_t* values, int64_t values_stride,
