@@ -296,8 +296,8 @@ __device__ inline Stretch stretch_of(const T* z, int64_t length, int tid) {
 
 // Rows that fit the registers of a group: kGroup threads hold kVecs times 16 bytes each. The logits are read once; maximum, sum
 // and gradient come from registers. Instructions bound short rows (307200 of 150 bf16: 81 us, 2.5 TB/s, vector instructions in
-// 98% of the cycles), memory bounds long ones (4096 of 65537 bf16: 1.07 GB in 234 us, 4.6 TB/s, a copy's rate). The loss alone takes
-// 52 and 113 us, the gradient in a later call 65 and 235 more.
+// 98% of the cycles), memory bounds long ones (4096 of 65537 bf16: 1.07 GB in 234 us, 4.6 TB/s, a copy's rate). The loss alone
+// takes 52 and 113 us, the gradient in a later call 65 and 235 more.
 template <typename T, int kGroup, int kVecs>
 __global__ __launch_bounds__(kGroup < 256 ? 256 : kGroup) void distill_held_kernel(DistillArgs a, const T* __restrict__ logits,
                                                                                    T* __restrict__ grad) {
@@ -529,10 +529,10 @@ gsx_hip_status distill_check(const DistillArgs& a, const void* logits, int32_t t
 
 // A row is held by 16 lanes of a wave (up to 1 KB, and 1792 bytes of LDS), by a wave (4 KB), by 256 threads (64 KB), 512 (128 KB)
 // or 1024 (256 KB): the smallest group that holds it in 16 vectors a thread, so that two or more rows share a CU and one loads
-// while another is computed. 307200 rows of 150 bf16 with 8 entries: a wave took 2.6 times as long as 16 lanes; 100000 of
-// 512 with 64 entries, 2 KB of LDS: 16 lanes 97 us, a wave 91. 4096 rows of 65536 bf16: 512 threads 227 us, 1024 with half the vectors each 289. Above 32 KB only
-// where there are rows enough for the GPU's 256 CUs; else, and beyond, a row is cut into slices of 16 KB or more, so that some
-// 2048 workgroups share the logits.
+// while another is computed. 307200 rows of 150 bf16 with 8 entries: a wave took 2.6 times as long as 16 lanes; 100000 of 512
+// with 64 entries, 2 KB of LDS: 16 lanes 97 us, a wave 91. 4096 rows of 65536 bf16: 512 threads 227 us, 1024 with half the
+// vectors each 289. Above 32 KB only where there are rows enough for the GPU's 256 CUs; else, and beyond, a row is cut into
+// slices of 16 KB or more, so that some 2048 workgroups share the logits.
 struct DistillPlan {
     int group, vecs;        // group = 0: slices
     int64_t slice, slices;  // logits of a slice

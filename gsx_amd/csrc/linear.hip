@@ -304,13 +304,13 @@ __global__ __launch_bounds__(kHeadThreads, 2) void linear_head_kernel(const T* _
 //   gw[i, j] = sum over rows r of blocks(dy^T)[i, r] blocks(x^T)[j, r]
 //
 // A workgroup takes a stretch of blocks of 128 rows. Of each it reads dy and x once, finds the columns' maxima, quantises the
-// columns into LDS (a column's 128 values in a row of kWeightPitch bytes, so that a read of 16 columns meets 16 different
-// banks) and multiplies them, 2 x 4 waves with NT x KT tiles of 16 x 16 each; the next block's rows are on their way meanwhile.
-// The stretches' sums are joined by another launch. Quantised copies of dy^T and x^T, written and read again, would double what
-// is moved. 307200 x 150 x 128 of bf16: 69 us for 171 MB, 2.5 TB/s. Registers leave one workgroup
-// a CU, whose phases (maxima, quantising, products) stand between barriers (the waves wait for 44% of their time, the vector units are
-// busy for 33%, the matrix units for 8%): with a second block's rows on their way it is no
-// faster; with 16 waves 4% for 16-bit types, whose float32 form spills.
+// columns into LDS (a column's 128 values in a row of kWeightPitch bytes, so that a read of 16 columns meets 16 different banks)
+// and multiplies them, 2 x 4 waves with NT x KT tiles of 16 x 16 each; the next block's rows are on their way meanwhile. The
+// stretches' sums are joined by another launch. Quantised copies of dy^T and x^T, written and read again, would double what is
+// moved. 307200 x 150 x 128 of bf16: 69 us for 171 MB, 2.5 TB/s. Registers leave one workgroup a CU, whose phases (maxima,
+// quantising, products) stand between barriers (the waves wait for 44% of their time, the vector units are busy for 33%, the
+// matrix units for 8%): with a second block's rows on their way it is no faster; with 16 waves 4% for 16-bit types, whose float32
+// form spills.
 constexpr int kWeightThreads = 512;
 constexpr int kWeightPitch = 144;
 constexpr int kWeightPatches = 3;  // of 8 rows by 4 columns a thread holds: up to 96 quads of columns
@@ -448,12 +448,12 @@ constexpr int kHeadMostBlocks = 6;
 
 enum class LinearWay { kFew, kHead, kTiles };
 
-// Few rows while the quantised rows fit a workgroup's LDS (k = n = 8192: 1 row 18 us against 24 through the tiled product, 4 rows 21
-// against 24.5, 8 rows, which do not fit, 28 against 24.5) and no wave's sum is longer than kSumMostBlocks (one row, k = 300000:
-// 64 columns 204 us and 1024 257 in longer sums, 19 and 96 through the tiled product). Few columns up to some blocks of k: three
-// (65536 x 150 x 384: 37 us either way, 512 47 against 44); up to 64 columns leave room for the weight's six in
-// LDS, which pays with many rows (40 columns, k = 768: 307200 rows 135 us against 186, 8000 rows 27 against 20); more than 192
-// columns one, two with few rows (250 columns, k = 256: 307200 rows 154 us against 127, 2000 rows 17 against 19).
+// Few rows while the quantised rows fit a workgroup's LDS (k = n = 8192: 1 row 18 us against 24 through the tiled product, 4 rows
+// 21 against 24.5, 8 rows, which do not fit, 28 against 24.5) and no wave's sum is longer than kSumMostBlocks (one row, k =
+// 300000: 64 columns 204 us and 1024 257 in longer sums, 19 and 96 through the tiled product). Few columns up to some blocks of
+// k: three (65536 x 150 x 384: 37 us either way, 512 47 against 44); up to 64 columns leave room for the weight's six in LDS,
+// which pays with many rows (40 columns, k = 768: 307200 rows 135 us against 186, 8000 rows 27 against 20); more than 192 columns
+// one, two with few rows (250 columns, k = 256: 307200 rows 154 us against 127, 2000 rows 17 against 19).
 LinearWay linear_way(int64_t m, int64_t n, int64_t k) {
     const int64_t blocks = ceil_div(k, kBlock);
     if (m <= kFewRows && (m <= 2 || m * blocks * kBlock <= kFewBytes) && blocks <= kFewLeastWaves * kSumMostBlocks)
