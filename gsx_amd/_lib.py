@@ -85,6 +85,16 @@ class AdamGroup(ctypes.Structure):
                 ("max_grad", _f), ("bias_correction1", _d), ("bias_correction2", _d)]
 
 
+class AdamwTensor(ctypes.Structure):
+    _fields_ = [("parameter", _vp), ("gradient", _vp), ("first", _vp), ("second", _vp), ("first_scale", _vp),
+                ("second_scale", _vp), ("count", _i64), ("parameter_type", _i32), ("gradient_type", _i32), ("bits", _i32),
+                ("group", _i32)]
+
+
+class AdamwGroup(ctypes.Structure):
+    _fields_ = [("beta1", _d), ("beta2", _d), ("learning_rate", _d), ("weight_decay", _d), ("epsilon", _d)]
+
+
 class AdcParams(ctypes.Structure):
     _fields_ = [("algorithm", _i32), ("pruning_opacity_threshold", _f), ("opacity_clamp_value", _f),
                 ("max_world_scale", _f), ("max_screen_scale", _f), ("duplicate_grad_threshold", _f),
@@ -179,6 +189,11 @@ SIGNATURES = {
                                                                ctypes.c_int, _vp]),
     "gsx_hip_adam_step_f32_kernel_launch": (_st, [_vp, _vp, _vp, _vp, _i64, _f, _f, _f, _f, _f, _f, _d, _d, _vp]),
     "gsx_hip_adam_step_multi_launch": (_st, [ctypes.POINTER(AdamGroup), _i32, _vp]),
+    "gsx_hip_adamw_table_bytes": (ctypes.c_size_t, [ctypes.POINTER(AdamwTensor), _i64]),
+    "gsx_hip_adamw_table_fill": (_st, [ctypes.POINTER(AdamwTensor), _i64, _vp, ctypes.POINTER(_i64)]),
+    "gsx_hip_adamw_step": (_st, [_vp, _i64, ctypes.POINTER(AdamwGroup), _i32, _f, _vp, _vp, _vp, _vp]),
+    "gsx_hip_moments_hold": (_st, [_vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp]),
+    "gsx_hip_moments_read": (_st, [_vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp]),
     "gsx_hip_adc_context_create": (_st, [ctypes.POINTER(_vp), ctypes.c_uint64]),
     "gsx_hip_adc_context_destroy": (_st, [_vp]),
     "gsx_hip_adc_step": (_st, [_vp, ctypes.POINTER(AdcParams), ctypes.c_uint64, ctypes.POINTER(GsRows), _i64,

@@ -17,7 +17,7 @@ import torch
 from . import _lib
 from ._lib import Camera, GaussianGrads, Gaussians, GsxHipError, check
 
-__all__ = ["Camera", "Renderer", "Loss", "Adam", "DensityControl", "GsxHipError", "stream_handle", "ptr"]
+__all__ = ["Camera", "Renderer", "Loss", "Adam", "AdamW", "DensityControl", "GsxHipError", "stream_handle", "ptr"]
 
 
 def ptr(t: torch.Tensor | None):
@@ -252,6 +252,140 @@ class Adam:
             a.bias_correction1 = 1.0 - math.pow(b1, float(g["step"]))
             a.bias_correction2 = 1.0 - math.pow(b2, float(g["step"]))
         check(self.lib.gsx_hip_adam_step_multi_launch(arr, len(self.groups), stream_handle(stream)), "adam step")
+
+
+class AdamW:
+    """AdamW over any number of tensors in one launch, with moments in 32 bits or in 8 (include/gsx_hip.h has the formulas and
+    the format).
+
+    groups: up to 16 dicts of `parameters` and `gradients` (lists of contiguous tensors of the same sizes, float32, bfloat16 or
+    float16, whose memory stays in use by this optimizer) and of learning_rate, beta1, beta2, weight_decay and epsilon, which may
+    be changed in `groups` between steps. All moments lie in one buffer, in the order of the tensors, each from a multiple of 128
+    values on (`offsets`). Steps are counted on the device: a step captured into a graph counts at every replay, with the
+    rates of its capture."""
+
+    BLOCK = 128
+    _TYPES = {torch.float32: 0, torch.bfloat16: 3, torch.float16: 4}  # GSX_HIP_DTYPE_*
+
+    def __init__(self, groups: list[dict], bits: int = 32):
+        self.lib = _lib.load()
+        if bits not in (8, 32):
+            raise GsxHipError(f"moments have 8 bits or 32, not {bits}")
+        if not 1 <= len(groups) <= _lib.ADAM_MAX_GROUPS:
+            raise GsxHipError(f"1 to {_lib.ADAM_MAX_GROUPS} groups, not {len(groups)}")
+        self.bits = bits
+        self.device = torch.cuda.current_device()
+        self.groups = []
+        self.offsets = []
+        self._tensors = []  # (group, parameter, gradient)
+        total = 0
+        for k, g in enumerate(groups):
+            parameters, gradients = list(g["parameters"]), list(g["gradients"])
+            if len(parameters) != len(gradients):
+                raise GsxHipError("a group needs a gradient for each parameter")
+            for p, d in zip(parameters, gradients):
+                for t in (p, d):
+                    if t.get_device() != self.device:
+                        raise GsxHipError("parameters and gradients must live on the current HIP device")
+                    if t.dtype not in self._TYPES:
+                        raise GsxHipError(f"parameters and gradients are float32, bfloat16 or float16, not {t.dtype}")
+                    if not t.is_contiguous():
+                        raise GsxHipError("parameters and gradients must be contiguous")
+                if p.shape != d.shape:
+                    raise GsxHipError(f"a gradient of shape {tuple(d.shape)} for a parameter of shape {tuple(p.shape)}")
+                self._tensors.append((k, p, d))
+                self.offsets.append(total)
+                total += -(-p.numel() // self.BLOCK) * self.BLOCK
+            self.groups.append(dict(learning_rate=float(g["learning_rate"]), beta1=float(g.get("beta1", 0.9)),
+                                    beta2=float(g.get("beta2", 0.999)), weight_decay=float(g.get("weight_decay", 0.01)),
+                                    epsilon=float(g.get("epsilon", 1e-8))))
+        self.size = total
+        kind = torch.uint8 if bits == 8 else torch.float32
+        self.first = torch.zeros(total, dtype=kind, device="cuda")
+        self.second = torch.zeros(total, dtype=kind, device="cuda")
+        self.first_scale = self.second_scale = None
+        if bits == 8:
+            self.first_scale = torch.full((total // self.BLOCK,), 2.0**-126, device="cuda")
+            self.second_scale = torch.full((total // self.BLOCK,), 2.0**-126, device="cuda")
+        self.steps = torch.zeros(1, dtype=torch.int64, device="cuda")
+        self._factors = torch.zeros(2 * _lib.ADAM_MAX_GROUPS, device="cuda")
+        self._lay_out()
+        self._stream = torch.cuda.current_stream()
+        self._stream.synchronize()  # steps may run on any stream
+
+    def _lay_out(self):
+        wide = self.first.element_size()
+        entries = (_lib.AdamwTensor * max(1, len(self._tensors)))()
+        for e, at, (k, p, d) in zip(entries, self.offsets, self._tensors):
+            e.parameter, e.gradient, e.count, e.group, e.bits = p.data_ptr(), d.data_ptr(), p.numel(), k, self.bits
+            e.parameter_type, e.gradient_type = self._TYPES[p.dtype], self._TYPES[d.dtype]
+            e.first, e.second = self.first.data_ptr() + at * wide, self.second.data_ptr() + at * wide
+            if self.bits == 8:
+                e.first_scale = self.first_scale.data_ptr() + at // self.BLOCK * 4
+                e.second_scale = self.second_scale.data_ptr() + at // self.BLOCK * 4
+        size = self.lib.gsx_hip_adamw_table_bytes(entries, len(self._tensors))
+        table = torch.empty(max(size, 16) // 8, dtype=torch.int64)
+        chunks = ctypes.c_int64(0)
+        check(self.lib.gsx_hip_adamw_table_fill(entries, len(self._tensors), table.data_ptr(), ctypes.byref(chunks)),
+              "adamw table")
+        self._table, self._chunks = table.cuda(), chunks.value
+
+    def _on(self, stream):
+        """The stream of a call, whose use of this optimizer's memory the allocator is told of."""
+        if torch.cuda.current_device() != self.device:
+            raise GsxHipError("the optimizer's device must be the current one")
+        s = stream if stream is not None else torch.cuda.current_stream()
+        if s != self._stream:
+            for t in (self.first, self.second, self.first_scale, self.second_scale, self.steps, self._factors, self._table):
+                if t is not None:
+                    t.record_stream(s)
+        return s
+
+    def step(self, grad_scale: float = 1.0, grad_factor: torch.Tensor | None = None, stream=None) -> None:
+        """One step. Gradients are multiplied by grad_scale and by what grad_factor, one float32 on the device, holds then."""
+        if grad_factor is not None and (grad_factor.get_device() != self.device or grad_factor.dtype != torch.float32 or
+                                        grad_factor.numel() != 1):
+            raise GsxHipError("grad_factor must be one float32 on the current HIP device")
+        s = self._on(stream)
+        arr = (_lib.AdamwGroup * len(self.groups))()
+        for a, g in zip(arr, self.groups):
+            a.beta1, a.beta2, a.learning_rate = g["beta1"], g["beta2"], g["learning_rate"]
+            a.weight_decay, a.epsilon = g["weight_decay"], g["epsilon"]
+        check(self.lib.gsx_hip_adamw_step(self._table.data_ptr(), self._chunks, arr, len(self.groups), grad_scale,
+                                          None if grad_factor is None else grad_factor.data_ptr(), self.steps.data_ptr(),
+                                          self._factors.data_ptr(), s.cuda_stream), "adamw step")
+
+    def moments(self, stream=None):
+        """(first, second) moments in float32, each [size]; tensor i's from offsets[i] on, 0 between the tensors. With 32 bits
+        they are the optimizer's own."""
+        if self.bits == 32:
+            return self.first, self.second
+        s = self._on(stream)
+        with torch.cuda.stream(s):
+            first, second = (torch.empty(self.size, device="cuda") for _ in range(2))
+        check(self.lib.gsx_hip_moments_read(self.first.data_ptr(), self.first_scale.data_ptr(), self.second.data_ptr(),
+                                            self.second_scale.data_ptr(), self.size // self.BLOCK, first.data_ptr(),
+                                            second.data_ptr(), s.cuda_stream), "moments")
+        return first, second
+
+    def load(self, first: torch.Tensor, second: torch.Tensor, steps: int, stream=None) -> None:
+        """Goes on from moments laid out as `moments` gives them (0 between the tensors, second ones >= 0) after `steps` steps."""
+        for t in (first, second):
+            if t.get_device() != self.device or t.dtype != torch.float32 or t.shape != (self.size,) or not t.is_contiguous():
+                raise GsxHipError(f"moments are {self.size} contiguous float32 values on the current HIP device")
+        if steps < 0:
+            raise GsxHipError("the number of steps must be >= 0")
+        s = self._on(stream)
+        with torch.cuda.stream(s):
+            self.steps.fill_(int(steps))
+            if self.bits == 32:
+                self.first.copy_(first)
+                self.second.copy_(second)
+            else:
+                check(self.lib.gsx_hip_moments_hold(first.data_ptr(), second.data_ptr(), self.size // self.BLOCK,
+                                                    self.first.data_ptr(), self.first_scale.data_ptr(),
+                                                    self.second.data_ptr(), self.second_scale.data_ptr(),
+                                                    s.cuda_stream), "moments")
 
 
 FIELD_WIDTHS = {"mean3d": 3, "rotation": 4, "logscale": 3, "opacity": 1, "sh0": 3, "sh1": 9, "sh2": 15, "sh3": 21}

@@ -400,6 +400,52 @@ gsx_hip_status gsx_hip_adam_step_f32_kernel_launch(float* parameter, const float
 gsx_hip_status gsx_hip_adam_step_multi_launch(const gsx_hip_adam_group* groups, int32_t group_count,
                                               hipStream_t stream);
 
+/* AdamW over any number of tensors in one launch (no counterpart in the reference). With t = *steps + 1, all in float32, one
+ * rounding for each operation:
+ *   g = gradient * grad_scale * grad_factor[0] (null: 1);  m' = beta1 m + (1 - beta1) g;  v' = beta2 v + (1 - beta2) (g g)
+ *   p' = p - (rate decay) p - (rate / (1 - beta1^t)) (m' / (sqrt(v') / sqrt(1 - beta2^t) + epsilon))
+ * Parameters and gradients are GSX_HIP_DTYPE_F32, BF16 or F16, a parameter rounded to nearest even. bits = 32: first and second
+ * are float32 [count]. bits = 8: they hold ceil(count / 128) whole blocks of 128 codes (8-byte aligned) and a float32 scale a
+ * block, 0 behind the count:
+ *   first:  scale s = max(max |m| * (float)(1/448), 2^-126), code E4M3 of m * (1 / s) (ties to even); stands for code * s
+ *   second: scale s = max(max v, 2^-126), ratio y = v * (1 / s) rounded to three bits behind the first (ties to even), code
+ *           (bits of y >> 20) - 762 within 1 to 254 for v > 0, 0 for v = 0; stands for ratio * s
+ * over a block's finite values; one that is not finite is held as NaN in the first and as 255, +inf, in the second. */
+typedef struct gsx_hip_adamw_tensor {
+    void* parameter;
+    const void* gradient;
+    void *first, *second;              /* moments */
+    float *first_scale, *second_scale; /* of 8-bit moments */
+    int64_t count;
+    int32_t parameter_type, gradient_type;
+    int32_t bits;  /* 8 or 32 */
+    int32_t group; /* of gsx_hip_adamw_step's groups */
+} gsx_hip_adamw_tensor;
+typedef struct gsx_hip_adamw_group {
+    double beta1, beta2, learning_rate, weight_decay, epsilon; /* 0 <= beta < 1, epsilon > 0 as a float, decay >= 0 */
+} gsx_hip_adamw_group;
+
+/* The table of a step's tensors: fill writes table_bytes bytes to host memory (8-byte aligned) and *out_chunks, what step is
+ * given; the caller copies the table to 8-byte aligned device memory and keeps it there as it is. Nothing that a step writes
+ * (parameters, moments, scales) may overlap another tensor's memory or the gradients. table_bytes is 0 where fill would refuse
+ * the tensors for anything but an overlap. At most 2^24 - 1 chunks of 2048 elements. */
+size_t gsx_hip_adamw_table_bytes(const gsx_hip_adamw_tensor* tensors, int64_t tensor_count);
+gsx_hip_status gsx_hip_adamw_table_fill(const gsx_hip_adamw_tensor* tensors, int64_t tensor_count, void* table,
+                                        int64_t* out_chunks);
+/* One step: counts *steps (on the device) and updates every tensor of the table; those of groups from group_count on stay as
+ * they are. `factors` is device memory of 8 * GSX_HIP_ADAM_MAX_GROUPS bytes (8-byte aligned) that steps on one stream may
+ * share. Captured into a graph, each replay counts a step, with the capture's groups and grad_scale and with what grad_factor
+ * holds then. */
+gsx_hip_status gsx_hip_adamw_step(const void* table, int64_t chunks, const gsx_hip_adamw_group* groups, int32_t group_count,
+                                  float grad_scale, const float* grad_factor, int64_t* steps, void* factors,
+                                  hipStream_t stream);
+/* Whole blocks of moments (128 * blocks values) from float32 to their codes and scales, and back. */
+gsx_hip_status gsx_hip_moments_hold(const float* first, const float* second, int64_t blocks, uint8_t* first_codes,
+                                    float* first_scale, uint8_t* second_codes, float* second_scale, hipStream_t stream);
+gsx_hip_status gsx_hip_moments_read(const uint8_t* first_codes, const float* first_scale, const uint8_t* second_codes,
+                                    const float* second_scale, int64_t blocks, float* first, float* second,
+                                    hipStream_t stream);
+
 /* ---- adaptive density control -----------------------------------------------------------------
  * Replaces the CUDA thrust pipeline (gsx/src/gsx-cuda/adc.cu:757-927) with the semantics of
  * the CPU default/ABSGS refine and opacity reset (gsx/src/gsx-cpu/adc/default.c:160-527,
