@@ -215,6 +215,10 @@ SIGNATURES = {
                                       _vp, _vp]),
     "gsx_hip_distill_backward": (_st, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _i32, _f, _vp, _vp, _vp, _f, _vp, _i64,
                                        _vp]),
+    "gsx_hip_log_probs_temp_bytes": (ctypes.c_size_t, [_i64, _i64, _i32]),
+    "gsx_hip_log_probs_forward": (_st, [_vp, _i32, _i64, _i64, _i64, _vp, _f, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _i64, _vp, _f,
+                                        _vp, _f, _vp, _vp]),
+    "gsx_hip_log_probs_backward": (_st, [_vp, _i32, _i64, _i64, _i64, _vp, _f, _vp, _vp, _f, _vp, _f, _vp, _i64, _vp]),
 }
 
 _LIB = None

@@ -1,0 +1,683 @@
+// logprobs.hip - log probabilities of given labels, entropies and top alternatives of rows of logits, and their gradient.
+//
+// One row: z [vocab], T the temperature, y = z / T, q = softmax(y), id the given label:
+//   chosen = log q_id,  entropy H = -sum_j q_j log q_j,  top: the largest z (of equal ones the lowest index) with their log q
+//   dz_j = (gl (delta_{j,id} - q_j) - gh q_j (log q_j + H)) / T   for upstream gradients gl of chosen and gh of H
+// With m = max z, u_j = (z_j - m) log2(e) / T and e_j = 2^u_j, all of it follows from s = sum e_j and w = sum e_j u_j:
+//   log q_j = ln2 u_j - ln s,  H = ln s - ln2 w / s    (terms of one sign: nothing cancels)
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "logits.hpp"
+
+namespace gsx_amd {
+
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kMostAlternatives = 64;
+constexpr float kLeastFloat = -3.402823466e38f;
+
+// Of a set of logits: m, s and w as above.
+struct RowSums {
+    float m, s, w;
+};
+
+struct LogProbsArgs {
+    int64_t rows, vocab, logits_stride, grad_stride;
+    const int32_t* ids;  // may be null
+    float inv_t;
+    float scale2;  // log2(e) / temperature
+    float* chosen;   // may be null
+    float* entropy;  // may be null
+    float* stats;    // may be null: m, s, H
+    int32_t top;
+    int32_t* top_ids;
+    float* top_logs;
+    const float* row_grad;      // may be null: 1
+    const float* entropy_grad;  // may be null: 1
+    float grad_scale, entropy_scale;
+    int64_t slice, slices;  // logits of a workgroup where a row has several, and how many
+    RowSums* partial;       // of each slice
+    uint64_t* partial_top;  // [slice][top] keys
+};
+
+// u_j where e_j is not 0 (2^-149 is the least float), and finite for z_j = -inf, so that e_j u_j = 0 there. NaN is left to e_j.
+__device__ inline float scaled_from(float z, float base, float scale2) { return fmaxf((z - base) * scale2, -256.0f); }
+
+// Whole numbers in the order of the logits: NaN above everything, -0 with 0. 0 is below all of them, 2^32 - 1 above.
+__device__ inline uint32_t ordered_bits(float x) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.0f);
+    if (x != x) return 0xfffffffeu;
+    return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+__device__ inline float ordered_value(uint32_t o) {
+    return __builtin_bit_cast(float, o & 0x80000000u ? o ^ 0x80000000u : ~o);
+}
+constexpr uint32_t kOrderedClosed = 0x007fffffu;  // of -inf
+
+// The order of the alternatives: by value, then by the lowest index. 0: none.
+__device__ inline uint64_t key_of(float x, int64_t index) {
+    return (uint64_t)ordered_bits(x) << 32 | (0xffffffffu - (uint32_t)index);
+}
+__device__ inline bool key_open(uint64_t key) { return (uint32_t)(key >> 32) > kOrderedClosed; }
+
+template <int kCtrl>
+__device__ inline uint64_t dpp_move_u64(uint64_t v) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, kCtrl, 0xf, 0xf, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), kCtrl, 0xf, 0xf, false);
+    return (uint64_t)hi << 32 | lo;
+}
+
+// The largest key of a group; s_keys holds one for each of its waves.
+template <int kGroup>
+__device__ inline uint64_t max_key(uint64_t v, uint64_t* s_keys) {
+    const auto larger = [](uint64_t a, uint64_t b) { return a > b ? a : b; };
+    v = larger(v, dpp_move_u64<0xb1>(v));
+    v = larger(v, dpp_move_u64<0x4e>(v));
+    v = larger(v, dpp_move_u64<0x141>(v));
+    v = larger(v, dpp_move_u64<0x140>(v));
+    if constexpr (kGroup == 16) return v;
+    v = larger(v, __shfl_xor((unsigned long long)v, 16, 64));
+    v = larger(v, __shfl_xor((unsigned long long)v, 32, 64));
+    if constexpr (kGroup == 64) return v;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) s_keys[threadIdx.x / 64] = v;
+    __syncthreads();
+    v = s_keys[0];
+#pragma unroll
+    for (int i = 1; i < kGroup / 64; ++i) v = larger(v, s_keys[i]);
+    return v;
+}
+
+// Sums of two values over a group.
+template <int kGroup>
+__device__ inline float2 sums_of_group(float2 v, float2* s_wave) {
+    if constexpr (kGroup <= 64) return make_float2(sum_of_group<kGroup>(v.x, nullptr), sum_of_group<kGroup>(v.y, nullptr));
+    v = make_float2(wave_reduce_sum(v.x), wave_reduce_sum(v.y));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) s_wave[threadIdx.x / 64] = v;
+    __syncthreads();
+    v = s_wave[0];
+#pragma unroll
+    for (int w = 1; w < kGroup / 64; ++w) {
+        v.x += s_wave[w].x;
+        v.y += s_wave[w].y;
+    }
+    return v;
+}
+
+constexpr int kCandidates = 512;
+
+template <int kGroup>
+struct TopScratch {
+    uint64_t keys[kGroup == 16 ? 1 : kCandidates];
+    uint64_t wave_key[kGroup / 64 + 1];
+    float lane[kGroup > 64 ? kGroup : 1];
+    float threshold;
+    int count;
+};
+
+// The largest of the wave's 64 * kN values that at least k of them reach, or a lower one: its ordered bits are found from the
+// highest on, until exactly k values are left.
+template <int kN>
+__device__ inline float reached_by(const float (&v)[kN], int k) {
+    uint32_t o[kN];
+#pragma unroll
+    for (int i = 0; i < kN; ++i) o[i] = ordered_bits(v[i]);
+    uint32_t t = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t up = t | 1u << bit;
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < kN; ++i) n += __builtin_popcountll(__builtin_amdgcn_ballot_w64(o[i] >= up));
+        if (n >= k) t = up;
+        if (n == k) break;
+    }
+    return t <= kOrderedClosed ? -INFINITY : ordered_value(t);
+}
+
+// The keys of `count` candidates (LDS) in order: emit(place, key) for the first `top`, 0 where there are fewer. Every candidate
+// counts those before it.
+template <int kGroup, typename Emit>
+__device__ inline void emit_ranked(const uint64_t* s_keys, int count, int top, int tid, Emit emit) {
+    for (int c = tid; c < count; c += kGroup) {
+        const uint64_t key = s_keys[c];
+        int place = 0;
+        for (int j = 0; j < count; ++j) place += s_keys[j] > key ? 1 : 0;
+        if (place < top) emit(place, key);
+    }
+    for (int c = count + tid; c < top; c += kGroup) emit(c, 0);
+}
+
+// The `top` first alternatives of what a group holds in registers (each(f) calls f(value, index) for every one), in order.
+// `mine` is the thread's largest value; special: NaN or +inf are among them.
+template <int kGroup, typename Each, typename Emit>
+__device__ inline void top_of_group(Each each, float mine, bool special, int top, int tid, TopScratch<kGroup>& s, Emit emit) {
+    if constexpr (kGroup > 16) {
+        if (!special) {
+            // a value that the group's k-th largest thread reaches: at least k values do
+            float least;
+            group_sync<kGroup>();  // the row before is done
+            if (tid == 0) s.count = 0;
+            if constexpr (kGroup == 64) {
+                const float v[1] = {mine};
+                least = reached_by(v, top);
+            } else {
+                s.lane[tid] = mine;
+                __syncthreads();
+                if (tid < 64) {
+                    float v[kGroup / 64];
+#pragma unroll
+                    for (int i = 0; i < kGroup / 64; ++i) v[i] = s.lane[i * 64 + tid];
+                    const float t = reached_by(v, top);
+                    if (tid == 0) s.threshold = t;
+                }
+                __syncthreads();
+                least = s.threshold;
+            }
+            group_sync<kGroup>();
+            least = fmaxf(least, kLeastFloat);  // closed logits are no alternatives
+            each([&](float x, int64_t index) {
+                if (x >= least) {
+                    const int at = atomicAdd(&s.count, 1);
+                    if (at < kCandidates) s.keys[at] = key_of(x, index);
+                }
+            });
+            group_sync<kGroup>();
+            const int count = s.count;
+            if (count <= kCandidates) {
+                emit_ranked<kGroup>(s.keys, count, top, tid, emit);
+                return;
+            }
+        }
+    }
+    // one after the other
+    uint64_t before = ~0ull;
+    for (int place = 0; place < top; ++place) {
+        uint64_t best = 0;
+        each([&](float x, int64_t index) {
+            const uint64_t key = key_of(x, index);
+            if (key < before && key > best) best = key;
+        });
+        best = max_key<kGroup>(best, s.wave_key);
+        if (!key_open(best)) best = 0;
+        if (tid == 0) emit(place, best);
+        before = best;
+    }
+}
+
+// What a row's sums say to the outside.
+struct RowAnswer {
+    float m, log_s, inv_t;
+    __device__ inline float log_q(float z) const {
+        return z == -INFINITY && log_s == log_s ? -INFINITY : (z - m) * inv_t - log_s;
+    }
+};
+__device__ inline RowAnswer answer_of(const LogProbsArgs& a, RowSums q) { return {q.m, logf(q.s), a.inv_t}; }
+__device__ inline float entropy_of(RowSums q) { return q.s == 0.0f ? 0.0f : logf(q.s) - kLn2 * (q.w / q.s); }
+
+__device__ inline bool known_id(const LogProbsArgs& a, int64_t row, int32_t& id) {
+    id = a.ids != nullptr ? a.ids[row] : -1;
+    return id >= 0 && id < a.vocab;
+}
+
+// By one thread: a row's chosen log probability, entropy and statistics.
+template <typename T>
+__device__ inline void write_row(const LogProbsArgs& a, int64_t row, const T* __restrict__ z, RowSums q) {
+    int32_t id;
+    const bool known = known_id(a, row, id);
+    if (a.chosen != nullptr) a.chosen[row] = known ? answer_of(a, q).log_q(to_float(z[id])) : 0.0f;
+    const float h = entropy_of(q);
+    if (a.entropy != nullptr) a.entropy[row] = h;
+    if (a.stats != nullptr) {
+        a.stats[3 * row] = q.m;
+        a.stats[3 * row + 1] = q.s;
+        a.stats[3 * row + 2] = h;
+    }
+}
+
+__device__ inline void write_alternative(const LogProbsArgs& a, int64_t row, int place, uint64_t key, RowAnswer r) {
+    const int64_t at = row * a.top + place;
+    a.top_ids[at] = key == 0 ? -1 : (int32_t)(0xffffffffu - (uint32_t)key);
+    a.top_logs[at] = key == 0 ? -INFINITY : r.log_q(ordered_value((uint32_t)(key >> 32)));
+}
+
+// A row's gradient: dz = e (rate + slope u), and `own` more at the given label.
+struct RowGrad {
+    bool live;
+    float base, rate, slope, own;
+    int32_t id;
+    __device__ inline float at(float z, float scale2) const {
+        const float u = scaled_from(z, base, scale2);
+        return __builtin_amdgcn_exp2f((z - base) * scale2) * (rate + slope * u);
+    }
+};
+__device__ inline RowGrad grad_of(const LogProbsArgs& a, int64_t row, float m, float s, float h) {
+    RowGrad g;
+    const bool known = known_id(a, row, g.id);
+    const float gl = known ? a.grad_scale * (a.row_grad != nullptr ? a.row_grad[row] : 1.0f) : 0.0f;
+    const float gh = a.entropy_scale * (a.entropy_grad != nullptr ? a.entropy_grad[row] : 1.0f);
+    g.live = (gl != 0.0f || gh != 0.0f) && s != 0.0f;
+    g.base = m == -INFINITY ? 0.0f : m;
+    const float over = g.live ? a.inv_t / s : 0.0f;
+    g.slope = -(gh * kLn2) * over;
+    g.rate = -(gl + gh * (h - logf(s))) * over;
+    g.own = gl * a.inv_t;
+    if (!known) g.id = -1;
+    return g;
+}
+
+// Rows that fit the registers of a group: kGroup threads hold kVecs times 16 bytes each.
+template <typename T, int kGroup, int kVecs>
+struct HeldRow {
+    static constexpr int kElements = Words<T>::kElements;
+    Words<T> x[kVecs];
+    float last;
+    Stretch st;
+
+    __device__ inline void load(const T* __restrict__ z, int64_t length, int tid) {
+        st = stretch_of<T>(z, length, tid);
+#pragma unroll
+        for (int u = 0; u < kVecs; ++u) x[u] = load_words<T>(z + st.lead + u * kGroup * kElements, tid, st.vecs - u * kGroup);
+        last = st.loose >= 0 ? to_float(z[st.loose]) : -INFINITY;
+    }
+    __device__ inline float largest() const {
+        float m = last == last ? last : -INFINITY;
+#pragma unroll
+        for (int u = 0; u < kVecs; ++u)
+#pragma unroll
+            for (int i = 0; i < kElements; ++i) m = fmaxf(m, element_of(x[u], i));
+        return m;
+    }
+    __device__ inline float2 sums(float base, float scale2) {
+        float2 r;
+        r.x = __builtin_amdgcn_exp2f((last - base) * scale2);
+        r.y = r.x * scaled_from(last, base, scale2);
+#pragma unroll
+        for (int u = 0; u < kVecs; ++u) {
+            repack(x[u]);
+#pragma unroll
+            for (int i = 0; i < kElements; ++i) {
+                const float z = element_of(x[u], i);
+                const float e = __builtin_amdgcn_exp2f((z - base) * scale2);
+                r.x += e;
+                r.y += e * scaled_from(z, base, scale2);
+            }
+        }
+        return r;
+    }
+    // f(value, index) for every logit; behind the row's end there are some -inf
+    template <typename F>
+    __device__ inline void each(int tid, int64_t from, F f) {
+#pragma unroll
+        for (int u = 0; u < kVecs; ++u) {
+            repack(x[u]);
+            const int64_t at = from + st.lead + (int64_t)(u * kGroup + tid) * kElements;
+#pragma unroll
+            for (int i = 0; i < kElements; ++i) f(element_of(x[u], i), at + i);
+        }
+        f(last, from + st.loose);
+    }
+};
+
+template <typename T, int kGroup, int kVecs>
+__global__ __launch_bounds__(kGroup < 256 ? 256 : kGroup) void logprobs_held_kernel(LogProbsArgs a,
+                                                                                    const T* __restrict__ logits,
+                                                                                    T* __restrict__ grad) {
+    constexpr int kGroups = kGroup < 256 ? 256 / kGroup : 1;  // rows of a workgroup
+    constexpr int kElements = Words<T>::kElements;
+    __shared__ TopScratch<kGroup> s_top[kGroups];
+    __shared__ float2 s_wave2[16];
+    __shared__ float s_wave[16];
+    const int group = kGroups == 1 ? 0 : threadIdx.x / kGroup, tid = kGroups == 1 ? threadIdx.x : threadIdx.x % kGroup;
+    for (int64_t row = (int64_t)blockIdx.x * kGroups + group; row < a.rows; row += (int64_t)gridDim.x * kGroups) {
+        const T* const z = logits + row * a.logits_stride;
+        HeldRow<T, kGroup, kVecs> x;
+        x.load(z, a.vocab, tid);
+        const float mine = x.largest();
+        RowSums q;
+        q.m = max_of_group<kGroup>(mine, s_wave);
+        const float base = q.m == -INFINITY ? 0.0f : q.m;
+        const float2 sums = sums_of_group<kGroup>(x.sums(base, a.scale2), s_wave2);
+        q.s = sums.x;
+        q.w = sums.y;
+        if (tid == 0) write_row(a, row, z, q);
+        if (a.top > 0) {
+            const RowAnswer r = answer_of(a, q);
+            top_of_group<kGroup>([&](auto f) { x.each(tid, 0, f); }, mine, q.s != q.s, a.top, tid, s_top[group],
+                                 [&](int place, uint64_t key) { write_alternative(a, row, place, key, r); });
+        }
+        if (grad == nullptr) continue;
+        T* const g = grad + row * a.grad_stride;
+        const RowGrad d = grad_of(a, row, q.m, q.s, entropy_of(q));
+#pragma unroll
+        for (int u = 0; u < kVecs; ++u) {
+            float y[kElements];
+            repack(x.x[u]);
+#pragma unroll
+            for (int i = 0; i < kElements; ++i) y[i] = d.live ? d.at(element_of(x.x[u], i), a.scale2) : 0.0f;
+            const int own = d.id - x.st.lead - (u * kGroup + tid) * kElements;
+            if (d.live && d.id >= 0 && own >= 0 && own < kElements) {
+#pragma unroll
+                for (int i = 0; i < kElements; ++i) y[i] += i == own ? d.own : 0.0f;
+            }
+            store_words<T>(g + x.st.lead + u * kGroup * kElements, tid, x.st.vecs - u * kGroup, y);
+        }
+        if (x.st.loose >= 0)
+            g[x.st.loose] = from_float<T>(d.live ? d.at(x.last, a.scale2) + (d.id == x.st.loose ? d.own : 0.0f) : 0.0f);
+    }
+}
+
+// Longer rows, and few of them: a row is cut into slices, each held by a workgroup. This launch leaves every slice's sums and its
+// first alternatives,
+constexpr int kSliceGroup = 256;
+
+template <typename T, int kVecs>
+__global__ __launch_bounds__(kSliceGroup) void logprobs_slices_kernel(LogProbsArgs a, const T* __restrict__ logits) {
+    __shared__ TopScratch<kSliceGroup> s_top;
+    __shared__ float2 s_wave2[16];
+    __shared__ float s_wave[16];
+    const int64_t total = a.rows * a.slices;
+    for (int64_t b = blockIdx.x; b < total; b += gridDim.x) {
+        const int64_t row = b / a.slices, from = b % a.slices * a.slice, to = min(from + a.slice, a.vocab);
+        HeldRow<T, kSliceGroup, kVecs> x;
+        x.load(logits + row * a.logits_stride + from, to - from, threadIdx.x);
+        const float mine = x.largest();
+        const float m = max_of_group<kSliceGroup>(mine, s_wave);
+        const float base = m == -INFINITY ? 0.0f : m;
+        const float2 sums = sums_of_group<kSliceGroup>(x.sums(base, a.scale2), s_wave2);
+        if (threadIdx.x == 0) a.partial[b] = {m, sums.x, sums.y};
+        if (a.top > 0)
+            top_of_group<kSliceGroup>([&](auto f) { x.each(threadIdx.x, from, f); }, mine, sums.x != sums.x, a.top,
+                                      threadIdx.x, s_top, [&](int place, uint64_t key) { a.partial_top[b * a.top + place] = key; });
+    }
+}
+
+// and this one joins a row's.
+template <typename T>
+__global__ __launch_bounds__(kSliceGroup) void logprobs_join_kernel(LogProbsArgs a, const T* __restrict__ logits) {
+    __shared__ uint64_t s_keys[kCandidates], s_kept[kMostAlternatives];
+    __shared__ float2 s_wave2[16];
+    __shared__ float s_wave[16];
+    __shared__ int s_count;
+    const int tid = threadIdx.x;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const RowSums* const part = a.partial + row * a.slices;
+        float m = -INFINITY;
+        for (int64_t i = tid; i < a.slices; i += kSliceGroup) m = fmaxf(m, part[i].m);
+        RowSums q;
+        q.m = max_of_group<kSliceGroup>(m, s_wave);
+        const float base = q.m == -INFINITY ? 0.0f : q.m;
+        float2 sums = make_float2(0.0f, 0.0f);
+        for (int64_t i = tid; i < a.slices; i += kSliceGroup) {
+            const RowSums p = part[i];
+            const float u = scaled_from(p.m, base, a.scale2), f = __builtin_amdgcn_exp2f((p.m - base) * a.scale2);
+            sums.x += f * p.s;
+            sums.y += f * (p.w + u * p.s);
+        }
+        sums = sums_of_group<kSliceGroup>(sums, s_wave2);
+        q.s = sums.x;
+        q.w = sums.y;
+        if (tid == 0) write_row(a, row, logits + row * a.logits_stride, q);
+        if (a.top == 0) continue;
+        const RowAnswer r = answer_of(a, q);
+        const uint64_t* const keys = a.partial_top + row * a.slices * a.top;
+        const int64_t all = a.slices * a.top;
+        // rounds of keys that come before the last of the `top` first ones so far
+        if (tid == 0) s_count = 0;
+        uint64_t least = 0;
+        __syncthreads();
+        for (int64_t i0 = 0; i0 < all; i0 += kSliceGroup) {
+            const uint64_t key = i0 + tid < all ? keys[i0 + tid] : 0;
+            if (key > least) s_keys[atomicAdd(&s_count, 1)] = key;
+            __syncthreads();
+            const int count = s_count;
+            if (count + kSliceGroup > kCandidates && i0 + kSliceGroup < all) {
+                emit_ranked<kSliceGroup>(s_keys, count, a.top, tid, [&](int place, uint64_t k) { s_kept[place] = k; });
+                __syncthreads();
+                if (tid < a.top) s_keys[tid] = s_kept[tid];
+                least = s_kept[a.top - 1];
+                if (tid == 0) s_count = a.top;
+            }
+            __syncthreads();
+        }
+        emit_ranked<kSliceGroup>(s_keys, s_count, a.top, tid,
+                                 [&](int place, uint64_t key) { write_alternative(a, row, place, key, r); });
+        __syncthreads();
+    }
+}
+
+// The gradient from a forward's statistics: kGroup threads take a stretch of a row.
+template <typename T, int kGroup>
+__global__ __launch_bounds__(256) void logprobs_grad_kernel(LogProbsArgs a, const T* __restrict__ logits,
+                                                            T* __restrict__ grad) {
+    constexpr int kGroups = 256 / kGroup, kElements = Words<T>::kElements, kAhead = 4;
+    const int group = threadIdx.x / kGroup, tid = threadIdx.x % kGroup;
+    const int64_t total = a.rows * a.slices;
+    for (int64_t b = (int64_t)blockIdx.x * kGroups + group; b < total; b += (int64_t)gridDim.x * kGroups) {
+        const int64_t row = b / a.slices, from = b % a.slices * a.slice, to = min(from + a.slice, a.vocab);
+        const T* const z = logits + row * a.logits_stride + from;
+        T* const g = grad + row * a.grad_stride + from;
+        const RowGrad d = grad_of(a, row, a.stats[3 * row], a.stats[3 * row + 1], a.stats[3 * row + 2]);
+        const Stretch st = stretch_of<T>(z, to - from, tid);
+        for (int v = tid; v < st.vecs; v += kGroup * kAhead) {
+            Words<T> x[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) x[u] = load_words<T>(z + st.lead, v + u * kGroup, d.live ? st.vecs : 0);
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                float y[kElements];
+#pragma unroll
+                for (int i = 0; i < kElements; ++i) y[i] = d.live ? d.at(element_of(x[u], i), a.scale2) : 0.0f;
+                const int64_t own = d.id - from - st.lead - (int64_t)(v + u * kGroup) * kElements;
+                if (d.live && d.id >= 0 && own >= 0 && own < kElements) {
+#pragma unroll
+                    for (int i = 0; i < kElements; ++i) y[i] += i == own ? d.own : 0.0f;
+                }
+                store_words<T>(g + st.lead, v + u * kGroup, st.vecs, y);
+            }
+        }
+        if (st.loose >= 0)
+            g[st.loose] = from_float<T>(
+                d.live ? d.at(to_float(z[st.loose]), a.scale2) + (d.id >= 0 && d.id - from == st.loose ? d.own : 0.0f) : 0.0f);
+    }
+}
+
+}  // namespace gsx_amd
+
+using namespace gsx_amd;
+
+namespace {
+
+// How a forward goes: by groups that hold whole rows (group > 0), or by slices. The smallest group that holds a row in 16 vectors
+// a thread; above 16 KB only where there are rows enough for the GPU's 256 CUs.
+struct LogProbsPlan {
+    int group, vecs;
+    int64_t slice, slices;
+};
+
+LogProbsPlan logprobs_plan(int64_t rows, int64_t vocab, int64_t bytes, int32_t top) {
+    LogProbsPlan p = {};
+    const int64_t vecs = vocab * bytes / 16;
+    if (vecs <= 16 * 4 && top <= 8) p.group = 16;
+    else if (vecs <= 64 * 4) p.group = 64;
+    else if (vecs <= 256 * 4 || (vecs <= 256 * 16 && rows >= 192)) p.group = 256;
+    else if (vecs <= 512 * 16 && rows >= 192) p.group = 512;
+    else if (vecs <= 1024 * 16 && rows >= 192) p.group = 1024;
+    if (p.group != 0) {
+        p.vecs = vecs > 0 ? (int)ceil_div(vecs, p.group) : 1;
+        return p;
+    }
+    // slices of 16 KB, or of 64 KB where that makes 1024 of them
+    const int64_t most = 65536 / bytes, least = 16384 / bytes;
+    p.slice = rows * ceil_div(vocab, most) >= 1024 ? most : least;
+    p.vecs = p.slice == most ? 16 : 4;
+    p.slices = ceil_div(vocab, p.slice);
+    return p;
+}
+
+int64_t sums_bytes(int64_t rows, int64_t slices) { return ceil_div(rows * slices * (int64_t)sizeof(RowSums), 16) * 16; }
+
+inline dim3 logprobs_grid(int64_t blocks) { return dim3((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20)); }
+
+template <typename T, int kGroup, int kVecs>
+gsx_hip_status launch_held(const LogProbsArgs& a, const T* logits, T* grad, hipStream_t stream) {
+    const int per = kGroup < 256 ? 256 / kGroup : 1;
+    hipLaunchKernelGGL((logprobs_held_kernel<T, kGroup, kVecs>), logprobs_grid(ceil_div(a.rows, per)),
+                       dim3(kGroup < 256 ? 256 : kGroup), 0, stream, a, logits, grad);
+    return fields_launched("log probabilities launch");
+}
+
+template <typename T>
+gsx_hip_status launch_grad(LogProbsArgs a, const T* logits, T* grad, hipStream_t stream) {
+    const int64_t vecs = a.vocab * (int64_t)sizeof(T) / 16;
+    const auto go = [&](auto kernel, int groups) {
+        hipLaunchKernelGGL(kernel, logprobs_grid(ceil_div(a.rows * a.slices, groups)), dim3(256), 0, stream, a, logits, grad);
+    };
+    a.slice = a.vocab;
+    a.slices = 1;
+    if (vecs <= 64) go(logprobs_grad_kernel<T, 16>, 16);
+    else if (vecs <= 256) go(logprobs_grad_kernel<T, 64>, 4);
+    else {
+        a.slice = 16384 / (int64_t)sizeof(T);
+        a.slices = ceil_div(a.vocab, a.slice);
+        go(logprobs_grad_kernel<T, 256>, 1);
+    }
+    return fields_launched("log probabilities launch");
+}
+
+template <typename T>
+gsx_hip_status launch_logprobs(const LogProbsPlan& p, LogProbsArgs a, const T* logits, T* grad, void* temp,
+                               hipStream_t stream) {
+    if (p.group == 16) {
+        if (p.vecs <= 1) return launch_held<T, 16, 1>(a, logits, grad, stream);
+        if (p.vecs <= 2) return launch_held<T, 16, 2>(a, logits, grad, stream);
+        return launch_held<T, 16, 4>(a, logits, grad, stream);
+    }
+    if (p.group == 64) {
+        if (p.vecs <= 1) return launch_held<T, 64, 1>(a, logits, grad, stream);
+        return launch_held<T, 64, 4>(a, logits, grad, stream);
+    }
+    if (p.group == 256) {
+        if (p.vecs <= 4) return launch_held<T, 256, 4>(a, logits, grad, stream);
+        if (p.vecs <= 8) return launch_held<T, 256, 8>(a, logits, grad, stream);
+        return launch_held<T, 256, 16>(a, logits, grad, stream);
+    }
+    if (p.group == 512) return launch_held<T, 512, 16>(a, logits, grad, stream);
+    if (p.group == 1024) return launch_held<T, 1024, 16>(a, logits, grad, stream);
+    a.slice = p.slice;
+    a.slices = p.slices;
+    a.partial = static_cast<RowSums*>(temp);
+    a.partial_top = reinterpret_cast<uint64_t*>(static_cast<uint8_t*>(temp) + sums_bytes(a.rows, p.slices));
+    const dim3 grid = logprobs_grid(a.rows * p.slices);
+    if (p.vecs == 16) hipLaunchKernelGGL((logprobs_slices_kernel<T, 16>), grid, dim3(kSliceGroup), 0, stream, a, logits);
+    else hipLaunchKernelGGL((logprobs_slices_kernel<T, 4>), grid, dim3(kSliceGroup), 0, stream, a, logits);
+    hipLaunchKernelGGL((logprobs_join_kernel<T>), logprobs_grid(a.rows), dim3(kSliceGroup), 0, stream, a, logits);
+    if (grad == nullptr) return fields_launched("log probabilities launch");
+    return launch_grad<T>(a, logits, grad, stream);
+}
+
+gsx_hip_status logprobs_check(const LogProbsArgs& a, const void* logits, int32_t type, float temperature, const void* grad) {
+    if (!known_type(type)) return fields_fail(GSX_HIP_ERROR_NOT_SUPPORTED, "log probabilities: logits are f32, bf16 or f16");
+    if (a.vocab < 1 || a.vocab > INT32_MAX)
+        return fields_fail(GSX_HIP_ERROR_OUT_OF_RANGE, "log probabilities: 1 to 2^31 - 1 logits a row");
+    if (a.top < 0 || a.top > kMostAlternatives || a.top > a.vocab)
+        return fields_fail(GSX_HIP_ERROR_OUT_OF_RANGE, "log probabilities: 0 to 64 alternatives, no more than logits");
+    if (!rows_fit(a.rows, a.logits_stride, a.vocab) ||
+        (grad != nullptr && !rows_fit(a.rows, a.grad_stride, a.vocab)))
+        return fields_fail(GSX_HIP_ERROR_INVALID_ARGUMENT,
+                           "log probabilities: rows must be >= 0 and strides at least the row's length");
+    if (!(temperature >= 1e-6f) || !(temperature <= 1e6f))
+        return fields_fail(GSX_HIP_ERROR_INVALID_ARGUMENT, "log probabilities: the temperature must lie between 1e-6 and 1e6");
+    if (a.rows > 0 && (logits == nullptr || (a.top > 0 && (a.top_ids == nullptr || a.top_logs == nullptr))))
+        return fields_fail(GSX_HIP_ERROR_INVALID_ARGUMENT, "log probabilities: null pointer");
+    if (!aligned_to(logits, type_bytes(type)) || !aligned_to(grad, type_bytes(type)) || !aligned_to(a.ids, 4) ||
+        !aligned_to(a.chosen, 4) || !aligned_to(a.entropy, 4) || !aligned_to(a.stats, 4) || !aligned_to(a.top_ids, 4) ||
+        !aligned_to(a.top_logs, 4) || !aligned_to(a.row_grad, 4) || !aligned_to(a.entropy_grad, 4))
+        return fields_fail(GSX_HIP_ERROR_INVALID_ARGUMENT, "log probabilities: pointers must be aligned to their elements");
+    if (logits != nullptr && logits == grad)
+        return fields_fail(GSX_HIP_ERROR_INVALID_ARGUMENT, "log probabilities: the gradient may not overwrite the logits");
+    return GSX_HIP_SUCCESS;
+}
+
+LogProbsArgs logprobs_args(int64_t logits_stride, int64_t rows, int64_t vocab, const int32_t* ids, float temperature,
+                           const float* row_grad, float grad_scale, const float* entropy_grad, float entropy_scale,
+                           int64_t grad_stride) {
+    LogProbsArgs a = {};
+    a.rows = rows;
+    a.vocab = vocab;
+    a.logits_stride = logits_stride;
+    a.grad_stride = grad_stride;
+    a.ids = ids;
+    a.inv_t = 1.0f / temperature;
+    a.scale2 = kLog2e / temperature;
+    a.row_grad = row_grad;
+    a.grad_scale = grad_scale;
+    a.entropy_grad = entropy_grad;
+    a.entropy_scale = entropy_scale;
+    return a;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t gsx_hip_log_probs_temp_bytes(int64_t rows, int64_t vocab, int32_t top) {
+    if (rows <= 0 || vocab <= 0 || vocab > INT32_MAX || top < 0 || top > kMostAlternatives || rows > (INT64_MAX >> 4) / vocab)
+        return 0;
+    int64_t most = 0;  // whatever the logits' type is
+    for (int64_t bytes = 2; bytes <= 4; bytes += 2) {
+        const LogProbsPlan p = logprobs_plan(rows, vocab, bytes, top);
+        if (p.group != 0) continue;
+        const int64_t need = sums_bytes(rows, p.slices) + rows * p.slices * top * 8;
+        if (need > most) most = need;
+    }
+    return (size_t)most;
+}
+
+gsx_hip_status gsx_hip_log_probs_forward(const void* logits, int32_t logits_type, int64_t logits_stride, int64_t rows,
+                                         int64_t vocab, const int32_t* ids, float temperature, float* chosen,
+                                         float* entropy, float* row_stats, int32_t top, int32_t* top_ids,
+                                         float* top_log_probs, void* grad_logits, int64_t grad_stride,
+                                         const float* row_grad, float grad_scale, const float* entropy_grad,
+                                         float entropy_scale, void* temp, hipStream_t stream) {
+    LogProbsArgs a = logprobs_args(logits_stride, rows, vocab, ids, temperature, row_grad, grad_scale, entropy_grad,
+                                   entropy_scale, grad_stride);
+    a.chosen = chosen;
+    a.entropy = entropy;
+    a.stats = row_stats;
+    a.top = top;
+    a.top_ids = top_ids;
+    a.top_logs = top_log_probs;
+    const gsx_hip_status st = logprobs_check(a, logits, logits_type, temperature, grad_logits);
+    if (st != GSX_HIP_SUCCESS || rows == 0) return st;
+    const LogProbsPlan p = logprobs_plan(rows, vocab, type_bytes(logits_type), top);
+    if (p.group == 0 && (temp == nullptr || !aligned_to(temp, 16)))
+        return fields_fail(GSX_HIP_ERROR_INVALID_ARGUMENT,
+                           "log probabilities: the workspace must be non-null and 16-byte aligned");
+    if (grad_logits != nullptr && row_stats == nullptr)
+        return fields_fail(GSX_HIP_ERROR_INVALID_ARGUMENT, "log probabilities: a gradient needs row_stats");
+    return with_type(logits_type, [&](auto t) {
+        using T = decltype(t);
+        return launch_logprobs<T>(p, a, static_cast<const T*>(logits), static_cast<T*>(grad_logits), temp, stream);
+    });
+}
+
+gsx_hip_status gsx_hip_log_probs_backward(const void* logits, int32_t logits_type, int64_t logits_stride, int64_t rows,
+                                          int64_t vocab, const int32_t* ids, float temperature, const float* row_stats,
+                                          const float* row_grad, float grad_scale, const float* entropy_grad,
+                                          float entropy_scale, void* grad_logits, int64_t grad_stride, hipStream_t stream) {
+    LogProbsArgs a = logprobs_args(logits_stride, rows, vocab, ids, temperature, row_grad, grad_scale, entropy_grad,
+                                   entropy_scale, grad_stride);
+    a.stats = const_cast<float*>(row_stats);  // read only
+    const gsx_hip_status st = logprobs_check(a, logits, logits_type, temperature, grad_logits);
+    if (st != GSX_HIP_SUCCESS || rows == 0) return st;
+    if (row_stats == nullptr || grad_logits == nullptr)
+        return fields_fail(GSX_HIP_ERROR_INVALID_ARGUMENT, "log probabilities backward: null pointer");
+    return with_type(logits_type, [&](auto t) {
+        using T = decltype(t);
+        return launch_grad<T>(a, static_cast<const T*>(logits), static_cast<T*>(grad_logits), stream);
+    });
+}
+
+}  // extern "C"

@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes
 from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 
@@ -20,7 +21,7 @@ from . import _lib
 from ._lib import GsxHipError, check
 
 __all__ = ["Blocks", "lookup", "lookup_backward", "quantize", "matmul", "linear", "linear_backward", "distill",
-           "distill_backward"]
+           "distill_backward", "LogProbs", "log_probs", "log_probs_backward"]
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 3, torch.float16: 4}  # GSX_HIP_DTYPE_*
 BLOCK = 128
@@ -309,6 +310,90 @@ def distill_backward(logits: torch.Tensor, row_stats: torch.Tensor, teacher_ids:
         to, to_stride = _rows(result, "grad", logits.dtype, (rows, vocab))
         check(lib.gsx_hip_distill_backward(base, code, stride, rows, vocab, ids, t, t_stride, top, temperature, weight,
                                            stats, upstream, grad_scale, to, to_stride, handle), "distill backward")
+        return result
+
+    return _run(stream, call)
+
+
+class LogProbs(NamedTuple):
+    """What `log_probs` says of each row; `top_ids` and `top_log_probs` are what `distill` takes as a teacher's entries."""
+
+    chosen: torch.Tensor         # float32 [rows]: log probability of the given label, 0 for a row without one
+    entropy: torch.Tensor        # float32 [rows]
+    top_ids: torch.Tensor        # int32 [rows, top], -1 where there are fewer alternatives
+    top_log_probs: torch.Tensor  # float32 [rows, top]
+    row_stats: torch.Tensor      # float32 [rows, 3], for `log_probs_backward`
+    grad: torch.Tensor | None    # the logits' gradient
+
+
+def log_probs(logits: torch.Tensor, ids: torch.Tensor | None = None, top: int = 0, temperature: float = 1.0,
+              grad_scale: float | None = None, row_grad: torch.Tensor | None = None, entropy_scale: float | None = None,
+              entropy_grad: torch.Tensor | None = None, grad: torch.Tensor | None = None, stream=None) -> LogProbs:
+    """Log probabilities of one int32 label a row (what lies outside the logits is no label), entropies and the `top` (at most 64)
+    likeliest labels. With grad_scale or entropy_scale, the logits' gradient comes from the same pass (into `grad` if given): for
+    upstream gradients grad_scale * row_grad of `chosen` and entropy_scale * entropy_grad of `entropy`."""
+    lib = _lib.load(require_device=False)
+    base, stride = _rows(logits, "logits")
+    code = _type(logits.dtype)
+    rows, vocab = logits.shape
+    id_ptr = _vector(ids, "ids", torch.int32, rows)
+    upstream = _vector(row_grad, "row_grad", torch.float32, rows)
+    entropy_upstream = _vector(entropy_grad, "entropy_grad", torch.float32, rows)
+    wanted = grad_scale is not None or entropy_scale is not None
+    if not wanted and not (grad is None and row_grad is None and entropy_grad is None):
+        raise GsxHipError("a gradient needs a grad_scale or an entropy_scale")
+    if (row_grad is not None and grad_scale is None) or (entropy_grad is not None and entropy_scale is None):
+        raise GsxHipError("row_grad needs a grad_scale, entropy_grad an entropy_scale")
+    if top < 0:
+        raise GsxHipError("the number of alternatives must be >= 0")
+
+    def call(handle):
+        def floats(*shape):
+            return torch.empty(shape, dtype=torch.float32, device=logits.device)
+
+        chosen, entropy, stats, top_logs = floats(rows), floats(rows), floats(rows, 3), floats(rows, top)
+        top_ids = torch.empty((rows, top), dtype=torch.int32, device=logits.device)
+        result, to, to_stride = grad, None, 0
+        if wanted:
+            if result is None:
+                result = torch.empty((rows, vocab), dtype=logits.dtype, device=logits.device)
+            to, to_stride = _rows(result, "grad", logits.dtype, (rows, vocab))
+        temp = _temp(lib.gsx_hip_log_probs_temp_bytes(rows, vocab, top))
+        check(lib.gsx_hip_log_probs_forward(base, code, stride, rows, vocab, id_ptr, temperature, chosen.data_ptr(),
+                                            entropy.data_ptr(), stats.data_ptr(), top, top_ids.data_ptr(),
+                                            top_logs.data_ptr(), to, to_stride, upstream, grad_scale or 0.0,
+                                            entropy_upstream, entropy_scale or 0.0, _address(temp), handle),
+              "log probabilities")
+        return LogProbs(chosen, entropy, top_ids, top_logs, stats, result)
+
+    return _run(stream, call)
+
+
+def log_probs_backward(logits: torch.Tensor, row_stats: torch.Tensor, ids: torch.Tensor | None = None,
+                       row_grad: torch.Tensor | None = None, entropy_grad: torch.Tensor | None = None,
+                       temperature: float = 1.0, grad_scale: float = 1.0, entropy_scale: float | None = None,
+                       grad: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """The logits' gradient for upstream gradients grad_scale * row_grad of `chosen` and entropy_scale * entropy_grad of `entropy`
+    (entropy_scale: 1 if there is an entropy_grad, else 0), from `log_probs`' row_stats."""
+    lib = _lib.load(require_device=False)
+    base, stride = _rows(logits, "logits")
+    code = _type(logits.dtype)
+    rows, vocab = logits.shape
+    id_ptr = _vector(ids, "ids", torch.int32, rows)
+    stats, stats_stride = _rows(row_stats, "row_stats", torch.float32, (rows, 3))
+    if stats_stride != 3:
+        raise GsxHipError("row_stats must be contiguous")
+    upstream = _vector(row_grad, "row_grad", torch.float32, rows)
+    entropy_upstream = _vector(entropy_grad, "entropy_grad", torch.float32, rows)
+    if entropy_scale is None:
+        entropy_scale = 0.0 if entropy_grad is None else 1.0
+
+    def call(handle):
+        result = torch.empty((rows, vocab), dtype=logits.dtype, device=logits.device) if grad is None else grad
+        to, to_stride = _rows(result, "grad", logits.dtype, (rows, vocab))
+        check(lib.gsx_hip_log_probs_backward(base, code, stride, rows, vocab, id_ptr, temperature, stats, upstream, grad_scale,
+                                             entropy_upstream, entropy_scale, to, to_stride, handle),
+              "log probabilities backward")
         return result
 
     return _run(stream, call)

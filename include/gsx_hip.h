@@ -601,6 +601,31 @@ gsx_hip_status gsx_hip_distill_backward(const void* logits, int32_t logits_type,
                                         const float* row_stats, const float* row_grad, float grad_scale,
                                         void* grad_logits, int64_t grad_stride, hipStream_t stream);
 
+/* Log probabilities of given labels, entropies and top alternatives. Row r of `logits` [rows, vocab] is z; with T the
+ * temperature (1e-6 to 1e6), q = softmax(z / T) and id = ids[r]:
+ *   chosen[r] = log q_id (0 where ids is null or id lies outside [0, vocab): a row without a label),
+ *   entropy[r] = -sum_j q_j log q_j (a logit of -inf has q = 0 and adds nothing),
+ *   top_ids, top_log_probs [rows, top] (contiguous, top at most 64 and vocab): the largest logits and their log q, of equal ones
+ *   the lowest index first (-0 equals 0); a logit of -inf is no alternative: where there are fewer, the id is -1 and log q -inf,
+ *   row_stats [rows][3]: max z, the sum of exp((z - max z) / T), the entropy; for the gradient,
+ *   dz_j = (gl (delta_{j,id} - q_j) - gh q_j (log q_j + entropy)) / T with gl = grad_scale * row_grad[r] (null: 1; 0 for a row
+ *   without a label) and gh = entropy_scale * entropy_grad[r] (null: 1), in the logits' type.
+ * A row with gl = gh = 0 has gradient 0 whatever its logits are. A row of nothing but -inf has no distribution: chosen -inf (if
+ * it has a label), entropy 0, gradient 0, no alternatives. NaN or +inf in a row's logits gives NaN for chosen, entropy and log
+ * q; alternatives are then ordered NaN, +inf, the others. Any of chosen, entropy and row_stats may be null, ids too; a gradient
+ * from forward (grad_logits not null) needs row_stats. The gradient may not overlap the logits. */
+size_t gsx_hip_log_probs_temp_bytes(int64_t rows, int64_t vocab, int32_t top);
+gsx_hip_status gsx_hip_log_probs_forward(const void* logits, int32_t logits_type, int64_t logits_stride, int64_t rows,
+                                         int64_t vocab, const int32_t* ids, float temperature, float* chosen,
+                                         float* entropy, float* row_stats, int32_t top, int32_t* top_ids,
+                                         float* top_log_probs, void* grad_logits, int64_t grad_stride,
+                                         const float* row_grad, float grad_scale, const float* entropy_grad,
+                                         float entropy_scale, void* temp, hipStream_t stream);
+gsx_hip_status gsx_hip_log_probs_backward(const void* logits, int32_t logits_type, int64_t logits_stride, int64_t rows,
+                                          int64_t vocab, const int32_t* ids, float temperature, const float* row_stats,
+                                          const float* row_grad, float grad_scale, const float* entropy_grad,
+                                          float entropy_scale, void* grad_logits, int64_t grad_stride, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

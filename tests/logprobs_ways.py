@@ -1,0 +1,25 @@
+"""Rows x logits, alternatives and the kernel that each takes (part of its name in the library), by the logits' type."""
+
+
+def _ways(t, wide):
+    k = 1 if wide else 2  # elements of 4 bytes
+    return [
+        (5, 3, 2, f"held_kernelI{t}Li16ELi1E"),
+        (33, 40 * k, 3, f"held_kernelI{t}Li16ELi1E"),
+        (9, 120 * k, 8, f"held_kernelI{t}Li16ELi2E"),
+        (21, 250 * k + 1, 5, f"held_kernelI{t}Li16ELi4E"),
+        (6, 150, 9, f"held_kernelI{t}Li64ELi1E"),
+        (6, 150, 64, f"held_kernelI{t}Li64ELi1E"),
+        (5, 1021 * k, 64, f"held_kernelI{t}Li64ELi4E"),
+        (4, 1500 * k + 1, 64, f"held_kernelI{t}Li256ELi4E"),
+        (3, 4111 * k, 20, f"slices_kernelI{t}Li4E"),
+        (193, 6001 * k, 33, f"held_kernelI{t}Li256ELi8E"),
+        (192, 16001 * k, 8, f"held_kernelI{t}Li256ELi16E"),
+        (193, 30011 * k, 20, f"held_kernelI{t}Li512ELi16E"),
+        (192, 65000 * k, 64, f"held_kernelI{t}Li1024ELi16E"),
+        (1, 65537 * k, 20, f"slices_kernelI{t}Li4E"),
+        (200, 90001 * k, 7, f"slices_kernelI{t}Li16E"),
+    ]
+
+
+WAYS = {"f": _ways("f", True), "DF16b": _ways("DF16b", False), "DF16_": _ways("DF16_", False)}
