@@ -129,31 +129,6 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_columns_kernel(const T
 // The matrix instructions take b as their first operand: a lane then holds four consecutive columns of one row of c. Which
 // row of b a lane brings for instruction j is chosen so that its 4 TN columns are consecutive too, and leave in wide stores.
 
-struct ProductTile {
-    int64_t m0, n0;
-    int64_t first, last;  // blocks of k
-    int64_t split;
-};
-
-// Tiles in bands of eight rows of tiles, so that workgroups that run together share operands in an L2; workgroup b runs on
-// XCD b % 8 and takes its share of the sequence in one piece.
-__device__ inline ProductTile product_tile(int64_t t, int64_t total, int64_t tiles_m, int64_t tiles_n, int bm, int bn,
-                                           int64_t blocks, int64_t splits) {
-    const int64_t per = (total + 7) / 8;
-    const int64_t whole = total / 8 * 8;
-    int64_t at = total % 8 == 0 ? (t % 8) * per + t / 8 : (t < whole ? (t % 8) * (total / 8) + t / 8 : t);
-    ProductTile r;
-    r.split = at % splits;
-    at /= splits;
-    const int64_t band = at / (8 * tiles_n), in_band = at % (8 * tiles_n);
-    const int64_t rows = min((int64_t)8, tiles_m - band * 8);
-    r.m0 = (band * 8 + in_band % rows) * bm;
-    r.n0 = in_band / rows * bn;
-    r.first = blocks * r.split / splits;
-    r.last = blocks * (r.split + 1) / splits;
-    return r;
-}
-
 // Begins a wave's loads of a whole block, which go straight to LDS.
 template <int kLoads, int BM, int kWaves>
 __device__ __forceinline__ void load_block(uint8_t* __restrict__ to, const uint8_t* a_from, const uint8_t* b_from,
@@ -384,7 +359,7 @@ bool product_sizes(int64_t m, int64_t n, int64_t k) {
 
 // Groups enough that no thread adds many splits, no more than there are (799 x 3734 in two parts: one group 9 us, sixteen 43).
 template <typename O>
-static void launch_join(const float* partial, int64_t m, int64_t n, int64_t splits, O* out, int64_t out_stride,
+void launch_join(const float* partial, int64_t m, int64_t n, int64_t splits, O* out, int64_t out_stride,
                         hipStream_t stream) {
     const auto go = [&](auto kernel, int64_t groups) {
         hipLaunchKernelGGL(kernel, dim3(blocks_grid(ceil_div(ceil_div(m * n, 4), 256 / groups))), dim3(256), 0, stream, partial, m,
@@ -394,6 +369,10 @@ static void launch_join(const float* partial, int64_t m, int64_t n, int64_t spli
     else if (splits >= 8) go(product_join_kernel<O, 4>, 4);
     else go(product_join_kernel<O, 1>, 1);
 }
+
+template void launch_join<float>(const float*, int64_t, int64_t, int64_t, float*, int64_t, hipStream_t);
+template void launch_join<__bf16>(const float*, int64_t, int64_t, int64_t, __bf16*, int64_t, hipStream_t);
+template void launch_join<_Float16>(const float*, int64_t, int64_t, int64_t, _Float16*, int64_t, hipStream_t);
 
 gsx_hip_status join_products(const float* partial, int64_t m, int64_t n, int64_t splits, float* out, int64_t out_stride,
                              hipStream_t stream) {

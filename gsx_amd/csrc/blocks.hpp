@@ -322,12 +322,39 @@ __device__ inline int swizzle_b(int row) {
     return (row & 3) | ((row / (4 * TN)) & 1) << 2;
 }
 
+struct ProductTile {
+    int64_t m0, n0;
+    int64_t first, last;  // blocks of k
+    int64_t split;
+};
+
+// Tiles in bands of eight rows of tiles, so that workgroups that run together share operands in an L2; workgroup b runs on
+// XCD b % 8 and takes its share of the sequence in one piece.
+__device__ inline ProductTile product_tile(int64_t t, int64_t total, int64_t tiles_m, int64_t tiles_n, int bm, int bn,
+                                           int64_t blocks, int64_t splits) {
+    const int64_t per = (total + 7) / 8;
+    const int64_t whole = total / 8 * 8;
+    int64_t at = total % 8 == 0 ? (t % 8) * per + t / 8 : (t < whole ? (t % 8) * (total / 8) + t / 8 : t);
+    ProductTile r;
+    r.split = at % splits;
+    at /= splits;
+    const int64_t band = at / (8 * tiles_n), in_band = at % (8 * tiles_n);
+    const int64_t rows = min((int64_t)8, tiles_m - band * 8);
+    r.m0 = (band * 8 + in_band % rows) * bm;
+    r.n0 = in_band / rows * bn;
+    r.first = blocks * r.split / splits;
+    r.last = blocks * (r.split + 1) / splits;
+    return r;
+}
+
 constexpr int64_t kMostSummands = (int64_t)1 << 27;
 constexpr int64_t kSumMostBlocks = 512;  // blocks of k after which a float sum starts anew, whatever way a product takes
 // 256 rows of a product's operand lie within 2^36 bytes (the kernel's offsets): value strides below 2^28.
 constexpr int64_t kMostStride = (int64_t)1 << 28;
 bool product_sizes(int64_t m, int64_t n, int64_t k);
 // out [m, n] = the sum of partial [splits][m][n] over the splits, in a fixed order.
+template <typename O>
+void launch_join(const float* partial, int64_t m, int64_t n, int64_t splits, O* out, int64_t out_stride, hipStream_t stream);
 gsx_hip_status join_products(const float* partial, int64_t m, int64_t n, int64_t splits, float* out, int64_t out_stride,
                              hipStream_t stream);
 gsx_hip_status block_matrix_check(const void* values, const void* exponents, int64_t rows, int64_t cols,

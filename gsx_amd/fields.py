@@ -20,11 +20,12 @@ import torch
 from . import _lib
 from ._lib import GsxHipError, check
 
-__all__ = ["Blocks", "lookup", "lookup_backward", "quantize", "matmul", "linear", "linear_backward", "distill",
+__all__ = ["Blocks", "Blocks4", "lookup", "lookup_backward", "quantize", "quantize4", "matmul", "linear", "linear_backward", "distill",
            "distill_backward", "LogProbs", "log_probs", "log_probs_backward"]
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 3, torch.float16: 4}  # GSX_HIP_DTYPE_*
 BLOCK = 128
+BLOCK4 = 32
 
 
 def _type(dtype) -> int:
@@ -180,27 +181,89 @@ def quantize(x: torch.Tensor, transpose: bool = False, stream=None) -> Blocks:
     return _run(stream, call)
 
 
-def matmul(a: Blocks, b: Blocks, out_dtype=torch.float32, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
-    """a b^T, [a.rows, b.rows]."""
+@dataclass
+class Blocks4:
+    """A matrix [rows, cols] in microscaled 4-bit blocks: values uint8 [rows, at least ceil(cols / 2)], two a byte, exponents uint8
+    [rows, at least ceil(cols / 32)], their rows 16 and 4 bytes aligned."""
+
+    values: torch.Tensor
+    exponents: torch.Tensor
+    cols: int
+
+    @property
+    def rows(self) -> int:
+        return int(self.values.shape[0])
+
+    def arguments(self):
+        v, v_stride = _rows(self.values, "values", torch.uint8)
+        e, e_stride = _rows(self.exponents, "exponents", torch.uint8)
+        if self.exponents.shape[0] != self.rows or self.values.shape[1] * 2 < self.cols or \
+                self.exponents.shape[1] < -(-self.cols // BLOCK4):
+            raise GsxHipError("values and exponents must cover the same rows and all columns")
+        return v, _padded(v_stride, 16, self.rows), e, _padded(e_stride, 4, self.rows)
+
+    def float(self, out_dtype=torch.float32, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+        """The values that the blocks stand for, [rows, cols]."""
+        lib = _lib.load(require_device=False)
+        args = self.arguments()
+
+        def call(handle):
+            shape = (self.rows, self.cols)
+            result = torch.empty(shape, dtype=out_dtype, device=self.values.device) if out is None else out
+            to, to_stride = _rows(result, "out", None, shape)
+            check(lib.gsx_hip_blocks4_expand(*args, *shape, to, _type(result.dtype), to_stride, handle), "4-bit blocks")
+            return result
+
+        return _run(stream, call)
+
+
+def quantize4(x: torch.Tensor, stream=None) -> Blocks4:
+    """x in microscaled 4-bit blocks along its rows."""
     lib = _lib.load(require_device=False)
+    base, stride = _rows(x, "x")
+    code = _type(x.dtype)
+    rows, cols = x.shape
+
+    def call(handle):
+        n = -(-cols // BLOCK4)
+        values = torch.empty((rows, n * BLOCK4 // 2), dtype=torch.uint8, device=x.device)
+        exponents = torch.empty((rows, -(-n // 4) * 4), dtype=torch.uint8, device=x.device)
+        check(lib.gsx_hip_blocks4_quantize(base, code, rows, cols, stride, values.data_ptr(), n * BLOCK4 // 2,
+                                           exponents.data_ptr(), -(-n // 4) * 4, handle), "quantize4")
+        return Blocks4(values, exponents, cols)
+
+    return _run(stream, call)
+
+
+def matmul(a: Blocks | Blocks4, b: Blocks | Blocks4, out_dtype=torch.float32, out: torch.Tensor | None = None,
+           stream=None) -> torch.Tensor:
+    """a b^T, [a.rows, b.rows], for operands in blocks of one kind."""
+    lib = _lib.load(require_device=False)
+    if isinstance(a, Blocks4) != isinstance(b, Blocks4):
+        raise GsxHipError("the operands must both be in 8-bit blocks, or both in 4-bit blocks")
     if a.cols != b.cols:
         raise GsxHipError(f"the operands' rows have {a.cols} and {b.cols} values")
     m, n, k = a.rows, b.rows, a.cols
     a_args, b_args = a.arguments(), b.arguments()
+    if isinstance(a, Blocks4):
+        temp_bytes, product = lib.gsx_hip_blocks4_matmul_temp_bytes, lib.gsx_hip_blocks4_matmul
+    else:
+        temp_bytes, product = lib.gsx_hip_blocks_matmul_temp_bytes, lib.gsx_hip_blocks_matmul
 
     def call(handle):
         result = torch.empty((m, n), dtype=out_dtype, device=a.values.device) if out is None else out
         to, to_stride = _rows(result, "out", None, (m, n))
-        temp = _temp(lib.gsx_hip_blocks_matmul_temp_bytes(m, n, k))
-        check(lib.gsx_hip_blocks_matmul(*a_args, *b_args, m, n, k, to, _type(result.dtype), to_stride, _address(temp),
-                                        handle), "block product")
+        temp = _temp(temp_bytes(m, n, k))
+        check(product(*a_args, *b_args, m, n, k, to, _type(result.dtype), to_stride, _address(temp), handle), "block product")
         return result
 
     return _run(stream, call)
 
 
-def linear(x: torch.Tensor, weight: Blocks, out_dtype=None, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
-    """x weight^T with the rows of x quantised on the way; the result has x's type unless out_dtype or out says otherwise."""
+def linear(x: torch.Tensor, weight: Blocks | Blocks4, out_dtype=None, out: torch.Tensor | None = None,
+           stream=None) -> torch.Tensor:
+    """x weight^T with the rows of x quantised on the way, to the weight's kind of blocks; the result has x's type unless out_dtype
+    or out says otherwise."""
     lib = _lib.load(require_device=False)
     base, stride = _rows(x, "x")
     code = _type(x.dtype)
@@ -209,13 +272,16 @@ def linear(x: torch.Tensor, weight: Blocks, out_dtype=None, out: torch.Tensor | 
     if weight.cols != k:
         raise GsxHipError(f"x has {k} columns, the weight {weight.cols}")
     w_args = weight.arguments()
+    if isinstance(weight, Blocks4):
+        temp_bytes, forward = lib.gsx_hip_linear4_temp_bytes, lib.gsx_hip_linear4_forward
+    else:
+        temp_bytes, forward = lib.gsx_hip_linear_temp_bytes, lib.gsx_hip_linear_forward
 
     def call(handle):
         result = torch.empty((m, n), dtype=out_dtype or x.dtype, device=x.device) if out is None else out
         to, to_stride = _rows(result, "out", out_dtype, (m, n))
-        temp = _temp(lib.gsx_hip_linear_temp_bytes(m, n, k))
-        check(lib.gsx_hip_linear_forward(base, code, stride, *w_args, m, n, k, to, _type(result.dtype), to_stride,
-                                         _address(temp), handle), "linear")
+        temp = _temp(temp_bytes(m, n, k))
+        check(forward(base, code, stride, *w_args, m, n, k, to, _type(result.dtype), to_stride, _address(temp), handle), "linear")
         return result
 
     return _run(stream, call)
@@ -235,6 +301,8 @@ def linear_backward(x: torch.Tensor, grad_out: torch.Tensor, weight_t: Blocks, g
     n = grad_out.shape[1]
     if grad_out.shape[0] != m:
         raise GsxHipError("x and grad_out must have the same number of rows")
+    if isinstance(weight_t, Blocks4):
+        raise GsxHipError("gradients go through 8-bit blocks: weight_t must be Blocks")
     if weight_t.cols != n or weight_t.rows != k:
         raise GsxHipError(f"weight_t must be [{k}, {n}], not [{weight_t.rows}, {weight_t.cols}]")
     grad_x = linear(grad_out, weight_t, stream=stream)

@@ -578,6 +578,36 @@ gsx_hip_status gsx_hip_linear_backward_weight(const void* x, int32_t x_type, int
                                               int32_t grad_type, int64_t grad_stride, int64_t m, int64_t n, int64_t k,
                                               float* grad_weight, int64_t weight_stride, void* temp, hipStream_t stream);
 
+/* Matrices in microscaled 4-bit blocks. A row of `cols` values is cut into blocks of 32; a block holds E2M1 values (OCP: 0, 0.5,
+ * 1, 1.5, 2, 3, 4, 6 and their negatives), two a byte, the first one in the low half, and one byte e + 127 for its scale 2^e, with
+ * e the least whole number >= -100 such that max |x| <= 6 * 2^e over the block (e = 0 where that maximum is 0). Each x * 2^-e is
+ * rounded to the nearest value, ties to the even code. A block that holds anything not finite gets the byte 255 and stands for NaN.
+ * Blocks with any byte are read: 0 to 254 for 2^-127 to 2^127, 255 for NaN. Value rows are 16-byte aligned (stride in bytes, a
+ * multiple of 16, >= ceil(cols / 2)), exponent rows 4-byte aligned (stride a multiple of 4, >= ceil(cols / 32)). A row's last
+ * block and its last 4 exponents are read whole, but what lies behind its last value is never used as one; quantize writes zeros
+ * up to the last block's end. */
+gsx_hip_status gsx_hip_blocks4_quantize(const void* src, int32_t src_type, int64_t rows, int64_t cols, int64_t src_stride,
+                                        uint8_t* values, int64_t values_stride, uint8_t* exponents, int64_t exponents_stride,
+                                        hipStream_t stream);
+/* out [rows, cols] = what the blocks stand for (exact in float32 and bfloat16 within their range). */
+gsx_hip_status gsx_hip_blocks4_expand(const uint8_t* values, int64_t values_stride, const uint8_t* exponents,
+                                      int64_t exponents_stride, int64_t rows, int64_t cols, void* out, int32_t out_type,
+                                      int64_t out_stride, hipStream_t stream);
+/* out [m, n] = a b^T for 4-bit block matrices a [m, k] and b [n, k]; m and n at most 2^31 - 1, k at most 2^27, value strides below
+ * 2^28. */
+size_t gsx_hip_blocks4_matmul_temp_bytes(int64_t m, int64_t n, int64_t k);
+gsx_hip_status gsx_hip_blocks4_matmul(const uint8_t* a_values, int64_t a_values_stride, const uint8_t* a_exponents,
+                                      int64_t a_exponents_stride, const uint8_t* b_values, int64_t b_values_stride,
+                                      const uint8_t* b_exponents, int64_t b_exponents_stride, int64_t m, int64_t n, int64_t k,
+                                      void* out, int32_t out_type, int64_t out_stride, void* temp, hipStream_t stream);
+/* out [m, n] = blocks(x) w^T: the rows of x [m, k] are quantised to 4-bit blocks as above and multiplied with the 4-bit block
+ * matrix w [n, k]. Where that takes a workspace, w's value stride is below 2^28. */
+size_t gsx_hip_linear4_temp_bytes(int64_t m, int64_t n, int64_t k);
+gsx_hip_status gsx_hip_linear4_forward(const void* x, int32_t x_type, int64_t x_stride, const uint8_t* w_values,
+                                       int64_t w_values_stride, const uint8_t* w_exponents, int64_t w_exponents_stride,
+                                       int64_t m, int64_t n, int64_t k, void* out, int32_t out_type, int64_t out_stride,
+                                       void* temp, hipStream_t stream);
+
 /* Distillation from a teacher's top logits. Row r of `logits` [rows, vocab] is the student's z; teacher_ids and teacher_logits
  * [rows, top] (rows teacher_stride apart, top at most 1024) name the teacher's entries. An entry counts if its id lies in
  * [0, vocab) and its logit is not -inf. With T the temperature (1e-6 to 1e6), p = softmax(t / T) over the entries that
