@@ -15,6 +15,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "blocks4.hpp"
 
 namespace gsx_amd {
@@ -89,119 +91,260 @@ __global__ __launch_bounds__(kQuant4Threads) void expand4_kernel(const uint8_t* 
 // A workgroup of WM x WN waves forms a tile of c: BM rows (of a) by BN columns (rows of b), a wave TM x TN times 16 x 16 of it.
 // Eight blocks, 256 k, of both operands' tiles lie in LDS, two such steps at a time: while one is multiplied the next is on its way
 // there, straight from memory. A row is eight chunks of 16 bytes, one block each; chunk c lies at place c ^ swizzle(row), and a lane
-// of group g = lane / 16 reads chunks g and g + 4: no two lanes of a read meet in a bank. Exponents lie as the words of four blocks
-// that they are in memory, [word][row].
+// of group g = lane / 16 reads chunks g and g + 4: no two lanes of a read meet in a bank. A row's eight exponents lie behind one
+// another, as in memory.
 //
 // The matrix instructions take b as their first operand: a lane then holds four consecutive columns of one row of c. Which
-// row of b a lane brings for instruction j is chosen so that its 4 TN columns are consecutive too, and leave in wide stores.
+// row of b a lane brings for instruction j is chosen so that it has 16 bytes of columns together and that the four lanes of a row
+// store 64 bytes in a piece: 32 columns by a pair of instructions in 16-bit types, 16 by one in float32.
 constexpr int kStep4 = 8;  // blocks
 
+template <typename O>
+constexpr int kPair = sizeof(O) == 2 ? 2 : 1;  // instructions whose columns of a lane lie together
+template <typename O>
+__device__ constexpr int column4_of(int j, int r) {
+    return j / kPair<O> * (16 * kPair<O>) + r / 4 * (4 * kPair<O>) + j % kPair<O> * 4 + r % 4;
+}
+template <typename O>
+__device__ inline int swizzle4_b(int row) {
+    return kPair<O> == 2 ? (row & 3) | (row >> 3 & 1) << 2 : row & 7;
+}
+
+// A lane's 4 TN columns of a row of n, the first of them at `col` + 4 kPair<O> (lane / 16).
+template <typename O, int TN, typename S>
+__device__ inline void store_row4(S* __restrict__ row, int64_t col, int64_t n, int lane, const v4f (&x)[TN]) {
+    constexpr int kP = kPair<O>;
+    struct __attribute__((packed, aligned(sizeof(S)))) Piece {
+        S v[4 * kP];
+    };
+#pragma unroll
+    for (int j = 0; j < TN; j += kP) {
+        const int64_t c = col + 16 * j + lane / 16 * (4 * kP);
+        if (c + 4 * kP <= n) {
+            Piece q;
+#pragma unroll
+            for (int i = 0; i < 4 * kP; ++i) q.v[i] = from_float<S>(x[j + i / 4][i % 4]);
+            *reinterpret_cast<Piece*>(row + c) = q;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4 * kP; ++i)
+                if (c + i < n) row[c + i] = from_float<S>(x[j + i / 4][i % 4]);
+        }
+    }
+}
+
+// Where a wave's loads begin: of the values of a step a load brings eight rows, of the exponents of two steps 64.
+template <int kLoads, int kExponentLoads>
+struct StepLoads4 {
+    const uint8_t *a, *b, *a_exponents, *b_exponents;  // the tile's rows
+    uint32_t offset[kLoads];                           // in units of 16 bytes
+    uint32_t exponent_offset[kExponentLoads];          // and of 4
+};
+
+// The chunk of a row that a lane of load u brings.
+template <typename O, int BM, int kWaves>
+__device__ __forceinline__ int chunk4_of(int u, int wave, int lane) {
+    const int row = 8 * (u * kWaves + wave) + lane / 8;
+    return (lane & 7) ^ (row < BM ? swizzle_a(row) : swizzle4_b<O>(row - BM));
+}
+
+// A step's values; of its chunks from `chunks` on (of a cut step, the last one) the last one before them is read again.
+template <typename O, int kLoads, int kExponentLoads, int BM, int kWaves>
+__device__ __forceinline__ void load_step4(uint8_t* __restrict__ to, const StepLoads4<kLoads, kExponentLoads>& from, int step,
+                                           int chunks, int wave, int lane) {
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+        const uint8_t* const base = (8 * (u * kWaves + wave) < BM ? from.a : from.b) + (uint32_t)step * 128;
+        uint32_t offset = from.offset[u];
+        if (chunks < kStep4) offset -= (uint32_t)max(chunk4_of<O, BM, kWaves>(u, wave, lane) - (chunks - 1), 0);
+        __builtin_amdgcn_global_load_lds((GlobalPtr)(base + (uint64_t)offset * 16), (LdsPtr)(to + (u * kWaves + wave) * 1024), 16,
+                                         0, 0);
+    }
+}
+
+template <int kLoads, int kExponentLoads, int kRows, int BM, int kWaves>
+__device__ __forceinline__ void load_exponents4(uint8_t* __restrict__ to, const StepLoads4<kLoads, kExponentLoads>& from, int pair,
+                                                int wave) {
+#pragma unroll
+    for (int u = 0; u < kExponentLoads; ++u) {
+        const int row = (u * kWaves + wave) * 64;
+        if (row >= kRows) continue;
+        const uint8_t* const base = (row < BM ? from.a_exponents : from.b_exponents) + (uint32_t)pair * 16;
+        __builtin_amdgcn_global_load_lds((GlobalPtr)(base + (uint64_t)from.exponent_offset[u] * 4),
+                                         (LdsPtr)(to + (u * kWaves + wave) * 1024), 16, 0, 0);
+    }
+}
+
+// The lane's places in a step: chunk lane / 16 of its first row of each operand (the one four further is 64 bytes away, up or
+// down), and its exponent there.
+struct StepPlaces4 {
+    int a, b, e_a, e_b;
+};
+
+// What a cut step's operands are masked with: of the lane's two chunks the bits that are there, and whether any are.
+struct Cut4 {
+    v4i keep[2];
+    bool some[2];
+};
+__device__ inline Cut4 cut4_of(int64_t left, int group) {  // values that are left of the step
+    Cut4 cut;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        const int mine = (int)max(min(left - (group + 4 * half) * kBlock4, (int64_t)kBlock4), (int64_t)0);
+        cut.some[half] = mine > 0;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) cut.keep[half][d] = (int)(0xffffffffull >> (32 - max(min(4 * (mine - 8 * d), 32), 0)));
+    }
+    return cut;
+}
+
+// One step: the loads of the next one are begun, then this one, which they do not touch, is multiplied. __restrict__ says so to the
+// compiler, which otherwise waits for the loads before it reads LDS. What the instructions of two rows of tiles need is read ahead.
+// kCut: this is the last step and cut. Zeros of a times anything of b are 0, but for a scale that is NaN.
+template <bool kCut, typename O, int TM, int TN, int kRows, int BM, int kWaves, int kLoads, int kExponentLoads>
+__device__ __forceinline__ void product4_step(const uint8_t* __restrict__ now, const uint8_t* __restrict__ exponents,
+                                              uint8_t* __restrict__ next, uint8_t* __restrict__ next_exponents, int load_chunks,
+                                              bool load_exponents, const StepLoads4<kLoads, kExponentLoads>& from, int step,
+                                              int wave, int lane, StepPlaces4 at, const Cut4& cut, v4f (&acc)[TM][TN]) {
+    if (load_chunks > 0) load_step4<O, kLoads, kExponentLoads, BM, kWaves>(next, from, step, load_chunks, wave, lane);
+    if (load_exponents) load_exponents4<kLoads, kExponentLoads, kRows, BM, kWaves>(next_exponents, from, step / 2, wave);
+    constexpr int kAhead = 3;
+    v4i va[kAhead], vb[2][TN];
+    uint32_t scale_a[kAhead], scale_b[2][TN];
+    const auto read_a = [&](int n) {  // of both halves' rows of tiles
+        const int i = n % TM, half = n / TM;
+        va[n % kAhead] = *reinterpret_cast<const v4i*>(now + (at.a ^ (half * 64)) + i * (16 * 128));
+        scale_a[n % kAhead] = exponents[at.e_a + half * 4 + i * (16 * 16)];
+        if constexpr (kCut) {
+            va[n % kAhead] &= cut.keep[half];
+            if (!cut.some[half]) scale_a[n % kAhead] = 127;
+        }
+    };
+    const auto read_b = [&](int half, int j) {
+        const int row = column4_of<O>(j, 0);
+        vb[half][j] = *reinterpret_cast<const v4i*>(now + (at.b ^ (half * 64)) + row * 128);
+        scale_b[half][j] = exponents[at.e_b + half * 4 + row * 16];
+        if constexpr (kCut) {
+            if (!cut.some[half]) scale_b[half][j] = 127;
+        }
+    };
+#pragma unroll
+    for (int j = 0; j < TN; ++j) read_b(0, j);
+#pragma unroll
+    for (int n = 0; n < kAhead - 1; ++n) read_a(n);
+#pragma unroll
+    for (int n = 0; n < 2 * TM; ++n) {
+        const int i = n % TM, half = n / TM;
+        if (n + kAhead - 1 < 2 * TM) read_a(n + kAhead - 1);
+        if (n < TN) read_b(1, n);
+        __builtin_amdgcn_sched_barrier(0);  // the reads stay ahead of the instructions
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+            acc[i][j] = multiply4<0, 0>(vb[half][j], va[n % kAhead], acc[i][j], scale_b[half][j], scale_a[n % kAhead]);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
 template <typename O, int TM, int TN, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN) void product4_kernel(BlockMatrix a, BlockMatrix b, int64_t m, int64_t n, int64_t k,
+__global__ __launch_bounds__(64 * WM * WN, 2) void product4_kernel(BlockMatrix a, BlockMatrix b, int64_t m, int64_t n, int64_t k,
                                                                 int64_t tiles_m, int64_t tiles_n, int64_t splits,
                                                                 O* __restrict__ out, int64_t out_stride,
                                                                 float* __restrict__ partial) {
     constexpr int kThreads = 64 * WM * WN, BM = 16 * TM * WM, BN = 16 * TN * WN;
     constexpr int kRows = BM + BN, kLoads = kRows * 8 / kThreads, kWaves = WM * WN;
-    static_assert(kRows * 8 % kThreads == 0 && BM % (8 * kWaves) == 0, "whole loads, each of one operand");
+    constexpr int kExponentLoads = (kRows / 64 + kWaves - 1) / kWaves;
+    static_assert(kRows * 8 % kThreads == 0 && BM % (8 * kWaves) == 0 && BM % 64 == 0, "whole loads, each of one operand");
+    static_assert(TN <= TM && TN % 2 == 0, "b's second half is read beside the first one's instructions");
     __shared__ __attribute__((aligned(1024))) uint8_t s_values[2][kRows * 128];
-    __shared__ uint32_t s_exponents[2][2][kRows];
+    __shared__ __attribute__((aligned(1024))) uint8_t s_exponents[2][kRows * 16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const int wm = wave / WN, wn = wave % WN;
-    const int64_t blocks = ceil_div(k, kBlock4), steps = ceil_div(blocks, kStep4), total = tiles_m * tiles_n * splits;
+    const int wm = wave / WN, wn = wave % WN, group = lane / 16;
+    const int blocks = (int)ceil_div(k, kBlock4), steps = (int)ceil_div(blocks, kStep4);
+    const int64_t total = tiles_m * tiles_n * splits;
+    const int row_a = wm * 16 * TM + (lane & 15), row_b = wn * 16 * TN + column4_of<O>(0, lane & 15);
+    const StepPlaces4 even = {row_a * 128 + ((group ^ swizzle_a(row_a)) * 16),
+                              (BM + row_b) * 128 + ((group ^ swizzle4_b<O>(row_b)) * 16), row_a * 16 + group,
+                              (BM + row_b) * 16 + group};
     for (int64_t t = blockIdx.x; t < total; t += gridDim.x) {
         const ProductTile tile = product_tile(t, total, tiles_m, tiles_n, BM, BN, steps, splits);
+        const int first = (int)tile.first, count = (int)(tile.last - tile.first);
         // Load u of a wave: eight rows (lane / 8) from row 8 (u kWaves + wave) on, a's rows before b's. Rows past the last one
-        // repeat it; what they give is not stored. Offsets from the tile's first row are kept in units of 16 bytes.
-        const uint8_t* const a_tile = a.values + tile.m0 * a.values_stride;
-        const uint8_t* const b_tile = b.values + tile.n0 * b.values_stride;
+        // repeat it; what they give is not stored.
         const int most_a = (int)min(m - 1 - tile.m0, (int64_t)BM), most_b = (int)min(n - 1 - tile.n0, (int64_t)BN);
         const uint32_t a_step = (uint32_t)(a.values_stride / 16), b_step = (uint32_t)(b.values_stride / 16);
-        uint32_t offset[kLoads];
+        const uint32_t a_words = (uint32_t)(a.exponents_stride / 4), b_words = (uint32_t)(b.exponents_stride / 4);
+        StepLoads4<kLoads, kExponentLoads> from;
+        from.a = a.values + tile.m0 * a.values_stride;
+        from.b = b.values + tile.n0 * b.values_stride;
+        from.a_exponents = a.exponents + tile.m0 * a.exponents_stride;
+        from.b_exponents = b.exponents + tile.n0 * b.exponents_stride;
+        const auto exponent_row = [&](int row) {
+            return row < BM ? min(row, most_a) * a_words : min(row - BM, most_b) * b_words;
+        };
 #pragma unroll
         for (int u = 0; u < kLoads; ++u) {
             const int row = 8 * (u * kWaves + wave) + lane / 8;
-            offset[u] = row < BM ? min(row, most_a) * a_step + (uint32_t)((lane & 7) ^ swizzle_a(row))
-                                 : min(row - BM, most_b) * b_step + (uint32_t)((lane & 7) ^ swizzle_b<TN>(row - BM));
+            from.offset[u] = (row < BM ? min(row, most_a) * a_step : min(row - BM, most_b) * b_step) +
+                             (uint32_t)chunk4_of<O, BM, kWaves>(u, wave, lane);
         }
-        const auto load_values4 = [&](int64_t step) {
 #pragma unroll
-            for (int u = 0; u < kLoads; ++u) {
-                const uint8_t* const base = (8 * (u * kWaves + wave) < BM ? a_tile : b_tile) + step * 128;
-                __builtin_amdgcn_global_load_lds((GlobalPtr)(base + (uint64_t)offset[u] * 16),
-                                                 (LdsPtr)(s_values[step & 1] + (u * kWaves + wave) * 1024), 16, 0, 0);
+        for (int u = 0; u < kExponentLoads; ++u)
+            from.exponent_offset[u] = exponent_row(min((u * kWaves + wave) * 64, kRows - 64) + lane);
+        // exponents of a pair of steps that is cut: through registers, a word a thread
+        const auto stage_exponents = [&](int pair, uint8_t* to) {
+            const int word = pair * 4 + (threadIdx.x & 3), at = min(word, (blocks - 1) / 4);
+            const int left = max(min(blocks - 4 * word, 4), 0);
+            const uint32_t keep = (uint32_t)((1ull << (8 * left)) - 1);
+#pragma unroll 2
+            for (int i = threadIdx.x; i < 4 * kRows; i += kThreads) {
+                const uint32_t* const p =
+                    reinterpret_cast<const uint32_t*>(i / 4 < BM ? from.a_exponents : from.b_exponents) + exponent_row(i / 4);
+                reinterpret_cast<uint32_t*>(to)[i] = (p[at] & keep) | (0x7f7f7f7fu & ~keep);
             }
         };
-        // a cut step, the last one: through registers, with zeros past the last k
-        const auto stage_values4 = [&](int64_t step) {
-#pragma unroll 1
-            for (int u = 0; u < kLoads; ++u) {
-                const int row = 8 * (u * kWaves + wave) + lane / 8;
-                const uint8_t* const p = row < BM ? a_tile + min(row, most_a) * a.values_stride
-                                                  : b_tile + min(row - BM, most_b) * b.values_stride;
-                const int chunk = (lane & 7) ^ (row < BM ? swizzle_a(row) : swizzle_b<TN>(row - BM));
-                *reinterpret_cast<v4i*>(s_values[step & 1] + (u * kWaves + wave) * 1024 + lane * 16) =
-                    load_block4(p, step * kStep4 + chunk, k);
-            }
-        };
-        const auto stage_exponents = [&](int64_t step) {
-            for (int i = threadIdx.x; i < 2 * kRows; i += kThreads) {
-                const int word = i / kRows, row = i % kRows;
-                const uint8_t* const p = row < BM ? a.exponents + (tile.m0 + min(row, most_a)) * a.exponents_stride
-                                                  : b.exponents + (tile.n0 + min(row - BM, most_b)) * b.exponents_stride;
-                s_exponents[step & 1][word][row] = load_exponents4(p, step * 2 + word, blocks);
-            }
-        };
-        const auto begin = [&](int64_t step) {
-            if ((step + 1) * kStep4 * kBlock4 <= k) load_values4(step);
-            else stage_values4(step);
-            stage_exponents(step);
-        };
+        const auto chunks_of = [&](int step) { return min(blocks - step * kStep4, kStep4); };
+        const auto whole_pair = [&](int step) { return (step / 2 * 2 + 2) * kStep4 <= blocks; };
         v4f acc[TM][TN];
 #pragma unroll
         for (int i = 0; i < TM; ++i)
 #pragma unroll
             for (int j = 0; j < TN; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-        if (tile.first < tile.last) begin(tile.first);
-        for (int64_t step = tile.first; step < tile.last; ++step) {
+        int held = 0;  // the buffer of this step's exponents
+        if (count > 0) {
+            load_step4<O, kLoads, kExponentLoads, BM, kWaves>(s_values[0], from, first, chunks_of(first), wave, lane);
+            if (whole_pair(first))
+                load_exponents4<kLoads, kExponentLoads, kRows, BM, kWaves>(s_exponents[0], from, first / 2, wave);
+            else
+                stage_exponents(first / 2, s_exponents[0]);
+        }
+        const auto multiply = [&](auto cut_step, int i) {
             // This step is in LDS (the barrier does not wait for loads that go there), the one before it has been read.
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
-            if (step + 1 < tile.last) begin(step + 1);
-            const uint8_t* const s_a = s_values[step & 1];
-            const uint8_t* const s_b = s_a + BM * 128;
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int c = lane / 16 + 4 * half;
-                const uint8_t* const e = reinterpret_cast<const uint8_t*>(s_exponents[step & 1][half]) + lane / 16;
-                v4i vb[TN];
-                uint32_t scale_b[TN];
-#pragma unroll
-                for (int j = 0; j < TN; ++j) {
-                    const int row = wn * 16 * TN + column_of<TN>(j, lane & 15);
-                    vb[j] = *reinterpret_cast<const v4i*>(s_b + row * 128 + ((c ^ swizzle_b<TN>(row)) * 16));
-                    scale_b[j] = e[(BM + row) * 4];
-                }
-#pragma unroll
-                for (int i = 0; i < TM; ++i) {
-                    const int row = wm * 16 * TM + i * 16 + (lane & 15);
-                    const v4i va = *reinterpret_cast<const v4i*>(s_a + row * 128 + ((c ^ swizzle_a(row)) * 16));
-                    const uint32_t scale_a = e[row * 4];
-#pragma unroll
-                    for (int j = 0; j < TN; ++j) acc[i][j] = multiply4<0, 0>(vb[j], va, acc[i][j], scale_b[j], scale_a);
-                }
-            }
-        }
+            constexpr bool kCut = decltype(cut_step)::value;
+            const int step = first + i, next = step + 1;
+            const bool more = !kCut && i + 1 < count, turns = more && next % 2 == 0, cut_pair = turns && !whole_pair(next);
+            if (cut_pair) stage_exponents(next / 2, s_exponents[held ^ 1]);
+            const StepPlaces4 places = {even.a, even.b, even.e_a + (step & 1) * 8, even.e_b + (step & 1) * 8};
+            const Cut4 cut = kCut ? cut4_of(k - (int64_t)step * kStep4 * kBlock4, group) : Cut4{};
+            product4_step<kCut, O, TM, TN, kRows, BM, kWaves, kLoads, kExponentLoads>(
+                s_values[i & 1], s_exponents[held], s_values[(i + 1) & 1], s_exponents[held ^ 1], more ? chunks_of(next) : 0,
+                turns && !cut_pair, from, next, wave, lane, places, cut, acc);
+            if (turns) held ^= 1;
+        };
+        const bool cut = count > 0 && (int64_t)(first + count) * kStep4 * kBlock4 > k;
+        for (int i = 0; i < count - (cut ? 1 : 0); ++i) multiply(std::false_type(), i);
+        if (cut) multiply(std::true_type(), count - 1);
         __syncthreads();  // the next tile's first step goes where this one's last was read
-        const int64_t col = tile.n0 + wn * 16 * TN + (lane / 16) * (4 * TN);
+        const int64_t col = tile.n0 + wn * 16 * TN;
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
             const int64_t row = tile.m0 + wm * 16 * TM + i * 16 + (lane & 15);
             if (row >= m) continue;
             if (splits == 1) {
-                store_columns<TN>(out + row * out_stride, col, n, acc[i]);
+                store_row4<O, TN>(out + row * out_stride, col, n, lane, acc[i]);
             } else {
-                store_columns<TN>(partial + (tile.split * m + row) * n, col, n, acc[i]);
+                store_row4<O, TN>(partial + (tile.split * m + row) * n, col, n, lane, acc[i]);
             }
         }
     }
@@ -324,8 +467,10 @@ gsx_hip_status gsx_hip_blocks4_matmul(const uint8_t* a_values, int64_t a_values_
     if (!product_sizes(m, n, k))
         return fields_fail(GSX_HIP_ERROR_OUT_OF_RANGE,
                            "4-bit blocks: a product has at most 2^31 - 1 rows and columns and 2^27 summands");
-    if (a_values_stride >= kMostStride || b_values_stride >= kMostStride)
-        return fields_fail(GSX_HIP_ERROR_OUT_OF_RANGE, "4-bit blocks: a product's value rows lie less than 2^28 bytes apart");
+    if (a_values_stride >= kMostStride || b_values_stride >= kMostStride || a_exponents_stride >= kMostStride / 4 ||
+        b_exponents_stride >= kMostStride / 4)
+        return fields_fail(GSX_HIP_ERROR_OUT_OF_RANGE,
+                           "4-bit blocks: a product's value rows lie less than 2^28 bytes apart, its exponent rows 2^26");
     gsx_hip_status st = blocks4_check(a_values, a_exponents, m, k, a_values_stride, a_exponents_stride);
     if (st != GSX_HIP_SUCCESS) return st;
     st = blocks4_check(b_values, b_exponents, n, k, b_values_stride, b_exponents_stride);
@@ -351,7 +496,7 @@ gsx_hip_status gsx_hip_blocks4_matmul(const uint8_t* a_values, int64_t a_values_
                                plan.splits, to, out_stride, partial);
         };
         if (plan.edge == 256) go(product4_kernel<O, 8, 4, 2, 4>, 512);
-        else if (plan.edge == 192) go(product4_kernel<O, 6, 3, 2, 4>, 512);
+        else if (plan.edge == 192) go(product4_kernel<O, 6, 4, 2, 3>, 384);
         else if (plan.edge == 128) go(product4_kernel<O, 4, 4, 2, 2>, 256);
         else go(product4_kernel<O, 2, 2, 2, 2>, 256);
         if (plan.splits > 1) launch_join(partial, m, n, plan.splits, to, out_stride, stream);
@@ -382,8 +527,9 @@ gsx_hip_status gsx_hip_linear4_forward(const void* x, int32_t x_type, int64_t x_
         return fields_fail(GSX_HIP_ERROR_INVALID_ARGUMENT, "4-bit linear: rows must be non-null and aligned to their elements");
     if (k > 0 && (temp == nullptr || !aligned_to(temp, 16)))
         return fields_fail(GSX_HIP_ERROR_INVALID_ARGUMENT, "4-bit linear: the workspace must be non-null and 16-byte aligned");
-    if (w_values_stride >= kMostStride)
-        return fields_fail(GSX_HIP_ERROR_OUT_OF_RANGE, "4-bit linear: a wide layer's value rows lie less than 2^28 bytes apart");
+    if (w_values_stride >= kMostStride || w_exponents_stride >= kMostStride / 4)
+        return fields_fail(GSX_HIP_ERROR_OUT_OF_RANGE,
+                           "4-bit linear: a wide layer's value rows lie less than 2^28 bytes apart, its exponent rows 2^26");
     const int64_t blocks = ceil_div(k, kBlock4), words = ceil_div(blocks, 4) * 4;
     uint8_t* const values = static_cast<uint8_t*>(temp);
     uint8_t* const exponents = values + m * blocks * 16;

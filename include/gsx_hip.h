@@ -594,14 +594,14 @@ gsx_hip_status gsx_hip_blocks4_expand(const uint8_t* values, int64_t values_stri
                                       int64_t exponents_stride, int64_t rows, int64_t cols, void* out, int32_t out_type,
                                       int64_t out_stride, hipStream_t stream);
 /* out [m, n] = a b^T for 4-bit block matrices a [m, k] and b [n, k]; m and n at most 2^31 - 1, k at most 2^27, value strides below
- * 2^28. */
+ * 2^28, exponent strides below 2^26. */
 size_t gsx_hip_blocks4_matmul_temp_bytes(int64_t m, int64_t n, int64_t k);
 gsx_hip_status gsx_hip_blocks4_matmul(const uint8_t* a_values, int64_t a_values_stride, const uint8_t* a_exponents,
                                       int64_t a_exponents_stride, const uint8_t* b_values, int64_t b_values_stride,
                                       const uint8_t* b_exponents, int64_t b_exponents_stride, int64_t m, int64_t n, int64_t k,
                                       void* out, int32_t out_type, int64_t out_stride, void* temp, hipStream_t stream);
 /* out [m, n] = blocks(x) w^T: the rows of x [m, k] are quantised to 4-bit blocks as above and multiplied with the 4-bit block
- * matrix w [n, k]. Where that takes a workspace, w's value stride is below 2^28. */
+ * matrix w [n, k]. Where that takes a workspace, w's value stride is below 2^28, its exponent stride below 2^26. */
 size_t gsx_hip_linear4_temp_bytes(int64_t m, int64_t n, int64_t k);
 gsx_hip_status gsx_hip_linear4_forward(const void* x, int32_t x_type, int64_t x_stride, const uint8_t* w_values,
                                        int64_t w_values_stride, const uint8_t* w_exponents, int64_t w_exponents_stride,

@@ -6,8 +6,8 @@ PRODUCTS = [
     (33, 17, 31, "Li2ELi2ELi2ELi2E"),
     (1601, 1099, 1100, "Li4ELi4ELi2ELi2E"),
     (300, 290, 255, "Li4ELi4ELi2ELi2E"),
-    (4001, 2050, 1100, "Li6ELi3ELi2ELi4E"),
-    (2899, 2900, 1301, "Li6ELi3ELi2ELi4E"),
+    (4001, 2050, 1100, "Li6ELi4ELi2ELi3E"),
+    (2899, 2900, 1301, "Li6ELi4ELi2ELi3E"),
     (3900, 3901, 1100, "Li8ELi4ELi2ELi4E"),
     (3557, 2529, 1027, "Li8ELi4ELi2ELi4E"),
 ]
