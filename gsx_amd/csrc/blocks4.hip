@@ -401,11 +401,6 @@ Product4Plan product4_plan(int64_t m, int64_t n, int64_t k) {
     return p;
 }
 
-int64_t linear4_rows_bytes(int64_t m, int64_t k) {  // of the rows of x in blocks: values, then exponents
-    const int64_t blocks = ceil_div(k, kBlock4);
-    return ceil_div(m * (blocks * 16 + ceil_div(blocks, 4) * 4), 256) * 256;
-}
-
 }  // namespace
 
 extern "C" {
@@ -502,42 +497,6 @@ gsx_hip_status gsx_hip_blocks4_matmul(const uint8_t* a_values, int64_t a_values_
         if (plan.splits > 1) launch_join(partial, m, n, plan.splits, to, out_stride, stream);
         return fields_launched("4-bit blocks matmul launch");
     });
-}
-
-size_t gsx_hip_linear4_temp_bytes(int64_t m, int64_t n, int64_t k) {
-    if (!product_sizes(m, n, k) || m == 0 || n == 0) return 0;
-    return (size_t)linear4_rows_bytes(m, k) + gsx_hip_blocks4_matmul_temp_bytes(m, n, k);
-}
-
-gsx_hip_status gsx_hip_linear4_forward(const void* x, int32_t x_type, int64_t x_stride, const uint8_t* w_values,
-                                       int64_t w_values_stride, const uint8_t* w_exponents, int64_t w_exponents_stride,
-                                       int64_t m, int64_t n, int64_t k, void* out, int32_t out_type, int64_t out_stride,
-                                       void* temp, hipStream_t stream) {
-    if (!known_type(x_type) || !known_type(out_type))
-        return fields_fail(GSX_HIP_ERROR_NOT_SUPPORTED, "4-bit linear: rows are f32, bf16 or f16");
-    if (!product_sizes(m, n, k))
-        return fields_fail(GSX_HIP_ERROR_OUT_OF_RANGE, "4-bit linear: at most 2^31 - 1 rows and columns and 2^27 summands");
-    if (!rows_fit(m, x_stride, k) || !rows_fit(m, out_stride, n))
-        return fields_fail(GSX_HIP_ERROR_INVALID_ARGUMENT, "4-bit linear: strides must be at least the rows' lengths");
-    const gsx_hip_status wrong = blocks4_check(w_values, w_exponents, n, k, w_values_stride, w_exponents_stride);
-    if (wrong != GSX_HIP_SUCCESS) return wrong;
-    if (m == 0 || n == 0) return GSX_HIP_SUCCESS;
-    if (out == nullptr || (k > 0 && x == nullptr) || !aligned_to(out, type_bytes(out_type)) ||
-        !aligned_to(x, type_bytes(x_type)))
-        return fields_fail(GSX_HIP_ERROR_INVALID_ARGUMENT, "4-bit linear: rows must be non-null and aligned to their elements");
-    if (k > 0 && (temp == nullptr || !aligned_to(temp, 16)))
-        return fields_fail(GSX_HIP_ERROR_INVALID_ARGUMENT, "4-bit linear: the workspace must be non-null and 16-byte aligned");
-    if (w_values_stride >= kMostStride || w_exponents_stride >= kMostStride / 4)
-        return fields_fail(GSX_HIP_ERROR_OUT_OF_RANGE,
-                           "4-bit linear: a wide layer's value rows lie less than 2^28 bytes apart, its exponent rows 2^26");
-    const int64_t blocks = ceil_div(k, kBlock4), words = ceil_div(blocks, 4) * 4;
-    uint8_t* const values = static_cast<uint8_t*>(temp);
-    uint8_t* const exponents = values + m * blocks * 16;
-    const gsx_hip_status st = gsx_hip_blocks4_quantize(x, x_type, m, k, x_stride, values, blocks * 16, exponents, words, stream);
-    if (st != GSX_HIP_SUCCESS) return st;
-    return gsx_hip_blocks4_matmul(values, blocks * 16, exponents, words, w_values, w_values_stride, w_exponents,
-                                  w_exponents_stride, m, n, k, out, out_type, out_stride, values + linear4_rows_bytes(m, k),
-                                  stream);
 }
 
 }  // extern "C"

@@ -1,7 +1,7 @@
 """What the 4-bit blocks' C entries refuse, and which kernels their sizes lead to: nothing runs on a GPU."""
 import pytest
 
-from blocks4_ways import PRODUCTS
+from blocks4_ways import LINEARS, PRODUCTS
 from gsx_amd import _lib
 from test_fields_ways_cpu import TYPES, host  # noqa: F401  (the stand-in for the runtime)
 
@@ -70,4 +70,20 @@ for m, n, k, name in {PRODUCTS!r}:
     _lib.check(lib.gsx_hip_blocks4_matmul(P, row, P, words, P, row, P, words, m, n, k, P, {TYPES[out]}, n, P, None), "product")
     assert fake.fake_launches_of(b"product4_kernel") == before + 1
     assert fake.fake_launches_of(("product4_kernelI{out}" + name).encode()) == one + 1, (m, n, k)
+""")
+
+
+@pytest.mark.parametrize("out", TYPES)
+@pytest.mark.parametrize("x", TYPES)
+def test_linears_take_the_kernels_that_the_tests_mean(host, x, out):  # noqa: F811
+    host(f"""
+for m, n, k, wide, name in {LINEARS!r}:
+    if wide != ({x!r} == "f") * 2 + 2:
+        continue
+    name = name.format(x={x!r}, out={out!r}).encode()
+    before = fake.fake_launches_of(name)
+    row, words = up(up(k, 32) // 2, 16), up(up(k, 32) // 32, 4)
+    temp = P if lib.gsx_hip_linear4_temp_bytes(m, n, k) else None
+    _lib.check(lib.gsx_hip_linear4_forward(P, {TYPES[x]}, k, P, row, P, words, m, n, k, P, {TYPES[out]}, n, temp, None), "linear")
+    assert fake.fake_launches_of(name) == before + 1, (m, n, k, name)
 """)

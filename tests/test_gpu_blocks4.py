@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 
 import blocks4_plain as plain
+from blocks4_ways import LINEARS as WAYS
 from blocks4_ways import PRODUCTS
 
 pytestmark = pytest.mark.gpu
@@ -72,64 +73,65 @@ def test_every_code_and_exponent_expands(kind):
         assert torch.equal(got.double().nan_to_num(nan=7e77), want.float().to(DTYPES[kind]).double().nan_to_num(nan=7e77))
 
 
-def _blocks(x, garbage=False):
-    """Blocks of a float array, by the definition; garbage: behind the last value there are other codes and NaN scales."""
+def _rows(rows, cols, seed):
+    """Rows whose columns and themselves differ in size."""
+    g = torch.Generator("cuda").manual_seed(seed)
+    x = torch.randn(rows, cols, device="cuda", generator=g, dtype=torch.float64)
+    x *= torch.exp(torch.randn(cols, device="cuda", generator=g))
+    return (x * 2.0 ** torch.randint(-3, 4, (rows, 1), device="cuda", generator=g)).float()
+
+
+def _blocks(x):
+    """x in blocks (whose making has tests of its own), and what they stand for; behind the last value there are other codes and NaN
+    scales."""
     from gsx_amd import fields
     rows, cols = x.shape
-    q, e = plain.blocks(x)
-    nb = e.shape[1]
-    values = np.zeros((rows, nb * 16 + (32 if garbage else 0)), np.uint8)
-    exponents = np.zeros((rows, -(-nb // 4) * 4 + (4 if garbage else 0)), np.uint8)
-    if garbage:
-        rng = np.random.default_rng(1)
-        values[:] = rng.integers(0, 256, values.shape)
-        exponents[:] = 255
-        q[:, cols:] = rng.integers(0, 16, q[:, cols:].shape)
-    values[:, : nb * 16] = plain.packed(q)
-    exponents[:, :nb] = e
-    return fields.Blocks4(torch.from_numpy(values).cuda(), torch.from_numpy(exponents).cuda(), cols), plain.values(q, e, cols)
+    made = fields.quantize4(x)
+    bytes_, blocks = -(-cols // 2), -(-cols // 32)
+    values = torch.randint(0, 256, (rows, made.values.shape[1] + 32), dtype=torch.uint8, device="cuda")
+    exponents = torch.full((rows, made.exponents.shape[1] + 4), 255, dtype=torch.uint8, device="cuda")
+    values[:, :bytes_] = made.values[:, :bytes_]
+    if cols % 2:
+        values[:, bytes_ - 1] = made.values[:, bytes_ - 1] & 15 | 0xA0
+    exponents[:, :blocks] = made.exponents[:, :blocks]
+    return fields.Blocks4(values, exponents, cols), made.float().double()
 
 
 def _room(a, b, k, kind, want):
     """How far a product may be: an instruction takes 128 k and rounds each of its four blocks' sums and what it adds them to, eight
     roundings at the most, each half a step of a number no larger than the terms' magnitudes together; then the result's type."""
-    size = np.abs(a) @ np.abs(b).T
-    off = 8 * (-(-k // 128) + 1) * U * size
+    off = 8 * (-(-k // 128) + 1) * U * (a.abs() @ b.abs().T)
     least = 2.0**-25 if kind == "f16" else 0.0
-    return off + UNIT[kind] * (np.abs(want) + off) + least
+    return off + UNIT[kind] * (want.abs() + off) + least
 
 
-def _rows(rng, m, k):
-    return rng.standard_normal((m, k)) * np.exp(rng.standard_normal(k)) * 2.0 ** rng.integers(-3, 4, (m, 1))
-
-
-@pytest.mark.parametrize("out", DTYPES)
-@pytest.mark.parametrize("m,n,k", [p[:3] for p in PRODUCTS])
-def test_products_against_64_bits(m, n, k, out):
-    from gsx_amd import fields
-    print(f"[case] 4-bit product {m} x {n} x {k} {out}", flush=True)
-    rng = np.random.default_rng(m + k)
-    a, va = _blocks(_rows(rng, m, k), garbage=True)
-    b, vb = _blocks(_rows(rng, n, k) * 0.1, garbage=True)
-    room = torch.full((m, n + 5), 7.0, dtype=DTYPES[out], device="cuda")
-    fields.matmul(a, b, out=room[:, :n])
-    assert (room[:, n:] == 7).all()
+def _check_product(call, va, vb, k):
+    m, n = va.shape[0], vb.shape[0]
     want = va @ vb.T
-    got = room[:, :n].double().cpu().numpy()
-    assert (np.abs(got - want) <= _room(va, vb, k, out, want)).all(), np.abs(got - want).max()
+    for kind in DTYPES:
+        room = torch.full((m, n + 3), 7.0, dtype=DTYPES[kind], device="cuda")
+        call(room[:, :n])
+        assert (room[:, n:] == 7).all()
+        got = room[:, :n].double()
+        # what lies beyond the type's range (float16: from 65520 on) is infinite there
+        beyond = want.to(DTYPES[kind]).isinf() & (got == want.to(DTYPES[kind]).double())
+        assert ((got - want).abs() <= _room(va, vb, k, kind, want)).logical_or(beyond).all(), kind
+
+
+@pytest.mark.parametrize("m,n,k", [p[:3] for p in PRODUCTS])
+def test_products_against_64_bits(m, n, k):
+    from gsx_amd import fields
+    print(f"[case] 4-bit product {m} x {n} x {k}", flush=True)
+    (a, va), (b, vb) = _blocks(_rows(m, k, m + k)), _blocks(_rows(n, k, n + k) * 0.1)
+    _check_product(lambda out: fields.matmul(a, b, out=out), va, vb, k)
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 5, 2), (3, 1, 33), (17, 16, 32), (16, 64, 64), (65, 65, 256), (64, 64, 257),
                                    (5, 7, 0), (2, 3, 70_001), (130, 70, 9000)])
 def test_products_of_small_and_long_shapes(m, n, k):
     from gsx_amd import fields
-    rng = np.random.default_rng(k)
-    a, va = _blocks(_rows(rng, m, k), garbage=k > 0)
-    b, vb = _blocks(_rows(rng, n, k), garbage=k > 0)
-    want = va @ vb.T
-    got = fields.matmul(a, b).double().cpu().numpy()
-    assert got.shape == (m, n)
-    assert (np.abs(got - want) <= _room(va, vb, k, "f32", want)).all()
+    (a, va), (b, vb) = _blocks(_rows(m, k, k)), _blocks(_rows(n, k, k + 1))
+    _check_product(lambda out: fields.matmul(a, b, out=out), va, vb, k)
 
 
 @pytest.mark.parametrize("m,n", [(3, 5), (70, 80), (300, 280), (2100, 2050), (3900, 3901)])
@@ -154,7 +156,7 @@ def test_products_of_any_exponents(m, n):
     va, vb, got = va[keep_a], vb[keep_b], got[keep_a][:, keep_b]
     with np.errstate(over="ignore"):
         want = va @ vb.T
-    room = _room(va, vb, k, "f32", want) + 2.0**-126 * 128
+    room = _room(*(torch.from_numpy(v) for v in (va, vb)), k, "f32", torch.from_numpy(want)).numpy() + 2.0**-126 * 128
     fits = (np.abs(va) @ np.abs(vb).T) < 3e38
     assert (np.abs(got - want) <= room)[fits].all()
     assert not fits.all()  # 2^103 times 2^103
@@ -188,9 +190,10 @@ def test_small_blocks_beside_large_ones_that_cancel(m, n, k, out):
     assert torch.equal(fields.linear(x, weight, out_dtype=DTYPES[out]), want)
 
 
-LINEARS = [(1, 1, 1), (1, 333, 130), (2, 50, 16_500), (7, 129, 257), (16, 32_771, 300), (17, 40, 96), (500, 64, 257),
-           (500, 128, 384), (500, 129, 128), (3001, 150, 257), (500, 193, 256), (300, 300, 300), (40_001, 150, 128), (600, 257, 40),
+LINEARS = [(1, 1, 1), (1, 333, 130), (2, 50, 16_500), (7, 129, 257), (17, 40, 96), (500, 64, 257),
+           (500, 128, 384), (500, 129, 128), (3001, 150, 257), (500, 193, 256), (300, 300, 300), (600, 257, 40),
            (5, 3, 0), (3000, 16, 1500), (999, 7, 33), (2000, 256, 777), (1, 50, 66_000)]
+LINEARS += [way[:3] for way in WAYS if way[:3] not in LINEARS]
 
 
 @pytest.mark.parametrize("kind", DTYPES)
@@ -198,31 +201,28 @@ LINEARS = [(1, 1, 1), (1, 333, 130), (2, 50, 16_500), (7, 129, 257), (16, 32_771
 def test_linear_layers_against_64_bits(m, n, k, kind):
     from gsx_amd import fields
     print(f"[case] 4-bit linear {m} x {n} x {k} {kind}", flush=True)
-    rng = np.random.default_rng(m + n + k)
-    x = _put(_rows(rng, m, k).astype(np.float32), kind, 5, 1)
-    w, vw = _blocks(_rows(rng, n, k) * 0.1, garbage=k > 0)
-    q, e = plain.blocks(x.double().cpu().numpy())
-    vx = plain.values(q, e, k)
-    want = vx @ vw.T
-    for out in DTYPES:
-        room = torch.full((m, n + 3), 7.0, dtype=DTYPES[out], device="cuda")
-        fields.linear(x, w, out=room[:, :n])
-        assert (room[:, n:] == 7).all()
-        got = room[:, :n].double().cpu().numpy()
-        assert (np.abs(got - want) <= _room(vx, vw, k, out, want)).all(), (out, np.abs(got - want).max())
+    room = torch.full((m, k + 5), float("nan"), dtype=DTYPES[kind], device="cuda")
+    x = room[:, 1: k + 1]
+    x.copy_(_rows(m, k, m + n + k))
+    w, vw = _blocks(_rows(n, k, n) * 0.1)
+    _check_product(lambda out: fields.linear(x, w, out=out), fields.quantize4(x).float().double(), vw, k)
+    if m * n * k > 0:  # rows of the result without a gap
+        whole = torch.empty(m, n, dtype=DTYPES[kind], device="cuda")
+        fields.linear(x, w, out=whole)
+        room = torch.empty(m, n + 1, dtype=DTYPES[kind], device="cuda")
+        fields.linear(x, w, out=room[:, 1:])
+        assert torch.equal(whole, room[:, 1:])
 
 
 @pytest.mark.parametrize("kind", DTYPES)
 @pytest.mark.parametrize("m,n,k", [(2, 40, 200), (16, 300, 130), (200, 150, 257), (300, 300, 500)])
 def test_rows_that_are_not_finite_are_nan_alone(m, n, k, kind):
     from gsx_amd import fields
-    rng = np.random.default_rng(3)
-    x = _rows(rng, m, k).astype(np.float32)
-    w, _ = _blocks(_rows(rng, n, k))
-    clean = fields.linear(_put(x, kind), w)
-    x[0, k - 1] = np.nan
-    x[1, 0] = -np.inf
-    got = fields.linear(_put(x, kind), w)
+    x = _rows(m, k, 3).to(DTYPES[kind])
+    w, _ = _blocks(_rows(n, k, 4))
+    clean = fields.linear(x, w)
+    x[0, k - 1], x[1, 0] = float("nan"), float("-inf")
+    got = fields.linear(x, w)
     assert got[:2].isnan().all() and torch.equal(got[2:], clean[2:])
 
 
