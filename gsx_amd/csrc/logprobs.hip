@@ -15,7 +15,7 @@ namespace gsx_amd {
 
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kMostAlternatives = 64;
-constexpr float kLeastFloat = -3.402823466e38f;
+constexpr float kLeastExponent2 = -256.0f;  // 2 to this is 0, a float's least is 2^-149
 
 // Of a set of logits: m, s and w as above.
 struct RowSums {
@@ -41,8 +41,8 @@ struct LogProbsArgs {
     uint64_t* partial_top;  // [slice][top] keys
 };
 
-// u_j where e_j is not 0 (2^-149 is the least float), and finite for z_j = -inf, so that e_j u_j = 0 there. NaN is left to e_j.
-__device__ inline float scaled_from(float z, float base, float scale2) { return fmaxf((z - base) * scale2, -256.0f); }
+// u_j where e_j is not 0, and finite for z_j = -inf, so that e_j u_j = 0 there. NaN is left to e_j.
+__device__ inline float scaled_from(float z, float base, float scale2) { return fmaxf((z - base) * scale2, kLeastExponent2); }
 
 // Whole numbers in the order of the logits: NaN above everything, -0 with 0. 0 is below all of them, 2^32 - 1 above.
 __device__ inline uint32_t ordered_bits(float x) {
@@ -55,44 +55,88 @@ __device__ inline float ordered_value(uint32_t o) {
 }
 constexpr uint32_t kOrderedClosed = 0x007fffffu;  // of -inf
 
-// The order of the alternatives: by value, then by the lowest index. 0: none.
+// The order of the alternatives: by value, then by the lowest index; 0: none. Rows of few logits in 16-bit types have 32 bits for it.
 __device__ inline uint64_t key_of(float x, int64_t index) {
     return (uint64_t)ordered_bits(x) << 32 | (0xffffffffu - (uint32_t)index);
 }
 __device__ inline bool key_open(uint64_t key) { return (uint32_t)(key >> 32) > kOrderedClosed; }
 
+template <typename T>
+struct RowKey {
+    typedef uint64_t Type;
+    static __device__ inline Type of(float x, int index) { return key_of(x, index); }
+    static __device__ inline uint64_t wide(Type k) { return key_open(k) ? k : 0; }
+};
+// 16 bits in the order of the values, then 16 of the index.
+__device__ inline uint32_t short_key(uint32_t bits, int index, uint32_t infinity) {
+    const uint32_t size = bits & 0x7fffu;
+    uint32_t o = bits & 0x8000u ? 0x8000u - size : 0x8000u + size;  // -0 with 0
+    if (size > infinity) o = 0xfffeu;
+    return o << 16 | (0xffffu - (uint32_t)index);
+}
+template <>
+struct RowKey<__bf16> {
+    typedef uint32_t Type;
+    static __device__ inline Type of(float x, int index) {
+        return short_key(__builtin_bit_cast(uint32_t, x) >> 16, index, 0x7f80u);
+    }
+    static __device__ inline uint64_t wide(Type k) {
+        const uint32_t o = k >> 16;
+        if (o <= 0x8000u - 0x7f80u) return 0;
+        const uint32_t bits = o >= 0x8000u ? o - 0x8000u : 0x8000u | (0x8000u - o);
+        return key_of(__builtin_bit_cast(float, bits << 16), 0xffff - (int)(k & 0xffffu));
+    }
+};
+template <>
+struct RowKey<_Float16> {
+    typedef uint32_t Type;
+    static __device__ inline Type of(float x, int index) {
+        return short_key(__builtin_bit_cast(uint16_t, (_Float16)x), index, 0x7c00u);
+    }
+    static __device__ inline uint64_t wide(Type k) {
+        const uint32_t o = k >> 16;
+        if (o <= 0x8000u - 0x7c00u) return 0;
+        const uint32_t bits = o >= 0x8000u ? o - 0x8000u : 0x8000u | (0x8000u - o);
+        return key_of((float)__builtin_bit_cast(_Float16, (uint16_t)bits), 0xffff - (int)(k & 0xffffu));
+    }
+};
+
+__device__ inline uint32_t larger_key(uint32_t a, uint32_t b) { return max(a, b); }
+__device__ inline uint64_t larger_key(uint64_t a, uint64_t b) { return a > b ? a : b; }
+
 template <int kCtrl>
-__device__ inline uint64_t dpp_move_u64(uint64_t v) {
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, kCtrl, 0xf, 0xf, false);
-    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), kCtrl, 0xf, 0xf, false);
-    return (uint64_t)hi << 32 | lo;
+__device__ inline uint32_t dpp_move_key(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kCtrl, 0xf, 0xf, false);
+}
+template <int kCtrl>
+__device__ inline uint64_t dpp_move_key(uint64_t v) {
+    return (uint64_t)dpp_move_key<kCtrl>((uint32_t)(v >> 32)) << 32 | dpp_move_key<kCtrl>((uint32_t)v);
 }
 
-// The largest key of a group; s_keys holds one for each of its waves.
-template <int kGroup>
-__device__ inline uint64_t max_key(uint64_t v, uint64_t* s_keys) {
-    const auto larger = [](uint64_t a, uint64_t b) { return a > b ? a : b; };
-    v = larger(v, dpp_move_u64<0xb1>(v));
-    v = larger(v, dpp_move_u64<0x4e>(v));
-    v = larger(v, dpp_move_u64<0x141>(v));
-    v = larger(v, dpp_move_u64<0x140>(v));
-    if constexpr (kGroup == 16) return v;
-    v = larger(v, __shfl_xor((unsigned long long)v, 16, 64));
-    v = larger(v, __shfl_xor((unsigned long long)v, 32, 64));
-    if constexpr (kGroup == 64) return v;
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) s_keys[threadIdx.x / 64] = v;
-    __syncthreads();
-    v = s_keys[0];
-#pragma unroll
-    for (int i = 1; i < kGroup / 64; ++i) v = larger(v, s_keys[i]);
+// The largest key of 8 or 16 lanes.
+template <int kGroup, typename Key>
+__device__ inline Key max_key(Key v) {
+    v = larger_key(v, dpp_move_key<0xb1>(v));
+    v = larger_key(v, dpp_move_key<0x4e>(v));
+    v = larger_key(v, dpp_move_key<0x141>(v));
+    if constexpr (kGroup == 16) v = larger_key(v, dpp_move_key<0x140>(v));
     return v;
 }
 
-// Sums of two values over a group.
+// Sums of two values, and a maximum, over a group.
+template <int kGroup>
+__device__ inline float sum_of_lanes(float v) {
+    if constexpr (kGroup == 8) {
+        v += dpp_move<0xb1, 0xf>(v);
+        v += dpp_move<0x4e, 0xf>(v);
+        return v + dpp_move<0x141, 0xf>(v);
+    } else {
+        return sum_of_group<kGroup>(v, nullptr);
+    }
+}
 template <int kGroup>
 __device__ inline float2 sums_of_group(float2 v, float2* s_wave) {
-    if constexpr (kGroup <= 64) return make_float2(sum_of_group<kGroup>(v.x, nullptr), sum_of_group<kGroup>(v.y, nullptr));
+    if constexpr (kGroup <= 64) return make_float2(sum_of_lanes<kGroup>(v.x), sum_of_lanes<kGroup>(v.y));
     v = make_float2(wave_reduce_sum(v.x), wave_reduce_sum(v.y));
     __syncthreads();
     if ((threadIdx.x & 63) == 0) s_wave[threadIdx.x / 64] = v;
@@ -105,105 +149,204 @@ __device__ inline float2 sums_of_group(float2 v, float2* s_wave) {
     }
     return v;
 }
-
-constexpr int kCandidates = 512;
-
 template <int kGroup>
-struct TopScratch {
-    uint64_t keys[kGroup == 16 ? 1 : kCandidates];
-    uint64_t wave_key[kGroup / 64 + 1];
-    float lane[kGroup > 64 ? kGroup : 1];
-    float threshold;
-    int count;
-};
-
-// The largest of the wave's 64 * kN values that at least k of them reach, or a lower one: its ordered bits are found from the
-// highest on, until exactly k values are left.
-template <int kN>
-__device__ inline float reached_by(const float (&v)[kN], int k) {
-    uint32_t o[kN];
-#pragma unroll
-    for (int i = 0; i < kN; ++i) o[i] = ordered_bits(v[i]);
-    uint32_t t = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t up = t | 1u << bit;
-        int n = 0;
-#pragma unroll
-        for (int i = 0; i < kN; ++i) n += __builtin_popcountll(__builtin_amdgcn_ballot_w64(o[i] >= up));
-        if (n >= k) t = up;
-        if (n == k) break;
+__device__ inline float largest_of_group(float v, float* s_wave) {
+    if constexpr (kGroup == 8) {
+        v = fmaxf(v, dpp_move<0xb1, 0xf>(v));
+        v = fmaxf(v, dpp_move<0x4e, 0xf>(v));
+        return fmaxf(v, dpp_move<0x141, 0xf>(v));
+    } else {
+        return max_of_group<kGroup>(v, s_wave);
     }
-    return t <= kOrderedClosed ? -INFINITY : ordered_value(t);
 }
 
-// The keys of `count` candidates (LDS) in order: emit(place, key) for the first `top`, 0 where there are fewer. Every candidate
-// counts those before it.
-template <int kGroup, typename Emit>
-__device__ inline void emit_ranked(const uint64_t* s_keys, int count, int top, int tid, Emit emit) {
+// The largest number that at least k of a wave's 64 * kN keys reach, or a lower one that exactly k of them do: its bits are found
+// from the highest on. 0 if there are fewer keys that are not 0.
+template <int kN, typename Key>
+__device__ inline Key reached_by(const Key (&v)[kN], int n, int k) {
+    Key t = 0;
+    for (int bit = 8 * (int)sizeof(Key) - 1; bit >= 0; --bit) {
+        const Key up = t | (Key)1 << bit;
+        int count = 0;
+#pragma unroll
+        for (int i = 0; i < kN; ++i)
+            if (i < n) count += __builtin_popcountll(__builtin_amdgcn_ballot_w64(v[i] >= up));
+        if (count >= k) t = up;
+        if (count == k) break;
+    }
+    return t;
+}
+
+constexpr int kCandidates = 1024;    // of a workgroup's row
+constexpr int kWaveCandidates = 256;  // of a wave's
+
+// Keys (LDS) in order: emit(place, key) for the first `top`, 0 where there are fewer. Every key counts those before it.
+template <int kGroup, typename Key, typename Emit>
+__device__ inline void emit_ranked(const Key* s_keys, int count, int top, int tid, Emit emit) {
     for (int c = tid; c < count; c += kGroup) {
-        const uint64_t key = s_keys[c];
+        const Key key = s_keys[c];
         int place = 0;
         for (int j = 0; j < count; ++j) place += s_keys[j] > key ? 1 : 0;
         if (place < top) emit(place, key);
     }
-    for (int c = count + tid; c < top; c += kGroup) emit(c, 0);
+    for (int c = count + tid; c < top; c += kGroup) emit(c, (Key)0);
 }
 
-// The `top` first alternatives of what a group holds in registers (each(f) calls f(value, index) for every one), in order.
-// `mine` is the thread's largest value; special: NaN or +inf are among them.
-template <int kGroup, typename Each, typename Emit>
-__device__ inline void top_of_group(Each each, float mine, bool special, int top, int tid, TopScratch<kGroup>& s, Emit emit) {
-    if constexpr (kGroup > 16) {
-        if (!special) {
-            // a value that the group's k-th largest thread reaches: at least k values do
-            float least;
-            group_sync<kGroup>();  // the row before is done
-            if (tid == 0) s.count = 0;
-            if constexpr (kGroup == 64) {
-                const float v[1] = {mine};
-                least = reached_by(v, top);
-            } else {
-                s.lane[tid] = mine;
-                __syncthreads();
-                if (tid < 64) {
-                    float v[kGroup / 64];
+// A wave's keys that are `least` or more, together in LDS; how many there are.
+template <int kN, typename Key>
+__device__ inline int collect_keys(const Key (&v)[kN], int n, Key least, Key* s_keys, int lane) {
+    int count = 0;
 #pragma unroll
-                    for (int i = 0; i < kGroup / 64; ++i) v[i] = s.lane[i * 64 + tid];
-                    const float t = reached_by(v, top);
-                    if (tid == 0) s.threshold = t;
-                }
-                __syncthreads();
-                least = s.threshold;
-            }
-            group_sync<kGroup>();
-            least = fmaxf(least, kLeastFloat);  // closed logits are no alternatives
-            each([&](float x, int64_t index) {
-                if (x >= least) {
-                    const int at = atomicAdd(&s.count, 1);
-                    if (at < kCandidates) s.keys[at] = key_of(x, index);
-                }
-            });
-            group_sync<kGroup>();
-            const int count = s.count;
-            if (count <= kCandidates) {
-                emit_ranked<kGroup>(s.keys, count, top, tid, emit);
-                return;
+    for (int i = 0; i < kN; ++i) {
+        const bool mine = i < n && v[i] >= least && v[i] != 0;
+        const uint64_t all = __builtin_amdgcn_ballot_w64(mine);
+        const int at = count + __builtin_amdgcn_mbcnt_hi((uint32_t)(all >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)all, 0));
+        if (mine && at < kWaveCandidates) s_keys[at] = v[i];
+        count += __builtin_popcountll(all);
+    }
+    return count;
+}
+
+// A row's alternatives by a wave. The row, which was just read, is read again, an element a lane. Where a lane has several, the
+// largest of each lane bound what the first `top` may be; what reaches that bound is ranked, or searched again where it is much.
+template <typename T, int kN, typename Emit>
+__device__ inline void top_of_wave(const T* __restrict__ z, int vocab, int top, int lane, typename RowKey<T>::Type* s_keys,
+                                   Emit emit) {
+    typedef typename RowKey<T>::Type Key;
+    const int n = (vocab + 63) / 64;
+    Key v[kN];
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+        const int at = i * 64 + lane;
+        v[i] = at < vocab ? RowKey<T>::of(to_float(z[at]), at) : (Key)0;
+        if (RowKey<T>::wide(v[i]) == 0) v[i] = 0;  // closed
+    }
+    wave_lds_sync();  // the row before is done
+    Key least = 0;
+    if (n >= 4) {
+        Key most[1] = {v[0]};
+#pragma unroll
+        for (int i = 1; i < kN; ++i) most[0] = larger_key(most[0], v[i]);
+        least = reached_by<1>(most, 1, top);
+    } else {
+        least = reached_by<kN>(v, n, top);
+    }
+    int count = collect_keys<kN>(v, n, least, s_keys, lane);
+    if (count > kWaveCandidates) {
+        least = reached_by<kN>(v, n, top);
+        count = collect_keys<kN>(v, n, least, s_keys, lane);
+    }
+    wave_lds_sync();
+    if (count > 64 && count > top) {
+        Key w[kWaveCandidates / 64];
+#pragma unroll
+        for (int i = 0; i < kWaveCandidates / 64; ++i) w[i] = i * 64 + lane < count ? s_keys[i * 64 + lane] : 0;
+        wave_lds_sync();
+        least = reached_by<kWaveCandidates / 64>(w, (count + 63) / 64, top);
+        count = collect_keys<kWaveCandidates / 64>(w, (count + 63) / 64, least, s_keys, lane);
+        wave_lds_sync();
+    }
+    emit_ranked<64>(s_keys, count, top, lane, [&](int place, Key k) { emit(place, RowKey<T>::wide(k)); });
+}
+
+template <int kGroup>
+struct TopScratch {
+    uint64_t keys[kCandidates];
+    uint32_t lane[kGroup];
+    uint32_t threshold;
+    int count, counts[2];
+};
+
+// A row's (or slice's) alternatives by a workgroup. `mine` is the thread's largest logit: the k-th largest of a wave's, or of all
+// where k is larger than 16, is reached by at least k logits, so only threads whose own reach it have candidates. Their logits are
+// read again, by their waves. special: there are NaN or +inf.
+template <typename T, int kGroup, int kVecs, typename Emit>
+__device__ inline void top_of_workgroup(const T* __restrict__ z, int64_t length, int64_t from, const Stretch& st, float mine,
+                                        float last, bool special, int top, TopScratch<kGroup>& s, Emit emit) {
+    constexpr int kElements = Words<T>::kElements;
+    const int tid = threadIdx.x, lane = tid & 63;
+    __syncthreads();  // the row before is done
+    if (tid == 0) {
+        s.count = 0;
+        s.threshold = 0;
+        s.counts[0] = 0;
+        s.counts[1] = 0;
+    }
+    const uint32_t most[1] = {ordered_bits(mine)};
+    if (top > 16) s.lane[tid] = most[0];
+    __syncthreads();
+    if (!special) {
+        if (top <= 16) {
+            const uint32_t t = reached_by<1>(most, 1, top);
+            if (lane == 0) atomicMax(&s.threshold, t);
+        } else if (tid < 64) {
+            uint32_t v[kGroup / 64];
+#pragma unroll
+            for (int i = 0; i < kGroup / 64; ++i) v[i] = s.lane[i * 64 + tid];
+            const uint32_t t = reached_by<kGroup / 64>(v, kGroup / 64, top);
+            if (tid == 0) s.threshold = t;
+        }
+        __syncthreads();
+        const uint32_t least = max(s.threshold, kOrderedClosed + 1);  // closed logits are no alternatives
+        const auto take = [&](float x, int64_t index) {
+            if (ordered_bits(x) < least) return;
+            const int at = atomicAdd(&s.count, 1);
+            if (at < kCandidates) s.keys[at] = key_of(x, from + index);
+        };
+        for (uint64_t hits = __builtin_amdgcn_ballot_w64(most[0] >= least); hits != 0; hits &= hits - 1) {
+            const int owner = (tid & ~63) + __builtin_ctzll(hits);
+            for (int i = lane; i < kVecs * kElements; i += 64) {
+                const int vec = i / kElements * kGroup + owner;
+                if (vec >= st.vecs) continue;
+                const int64_t at = st.lead + (int64_t)vec * kElements + i % kElements;
+                take(to_float(z[at]), at);
             }
         }
+        if (st.loose >= 0) take(last, st.loose);
+        __syncthreads();
+        const int count = s.count;
+        if (count <= kCandidates) {
+            emit_ranked<kGroup>(s.keys, count, top, tid, emit);
+            return;
+        }
     }
-    // one after the other
-    uint64_t before = ~0ull;
-    for (int place = 0; place < top; ++place) {
-        uint64_t best = 0;
-        each([&](float x, int64_t index) {
-            const uint64_t key = key_of(x, index);
-            if (key < before && key > best) best = key;
-        });
-        best = max_key<kGroup>(best, s.wave_key);
-        if (!key_open(best)) best = 0;
-        if (tid == 0) emit(place, best);
-        before = best;
+    // Many equal logits, or some that are not finite: the value of the last alternative is found bit by bit, then the last index that
+    // has it. Each count is one more look at the row.
+    int turn = 0;
+    const auto counted = [&](auto belongs) {
+        int n = 0;
+        for (int64_t i = tid; i < length; i += kGroup) n += belongs(ordered_bits(to_float(z[i])), (uint32_t)i) ? 1 : 0;
+        for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off, 64);
+        if (lane == 0) atomicAdd(&s.counts[turn], n);
+        __syncthreads();
+        n = s.counts[turn];
+        turn ^= 1;
+        if (tid == 0) s.counts[turn] = 0;
+        __syncthreads();
+        return n;
+    };
+    const int open = counted([](uint32_t o, uint32_t) { return o > kOrderedClosed; }), need = min(top, open);
+    uint32_t value = 0, end = 0;
+    if (need > 0) {
+        for (int bit = 31; bit >= 0; --bit) {
+            const uint32_t up = value | 1u << bit;
+            if (counted([&](uint32_t o, uint32_t) { return o >= up; }) >= need) value = up;
+        }
+        const int equal = need - counted([&](uint32_t o, uint32_t) { return o > value; });
+        for (int bit = 30; bit >= 0; --bit) {  // as many indices lie below `end` as leave less than `equal` before it
+            const uint32_t up = end + (1u << bit);
+            if (counted([&](uint32_t o, uint32_t i) { return o == value && i < up; }) < equal) end = up;
+        }
     }
+    if (tid == 0) s.count = 0;
+    __syncthreads();
+    for (int64_t i = tid; need > 0 && i < length; i += kGroup) {
+        const float x = to_float(z[i]);
+        const uint32_t o = ordered_bits(x);
+        if (o > value || (o == value && (uint32_t)i <= end)) s.keys[atomicAdd(&s.count, 1)] = key_of(x, from + i);
+    }
+    __syncthreads();
+    emit_ranked<kGroup>(s.keys, need, top, tid, emit);
 }
 
 // What a row's sums say to the outside.
@@ -247,9 +390,9 @@ struct RowGrad {
     bool live;
     float base, rate, slope, own;
     int32_t id;
-    __device__ inline float at(float z, float scale2) const {
-        const float u = scaled_from(z, base, scale2);
-        return __builtin_amdgcn_exp2f((z - base) * scale2) * (rate + slope * u);
+    __device__ inline float at(float z, float scale2, bool sloped) const {
+        const float u = (z - base) * scale2, e = __builtin_amdgcn_exp2f(u);
+        return sloped ? e * __builtin_fmaf(slope, fmaxf(u, kLeastExponent2), rate) : e * rate;
     }
 };
 __device__ inline RowGrad grad_of(const LogProbsArgs& a, int64_t row, float m, float s, float h) {
@@ -267,7 +410,8 @@ __device__ inline RowGrad grad_of(const LogProbsArgs& a, int64_t row, float m, f
     return g;
 }
 
-// Rows that fit the registers of a group: kGroup threads hold kVecs times 16 bytes each.
+// Rows that fit the registers of a group: kGroup threads hold kVecs times 16 bytes each. Groups of 8 lanes take their vectors from the
+// row's start on, at whatever address that is, and at most one logit a thread behind the last vector.
 template <typename T, int kGroup, int kVecs>
 struct HeldRow {
     static constexpr int kElements = Words<T>::kElements;
@@ -276,7 +420,13 @@ struct HeldRow {
     Stretch st;
 
     __device__ inline void load(const T* __restrict__ z, int64_t length, int tid) {
-        st = stretch_of<T>(z, length, tid);
+        if constexpr (kGroup == 8) {
+            st.lead = 0;
+            st.vecs = (int)length / kElements;
+            st.loose = st.vecs * kElements + tid < length ? st.vecs * kElements + tid : -1;
+        } else {
+            st = stretch_of<T>(z, length, tid);
+        }
 #pragma unroll
         for (int u = 0; u < kVecs; ++u) x[u] = load_words<T>(z + st.lead + u * kGroup * kElements, tid, st.vecs - u * kGroup);
         last = st.loose >= 0 ? to_float(z[st.loose]) : -INFINITY;
@@ -298,35 +448,51 @@ struct HeldRow {
             repack(x[u]);
 #pragma unroll
             for (int i = 0; i < kElements; ++i) {
-                const float z = element_of(x[u], i);
-                const float e = __builtin_amdgcn_exp2f((z - base) * scale2);
+                const float v = (element_of(x[u], i) - base) * scale2;
+                const float e = __builtin_amdgcn_exp2f(v);
                 r.x += e;
-                r.y += e * scaled_from(z, base, scale2);
+                r.y = __builtin_fmaf(e, fmaxf(v, kLeastExponent2), r.y);
             }
+            asm volatile("" : "+v"(r.x), "+v"(r.y));  // both sums go on with each vector: no e is kept for later
         }
         return r;
     }
-    // f(value, index) for every logit; behind the row's end there are some -inf
-    template <typename F>
-    __device__ inline void each(int tid, int64_t from, F f) {
-#pragma unroll
-        for (int u = 0; u < kVecs; ++u) {
-            repack(x[u]);
-            const int64_t at = from + st.lead + (int64_t)(u * kGroup + tid) * kElements;
-#pragma unroll
-            for (int i = 0; i < kElements; ++i) f(element_of(x[u], i), at + i);
-        }
-        f(last, from + st.loose);
-    }
 };
 
+// One alternative after the other, from keys in the registers of 8 or 16 lanes.
+template <typename T, int kGroup, int kVecs, typename Emit>
+__device__ inline void top_of_lanes(const HeldRow<T, kGroup, kVecs>& x, int top, int tid, Emit emit) {
+    typedef typename RowKey<T>::Type Key;
+    constexpr int kElements = Words<T>::kElements, kKeys = kVecs * kElements + 1;
+    Key keys[kKeys];
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u) {
+        const int vec = u * kGroup + tid;
+#pragma unroll
+        for (int i = 0; i < kElements; ++i)
+            keys[u * kElements + i] =
+                vec < x.st.vecs ? RowKey<T>::of(element_of(x.x[u], i), x.st.lead + vec * kElements + i) : (Key)0;
+    }
+    keys[kKeys - 1] = x.st.loose >= 0 ? RowKey<T>::of(x.last, (int)x.st.loose) : (Key)0;
+    for (int place = 0; place < top; ++place) {
+        Key best = keys[0];
+#pragma unroll
+        for (int i = 1; i < kKeys; ++i) best = larger_key(best, keys[i]);
+        best = max_key<kGroup>(best);
+        if (tid == 0) emit(place, RowKey<T>::wide(best));
+#pragma unroll
+        for (int i = 0; i < kKeys; ++i) keys[i] = keys[i] == best ? 0 : keys[i];
+    }
+}
+
 template <typename T, int kGroup, int kVecs>
-__global__ __launch_bounds__(kGroup < 256 ? 256 : kGroup) void logprobs_held_kernel(LogProbsArgs a,
-                                                                                    const T* __restrict__ logits,
-                                                                                    T* __restrict__ grad) {
+__global__ __launch_bounds__(kGroup < 256 ? 256 : kGroup, 4) void logprobs_held_kernel(LogProbsArgs a,
+                                                                                       const T* __restrict__ logits,
+                                                                                       T* __restrict__ grad) {
     constexpr int kGroups = kGroup < 256 ? 256 / kGroup : 1;  // rows of a workgroup
     constexpr int kElements = Words<T>::kElements;
-    __shared__ TopScratch<kGroup> s_top[kGroups];
+    __shared__ TopScratch<kGroups == 1 ? kGroup : 1> s_top[1];
+    __shared__ typename RowKey<T>::Type s_keys[kGroup == 64 ? kGroups : 1][kWaveCandidates];
     __shared__ float2 s_wave2[16];
     __shared__ float s_wave[16];
     const int group = kGroups == 1 ? 0 : threadIdx.x / kGroup, tid = kGroups == 1 ? threadIdx.x : threadIdx.x % kGroup;
@@ -336,35 +502,39 @@ __global__ __launch_bounds__(kGroup < 256 ? 256 : kGroup) void logprobs_held_ker
         x.load(z, a.vocab, tid);
         const float mine = x.largest();
         RowSums q;
-        q.m = max_of_group<kGroup>(mine, s_wave);
+        q.m = largest_of_group<kGroup>(mine, s_wave);
         const float base = q.m == -INFINITY ? 0.0f : q.m;
         const float2 sums = sums_of_group<kGroup>(x.sums(base, a.scale2), s_wave2);
         q.s = sums.x;
         q.w = sums.y;
         if (tid == 0) write_row(a, row, z, q);
-        if (a.top > 0) {
-            const RowAnswer r = answer_of(a, q);
-            top_of_group<kGroup>([&](auto f) { x.each(tid, 0, f); }, mine, q.s != q.s, a.top, tid, s_top[group],
-                                 [&](int place, uint64_t key) { write_alternative(a, row, place, key, r); });
-        }
-        if (grad == nullptr) continue;
-        T* const g = grad + row * a.grad_stride;
-        const RowGrad d = grad_of(a, row, q.m, q.s, entropy_of(q));
+        if (grad != nullptr) {
+            T* const g = grad + row * a.grad_stride;
+            const RowGrad d = grad_of(a, row, q.m, q.s, entropy_of(q));
+            const bool sloped = d.slope != 0.0f;
 #pragma unroll
-        for (int u = 0; u < kVecs; ++u) {
-            float y[kElements];
-            repack(x.x[u]);
+            for (int u = 0; u < kVecs; ++u) {
+                float y[kElements];
+                repack(x.x[u]);
 #pragma unroll
-            for (int i = 0; i < kElements; ++i) y[i] = d.live ? d.at(element_of(x.x[u], i), a.scale2) : 0.0f;
-            const int own = d.id - x.st.lead - (u * kGroup + tid) * kElements;
-            if (d.live && d.id >= 0 && own >= 0 && own < kElements) {
+                for (int i = 0; i < kElements; ++i) y[i] = d.live ? d.at(element_of(x.x[u], i), a.scale2, sloped) : 0.0f;
+                const int own = d.id - x.st.lead - (u * kGroup + tid) * kElements;
+                if (d.live && d.id >= 0 && own >= 0 && own < kElements) {
 #pragma unroll
-                for (int i = 0; i < kElements; ++i) y[i] += i == own ? d.own : 0.0f;
+                    for (int i = 0; i < kElements; ++i) y[i] += i == own ? d.own : 0.0f;
+                }
+                store_words<T>(g + x.st.lead + u * kGroup * kElements, tid, x.st.vecs - u * kGroup, y);
             }
-            store_words<T>(g + x.st.lead + u * kGroup * kElements, tid, x.st.vecs - u * kGroup, y);
+            if (x.st.loose >= 0)
+                g[x.st.loose] =
+                    from_float<T>(d.live ? d.at(x.last, a.scale2, sloped) + (d.id == x.st.loose ? d.own : 0.0f) : 0.0f);
         }
-        if (x.st.loose >= 0)
-            g[x.st.loose] = from_float<T>(d.live ? d.at(x.last, a.scale2) + (d.id == x.st.loose ? d.own : 0.0f) : 0.0f);
+        if (a.top == 0) continue;
+        const RowAnswer r = answer_of(a, q);
+        const auto emit = [&](int place, uint64_t key) { write_alternative(a, row, place, key, r); };
+        if constexpr (kGroup < 64) top_of_lanes<T, kGroup, kVecs>(x, a.top, tid, emit);
+        else if constexpr (kGroup == 64) top_of_wave<T, kVecs * kElements + 1>(z, (int)a.vocab, a.top, tid, s_keys[group], emit);
+        else top_of_workgroup<T, kGroup, kVecs>(z, a.vocab, 0, x.st, mine, x.last, q.s != q.s, a.top, s_top[0], emit);
     }
 }
 
@@ -388,23 +558,32 @@ __global__ __launch_bounds__(kSliceGroup) void logprobs_slices_kernel(LogProbsAr
         const float2 sums = sums_of_group<kSliceGroup>(x.sums(base, a.scale2), s_wave2);
         if (threadIdx.x == 0) a.partial[b] = {m, sums.x, sums.y};
         if (a.top > 0)
-            top_of_group<kSliceGroup>([&](auto f) { x.each(threadIdx.x, from, f); }, mine, sums.x != sums.x, a.top,
-                                      threadIdx.x, s_top, [&](int place, uint64_t key) { a.partial_top[b * a.top + place] = key; });
+            top_of_workgroup<T, kSliceGroup, kVecs>(logits + row * a.logits_stride + from, to - from, from, x.st, mine, x.last,
+                                                    sums.x != sums.x, a.top, s_top,
+                                                    [&](int place, uint64_t key) { a.partial_top[b * a.top + place] = key; });
     }
 }
 
 // and this one joins a row's.
 template <typename T>
 __global__ __launch_bounds__(kSliceGroup) void logprobs_join_kernel(LogProbsArgs a, const T* __restrict__ logits) {
-    __shared__ uint64_t s_keys[kCandidates], s_kept[kMostAlternatives];
+    __shared__ uint64_t s_keys[kCandidates], s_kept[kMostAlternatives], s_least;
     __shared__ float2 s_wave2[16];
     __shared__ float s_wave[16];
     __shared__ int s_count;
     const int tid = threadIdx.x;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const RowSums* const part = a.partial + row * a.slices;
+        const uint64_t* const keys = a.partial_top + row * a.slices * a.top;
+        // Of each slice the key at place p, top <= slices (p + 1): those that reach the k-th largest of them, k (p + 1) >= top,
+        // come from slices that have enough keys together, so no alternative is below it.
+        uint64_t most[1] = {0};
+        const int p = a.top > 0 ? (int)((a.top - 1) / a.slices) : 0;
         float m = -INFINITY;
-        for (int64_t i = tid; i < a.slices; i += kSliceGroup) m = fmaxf(m, part[i].m);
+        for (int64_t i = tid; i < a.slices; i += kSliceGroup) {
+            m = fmaxf(m, part[i].m);
+            if (a.top > 0) most[0] = larger_key(most[0], keys[i * a.top + p]);
+        }
         RowSums q;
         q.m = max_of_group<kSliceGroup>(m, s_wave);
         const float base = q.m == -INFINITY ? 0.0f : q.m;
@@ -415,28 +594,38 @@ __global__ __launch_bounds__(kSliceGroup) void logprobs_join_kernel(LogProbsArgs
             sums.x += f * p.s;
             sums.y += f * (p.w + u * p.s);
         }
+        if (tid == 0) {
+            s_count = 0;
+            s_least = 0;
+        }
+        if (a.top > 0) s_keys[tid] = most[0];
         sums = sums_of_group<kSliceGroup>(sums, s_wave2);
         q.s = sums.x;
         q.w = sums.y;
         if (tid == 0) write_row(a, row, logits + row * a.logits_stride, q);
         if (a.top == 0) continue;
         const RowAnswer r = answer_of(a, q);
-        const uint64_t* const keys = a.partial_top + row * a.slices * a.top;
+        if (tid < 64) {
+            uint64_t v[kSliceGroup / 64];
+#pragma unroll
+            for (int i = 0; i < kSliceGroup / 64; ++i) v[i] = s_keys[i * 64 + tid];
+            const uint64_t t = reached_by<kSliceGroup / 64>(v, kSliceGroup / 64, (a.top + p) / (p + 1));
+            if (tid == 0) s_least = t;
+        }
+        __syncthreads();
         const int64_t all = a.slices * a.top;
         // rounds of keys that come before the last of the `top` first ones so far
-        if (tid == 0) s_count = 0;
-        uint64_t least = 0;
-        __syncthreads();
+        uint64_t least = larger_key(s_least, (uint64_t)1);
         for (int64_t i0 = 0; i0 < all; i0 += kSliceGroup) {
             const uint64_t key = i0 + tid < all ? keys[i0 + tid] : 0;
-            if (key > least) s_keys[atomicAdd(&s_count, 1)] = key;
+            if (key >= least) s_keys[atomicAdd(&s_count, 1)] = key;
             __syncthreads();
             const int count = s_count;
             if (count + kSliceGroup > kCandidates && i0 + kSliceGroup < all) {
                 emit_ranked<kSliceGroup>(s_keys, count, a.top, tid, [&](int place, uint64_t k) { s_kept[place] = k; });
                 __syncthreads();
                 if (tid < a.top) s_keys[tid] = s_kept[tid];
-                least = s_kept[a.top - 1];
+                least = s_kept[a.top - 1] + 1;
                 if (tid == 0) s_count = a.top;
             }
             __syncthreads();
@@ -459,6 +648,7 @@ __global__ __launch_bounds__(256) void logprobs_grad_kernel(LogProbsArgs a, cons
         const T* const z = logits + row * a.logits_stride + from;
         T* const g = grad + row * a.grad_stride + from;
         const RowGrad d = grad_of(a, row, a.stats[3 * row], a.stats[3 * row + 1], a.stats[3 * row + 2]);
+        const bool sloped = d.slope != 0.0f;
         const Stretch st = stretch_of<T>(z, to - from, tid);
         for (int v = tid; v < st.vecs; v += kGroup * kAhead) {
             Words<T> x[kAhead];
@@ -468,7 +658,7 @@ __global__ __launch_bounds__(256) void logprobs_grad_kernel(LogProbsArgs a, cons
             for (int u = 0; u < kAhead; ++u) {
                 float y[kElements];
 #pragma unroll
-                for (int i = 0; i < kElements; ++i) y[i] = d.live ? d.at(element_of(x[u], i), a.scale2) : 0.0f;
+                for (int i = 0; i < kElements; ++i) y[i] = d.live ? d.at(element_of(x[u], i), a.scale2, sloped) : 0.0f;
                 const int64_t own = d.id - from - st.lead - (int64_t)(v + u * kGroup) * kElements;
                 if (d.live && d.id >= 0 && own >= 0 && own < kElements) {
 #pragma unroll
@@ -479,7 +669,7 @@ __global__ __launch_bounds__(256) void logprobs_grad_kernel(LogProbsArgs a, cons
         }
         if (st.loose >= 0)
             g[st.loose] = from_float<T>(
-                d.live ? d.at(to_float(z[st.loose]), a.scale2) + (d.id >= 0 && d.id - from == st.loose ? d.own : 0.0f) : 0.0f);
+                d.live ? d.at(to_float(z[st.loose]), a.scale2, sloped) + (d.id >= 0 && d.id - from == st.loose ? d.own : 0.0f) : 0.0f);
     }
 }
 
@@ -499,7 +689,8 @@ struct LogProbsPlan {
 LogProbsPlan logprobs_plan(int64_t rows, int64_t vocab, int64_t bytes, int32_t top) {
     LogProbsPlan p = {};
     const int64_t vecs = vocab * bytes / 16;
-    if (vecs <= 16 * 4 && top <= 8) p.group = 16;
+    if (vecs <= 8 * 4 && top <= 8) p.group = 8;
+    else if (vecs <= 16 * 4 && top <= 8) p.group = 16;
     else if (vecs <= 64 * 4) p.group = 64;
     else if (vecs <= 256 * 4 || (vecs <= 256 * 16 && rows >= 192)) p.group = 256;
     else if (vecs <= 512 * 16 && rows >= 192) p.group = 512;
@@ -549,9 +740,14 @@ gsx_hip_status launch_grad(LogProbsArgs a, const T* logits, T* grad, hipStream_t
 template <typename T>
 gsx_hip_status launch_logprobs(const LogProbsPlan& p, LogProbsArgs a, const T* logits, T* grad, void* temp,
                                hipStream_t stream) {
+    if (p.group == 8) {
+        if (p.vecs <= 1) return launch_held<T, 8, 1>(a, logits, grad, stream);
+        if (p.vecs <= 2) return launch_held<T, 8, 2>(a, logits, grad, stream);
+        if (p.vecs <= 3) return launch_held<T, 8, 3>(a, logits, grad, stream);
+        return launch_held<T, 8, 4>(a, logits, grad, stream);
+    }
     if (p.group == 16) {
-        if (p.vecs <= 1) return launch_held<T, 16, 1>(a, logits, grad, stream);
-        if (p.vecs <= 2) return launch_held<T, 16, 2>(a, logits, grad, stream);
+        if (p.vecs <= 3) return launch_held<T, 16, 3>(a, logits, grad, stream);
         return launch_held<T, 16, 4>(a, logits, grad, stream);
     }
     if (p.group == 64) {

@@ -4,13 +4,17 @@
 def _ways(t, wide):
     k = 1 if wide else 2  # elements of 4 bytes
     return [
-        (5, 3, 2, f"held_kernelI{t}Li16ELi1E"),
-        (33, 40 * k, 3, f"held_kernelI{t}Li16ELi1E"),
-        (9, 120 * k, 8, f"held_kernelI{t}Li16ELi2E"),
+        (5, 3, 2, f"held_kernelI{t}Li8ELi1E"),
+        (33, 40 * k, 3, f"held_kernelI{t}Li8ELi2E"),
+        (300, 76 * k - 1, 8, f"held_kernelI{t}Li8ELi3E"),
+        (9, 120 * k, 8, f"held_kernelI{t}Li8ELi4E"),
+        (37, 180 * k + 1, 5, f"held_kernelI{t}Li16ELi3E"),
         (21, 250 * k + 1, 5, f"held_kernelI{t}Li16ELi4E"),
         (6, 150, 9, f"held_kernelI{t}Li64ELi1E"),
         (6, 150, 64, f"held_kernelI{t}Li64ELi1E"),
+        (70, 250 * k, 40, f"held_kernelI{t}Li64ELi1E"),
         (5, 1021 * k, 64, f"held_kernelI{t}Li64ELi4E"),
+        (66, 700 * k, 5, f"held_kernelI{t}Li64ELi4E"),
         (4, 1500 * k + 1, 64, f"held_kernelI{t}Li256ELi4E"),
         (3, 4111 * k, 20, f"slices_kernelI{t}Li4E"),
         (193, 6001 * k, 33, f"held_kernelI{t}Li256ELi8E"),
