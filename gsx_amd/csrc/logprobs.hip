@@ -65,44 +65,43 @@ template <typename T>
 struct RowKey {
     typedef uint64_t Type;
     static __device__ inline Type of(float x, int index) { return key_of(x, index); }
+    static __device__ inline Type of_number(float x, int index) {
+        const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.0f);
+        return (uint64_t)(b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u)) << 32 | (0xffffffffu - (uint32_t)index);
+    }
     static __device__ inline uint64_t wide(Type k) { return key_open(k) ? k : 0; }
 };
-// 16 bits in the order of the values, then 16 of the index.
-__device__ inline uint32_t short_key(uint32_t bits, int index, uint32_t infinity) {
-    const uint32_t size = bits & 0x7fffu;
-    uint32_t o = bits & 0x8000u ? 0x8000u - size : 0x8000u + size;  // -0 with 0
-    if (size > infinity) o = 0xfffeu;
-    return o << 16 | (0xffffu - (uint32_t)index);
+// A float32 that holds a 16-bit one has zeros in its last 13 bits: the index (of at most 2^13 logits) takes their place.
+template <bool kFinite>
+__device__ inline uint32_t short_key(float x, int index) {
+    uint32_t o;
+    if constexpr (kFinite) {
+        const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.0f);
+        o = b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+    } else {
+        o = ordered_bits(x);
+    }
+    return (o & ~0x1fffu) | (0x1fffu - (uint32_t)index);
 }
-template <>
-struct RowKey<__bf16> {
+struct ShortRowKey {
     typedef uint32_t Type;
-    static __device__ inline Type of(float x, int index) {
-        return short_key(__builtin_bit_cast(uint32_t, x) >> 16, index, 0x7f80u);
-    }
+    static __device__ inline Type of(float x, int index) { return short_key<false>(x, index); }
+    static __device__ inline Type of_number(float x, int index) { return short_key<true>(x, index); }  // no NaN with a sign
     static __device__ inline uint64_t wide(Type k) {
-        const uint32_t o = k >> 16;
-        if (o <= 0x8000u - 0x7f80u) return 0;
-        const uint32_t bits = o >= 0x8000u ? o - 0x8000u : 0x8000u | (0x8000u - o);
-        return key_of(__builtin_bit_cast(float, bits << 16), 0xffff - (int)(k & 0xffffu));
+        if (k <= (kOrderedClosed | 0x1fffu)) return 0;
+        const uint32_t o = k & 0x80000000u ? k & ~0x1fffu : k | 0x1fffu;
+        return (uint64_t)o << 32 | (0xffffffffu - (0x1fffu - (k & 0x1fffu)));
     }
 };
 template <>
-struct RowKey<_Float16> {
-    typedef uint32_t Type;
-    static __device__ inline Type of(float x, int index) {
-        return short_key(__builtin_bit_cast(uint16_t, (_Float16)x), index, 0x7c00u);
-    }
-    static __device__ inline uint64_t wide(Type k) {
-        const uint32_t o = k >> 16;
-        if (o <= 0x8000u - 0x7c00u) return 0;
-        const uint32_t bits = o >= 0x8000u ? o - 0x8000u : 0x8000u | (0x8000u - o);
-        return key_of((float)__builtin_bit_cast(_Float16, (uint16_t)bits), 0xffff - (int)(k & 0xffffu));
-    }
-};
+struct RowKey<__bf16> : ShortRowKey {};
+template <>
+struct RowKey<_Float16> : ShortRowKey {};
 
 __device__ inline uint32_t larger_key(uint32_t a, uint32_t b) { return max(a, b); }
 __device__ inline uint64_t larger_key(uint64_t a, uint64_t b) { return a > b ? a : b; }
+__device__ inline uint32_t smaller_key(uint32_t a, uint32_t b) { return min(a, b); }
+__device__ inline uint64_t smaller_key(uint64_t a, uint64_t b) { return a < b ? a : b; }
 
 template <int kCtrl>
 __device__ inline uint32_t dpp_move_key(uint32_t v) {
@@ -113,13 +112,13 @@ __device__ inline uint64_t dpp_move_key(uint64_t v) {
     return (uint64_t)dpp_move_key<kCtrl>((uint32_t)(v >> 32)) << 32 | dpp_move_key<kCtrl>((uint32_t)v);
 }
 
-// The largest key of 8 or 16 lanes.
+// The smallest number of 8 or 16 lanes.
 template <int kGroup, typename Key>
-__device__ inline Key max_key(Key v) {
-    v = larger_key(v, dpp_move_key<0xb1>(v));
-    v = larger_key(v, dpp_move_key<0x4e>(v));
-    v = larger_key(v, dpp_move_key<0x141>(v));
-    if constexpr (kGroup == 16) v = larger_key(v, dpp_move_key<0x140>(v));
+__device__ inline Key smallest_of_lanes(Key v) {
+    v = smaller_key(v, dpp_move_key<0xb1>(v));
+    v = smaller_key(v, dpp_move_key<0x4e>(v));
+    v = smaller_key(v, dpp_move_key<0x141>(v));
+    if constexpr (kGroup == 16) v = smaller_key(v, dpp_move_key<0x140>(v));
     return v;
 }
 
@@ -163,14 +162,13 @@ __device__ inline float largest_of_group(float v, float* s_wave) {
 // The largest number that at least k of a wave's 64 * kN keys reach, or a lower one that exactly k of them do: its bits are found
 // from the highest on. 0 if there are fewer keys that are not 0.
 template <int kN, typename Key>
-__device__ inline Key reached_by(const Key (&v)[kN], int n, int k) {
+__device__ inline Key reached_by(const Key (&v)[kN], int k) {
     Key t = 0;
     for (int bit = 8 * (int)sizeof(Key) - 1; bit >= 0; --bit) {
         const Key up = t | (Key)1 << bit;
         int count = 0;
 #pragma unroll
-        for (int i = 0; i < kN; ++i)
-            if (i < n) count += __builtin_popcountll(__builtin_amdgcn_ballot_w64(v[i] >= up));
+        for (int i = 0; i < kN; ++i) count += __builtin_popcountll(__builtin_amdgcn_ballot_w64(v[i] >= up));
         if (count >= k) t = up;
         if (count == k) break;
     }
@@ -178,6 +176,7 @@ __device__ inline Key reached_by(const Key (&v)[kN], int n, int k) {
 }
 
 constexpr int kCandidates = 1024;    // of a workgroup's row
+constexpr int kManyCandidates = 160;  // from here on the k-th of them is searched before they are ranked
 constexpr int kWaveCandidates = 256;  // of a wave's
 
 // Keys (LDS) in order: emit(place, key) for the first `top`, 0 where there are fewer. Every key counts those before it.
@@ -192,60 +191,98 @@ __device__ inline void emit_ranked(const Key* s_keys, int count, int top, int ti
     for (int c = count + tid; c < top; c += kGroup) emit(c, (Key)0);
 }
 
-// A wave's keys that are `least` or more, together in LDS; how many there are.
-template <int kN, typename Key>
-__device__ inline int collect_keys(const Key (&v)[kN], int n, Key least, Key* s_keys, int lane) {
+// A wave's keys that are `least` or more (least > 0), together in LDS, at most kMost of them; how many there are.
+template <int kN, int kMost, typename Key>
+__device__ inline int collect_keys(const Key (&v)[kN], Key least, Key* s_keys, int lane) {
     int count = 0;
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
-        const bool mine = i < n && v[i] >= least && v[i] != 0;
+        const bool mine = v[i] >= least;
         const uint64_t all = __builtin_amdgcn_ballot_w64(mine);
         const int at = count + __builtin_amdgcn_mbcnt_hi((uint32_t)(all >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)all, 0));
-        if (mine && at < kWaveCandidates) s_keys[at] = v[i];
+        if (mine && at < kMost) s_keys[at] = v[i];
         count += __builtin_popcountll(all);
     }
     return count;
 }
 
-// A row's alternatives by a wave. The row, which was just read, is read again, an element a lane. Where a lane has several, the
-// largest of each lane bound what the first `top` may be; what reaches that bound is ranked, or searched again where it is much.
-template <typename T, int kN, typename Emit>
-__device__ inline void top_of_wave(const T* __restrict__ z, int vocab, int top, int lane, typename RowKey<T>::Type* s_keys,
-                                   Emit emit) {
+// Of `count` keys in LDS (at most kMost) the first `top`, in no order, by one wave: how many are left.
+template <int kMost, typename Key>
+__device__ inline int keep_first(Key* s_keys, int count, int top, int lane) {
+    if (count <= 64 || count <= top) return count;
+    Key v[kMost / 64];
+#pragma unroll
+    for (int i = 0; i < kMost / 64; ++i) v[i] = i * 64 + lane < count ? s_keys[i * 64 + lane] : 0;
+    wave_lds_sync();
+    const Key least = reached_by<kMost / 64>(v, top);
+    return collect_keys<kMost / 64, kMost>(v, least, s_keys, lane);
+}
+
+// A row's alternatives by a wave. The row, which was just read, is read again. Up to 256 logits are searched for the k-th largest;
+// of longer rows only lanes have candidates whose own largest logit (mine) reaches what `top` lanes' do.
+template <typename T, int kVecs, typename Emit>
+__device__ inline void top_of_wave(const T* __restrict__ z, int vocab, const Stretch& st, float mine, float last, int top, int lane,
+                                   typename RowKey<T>::Type* s_keys, Emit emit) {
     typedef typename RowKey<T>::Type Key;
-    const int n = (vocab + 63) / 64;
-    Key v[kN];
-#pragma unroll
-    for (int i = 0; i < kN; ++i) {
-        const int at = i * 64 + lane;
-        v[i] = at < vocab ? RowKey<T>::of(to_float(z[at]), at) : (Key)0;
-        if (RowKey<T>::wide(v[i]) == 0) v[i] = 0;  // closed
-    }
+    constexpr int kElements = Words<T>::kElements, kFew = 4;
+    const Key closed = RowKey<T>::of(-INFINITY, 0);  // of those the largest
+    int count;
     wave_lds_sync();  // the row before is done
-    Key least = 0;
-    if (n >= 4) {
-        Key most[1] = {v[0]};
+    if (vocab <= 64 * kFew) {
+        Key v[kFew];
 #pragma unroll
-        for (int i = 1; i < kN; ++i) most[0] = larger_key(most[0], v[i]);
-        least = reached_by<1>(most, 1, top);
+        for (int i = 0; i < kFew; ++i) {
+            const int at = i * 64 + lane;
+            v[i] = at < vocab ? RowKey<T>::of(to_float(z[at]), at) : (Key)0;
+            if (v[i] <= closed) v[i] = 0;
+        }
+        const Key least = reached_by<kFew>(v, top);
+        count = collect_keys<kFew, kWaveCandidates>(v, least > 0 ? least : (Key)1, s_keys, lane);
     } else {
-        least = reached_by<kN>(v, n, top);
-    }
-    int count = collect_keys<kN>(v, n, least, s_keys, lane);
-    if (count > kWaveCandidates) {
-        least = reached_by<kN>(v, n, top);
-        count = collect_keys<kN>(v, n, least, s_keys, lane);
+        const uint32_t most[1] = {ordered_bits(mine)};
+        uint32_t least = reached_by<1>(most, top);
+        least = max(least, kOrderedClosed + 1);
+        count = 0;
+        const auto take = [&](bool some, float x, int index) {
+            const Key key = RowKey<T>::of(x, index);
+            const bool in = some && ordered_bits(x) >= least;
+            const uint64_t all = __builtin_amdgcn_ballot_w64(in);
+            const int at = count + __builtin_amdgcn_mbcnt_hi((uint32_t)(all >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)all, 0));
+            if (in && at < kWaveCandidates) s_keys[at] = key;
+            count += __builtin_popcountll(all);
+        };
+        // NaN does not show in a lane's largest logit: such rows are looked through as a whole
+        const bool odd = __builtin_amdgcn_ballot_w64(!(mine < INFINITY)) != 0;
+        if (!odd) {
+            for (uint64_t hits = __builtin_amdgcn_ballot_w64(most[0] >= least); hits != 0; hits &= hits - 1) {
+                const int owner = __builtin_ctzll(hits);
+#pragma unroll
+                for (int i0 = 0; i0 < kVecs * kElements; i0 += 64) {
+                    const int i = i0 + lane, vec = i / kElements * 64 + owner;
+                    const bool some = i < kVecs * kElements && vec < st.vecs;
+                    const int at = some ? st.lead + vec * kElements + i % kElements : 0;
+                    take(some, to_float(z[at]), at);
+                }
+            }
+            take(st.loose >= 0, last, (int)st.loose);
+        }
+        if (odd || count > kWaveCandidates) {  // the first ones so far and 64 more at a time
+            count = 0;
+            least = kOrderedClosed + 1;
+            for (int i0 = 0; i0 < vocab; i0 += 64) {
+                const int at = min(i0 + lane, vocab - 1);
+                take(i0 + lane < vocab, to_float(z[at]), at);
+                if (count + 64 > kWaveCandidates) {
+                    wave_lds_sync();
+                    count = keep_first<kWaveCandidates>(s_keys, count, top, lane);
+                    wave_lds_sync();
+                }
+            }
+        }
     }
     wave_lds_sync();
-    if (count > 64 && count > top) {
-        Key w[kWaveCandidates / 64];
-#pragma unroll
-        for (int i = 0; i < kWaveCandidates / 64; ++i) w[i] = i * 64 + lane < count ? s_keys[i * 64 + lane] : 0;
-        wave_lds_sync();
-        least = reached_by<kWaveCandidates / 64>(w, (count + 63) / 64, top);
-        count = collect_keys<kWaveCandidates / 64>(w, (count + 63) / 64, least, s_keys, lane);
-        wave_lds_sync();
-    }
+    count = keep_first<kWaveCandidates>(s_keys, count, top, lane);
+    wave_lds_sync();
     emit_ranked<64>(s_keys, count, top, lane, [&](int place, Key k) { emit(place, RowKey<T>::wide(k)); });
 }
 
@@ -277,13 +314,13 @@ __device__ inline void top_of_workgroup(const T* __restrict__ z, int64_t length,
     __syncthreads();
     if (!special) {
         if (top <= 16) {
-            const uint32_t t = reached_by<1>(most, 1, top);
+            const uint32_t t = reached_by<1>(most, top);
             if (lane == 0) atomicMax(&s.threshold, t);
         } else if (tid < 64) {
             uint32_t v[kGroup / 64];
 #pragma unroll
             for (int i = 0; i < kGroup / 64; ++i) v[i] = s.lane[i * 64 + tid];
-            const uint32_t t = reached_by<kGroup / 64>(v, kGroup / 64, top);
+            const uint32_t t = reached_by<kGroup / 64>(v, top);
             if (tid == 0) s.threshold = t;
         }
         __syncthreads();
@@ -304,8 +341,16 @@ __device__ inline void top_of_workgroup(const T* __restrict__ z, int64_t length,
         }
         if (st.loose >= 0) take(last, st.loose);
         __syncthreads();
-        const int count = s.count;
+        int count = s.count;
         if (count <= kCandidates) {
+            if (count > kManyCandidates) {
+                if (tid < 64) {
+                    const int left = keep_first<kCandidates>(s.keys, count, top, lane);
+                    if (tid == 0) s.count = left;
+                }
+                __syncthreads();
+                count = s.count;
+            }
             emit_ranked<kGroup>(s.keys, count, top, tid, emit);
             return;
         }
@@ -459,29 +504,52 @@ struct HeldRow {
     }
 };
 
-// One alternative after the other, from keys in the registers of 8 or 16 lanes.
+// NaN of a word's one or two logits without their signs, which comes before every number.
+template <typename T>
+__device__ inline uint32_t positive_nans(uint32_t w) {
+    if constexpr (sizeof(T) == 4) {
+        return (w & 0x7fffffffu) > 0x7f800000u ? 0x7fffffffu : w;
+    } else {
+        constexpr uint32_t kInf = __is_same(T, __bf16) ? 0x7f80u : 0x7c00u;
+        if ((w & 0x7fffu) > kInf) w = (w | 0x7fffu) & ~0x8000u;
+        if ((w >> 16 & 0x7fffu) > kInf) w = (w | 0x7fff0000u) & 0x7fffffffu;
+        return w;
+    }
+}
+
+// One alternative after the other, from keys in the registers of 8 or 16 lanes: of the keys up to a bound, the nearest. How far
+// a key lies below it wraps around for those that do not. special: there is NaN in the wave's rows.
 template <typename T, int kGroup, int kVecs, typename Emit>
-__device__ inline void top_of_lanes(const HeldRow<T, kGroup, kVecs>& x, int top, int tid, Emit emit) {
+__device__ inline void top_of_lanes(HeldRow<T, kGroup, kVecs>& x, bool special, int top, int tid, Emit emit) {
     typedef typename RowKey<T>::Type Key;
     constexpr int kElements = Words<T>::kElements, kKeys = kVecs * kElements + 1;
     Key keys[kKeys];
+    if (special) {
+#pragma unroll
+        for (int u = 0; u < kVecs; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x.x[u].w[i] = positive_nans<T>(x.x[u].w[i]);
+        if (x.last != x.last) x.last = __builtin_nanf("");
+    }
 #pragma unroll
     for (int u = 0; u < kVecs; ++u) {
         const int vec = u * kGroup + tid;
+        repack(x.x[u]);
 #pragma unroll
-        for (int i = 0; i < kElements; ++i)
-            keys[u * kElements + i] =
-                vec < x.st.vecs ? RowKey<T>::of(element_of(x.x[u], i), x.st.lead + vec * kElements + i) : (Key)0;
+        for (int i = 0; i < kElements; ++i)  // behind the row's end lies -inf
+            keys[u * kElements + i] = RowKey<T>::of_number(element_of(x.x[u], i), x.st.lead + vec * kElements + i);
     }
-    keys[kKeys - 1] = x.st.loose >= 0 ? RowKey<T>::of(x.last, (int)x.st.loose) : (Key)0;
+    keys[kKeys - 1] = RowKey<T>::of_number(x.last, max((int)x.st.loose, 0));
+    Key most = ~(Key)0;
     for (int place = 0; place < top; ++place) {
-        Key best = keys[0];
+        Key apart = most - keys[0];
 #pragma unroll
-        for (int i = 1; i < kKeys; ++i) best = larger_key(best, keys[i]);
-        best = max_key<kGroup>(best);
-        if (tid == 0) emit(place, RowKey<T>::wide(best));
-#pragma unroll
-        for (int i = 0; i < kKeys; ++i) keys[i] = keys[i] == best ? 0 : keys[i];
+        for (int i = 1; i < kKeys; ++i) apart = smaller_key(apart, most - keys[i]);
+        apart = smallest_of_lanes<kGroup>(apart);
+        const Key best = most - apart;
+        const uint64_t key = best <= most ? RowKey<T>::wide(best) : 0;  // none is left where it wraps
+        if (tid == 0) emit(place, key);
+        if (key != 0) most = best - 1;
     }
 }
 
@@ -532,8 +600,10 @@ __global__ __launch_bounds__(kGroup < 256 ? 256 : kGroup, 4) void logprobs_held_
         if (a.top == 0) continue;
         const RowAnswer r = answer_of(a, q);
         const auto emit = [&](int place, uint64_t key) { write_alternative(a, row, place, key, r); };
-        if constexpr (kGroup < 64) top_of_lanes<T, kGroup, kVecs>(x, a.top, tid, emit);
-        else if constexpr (kGroup == 64) top_of_wave<T, kVecs * kElements + 1>(z, (int)a.vocab, a.top, tid, s_keys[group], emit);
+        if constexpr (kGroup < 64)
+            top_of_lanes<T, kGroup, kVecs>(x, __builtin_amdgcn_ballot_w64(q.s != q.s) != 0, a.top, tid, emit);
+        else if constexpr (kGroup == 64)
+            top_of_wave<T, kVecs>(z, (int)a.vocab, x.st, q.s != q.s ? INFINITY : mine, x.last, a.top, tid, s_keys[group], emit);
         else top_of_workgroup<T, kGroup, kVecs>(z, a.vocab, 0, x.st, mine, x.last, q.s != q.s, a.top, s_top[0], emit);
     }
 }
@@ -567,7 +637,7 @@ __global__ __launch_bounds__(kSliceGroup) void logprobs_slices_kernel(LogProbsAr
 // and this one joins a row's.
 template <typename T>
 __global__ __launch_bounds__(kSliceGroup) void logprobs_join_kernel(LogProbsArgs a, const T* __restrict__ logits) {
-    __shared__ uint64_t s_keys[kCandidates], s_kept[kMostAlternatives], s_least;
+    __shared__ uint64_t s_keys[kCandidates], s_least;
     __shared__ float2 s_wave2[16];
     __shared__ float s_wave[16];
     __shared__ int s_count;
@@ -609,26 +679,25 @@ __global__ __launch_bounds__(kSliceGroup) void logprobs_join_kernel(LogProbsArgs
             uint64_t v[kSliceGroup / 64];
 #pragma unroll
             for (int i = 0; i < kSliceGroup / 64; ++i) v[i] = s_keys[i * 64 + tid];
-            const uint64_t t = reached_by<kSliceGroup / 64>(v, kSliceGroup / 64, (a.top + p) / (p + 1));
+            const uint64_t t = reached_by<kSliceGroup / 64>(v, (a.top + p) / (p + 1));
             if (tid == 0) s_least = t;
         }
         __syncthreads();
         const int64_t all = a.slices * a.top;
-        // rounds of keys that come before the last of the `top` first ones so far
-        uint64_t least = larger_key(s_least, (uint64_t)1);
+        const uint64_t least = larger_key(s_least, (uint64_t)1);
         for (int64_t i0 = 0; i0 < all; i0 += kSliceGroup) {
             const uint64_t key = i0 + tid < all ? keys[i0 + tid] : 0;
             if (key >= least) s_keys[atomicAdd(&s_count, 1)] = key;
             __syncthreads();
             const int count = s_count;
-            if (count + kSliceGroup > kCandidates && i0 + kSliceGroup < all) {
-                emit_ranked<kSliceGroup>(s_keys, count, a.top, tid, [&](int place, uint64_t k) { s_kept[place] = k; });
+            __syncthreads();  // everybody has read it
+            if (count + kSliceGroup > kCandidates || (i0 + kSliceGroup >= all && count > kManyCandidates)) {
+                if (tid < 64) {
+                    const int left = keep_first<kCandidates>(s_keys, count, a.top, tid);
+                    if (tid == 0) s_count = left;
+                }
                 __syncthreads();
-                if (tid < a.top) s_keys[tid] = s_kept[tid];
-                least = s_kept[a.top - 1] + 1;
-                if (tid == 0) s_count = a.top;
             }
-            __syncthreads();
         }
         emit_ranked<kSliceGroup>(s_keys, s_count, a.top, tid,
                                  [&](int place, uint64_t key) { write_alternative(a, row, place, key, r); });
@@ -656,6 +725,7 @@ __global__ __launch_bounds__(256) void logprobs_grad_kernel(LogProbsArgs a, cons
             for (int u = 0; u < kAhead; ++u) x[u] = load_words<T>(z + st.lead, v + u * kGroup, d.live ? st.vecs : 0);
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
+                if (v + u * kGroup >= st.vecs) continue;
                 float y[kElements];
 #pragma unroll
                 for (int i = 0; i < kElements; ++i) y[i] = d.live ? d.at(element_of(x[u], i), a.scale2, sloped) : 0.0f;
