@@ -1,12 +1,16 @@
-"""A label field over a Gaussian scene, trained against a teacher's top logits: every operator of `gsx_amd.fields` as a program
-uses them, one step after another.
+"""A label field over a Gaussian scene, trained against a teacher's top logits or against given labels: every operator of
+`gsx_amd.fields` as a program uses them, one step after another.
 
-    python -m gsx_amd.label_field [--gaussians N] [--labels L] [--steps K]
+    python -m gsx_amd.label_field [--gaussians N] [--labels L] [--steps K] [--given] [--moments 32|8] [--answers K]
 
 Each Gaussian holds the code of the grid cell it lies in. A field is a table with a row for each code and a head with a row for
 each label. A step looks the rows up, multiplies them with the head in 8-bit blocks, compares the logits with the teacher's and
 carries the gradient back to head and table, which Adam updates in float32; the head's blocks are laid out anew from them.
 `LabelField.labels` answers for any Gaussians, one among them.
+
+With given labels a step's loss is the labels' negative log probability. AdamW takes Adam's place where moments are asked for in 32
+or 8 bits. `LabelField.answers` gives the likeliest labels with their log probabilities from a head in 4-bit blocks, half the bytes
+of the 8-bit one; what it gives is also a teacher for another field's steps.
 """
 from __future__ import annotations
 
@@ -16,15 +20,18 @@ import torch
 
 from . import fields, scenes
 from ._lib import GsxHipError
-from .backend import Adam
+from .backend import Adam, AdamW
 
 
 class LabelField:
     """codes: rows of the table; features: columns of table and head; labels: rows of the head. Rows travel in `dtype`, table,
-    head, their gradients and Adam's moments are float32."""
+    head, their gradients and Adam's moments are float32. moments: None for Adam, 32 or 8 for AdamW with moments of as many bits and
+    with weight_decay."""
 
     def __init__(self, codes: int, features: int, labels: int, temperature: float = 2.0, learning_rate: float = 1e-2,
-                 dtype=torch.bfloat16, seed: int = 0):
+                 dtype=torch.bfloat16, seed: int = 0, moments: int | None = None, weight_decay: float = 0.0):
+        if moments is None and weight_decay != 0.0:
+            raise GsxHipError("weight decay needs AdamW: moments of 32 or 8 bits")
         g = torch.Generator(device="cuda").manual_seed(seed)
         self.scale = 1.0 / features ** 0.5
         self.temperature = temperature
@@ -33,14 +40,25 @@ class LabelField:
         self.head = torch.randn(labels, features, device="cuda", generator=g) * 0.1
         self.table_grad = torch.zeros_like(self.table)
         self.head_grad = torch.zeros_like(self.head)
-        self.optimizer = Adam([dict(parameter=self.table, gradient=self.table_grad, learning_rate=learning_rate),
-                               dict(parameter=self.head, gradient=self.head_grad, learning_rate=learning_rate)])
+        if moments is None:
+            self.optimizer = Adam([dict(parameter=self.table, gradient=self.table_grad, learning_rate=learning_rate),
+                                   dict(parameter=self.head, gradient=self.head_grad, learning_rate=learning_rate)])
+        else:
+            self.optimizer = AdamW([dict(parameters=[self.table, self.head], gradients=[self.table_grad, self.head_grad],
+                                         learning_rate=learning_rate, weight_decay=weight_decay)], bits=moments)
         self._lay_out()
 
     def _lay_out(self):
         """The head's blocks, along features for the product and along labels for its gradient."""
         self.blocks = fields.quantize(self.head)
         self.blocks_t = fields.quantize(self.head, transpose=True)
+        self._blocks4 = None  # laid out when the first answer after a step is asked for
+
+    def head_blocks4(self) -> fields.Blocks4:
+        """The head in 4-bit blocks."""
+        if self._blocks4 is None:
+            self._blocks4 = fields.quantize4(self.head)
+        return self._blocks4
 
     def logits(self, codes: torch.Tensor) -> torch.Tensor:
         """Logits [count, labels] of int32 codes; a Gaussian without a code (-1) has equal ones."""
@@ -48,6 +66,26 @@ class LabelField:
 
     def labels(self, codes: torch.Tensor) -> torch.Tensor:
         return self.logits(codes).argmax(1)
+
+    def answers(self, codes: torch.Tensor, top: int = 1, labels: torch.Tensor | None = None) -> fields.LogProbs:
+        """The `top` likeliest labels of int32 codes with their log probabilities, the distribution's entropy, and the log
+        probability of given labels, by the head in 4-bit blocks."""
+        rows = fields.lookup(self.table, codes, self.scale, out_dtype=self.dtype)
+        return fields.log_probs(fields.linear(rows, self.head_blocks4(), out_dtype=torch.float32), labels, top)
+
+    def step_labels(self, codes: torch.Tensor, labels: torch.Tensor, row_weight: torch.Tensor | None = None,
+                    entropy_weight: float = 0.0) -> torch.Tensor:
+        """One training step against given int32 labels (a row whose label lies outside of the field's has none); the rows'
+        losses, -log p(label) times the row's weight less entropy_weight times the entropy. The gradient is that of their mean."""
+        if codes.numel() == 0:
+            raise GsxHipError("a step needs at least one row")
+        rows = fields.lookup(self.table, codes, self.scale, out_dtype=self.dtype)
+        logits = fields.linear(rows, self.blocks)
+        mean = 1.0 / codes.numel()
+        q = fields.log_probs(logits, labels, grad_scale=-mean, row_grad=row_weight, entropy_scale=-mean * entropy_weight)
+        self._descend(rows, q.grad, codes)
+        loss = -q.chosen if row_weight is None else torch.where(row_weight != 0, -q.chosen * row_weight, 0.0)
+        return loss if entropy_weight == 0.0 else loss - entropy_weight * q.entropy
 
     def step(self, codes: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor,
              row_weight: torch.Tensor | None = None) -> torch.Tensor:
@@ -58,11 +96,15 @@ class LabelField:
         logits = fields.linear(rows, self.blocks)
         loss, _, grad = fields.distill(logits, teacher_ids, teacher_logits, self.temperature, row_weight,
                                        grad_scale=1.0 / codes.numel())
+        self._descend(rows, grad, codes)
+        return loss
+
+    def _descend(self, rows, grad, codes):
+        """The logits' gradient carried back, and the optimizer's step."""
         grad_rows, _ = fields.linear_backward(rows, grad, self.blocks_t, grad_weight=self.head_grad)
         fields.lookup_backward(grad_rows, codes, self.table.shape[0], self.scale, grad_table=self.table_grad)
         self.optimizer.step()
         self._lay_out()
-        return loss
 
 
 def cell_codes(mean3d: torch.Tensor, cells: int) -> torch.Tensor:
@@ -93,20 +135,33 @@ def main(argv=None) -> float:
     p.add_argument("--top", type=int, default=8)
     p.add_argument("--steps", type=int, default=60)
     p.add_argument("--rate", type=float, default=0.05)
+    p.add_argument("--given", action="store_true", help="train against the teacher's first labels alone")
+    p.add_argument("--moments", type=int, choices=(32, 8), help="AdamW with moments of so many bits instead of Adam")
+    p.add_argument("--decay", type=float, default=0.0, help="AdamW's weight decay")
+    p.add_argument("--answers", type=int, default=0, help="print so many likeliest labels of one Gaussian, by a 4-bit head")
     a = p.parse_args(argv)
     mean3d = torch.from_numpy(scenes.config0(n=a.gaussians).scene.mean3d).cuda()
     codes = cell_codes(mean3d, a.cells)
     ids, logits = teacher_of(mean3d, a.labels, a.top)
     weight = (codes >= 0).float()
-    field = LabelField(a.cells ** 3, a.features, a.labels, learning_rate=a.rate)
+    field = LabelField(a.cells ** 3, a.features, a.labels, learning_rate=a.rate, moments=a.moments, weight_decay=a.decay)
+    first = ids[:, 0].contiguous()
     for k in range(a.steps):
-        loss = field.step(codes, ids, logits, weight)
+        loss = field.step_labels(codes, first, weight) if a.given else field.step(codes, ids, logits, weight)
         if k % 20 == 0 or k == a.steps - 1:
             print(f"step {k}: loss {loss.sum().item() / weight.sum().item():.4f}", flush=True)
     inside = codes >= 0
     agree = (field.labels(codes) == ids[:, 0])[inside].float().mean().item()
     print(f"the field's first label is the teacher's for {100 * agree:.1f}% of {int(inside.sum())} Gaussians")
     print(f"one Gaussian's label: {field.labels(codes[inside][:1]).item()}")
+    if a.answers > 0:
+        q = field.answers(codes, a.answers, first)
+        agree4 = (q.top_ids[:, 0] == first)[inside].float().mean().item()
+        print(f"by the 4-bit head for {100 * agree4:.1f}%, with {q.chosen[inside].mean().item():.3f} for the mean log probability "
+              f"of the teacher's")
+        one = field.answers(codes[inside][:1], a.answers)
+        for label, log_q in zip(one.top_ids[0].tolist(), one.top_log_probs[0].tolist()):
+            print(f"  label {label}: log probability {log_q:.3f}")
     return agree
 
 
