@@ -8,6 +8,7 @@ every computation runs in the HIP kernels of libgsx_hip.so.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 from dataclasses import dataclass
@@ -16,6 +17,7 @@ import torch
 
 from . import _lib
 from ._lib import Camera, GaussianGrads, Gaussians, GsxHipError, check
+from .fields import _current_stream
 
 __all__ = ["Camera", "Renderer", "Loss", "Adam", "AdamW", "DensityControl", "GsxHipError", "stream_handle", "ptr"]
 
@@ -310,8 +312,9 @@ class AdamW:
         self.steps = torch.zeros(1, dtype=torch.int64, device="cuda")
         self._factors = torch.zeros(2 * _lib.ADAM_MAX_GROUPS, device="cuda")
         self._lay_out()
-        self._stream = torch.cuda.current_stream()
-        self._stream.synchronize()  # steps may run on any stream
+        stream = torch.cuda.current_stream()
+        stream.synchronize()  # steps may run on any stream
+        self._stream = stream.cuda_stream
 
     def _lay_out(self):
         wide = self.first.element_size()
@@ -331,41 +334,42 @@ class AdamW:
         self._table, self._chunks = table.cuda(), chunks.value
 
     def _on(self, stream):
-        """The stream of a call, whose use of this optimizer's memory the allocator is told of."""
+        """The handle of a call's stream, whose use of this optimizer's memory the allocator is told of."""
         if torch.cuda.current_device() != self.device:
             raise GsxHipError("the optimizer's device must be the current one")
-        s = stream if stream is not None else torch.cuda.current_stream()
-        if s != self._stream:
+        handle = _current_stream(self.device) if stream is None else stream.cuda_stream
+        if handle != self._stream:
+            s = torch.cuda.current_stream() if stream is None else stream
             for t in (self.first, self.second, self.first_scale, self.second_scale, self.steps, self._factors, self._table):
                 if t is not None:
                     t.record_stream(s)
-        return s
+        return handle
 
     def step(self, grad_scale: float = 1.0, grad_factor: torch.Tensor | None = None, stream=None) -> None:
         """One step. Gradients are multiplied by grad_scale and by what grad_factor, one float32 on the device, holds then."""
         if grad_factor is not None and (grad_factor.get_device() != self.device or grad_factor.dtype != torch.float32 or
                                         grad_factor.numel() != 1):
             raise GsxHipError("grad_factor must be one float32 on the current HIP device")
-        s = self._on(stream)
+        handle = self._on(stream)
         arr = (_lib.AdamwGroup * len(self.groups))()
         for a, g in zip(arr, self.groups):
             a.beta1, a.beta2, a.learning_rate = g["beta1"], g["beta2"], g["learning_rate"]
             a.weight_decay, a.epsilon = g["weight_decay"], g["epsilon"]
         check(self.lib.gsx_hip_adamw_step(self._table.data_ptr(), self._chunks, arr, len(self.groups), grad_scale,
                                           None if grad_factor is None else grad_factor.data_ptr(), self.steps.data_ptr(),
-                                          self._factors.data_ptr(), s.cuda_stream), "adamw step")
+                                          self._factors.data_ptr(), handle), "adamw step")
 
     def moments(self, stream=None):
         """(first, second) moments in float32, each [size]; tensor i's from offsets[i] on, 0 between the tensors. With 32 bits
         they are the optimizer's own."""
         if self.bits == 32:
             return self.first, self.second
-        s = self._on(stream)
-        with torch.cuda.stream(s):
+        handle = self._on(stream)
+        with contextlib.nullcontext() if stream is None else torch.cuda.stream(stream):
             first, second = (torch.empty(self.size, device="cuda") for _ in range(2))
         check(self.lib.gsx_hip_moments_read(self.first.data_ptr(), self.first_scale.data_ptr(), self.second.data_ptr(),
                                             self.second_scale.data_ptr(), self.size // self.BLOCK, first.data_ptr(),
-                                            second.data_ptr(), s.cuda_stream), "moments")
+                                            second.data_ptr(), handle), "moments")
         return first, second
 
     def load(self, first: torch.Tensor, second: torch.Tensor, steps: int, stream=None) -> None:
@@ -375,8 +379,8 @@ class AdamW:
                 raise GsxHipError(f"moments are {self.size} contiguous float32 values on the current HIP device")
         if steps < 0:
             raise GsxHipError("the number of steps must be >= 0")
-        s = self._on(stream)
-        with torch.cuda.stream(s):
+        handle = self._on(stream)
+        with contextlib.nullcontext() if stream is None else torch.cuda.stream(stream):
             self.steps.fill_(int(steps))
             if self.bits == 32:
                 self.first.copy_(first)
@@ -384,8 +388,7 @@ class AdamW:
             else:
                 check(self.lib.gsx_hip_moments_hold(first.data_ptr(), second.data_ptr(), self.size // self.BLOCK,
                                                     self.first.data_ptr(), self.first_scale.data_ptr(),
-                                                    self.second.data_ptr(), self.second_scale.data_ptr(),
-                                                    s.cuda_stream), "moments")
+                                                    self.second.data_ptr(), self.second_scale.data_ptr(), handle), "moments")
 
 
 FIELD_WIDTHS = {"mean3d": 3, "rotation": 4, "logscale": 3, "opacity": 1, "sh0": 3, "sh1": 9, "sh2": 15, "sh3": 21}
