@@ -110,10 +110,44 @@ __device__ inline int swizzle4_b(int row) {
     return kPair<O> == 2 ? (row & 3) | (row >> 3 & 1) << 2 : row & 7;
 }
 
+// store_row4 for 16-bit rows that begin between two words: a lane's pieces go one column on, the column behind comes from the next
+// lane of the row. Whole words cost half as much as the same vectors two bytes off: 29681 x 2261 x 22 80 us that way, 64 this way.
+template <int TN, typename S>
+__device__ inline void store_shifted4(S* __restrict__ row, int64_t col, int64_t n, int lane, const v4f (&x)[TN]) {
+    struct __attribute__((packed, aligned(4))) Piece {
+        S v[8];
+    };
+    const int group = lane / 16;
+    if (group == 0 && col < n) row[col] = from_float<S>(x[0][0]);
+#pragma unroll
+    for (int j = 0; j < TN; j += 2) {
+        const bool last = group == 3 && j + 2 >= TN;
+        const float behind = __shfl(group == 0 && j + 2 < TN ? x[j + 2 < TN ? j + 2 : j][0] : x[j][0], (lane + 16) & 63, 64);
+        const int64_t c = col + 16 * j + group * 8 + 1;
+        Piece q;
+#pragma unroll
+        for (int i = 0; i < 7; ++i) q.v[i] = from_float<S>(x[j + (i + 1) / 4][(i + 1) % 4]);
+        q.v[7] = from_float<S>(behind);
+        if (c + 8 <= n && !last) {
+            *reinterpret_cast<Piece*>(row + c) = q;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (c + i < n && !(last && i == 7)) row[c + i] = q.v[i];
+        }
+    }
+}
+
 // A lane's 4 TN columns of a row of n, the first of them at `col` + 4 kPair<O> (lane / 16).
 template <typename O, int TN, typename S>
 __device__ inline void store_row4(S* __restrict__ row, int64_t col, int64_t n, int lane, const v4f (&x)[TN]) {
     constexpr int kP = kPair<O>;
+    if constexpr (sizeof(S) == 2) {
+        if (reinterpret_cast<uintptr_t>(row + col) % 4 != 0) {
+            store_shifted4<TN>(row, col, n, lane, x);
+            return;
+        }
+    }
     struct __attribute__((packed, aligned(sizeof(S)))) Piece {
         S v[4 * kP];
     };
@@ -369,9 +403,11 @@ using namespace gsx_amd;
 
 namespace {
 
-// Tiles and splits of a product by its sizes alone. Tiles of 256 and 192 run one to a CU, of 128 two; the edge is the one whose
-// whole rounds of tiles cover the product with the least work, the larger one where two do. What fills less than half a round is
-// split over k, two steps of 256 or more to a part.
+// Tiles and splits of a product by its sizes alone: what is estimated to take the least time. A round of tiles (256 or 192 wide one
+// to a CU, 128 two, 64 four) takes a fixed time, most of it the stores, and one a step of 256 k; in tenths of a microsecond, from
+// 8192 x 8192 x 256 to 8192: 8192 with tiles of 64 498 us, 128 346, 192 391, 256 285; 256 63, 50, 59 and 46. Narrow tiles pay where
+// wide ones leave CUs without work (493 x 7309 x 1940: 17 us, 27, 29 and 35) or fill the last round badly. What fills less than
+// half a round may also be split over k, two steps or more to a part; the parts' sums are then written, read and joined.
 struct Product4Plan {
     int edge;
     int64_t tiles_m, tiles_n, splits;
@@ -381,22 +417,31 @@ struct Product4Plan {
 constexpr int64_t kSum4MostSteps = kSumMostBlocks * kBlock / (kStep4 * kBlock4);  // 65536 k, after which a float sum starts anew
 
 Product4Plan product4_plan(int64_t m, int64_t n, int64_t k) {
-    Product4Plan p;
-    const auto cost = [&](int64_t edge, int64_t slots) {
-        return ceil_div(ceil_div(m, edge) * ceil_div(n, edge), slots) * (slots / 256) * edge * edge;
+    struct Tiles {
+        int edge;
+        int64_t slots, round, step;
     };
-    p.edge = 256;
-    if (cost(192, 256) < cost(256, 256)) p.edge = 192;
-    if (cost(128, 512) < cost(p.edge, 256)) p.edge = 128;
-    if (m <= 64 || n <= 64) p.edge = 64;
+    constexpr Tiles kTiles[] = {{256, 256, 90, 19}, {192, 256, 60, 15}, {128, 512, 50, 12}, {64, 1024, 25, 9}};
+    const int64_t steps = ceil_div(k, kStep4 * kBlock4), least = k > 0 ? ceil_div(steps, kSum4MostSteps) : 1;
+    Product4Plan p = {};
+    int64_t best = INT64_MAX;
+    for (const Tiles& t : kTiles) {
+        if (t.edge > 64 && (m <= 64 || n <= 64)) continue;
+        const int64_t count = ceil_div(m, t.edge) * ceil_div(n, t.edge);
+        int64_t most = count < t.slots / 2 ? t.slots / count : 1;  // one round of workgroups
+        if (most > steps / 2) most = steps / 2;
+        for (const int64_t splits : {least, most / 2, most}) {
+            if (splits < least) continue;
+            int64_t cost = ceil_div(count * splits, t.slots) * (t.round + t.step * ceil_div(steps, splits));
+            if (splits > 1) cost += 40 + splits * (m * n / 50000);
+            if (cost >= best) continue;
+            best = cost;
+            p.edge = t.edge;
+            p.splits = splits;
+        }
+    }
     p.tiles_m = ceil_div(m, p.edge);
     p.tiles_n = ceil_div(n, p.edge);
-    const int64_t steps = ceil_div(k, kStep4 * kBlock4), count = p.tiles_m * p.tiles_n;
-    const int64_t slots = p.edge >= 192 ? 256 : 512;
-    int64_t splits = count >= slots / 2 ? 1 : slots / count;  // one round of workgroups
-    if (splits > steps / 2) splits = steps / 2;
-    if (splits < ceil_div(steps, kSum4MostSteps)) splits = ceil_div(steps, kSum4MostSteps);
-    p.splits = splits < 1 ? 1 : splits;
     p.temp_bytes = p.splits > 1 ? p.splits * m * n * 4 : 0;
     return p;
 }

@@ -4,8 +4,11 @@
 PRODUCTS = [
     (60, 301, 1100, "Li2ELi2ELi2ELi2E"),
     (33, 17, 31, "Li2ELi2ELi2ELi2E"),
-    (1601, 1099, 1100, "Li4ELi4ELi2ELi2E"),
-    (300, 290, 255, "Li4ELi4ELi2ELi2E"),
+    (300, 290, 255, "Li2ELi2ELi2ELi2E"),
+    (300, 290, 4100, "Li2ELi2ELi2ELi2E"),
+    (1601, 1099, 1100, "Li2ELi2ELi2ELi2E"),
+    (1901, 2300, 1301, "Li4ELi4ELi2ELi2E"),
+    (20000, 257, 128, "Li4ELi4ELi2ELi2E"),
     (4001, 2050, 1100, "Li6ELi4ELi2ELi3E"),
     (2899, 2900, 1301, "Li6ELi4ELi2ELi3E"),
     (3900, 3901, 1100, "Li8ELi4ELi2ELi4E"),
@@ -31,6 +34,7 @@ LINEARS = [
     (12301, 193, 300, 2, "linear4_head_kernelI{x}{out}Li16E"),
     (4999, 256, 128, 4, "linear4_head_kernelI{x}{out}Li16E"),
     (16390, 16, 500, 2, "linear4_head_kernelI{x}{out}Li4E"),
-    (5000, 257, 128, 2, "product4_kernelI{out}Li4ELi4ELi2ELi2E"),
-    (300, 300, 300, 2, "product4_kernelI{out}Li4ELi4ELi2ELi2E"),
+    (5000, 257, 128, 2, "product4_kernelI{out}Li2ELi2ELi2ELi2E"),
+    (300, 300, 300, 2, "product4_kernelI{out}Li2ELi2ELi2ELi2E"),
+    (2333, 3001, 1100, 2, "product4_kernelI{out}Li4ELi4ELi2ELi2E"),
 ]
