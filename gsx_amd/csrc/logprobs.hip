@@ -45,11 +45,11 @@ struct LogProbsArgs {
 __device__ inline float scaled_from(float z, float base, float scale2) { return fmaxf((z - base) * scale2, kLeastExponent2); }
 
 // Whole numbers in the order of the logits: NaN above everything, -0 with 0. 0 is below all of them, 2^32 - 1 above.
-__device__ inline uint32_t ordered_bits(float x) {
+__device__ inline uint32_t ordered_number(float x) {  // of a number, or NaN without a sign
     const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.0f);
-    if (x != x) return 0xfffffffeu;
     return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
+__device__ inline uint32_t ordered_bits(float x) { return x != x ? 0xfffffffeu : ordered_number(x); }
 __device__ inline float ordered_value(uint32_t o) {
     return __builtin_bit_cast(float, o & 0x80000000u ? o ^ 0x80000000u : ~o);
 }
@@ -66,29 +66,18 @@ struct RowKey {
     typedef uint64_t Type;
     static __device__ inline Type of(float x, int index) { return key_of(x, index); }
     static __device__ inline Type of_number(float x, int index) {
-        const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.0f);
-        return (uint64_t)(b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u)) << 32 | (0xffffffffu - (uint32_t)index);
+        return (uint64_t)ordered_number(x) << 32 | (0xffffffffu - (uint32_t)index);
     }
     static __device__ inline uint64_t wide(Type k) { return key_open(k) ? k : 0; }
 };
 // A float32 that holds a 16-bit one has zeros in its last 13 bits: the index (of at most 2^13 logits) takes their place.
-template <bool kFinite>
-__device__ inline uint32_t short_key(float x, int index) {
-    uint32_t o;
-    if constexpr (kFinite) {
-        const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.0f);
-        o = b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
-    } else {
-        o = ordered_bits(x);
-    }
-    return (o & ~0x1fffu) | (0x1fffu - (uint32_t)index);
-}
 struct ShortRowKey {
     typedef uint32_t Type;
-    static __device__ inline Type of(float x, int index) { return short_key<false>(x, index); }
-    static __device__ inline Type of_number(float x, int index) { return short_key<true>(x, index); }  // no NaN with a sign
+    static __device__ inline Type with(uint32_t order, int index) { return (order & ~0x1fffu) | (0x1fffu - (uint32_t)index); }
+    static __device__ inline Type of(float x, int index) { return with(ordered_bits(x), index); }
+    static __device__ inline Type of_number(float x, int index) { return with(ordered_number(x), index); }
     static __device__ inline uint64_t wide(Type k) {
-        if (k <= (kOrderedClosed | 0x1fffu)) return 0;
+        if (k <= kOrderedClosed) return 0;
         const uint32_t o = k & 0x80000000u ? k & ~0x1fffu : k | 0x1fffu;
         return (uint64_t)o << 32 | (0xffffffffu - (0x1fffu - (k & 0x1fffu)));
     }
@@ -120,6 +109,11 @@ __device__ inline Key smallest_of_lanes(Key v) {
     v = smaller_key(v, dpp_move_key<0x141>(v));
     if constexpr (kGroup == 16) v = smaller_key(v, dpp_move_key<0x140>(v));
     return v;
+}
+
+__device__ inline uint32_t key_of_lane(uint32_t v, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); }
+__device__ inline uint64_t key_of_lane(uint64_t v, int lane) {
+    return (uint64_t)key_of_lane((uint32_t)(v >> 32), lane) << 32 | key_of_lane((uint32_t)v, lane);
 }
 
 // Sums of two values, and a maximum, over a group.
@@ -160,11 +154,11 @@ __device__ inline float largest_of_group(float v, float* s_wave) {
 }
 
 // The largest number that at least k of a wave's 64 * kN keys reach, or a lower one that exactly k of them do: its bits are found
-// from the highest on. 0 if there are fewer keys that are not 0.
-template <int kN, typename Key>
+// from the highest on, down to kLast (the rest of them 0). 0 if there are fewer keys that are not 0.
+template <int kN, int kLast = 0, typename Key>
 __device__ inline Key reached_by(const Key (&v)[kN], int k) {
     Key t = 0;
-    for (int bit = 8 * (int)sizeof(Key) - 1; bit >= 0; --bit) {
+    for (int bit = 8 * (int)sizeof(Key) - 1; bit >= kLast; --bit) {
         const Key up = t | (Key)1 << bit;
         int count = 0;
 #pragma unroll
@@ -177,7 +171,6 @@ __device__ inline Key reached_by(const Key (&v)[kN], int k) {
 
 constexpr int kCandidates = 1024;    // of a workgroup's row
 constexpr int kManyCandidates = 160;  // from here on the k-th of them is searched before they are ranked
-constexpr int kWaveCandidates = 256;  // of a wave's
 
 // Keys (LDS) in order: emit(place, key) for the first `top`, 0 where there are fewer. Every key counts those before it.
 template <int kGroup, typename Key, typename Emit>
@@ -218,74 +211,6 @@ __device__ inline int keep_first(Key* s_keys, int count, int top, int lane) {
     return collect_keys<kMost / 64, kMost>(v, least, s_keys, lane);
 }
 
-// A row's alternatives by a wave. The row, which was just read, is read again. Up to 256 logits are searched for the k-th largest;
-// of longer rows only lanes have candidates whose own largest logit (mine) reaches what `top` lanes' do.
-template <typename T, int kVecs, typename Emit>
-__device__ inline void top_of_wave(const T* __restrict__ z, int vocab, const Stretch& st, float mine, float last, int top, int lane,
-                                   typename RowKey<T>::Type* s_keys, Emit emit) {
-    typedef typename RowKey<T>::Type Key;
-    constexpr int kElements = Words<T>::kElements, kFew = 4;
-    const Key closed = RowKey<T>::of(-INFINITY, 0);  // of those the largest
-    int count;
-    wave_lds_sync();  // the row before is done
-    if (vocab <= 64 * kFew) {
-        Key v[kFew];
-#pragma unroll
-        for (int i = 0; i < kFew; ++i) {
-            const int at = i * 64 + lane;
-            v[i] = at < vocab ? RowKey<T>::of(to_float(z[at]), at) : (Key)0;
-            if (v[i] <= closed) v[i] = 0;
-        }
-        const Key least = reached_by<kFew>(v, top);
-        count = collect_keys<kFew, kWaveCandidates>(v, least > 0 ? least : (Key)1, s_keys, lane);
-    } else {
-        const uint32_t most[1] = {ordered_bits(mine)};
-        uint32_t least = reached_by<1>(most, top);
-        least = max(least, kOrderedClosed + 1);
-        count = 0;
-        const auto take = [&](bool some, float x, int index) {
-            const Key key = RowKey<T>::of(x, index);
-            const bool in = some && ordered_bits(x) >= least;
-            const uint64_t all = __builtin_amdgcn_ballot_w64(in);
-            const int at = count + __builtin_amdgcn_mbcnt_hi((uint32_t)(all >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)all, 0));
-            if (in && at < kWaveCandidates) s_keys[at] = key;
-            count += __builtin_popcountll(all);
-        };
-        // NaN does not show in a lane's largest logit: such rows are looked through as a whole
-        const bool odd = __builtin_amdgcn_ballot_w64(!(mine < INFINITY)) != 0;
-        if (!odd) {
-            for (uint64_t hits = __builtin_amdgcn_ballot_w64(most[0] >= least); hits != 0; hits &= hits - 1) {
-                const int owner = __builtin_ctzll(hits);
-#pragma unroll
-                for (int i0 = 0; i0 < kVecs * kElements; i0 += 64) {
-                    const int i = i0 + lane, vec = i / kElements * 64 + owner;
-                    const bool some = i < kVecs * kElements && vec < st.vecs;
-                    const int at = some ? st.lead + vec * kElements + i % kElements : 0;
-                    take(some, to_float(z[at]), at);
-                }
-            }
-            take(st.loose >= 0, last, (int)st.loose);
-        }
-        if (odd || count > kWaveCandidates) {  // the first ones so far and 64 more at a time
-            count = 0;
-            least = kOrderedClosed + 1;
-            for (int i0 = 0; i0 < vocab; i0 += 64) {
-                const int at = min(i0 + lane, vocab - 1);
-                take(i0 + lane < vocab, to_float(z[at]), at);
-                if (count + 64 > kWaveCandidates) {
-                    wave_lds_sync();
-                    count = keep_first<kWaveCandidates>(s_keys, count, top, lane);
-                    wave_lds_sync();
-                }
-            }
-        }
-    }
-    wave_lds_sync();
-    count = keep_first<kWaveCandidates>(s_keys, count, top, lane);
-    wave_lds_sync();
-    emit_ranked<64>(s_keys, count, top, lane, [&](int place, Key k) { emit(place, RowKey<T>::wide(k)); });
-}
-
 template <int kGroup>
 struct TopScratch {
     uint64_t keys[kCandidates];
@@ -314,13 +239,13 @@ __device__ inline void top_of_workgroup(const T* __restrict__ z, int64_t length,
     __syncthreads();
     if (!special) {
         if (top <= 16) {
-            const uint32_t t = reached_by<1>(most, top);
+            const uint32_t t = reached_by<1, 16>(most, top);
             if (lane == 0) atomicMax(&s.threshold, t);
         } else if (tid < 64) {
             uint32_t v[kGroup / 64];
 #pragma unroll
             for (int i = 0; i < kGroup / 64; ++i) v[i] = s.lane[i * 64 + tid];
-            const uint32_t t = reached_by<kGroup / 64>(v, top);
+            const uint32_t t = reached_by<kGroup / 64, 16>(v, top);
             if (tid == 0) s.threshold = t;
         }
         __syncthreads();
@@ -404,17 +329,28 @@ struct RowAnswer {
 __device__ inline RowAnswer answer_of(const LogProbsArgs& a, RowSums q) { return {q.m, logf(q.s), a.inv_t}; }
 __device__ inline float entropy_of(RowSums q) { return q.s == 0.0f ? 0.0f : logf(q.s) - kLn2 * (q.w / q.s); }
 
-__device__ inline bool known_id(const LogProbsArgs& a, int64_t row, int32_t& id) {
-    id = a.ids != nullptr ? a.ids[row] : -1;
-    return id >= 0 && id < a.vocab;
+__device__ inline int32_t id_of(const LogProbsArgs& a, int64_t row) { return a.ids != nullptr ? a.ids[row] : -1; }
+
+// A row's given label and its logit, two loads of which the second waits for the first. Groups of 8 and 16 lanes ask for them
+// beside the row (307200 x 150 with the gradient 58 us, 62 at the row's end), larger ones, whose other waves go on meanwhile, at
+// its end (100000 x 1000 in bf16 65 us, beside the row 71).
+struct GivenLabel {
+    int32_t id;
+    bool known;
+    float z;
+};
+template <typename T>
+__device__ inline GivenLabel given_label(const LogProbsArgs& a, int64_t row, const T* __restrict__ z) {
+    GivenLabel g;
+    g.id = id_of(a, row);
+    g.known = g.id >= 0 && g.id < a.vocab;
+    g.z = g.known ? to_float(z[g.id]) : 0.0f;
+    return g;
 }
 
 // By one thread: a row's chosen log probability, entropy and statistics.
-template <typename T>
-__device__ inline void write_row(const LogProbsArgs& a, int64_t row, const T* __restrict__ z, RowSums q) {
-    int32_t id;
-    const bool known = known_id(a, row, id);
-    if (a.chosen != nullptr) a.chosen[row] = known ? answer_of(a, q).log_q(to_float(z[id])) : 0.0f;
+__device__ inline void write_row(const LogProbsArgs& a, int64_t row, const GivenLabel& given, RowSums q) {
+    if (a.chosen != nullptr) a.chosen[row] = given.known ? answer_of(a, q).log_q(given.z) : 0.0f;
     const float h = entropy_of(q);
     if (a.entropy != nullptr) a.entropy[row] = h;
     if (a.stats != nullptr) {
@@ -435,14 +371,17 @@ struct RowGrad {
     bool live;
     float base, rate, slope, own;
     int32_t id;
+    __device__ inline float of(float z, float e, float scale2, bool sloped) const {
+        return sloped ? e * __builtin_fmaf(slope, fmaxf((z - base) * scale2, kLeastExponent2), rate) : e * rate;
+    }
     __device__ inline float at(float z, float scale2, bool sloped) const {
-        const float u = (z - base) * scale2, e = __builtin_amdgcn_exp2f(u);
-        return sloped ? e * __builtin_fmaf(slope, fmaxf(u, kLeastExponent2), rate) : e * rate;
+        return of(z, __builtin_amdgcn_exp2f((z - base) * scale2), scale2, sloped);
     }
 };
-__device__ inline RowGrad grad_of(const LogProbsArgs& a, int64_t row, float m, float s, float h) {
+__device__ inline RowGrad grad_of(const LogProbsArgs& a, int64_t row, int32_t id, float m, float s, float h) {
     RowGrad g;
-    const bool known = known_id(a, row, g.id);
+    const bool known = id >= 0 && id < a.vocab;
+    g.id = id;
     const float gl = known ? a.grad_scale * (a.row_grad != nullptr ? a.row_grad[row] : 1.0f) : 0.0f;
     const float gh = a.entropy_scale * (a.entropy_grad != nullptr ? a.entropy_grad[row] : 1.0f);
     g.live = (gl != 0.0f || gh != 0.0f) && s != 0.0f;
@@ -460,7 +399,9 @@ __device__ inline RowGrad grad_of(const LogProbsArgs& a, int64_t row, float m, f
 template <typename T, int kGroup, int kVecs>
 struct HeldRow {
     static constexpr int kElements = Words<T>::kElements;
+    static constexpr bool kKeeps = kGroup == 8;  // what sums() computes, for a gradient of the same pass
     Words<T> x[kVecs];
+    float e[kKeeps ? kVecs * kElements : 1];
     float last;
     Stretch st;
 
@@ -494,15 +435,86 @@ struct HeldRow {
 #pragma unroll
             for (int i = 0; i < kElements; ++i) {
                 const float v = (element_of(x[u], i) - base) * scale2;
-                const float e = __builtin_amdgcn_exp2f(v);
-                r.x += e;
-                r.y = __builtin_fmaf(e, fmaxf(v, kLeastExponent2), r.y);
+                const float power = __builtin_amdgcn_exp2f(v);
+                r.x += power;
+                r.y = __builtin_fmaf(power, fmaxf(v, kLeastExponent2), r.y);
+                if constexpr (kKeeps) e[u * kElements + i] = power;
             }
             asm volatile("" : "+v"(r.x), "+v"(r.y));  // both sums go on with each vector: no e is kept for later
         }
         return r;
     }
 };
+
+// A row's alternatives by a wave, from the registers that hold the row. `mine` is the lane's largest logit: what `top` lanes' reach
+// is reached by at least `top` logits, so all others are none. (16 bits of that bound are enough: a lower one lets in a few more.)
+// The candidates come together in LDS, thinned out where they are many, and the last 64 of them are ranked lane against lane.
+// special: there are NaN or +inf, the row is read again.
+template <typename T>
+constexpr int kWaveCandidates = 64 * Words<T>::kElements + 128;  // what is left of the ones before, and all of a vector
+
+template <typename T, int kVecs, typename Emit>
+__device__ inline void top_of_wave(const T* __restrict__ z, int vocab, HeldRow<T, 64, kVecs>& x, float mine, bool special, int top,
+                                   int lane, typename RowKey<T>::Type* s_keys, Emit emit) {
+    typedef typename RowKey<T>::Type Key;
+    constexpr int kElements = Words<T>::kElements, kFew = 4;
+    int count = 0;
+    wave_lds_sync();  // the row before is done
+    const auto put = [&](bool in, uint64_t all, float v, int index) {
+        const int at = count + __builtin_amdgcn_mbcnt_hi((uint32_t)(all >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)all, 0));
+        if (in) s_keys[at] = RowKey<T>::of(v, index);
+        count += __builtin_popcountll(all);
+    };
+    const auto thin = [&] {
+        wave_lds_sync();
+        if (count <= 128) count = keep_first<128>(s_keys, count, top, lane);
+        else count = keep_first<kWaveCandidates<T>>(s_keys, count, top, lane);
+        wave_lds_sync();
+    };
+    if (vocab <= 64 * kFew) {  // few lanes hold the row: every lane takes some of it again
+        Key v[kFew];
+#pragma unroll
+        for (int i = 0; i < kFew; ++i) {
+            const int at = i * 64 + lane;
+            v[i] = at < vocab ? RowKey<T>::of(to_float(z[at]), at) : (Key)0;
+            if (v[i] <= RowKey<T>::of(-INFINITY, 0)) v[i] = 0;
+        }
+        const Key least = reached_by<kFew>(v, top);
+        count = collect_keys<kFew, kWaveCandidates<T>>(v, least > 0 ? least : (Key)1, s_keys, lane);
+    } else if (!special) {
+        const uint32_t most[1] = {ordered_bits(mine)};
+        const float bound = ordered_value(max(reached_by<1, 16>(most, top), kOrderedClosed + 1));
+#pragma unroll
+        for (int u = 0; u < kVecs; ++u) {
+            if (count > 128) thin();
+            repack(x.x[u]);
+#pragma unroll
+            for (int i = 0; i < kElements; ++i) {
+                const float v = element_of(x.x[u], i);
+                const bool in = v >= bound;
+                const uint64_t all = __builtin_amdgcn_ballot_w64(in);
+                if (all != 0) put(in, all, v, x.st.lead + (u * 64 + lane) * kElements + i);
+            }
+        }
+        const bool in = x.st.loose >= 0 && x.last >= bound;
+        if (count > 128) thin();
+        put(in, __builtin_amdgcn_ballot_w64(in), x.last, (int)x.st.loose);
+    } else {
+        for (int i0 = 0; i0 < vocab; i0 += 64) {
+            if (count > 128) thin();
+            const int at = min(i0 + lane, vocab - 1);
+            const float v = to_float(z[at]);
+            const bool in = i0 + lane < vocab && v != -INFINITY;
+            put(in, __builtin_amdgcn_ballot_w64(in), v, at);
+        }
+    }
+    if (count > 64) thin();
+    wave_lds_sync();
+    const Key key = lane < count ? s_keys[lane] : 0;
+    int place = 0;
+    for (int j = 0; j < count; ++j) place += key_of_lane(key, j) > key ? 1 : 0;
+    if (lane < count ? place < top : lane < top) emit(lane < count ? place : lane, RowKey<T>::wide(key));
+}
 
 // NaN of a word's one or two logits without their signs, which comes before every number.
 template <typename T>
@@ -517,8 +529,9 @@ __device__ inline uint32_t positive_nans(uint32_t w) {
     }
 }
 
-// One alternative after the other, from keys in the registers of 8 or 16 lanes: of the keys up to a bound, the nearest. How far
-// a key lies below it wraps around for those that do not. special: there is NaN in the wave's rows.
+// One alternative after the other, from keys in the registers of 8 or 16 lanes: of the keys up to a bound, the nearest. How far a
+// key lies below it wraps around for those that do not. Lane p keeps the one at place p (top <= kGroup). special: there is NaN in
+// the wave's rows.
 template <typename T, int kGroup, int kVecs, typename Emit>
 __device__ inline void top_of_lanes(HeldRow<T, kGroup, kVecs>& x, bool special, int top, int tid, Emit emit) {
     typedef typename RowKey<T>::Type Key;
@@ -540,17 +553,17 @@ __device__ inline void top_of_lanes(HeldRow<T, kGroup, kVecs>& x, bool special, 
             keys[u * kElements + i] = RowKey<T>::of_number(element_of(x.x[u], i), x.st.lead + vec * kElements + i);
     }
     keys[kKeys - 1] = RowKey<T>::of_number(x.last, max((int)x.st.loose, 0));
-    Key most = ~(Key)0;
+    Key most = ~(Key)0, mine = 0;
     for (int place = 0; place < top; ++place) {
         Key apart = most - keys[0];
 #pragma unroll
         for (int i = 1; i < kKeys; ++i) apart = smaller_key(apart, most - keys[i]);
         apart = smallest_of_lanes<kGroup>(apart);
-        const Key best = most - apart;
-        const uint64_t key = best <= most ? RowKey<T>::wide(best) : 0;  // none is left where it wraps
-        if (tid == 0) emit(place, key);
-        if (key != 0) most = best - 1;
+        const Key best = most - apart;  // above the bound where none is left
+        if (place == tid) mine = best <= most ? best : 0;
+        if (best <= most) most = best - 1;
     }
+    if (tid < top) emit(tid, RowKey<T>::wide(mine));
 }
 
 template <typename T, int kGroup, int kVecs>
@@ -560,7 +573,7 @@ __global__ __launch_bounds__(kGroup < 256 ? 256 : kGroup, 4) void logprobs_held_
     constexpr int kGroups = kGroup < 256 ? 256 / kGroup : 1;  // rows of a workgroup
     constexpr int kElements = Words<T>::kElements;
     __shared__ TopScratch<kGroups == 1 ? kGroup : 1> s_top[1];
-    __shared__ typename RowKey<T>::Type s_keys[kGroup == 64 ? kGroups : 1][kWaveCandidates];
+    __shared__ typename RowKey<T>::Type s_keys[kGroup == 64 ? kGroups : 1][kWaveCandidates<T>];
     __shared__ float2 s_wave2[16];
     __shared__ float s_wave[16];
     const int group = kGroups == 1 ? 0 : threadIdx.x / kGroup, tid = kGroups == 1 ? threadIdx.x : threadIdx.x % kGroup;
@@ -568,6 +581,8 @@ __global__ __launch_bounds__(kGroup < 256 ? 256 : kGroup, 4) void logprobs_held_
         const T* const z = logits + row * a.logits_stride;
         HeldRow<T, kGroup, kVecs> x;
         x.load(z, a.vocab, tid);
+        GivenLabel given;
+        if (kGroup < 64) given = given_label(a, row, z);
         const float mine = x.largest();
         RowSums q;
         q.m = largest_of_group<kGroup>(mine, s_wave);
@@ -575,17 +590,26 @@ __global__ __launch_bounds__(kGroup < 256 ? 256 : kGroup, 4) void logprobs_held_
         const float2 sums = sums_of_group<kGroup>(x.sums(base, a.scale2), s_wave2);
         q.s = sums.x;
         q.w = sums.y;
-        if (tid == 0) write_row(a, row, z, q);
+        if (tid == 0) {
+            if (kGroup >= 64) given = given_label(a, row, z);
+            write_row(a, row, given, q);
+        }
         if (grad != nullptr) {
             T* const g = grad + row * a.grad_stride;
-            const RowGrad d = grad_of(a, row, q.m, q.s, entropy_of(q));
+            const RowGrad d = grad_of(a, row, kGroup < 64 ? given.id : id_of(a, row), q.m, q.s, entropy_of(q));
             const bool sloped = d.slope != 0.0f;
 #pragma unroll
             for (int u = 0; u < kVecs; ++u) {
                 float y[kElements];
                 repack(x.x[u]);
 #pragma unroll
-                for (int i = 0; i < kElements; ++i) y[i] = d.live ? d.at(element_of(x.x[u], i), a.scale2, sloped) : 0.0f;
+                for (int i = 0; i < kElements; ++i) {
+                    const float v = element_of(x.x[u], i);
+                    if constexpr (HeldRow<T, kGroup, kVecs>::kKeeps)
+                        y[i] = d.live ? d.of(v, x.e[u * kElements + i], a.scale2, sloped) : 0.0f;
+                    else
+                        y[i] = d.live ? d.at(v, a.scale2, sloped) : 0.0f;
+                }
                 const int own = d.id - x.st.lead - (u * kGroup + tid) * kElements;
                 if (d.live && d.id >= 0 && own >= 0 && own < kElements) {
 #pragma unroll
@@ -603,7 +627,7 @@ __global__ __launch_bounds__(kGroup < 256 ? 256 : kGroup, 4) void logprobs_held_
         if constexpr (kGroup < 64)
             top_of_lanes<T, kGroup, kVecs>(x, __builtin_amdgcn_ballot_w64(q.s != q.s) != 0, a.top, tid, emit);
         else if constexpr (kGroup == 64)
-            top_of_wave<T, kVecs>(z, (int)a.vocab, x.st, q.s != q.s ? INFINITY : mine, x.last, a.top, tid, s_keys[group], emit);
+            top_of_wave<T, kVecs>(z, (int)a.vocab, x, mine, q.s != q.s, a.top, tid, s_keys[group], emit);
         else top_of_workgroup<T, kGroup, kVecs>(z, a.vocab, 0, x.st, mine, x.last, q.s != q.s, a.top, s_top[0], emit);
     }
 }
@@ -644,6 +668,7 @@ __global__ __launch_bounds__(kSliceGroup) void logprobs_join_kernel(LogProbsArgs
     const int tid = threadIdx.x;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const RowSums* const part = a.partial + row * a.slices;
+        const GivenLabel given = given_label(a, row, logits + row * a.logits_stride);
         const uint64_t* const keys = a.partial_top + row * a.slices * a.top;
         // Of each slice the key at place p, top <= slices (p + 1): those that reach the k-th largest of them, k (p + 1) >= top,
         // come from slices that have enough keys together, so no alternative is below it.
@@ -672,7 +697,7 @@ __global__ __launch_bounds__(kSliceGroup) void logprobs_join_kernel(LogProbsArgs
         sums = sums_of_group<kSliceGroup>(sums, s_wave2);
         q.s = sums.x;
         q.w = sums.y;
-        if (tid == 0) write_row(a, row, logits + row * a.logits_stride, q);
+        if (tid == 0) write_row(a, row, given, q);
         if (a.top == 0) continue;
         const RowAnswer r = answer_of(a, q);
         if (tid < 64) {
@@ -716,7 +741,7 @@ __global__ __launch_bounds__(256) void logprobs_grad_kernel(LogProbsArgs a, cons
         const int64_t row = b / a.slices, from = b % a.slices * a.slice, to = min(from + a.slice, a.vocab);
         const T* const z = logits + row * a.logits_stride + from;
         T* const g = grad + row * a.grad_stride + from;
-        const RowGrad d = grad_of(a, row, a.stats[3 * row], a.stats[3 * row + 1], a.stats[3 * row + 2]);
+        const RowGrad d = grad_of(a, row, id_of(a, row), a.stats[3 * row], a.stats[3 * row + 1], a.stats[3 * row + 2]);
         const bool sloped = d.slope != 0.0f;
         const Stretch st = stretch_of<T>(z, to - from, tid);
         for (int v = tid; v < st.vecs; v += kGroup * kAhead) {
