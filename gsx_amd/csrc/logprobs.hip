@@ -214,14 +214,15 @@ __device__ inline int keep_first(Key* s_keys, int count, int top, int lane) {
 template <int kGroup>
 struct TopScratch {
     uint64_t keys[kCandidates];
-    uint32_t lane[kGroup];
+    uint32_t most[kGroup];
     uint32_t threshold;
     int count, counts[2];
 };
 
-// A row's (or slice's) alternatives by a workgroup. `mine` is the thread's largest logit: the k-th largest of a wave's, or of all
-// where k is larger than 16, is reached by at least k logits, so only threads whose own reach it have candidates. Their logits are
-// read again, by their waves. special: there are NaN or +inf.
+// A row's (or slice's) alternatives by a workgroup. `mine` is the thread's largest logit: what k of them reach is reached by at least k
+// logits, so only threads whose own reach it have candidates. Their logits are read again, by their waves. For up to 16 alternatives
+// the largest of four threads stand for them, which every wave searches for itself; for more one wave searches all. special: there
+// are NaN or +inf.
 template <typename T, int kGroup, int kVecs, typename Emit>
 __device__ inline void top_of_workgroup(const T* __restrict__ z, int64_t length, int64_t from, const Stretch& st, float mine,
                                         float last, bool special, int top, TopScratch<kGroup>& s, Emit emit) {
@@ -230,39 +231,57 @@ __device__ inline void top_of_workgroup(const T* __restrict__ z, int64_t length,
     __syncthreads();  // the row before is done
     if (tid == 0) {
         s.count = 0;
-        s.threshold = 0;
         s.counts[0] = 0;
         s.counts[1] = 0;
     }
-    const uint32_t most[1] = {ordered_bits(mine)};
-    if (top > 16) s.lane[tid] = most[0];
+    const uint32_t most = ordered_bits(mine);
+    const bool few = top <= kGroup / 16 && top <= 16;
+    if (few) {
+        uint32_t quad = max(most, dpp_move_key<0xb1>(most));
+        quad = max(quad, dpp_move_key<0x4e>(quad));
+        if (lane % 4 == 0) s.most[tid / 4] = quad;
+    } else {
+        s.most[tid] = most;
+    }
     __syncthreads();
     if (!special) {
-        if (top <= 16) {
-            const uint32_t t = reached_by<1, 16>(most, top);
-            if (lane == 0) atomicMax(&s.threshold, t);
-        } else if (tid < 64) {
-            uint32_t v[kGroup / 64];
+        uint32_t threshold;
+        if (few) {
+            uint32_t v[kGroup / 256];
 #pragma unroll
-            for (int i = 0; i < kGroup / 64; ++i) v[i] = s.lane[i * 64 + tid];
-            const uint32_t t = reached_by<kGroup / 64, 16>(v, top);
-            if (tid == 0) s.threshold = t;
+            for (int i = 0; i < kGroup / 256; ++i) v[i] = s.most[i * 64 + lane];
+            threshold = reached_by<kGroup / 256, 16>(v, top);
+        } else {
+            if (tid < 64) {
+                uint32_t v[kGroup / 64];
+#pragma unroll
+                for (int i = 0; i < kGroup / 64; ++i) v[i] = s.most[i * 64 + tid];
+                const uint32_t t = reached_by<kGroup / 64, 16>(v, top);
+                if (tid == 0) s.threshold = t;
+            }
+            __syncthreads();
+            threshold = s.threshold;
         }
-        __syncthreads();
-        const uint32_t least = max(s.threshold, kOrderedClosed + 1);  // closed logits are no alternatives
+        const uint32_t least = max(threshold, kOrderedClosed + 1);  // closed logits are no alternatives
         const auto take = [&](float x, int64_t index) {
             if (ordered_bits(x) < least) return;
             const int at = atomicAdd(&s.count, 1);
             if (at < kCandidates) s.keys[at] = key_of(x, from + index);
         };
-        for (uint64_t hits = __builtin_amdgcn_ballot_w64(most[0] >= least); hits != 0; hits &= hits - 1) {
+        for (uint64_t hits = __builtin_amdgcn_ballot_w64(most >= least); hits != 0; hits &= hits - 1) {
             const int owner = (tid & ~63) + __builtin_ctzll(hits);
-            for (int i = lane; i < kVecs * kElements; i += 64) {
-                const int vec = i / kElements * kGroup + owner;
-                if (vec >= st.vecs) continue;
-                const int64_t at = st.lead + (int64_t)vec * kElements + i % kElements;
-                take(to_float(z[at]), at);
+            constexpr int kSteps = (kVecs * kElements + 63) / 64;
+            float x[kSteps];
+            int64_t at[kSteps];
+#pragma unroll
+            for (int u = 0; u < kSteps; ++u) {
+                const int i = u * 64 + lane, vec = i / kElements * kGroup + owner;
+                const bool some = i < kVecs * kElements && vec < st.vecs;
+                at[u] = some ? st.lead + (int64_t)vec * kElements + i % kElements : -1;
+                x[u] = some ? to_float(z[at[u]]) : -INFINITY;  // which is no alternative
             }
+#pragma unroll
+            for (int u = 0; u < kSteps; ++u) take(x[u], at[u]);
         }
         if (st.loose >= 0) take(last, st.loose);
         __syncthreads();

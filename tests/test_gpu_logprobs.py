@@ -282,3 +282,29 @@ def test_refusals():
                  lambda: fields.log_probs_backward(z, r.row_stats, ids, up[:2])):
         with pytest.raises(GsxHipError):
             call()
+
+
+@pytest.mark.parametrize("kind", list(DTYPES))
+@pytest.mark.parametrize("vocab,top", [(3, 3), (150, 3), (250, 8), (300, 5), (500, 5), (150, 20), (900, 7), (1500, 64), (5000, 9)])
+def test_nan_of_either_sign_comes_first(kind, vocab, top):
+    """In the order of their indices, the first and the last logit among them, before +inf; equal numbers and zeros of either sign
+    follow by their indices."""
+    from gsx_amd import fields
+    bits = {"f32": torch.int32, "bf16": torch.int16, "f16": torch.int16}[kind]
+    minus = {"f32": -(2**31) + 0x7FC00000, "bf16": -(2**15) + 0x7FC0, "f16": -(2**15) + 0x7E00}[kind]
+    z = torch.zeros(6, vocab, device="cuda", dtype=DTYPES[kind])
+    z[:, 1::2] = -0.0
+    z.view(bits)[0, 0] = minus
+    z[1, vocab - 1] = float("nan")
+    z.view(bits)[2, vocab - 1] = minus
+    z[2, 0] = float("nan")
+    z[2, 1] = float("inf")
+    z.view(bits)[3, 1] = minus
+    z[3, 0] = float("inf")
+    z[4] = -float("inf")
+    z.view(bits)[4, vocab // 2] = minus
+    r = fields.log_probs(z, None, top)
+    ids = r.top_ids.cpu().numpy()
+    for i, row in enumerate(z.float().cpu().numpy()):
+        assert np.array_equal(ids[i], plain.order(row, top)), i
+    assert r.entropy[:5].isnan().all() and r.entropy[5].isfinite()
