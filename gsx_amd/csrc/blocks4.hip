@@ -24,8 +24,8 @@ namespace gsx_amd {
 constexpr int kQuant4Threads = 256;
 constexpr int kQuant4Unroll = 4;
 
-// Four lanes per block, eight values a lane, kQuant4Unroll stretches of a row's 64 blocks' worth a group of lanes: the loads are
-// issued together.
+// Four lanes per block, eight values a lane, kQuant4Unroll blocks one after the other: their loads are issued together. Bound by
+// memory: 8192 x 8192 in bf16 26 to 32 us in a loop (5.3 to 6.5 TB/s).
 template <typename T>
 __global__ __launch_bounds__(kQuant4Threads) void quantize4_kernel(const T* __restrict__ src, int64_t src_stride, int64_t rows,
                                                                    int64_t cols, int64_t blocks, uint8_t* __restrict__ values,
@@ -57,31 +57,69 @@ __global__ __launch_bounds__(kQuant4Threads) void quantize4_kernel(const T* __re
     }
 }
 
-// Eight values a thread.
+// 16 bytes of the result a thread and store, so that a wave's stores follow one another without a gap, kExpand4Unroll of them 256
+// threads apart. They pass the caches by. Bound by memory: 8192 x 8192 to float32 44 us
+// (7 TB/s), 66 with 32 bytes a thread in two stores through them.
+constexpr int kExpand4Unroll = 4;
 template <typename O>
 __global__ __launch_bounds__(kQuant4Threads) void expand4_kernel(const uint8_t* __restrict__ values, int64_t values_stride,
                                                                  const uint8_t* __restrict__ exponents,
                                                                  int64_t exponents_stride, int64_t rows, int64_t cols,
                                                                  O* __restrict__ out, int64_t out_stride) {
-    const int64_t octets = ceil_div(cols, 8), total = rows * octets;
-    for (int64_t i = (int64_t)blockIdx.x * kQuant4Threads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kQuant4Threads) {
-        const int64_t r = i / octets, at = i % octets * 8;
-        const uint32_t q = *reinterpret_cast<const uint32_t*>(values + r * values_stride + at / 2);
-        const float scale = block4_scale(exponents[r * exponents_stride + at / kBlock4]);
-        const v2f a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 1);
-        const v2f c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.0f, 3);
-        const float x[8] = {a[0] * scale, a[1] * scale, b[0] * scale, b[1] * scale,
-                            c[0] * scale, c[1] * scale, d[0] * scale, d[1] * scale};
-        O* const to = out + r * out_stride + at;
-        if (at + 8 <= cols) {
-            Octet<O> y;
+    constexpr int kEach = 16 / (int)sizeof(O);
+    struct __attribute__((packed, aligned(sizeof(O)))) Loose {
+        v4i v;
+    };
+    struct Piece {
+        O v[kEach];
+    };
+    const int64_t pieces = ceil_div(cols, kEach), total = rows * pieces;
+    const int64_t whole = kQuant4Threads / pieces, rest = kQuant4Threads % pieces;  // 256 pieces on
+    for (int64_t b = blockIdx.x; b * (kQuant4Threads * kExpand4Unroll) < total; b += gridDim.x) {
+        const int64_t i = b * (kQuant4Threads * kExpand4Unroll) + threadIdx.x;
+        int64_t r = total <= UINT32_MAX ? (int64_t)((uint32_t)i / (uint32_t)pieces) : i / pieces, piece = i - r * pieces;
+        const auto on = [&] {
+            r += whole;
+            piece += rest;
+            if (piece >= pieces) {
+                piece -= pieces;
+                ++r;
+            }
+        };
+        int64_t row[kExpand4Unroll], at[kExpand4Unroll];
+        uint32_t q[kExpand4Unroll], e[kExpand4Unroll];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) y.v[j] = from_float<O>(x[j]);
-            *reinterpret_cast<Octet<O>*>(to) = y;
-        } else {
+        for (int u = 0; u < kExpand4Unroll; ++u) {
+            row[u] = r;
+            at[u] = piece * kEach;
+            q[u] = e[u] = 0;
+            if (r < rows) {
+                const uint8_t* const from = values + r * values_stride + at[u] / 2;
+                if constexpr (kEach == 8) q[u] = *reinterpret_cast<const uint32_t*>(from);
+                else q[u] = *reinterpret_cast<const uint16_t*>(from);
+                e[u] = exponents[r * exponents_stride + at[u] / kBlock4];
+            }
+            on();
+        }
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (at + j < cols) to[j] = from_float<O>(x[j]);
+        for (int u = 0; u < kExpand4Unroll; ++u) {
+            if (row[u] >= rows) break;
+            const float scale = block4_scale(e[u]);
+            const v2f x[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[u], 1.0f, 0),
+                              __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[u], 1.0f, 1),
+                              __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[u], 1.0f, 2),
+                              __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q[u], 1.0f, 3)};
+            Piece y;
+#pragma unroll
+            for (int j = 0; j < kEach; ++j) y.v[j] = from_float<O>(x[j / 2][j % 2] * scale);
+            O* const to = out + row[u] * out_stride + at[u];
+            if (at[u] + kEach <= cols) {
+                __builtin_nontemporal_store(__builtin_bit_cast(v4i, y), &reinterpret_cast<Loose*>(to)->v);
+            } else {
+#pragma unroll
+                for (int j = 0; j < kEach; ++j)
+                    if (at[u] + j < cols) to[j] = y.v[j];
+            }
         }
     }
 }
@@ -97,6 +135,11 @@ __global__ __launch_bounds__(kQuant4Threads) void expand4_kernel(const uint8_t* 
 // The matrix instructions take b as their first operand: a lane then holds four consecutive columns of one row of c. Which
 // row of b a lane brings for instruction j is chosen so that it has 16 bytes of columns together and that the four lanes of a row
 // store 64 bytes in a piece: 32 columns by a pair of instructions in 16-bit types, 16 by one in float32.
+//
+// 8192^3 to bf16: 285 to 300 us by the card, 3.7 to 3.85 PFLOP/s, 471 before the loads of the next step were in flight beside the
+// instructions, exponents came two steps at a time and rows left in pieces of 64 bytes. The matrix units are busy for 41% of it, at a
+// clock that falls under this load: four rows of tiles read ahead instead of two, a higher priority for the instructions or 4 waves
+// of 128 x 128 made it no faster (0, 0 and -7%).
 constexpr int kStep4 = 8;  // blocks
 
 template <typename O>
@@ -111,7 +154,7 @@ __device__ inline int swizzle4_b(int row) {
 }
 
 // store_row4 for 16-bit rows that begin between two words: a lane's pieces go one column on, the column behind comes from the next
-// lane of the row. Whole words cost half as much as the same vectors two bytes off: 29681 x 2261 x 22 80 us that way, 64 this way.
+// lane of the row. Whole words cost less than the same vectors two bytes off: 29681 x 2261 x 22 64 us, the latter way 80.
 template <int TN, typename S>
 __device__ inline void store_shifted4(S* __restrict__ row, int64_t col, int64_t n, int lane, const v4f (&x)[TN]) {
     struct __attribute__((packed, aligned(4))) Piece {
@@ -138,7 +181,8 @@ __device__ inline void store_shifted4(S* __restrict__ row, int64_t col, int64_t 
     }
 }
 
-// A lane's 4 TN columns of a row of n, the first of them at `col` + 4 kPair<O> (lane / 16).
+// A lane's 4 TN columns of a row of n, the first of them at `col` + 4 kPair<O> (lane / 16). A store has 64 bytes of 16 rows; 128 of 8
+// rows, after an exchange between lanes, were slower (29681 x 2304 x 256 to bf16 53 us, 71), stores past the caches too (58).
 template <typename O, int TN, typename S>
 __device__ inline void store_row4(S* __restrict__ row, int64_t col, int64_t n, int lane, const v4f (&x)[TN]) {
     constexpr int kP = kPair<O>;
@@ -487,7 +531,7 @@ gsx_hip_status gsx_hip_blocks4_expand(const uint8_t* values, int64_t values_stri
         return fields_fail(GSX_HIP_ERROR_INVALID_ARGUMENT, "4-bit blocks: values must be non-null and aligned to their elements");
     return with_type(out_type, [&](auto t) {
         using O = decltype(t);
-        hipLaunchKernelGGL((expand4_kernel<O>), dim3(blocks_grid(ceil_div(rows * ceil_div(cols, 8), kQuant4Threads))),
+        hipLaunchKernelGGL((expand4_kernel<O>), dim3(blocks_grid(ceil_div(rows * ceil_div(cols, 16 / (int64_t)sizeof(O)), kQuant4Threads * kExpand4Unroll))),
                            dim3(kQuant4Threads), 0, stream, values, values_stride, exponents, exponents_stride, rows, cols,
                            static_cast<O*>(out), out_stride);
         return fields_launched("4-bit blocks expand launch");

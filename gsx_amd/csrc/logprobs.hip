@@ -585,6 +585,10 @@ __device__ inline void top_of_lanes(HeldRow<T, kGroup, kVecs>& x, bool special, 
     if (tid < top) emit(tid, RowKey<T>::wide(mine));
 }
 
+// A row is read once: its largest logit, both sums, the gradient and the alternatives come from registers. Long rows are bound by
+// memory (4096 x 65537 in bf16: sums 111 us, 4.8 TB/s; with the gradient 224, 4.8; 8 alternatives more 24 and 17). Short ones are
+// bound by the vector units, never idle (307200 x 150 in bf16: sums 25 us, 3.6 TB/s; with the gradient 55, 3.3; three alternatives
+// more 18 and 12). Four waves a SIMD at least: 128 registers, of which a row has 64.
 template <typename T, int kGroup, int kVecs>
 __global__ __launch_bounds__(kGroup < 256 ? 256 : kGroup, 4) void logprobs_held_kernel(LogProbsArgs a,
                                                                                        const T* __restrict__ logits,
@@ -719,11 +723,18 @@ __global__ __launch_bounds__(kSliceGroup) void logprobs_join_kernel(LogProbsArgs
         if (tid == 0) write_row(a, row, given, q);
         if (a.top == 0) continue;
         const RowAnswer r = answer_of(a, q);
-        if (tid < 64) {
+        if (tid < 64) {  // by the logits' bits alone
+            const int k = (a.top + p) / (p + 1);
             uint64_t v[kSliceGroup / 64];
 #pragma unroll
             for (int i = 0; i < kSliceGroup / 64; ++i) v[i] = s_keys[i * 64 + tid];
-            const uint64_t t = reached_by<kSliceGroup / 64>(v, (a.top + p) / (p + 1));
+            uint64_t t;
+            if (a.slices <= 64) {
+                const uint64_t few[1] = {v[0]};
+                t = reached_by<1, 32>(few, k);
+            } else {
+                t = reached_by<kSliceGroup / 64, 32>(v, k);
+            }
             if (tid == 0) s_least = t;
         }
         __syncthreads();
@@ -749,7 +760,8 @@ __global__ __launch_bounds__(kSliceGroup) void logprobs_join_kernel(LogProbsArgs
     }
 }
 
-// The gradient from a forward's statistics: kGroup threads take a stretch of a row.
+// The gradient from a forward's statistics: kGroup threads take a stretch of a row. Bound by memory (4096 x 65537 in bf16 184 us, 5.8
+// TB/s; 307200 x 150 54, 3.4: rows of 300 bytes begin and end between vectors).
 template <typename T, int kGroup>
 __global__ __launch_bounds__(256) void logprobs_grad_kernel(LogProbsArgs a, const T* __restrict__ logits,
                                                             T* __restrict__ grad) {
@@ -793,8 +805,10 @@ using namespace gsx_amd;
 
 namespace {
 
-// How a forward goes: by groups that hold whole rows (group > 0), or by slices. The smallest group that holds a row in 16 vectors
-// a thread; above 16 KB only where there are rows enough for the GPU's 256 CUs.
+// How a forward goes: by groups that hold whole rows (group > 0), or by slices. The smallest group that holds a row in 4 vectors a
+// thread, or 16 above 16 KB, where there are rows enough for the GPU's 256 CUs (4096 x 65537 with 8 alternatives 135 us, in slices
+// 189 to 213; one row of 131072 15 us in slices). More than 8 alternatives of a short row are a wave's: one after the other they
+// would cost what the row does, each.
 struct LogProbsPlan {
     int group, vecs;
     int64_t slice, slices;

@@ -1,10 +1,12 @@
-"""Label fields over libgsx_hip.so: rows looked up by code, a head in 8-bit blocks, distillation from a teacher's top logits.
+"""Label fields over libgsx_hip.so: rows looked up by code, a head in 8-bit or 4-bit blocks, distillation from a teacher's top
+logits, log probabilities of given labels.
 
 A field gives each Gaussian or pixel the id of a code. `lookup` fetches the codes' rows, `linear` multiplies them with a head
 whose weights are `Blocks` (8-bit values with a power-of-two scale for each block of 128), `distill` compares the logits with
 a teacher's top logits and gives their gradient, and `linear_backward` and `lookup_backward` carry it to the weights and the
-table, in float32 for `gsx_amd.backend.Adam`. Definitions, rounding and the treatment of masked ids and rows are those of
-include/gsx_hip.h.
+table, in float32 for `gsx_amd.backend.Adam` or `AdamW`. `log_probs` compares the logits with given labels instead, or gives the
+likeliest ones; a head that only answers can be `Blocks4` (4-bit values, a scale for each block of 32). Definitions, rounding and
+the treatment of masked ids and rows are those of include/gsx_hip.h.
 
 Tensors are two-dimensional with contiguous rows of any stride (ids and weights one-dimensional and contiguous), all on the
 current device. Results and workspaces that a call allocates belong to the stream it runs on: `stream`, or torch's current one.
