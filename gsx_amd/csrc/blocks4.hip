@@ -77,7 +77,7 @@ __global__ __launch_bounds__(kQuant4Threads) void expand4_kernel(const uint8_t* 
     const int64_t whole = kQuant4Threads / pieces, rest = kQuant4Threads % pieces;  // 256 pieces on
     for (int64_t b = blockIdx.x; b * (kQuant4Threads * kExpand4Unroll) < total; b += gridDim.x) {
         const int64_t i = b * (kQuant4Threads * kExpand4Unroll) + threadIdx.x;
-        int64_t r = total <= UINT32_MAX ? (int64_t)((uint32_t)i / (uint32_t)pieces) : i / pieces, piece = i - r * pieces;
+        int64_t r = total <= INT32_MAX ? (int64_t)((uint32_t)i / (uint32_t)pieces) : i / pieces, piece = i - r * pieces;
         const auto on = [&] {
             r += whole;
             piece += rest;

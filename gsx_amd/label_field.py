@@ -55,7 +55,9 @@ class LabelField:
         self._blocks4 = None  # laid out when the first answer after a step is asked for
 
     def head_blocks4(self) -> fields.Blocks4:
-        """The head in 4-bit blocks."""
+        """The head in 4-bit blocks. A graph that is captured lays them out at each replay, from the head as it is then."""
+        if torch.cuda.is_current_stream_capturing():
+            return fields.quantize4(self.head)
         if self._blocks4 is None:
             self._blocks4 = fields.quantize4(self.head)
         return self._blocks4
@@ -140,6 +142,8 @@ def main(argv=None) -> float:
     p.add_argument("--decay", type=float, default=0.0, help="AdamW's weight decay")
     p.add_argument("--answers", type=int, default=0, help="print so many likeliest labels of one Gaussian, by a 4-bit head")
     a = p.parse_args(argv)
+    if not 0 <= a.answers <= min(64, a.labels):
+        p.error("--answers takes 0 to 64 labels, no more than there are")
     mean3d = torch.from_numpy(scenes.config0(n=a.gaussians).scene.mean3d).cuda()
     codes = cell_codes(mean3d, a.cells)
     ids, logits = teacher_of(mean3d, a.labels, a.top)
