@@ -87,19 +87,19 @@ __device__ inline float max_of_group(float v, float* s_wave) {
     return v;
 }
 
-// 16 bytes of logits at any element's address.
-template <typename T>
+// A vector of logits, 16 bytes unless said otherwise, at any element's address.
+template <typename T, int kWords = 4>
 struct Words {
-    static constexpr int kElements = 16 / (int)sizeof(T);
-    uint32_t w[4];
+    static constexpr int kElements = 4 * kWords / (int)sizeof(T);
+    uint32_t w[kWords];
 };
-template <typename T>
+template <typename T, int kWords>
 struct __attribute__((packed, aligned(sizeof(T)))) LooseWords {
-    uint32_t w[4];
+    uint32_t w[kWords];
 };
 
-template <typename T>
-__device__ inline float element_of(const Words<T>& x, int i) {
+template <typename T, int kWords>
+__device__ inline float element_of(const Words<T, kWords>& x, int i) {
     if constexpr (sizeof(T) == 4) {
         return __builtin_bit_cast(float, x.w[i]);
     } else if constexpr (__is_same(T, __bf16)) {
@@ -111,10 +111,10 @@ __device__ inline float element_of(const Words<T>& x, int i) {
 
 // Keeps the compiler from holding what it unpacked or computed from x beside x itself until the next use: registers are what
 // bounds the rows that fit.
-template <typename T>
-__device__ inline void repack(Words<T>& x) {
+template <typename T, int kWords>
+__device__ inline void repack(Words<T, kWords>& x) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(x.w[i]));
+    for (int i = 0; i < kWords; ++i) asm volatile("" : "+v"(x.w[i]));
 }
 
 template <typename T>
@@ -124,34 +124,40 @@ __device__ inline uint32_t element_bits(float x) {
 }
 
 // Vector v of a row, -inf in all its elements where there is none (v >= vecs).
-template <typename T>
-__device__ inline Words<T> load_words(const T* __restrict__ z, int v, int vecs) {
+template <typename T, int kWords = 4>
+__device__ inline Words<T, kWords> load_words(const T* __restrict__ z, int v, int vecs) {
     constexpr uint32_t kNone = sizeof(T) == 4 ? 0xff800000u : __is_same(T, __bf16) ? 0xff80ff80u : 0xfc00fc00u;
-    Words<T> x = {{kNone, kNone, kNone, kNone}};
-    if (v < vecs) {
-        const LooseWords<T> y = *reinterpret_cast<const LooseWords<T>*>(z + (uint32_t)v * Words<T>::kElements);
+    Words<T, kWords> x;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x.w[i] = y.w[i];
+    for (int i = 0; i < kWords; ++i) x.w[i] = kNone;
+    if (v < vecs) {
+        const LooseWords<T, kWords> y =
+            *reinterpret_cast<const LooseWords<T, kWords>*>(z + (uint32_t)v * Words<T, kWords>::kElements);
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) x.w[i] = y.w[i];
     }
     return x;
 }
 
-template <typename T>
-__device__ inline void store_words(T* __restrict__ g, int v, int vecs, const float (&y)[Words<T>::kElements]) {
+// Past the caches, unless a line is written by several stores (kPast false; 8 lanes of 8 bytes, 307200 x 150: 45 us, past them 72).
+template <typename T, int kWords = 4, bool kPast = true>
+__device__ inline void store_words(T* __restrict__ g, int v, int vecs, const float (&y)[Words<T, kWords>::kElements]) {
     if (v >= vecs) return;
-    LooseWords<T> x;
+    LooseWords<T, kWords> x;
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x.w[i] = element_bits<T>(y[i]);
+        for (int i = 0; i < kWords; ++i) x.w[i] = element_bits<T>(y[i]);
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x.w[i] = element_bits<T>(y[2 * i]) | element_bits<T>(y[2 * i + 1]) << 16;
+        for (int i = 0; i < kWords; ++i) x.w[i] = element_bits<T>(y[2 * i]) | element_bits<T>(y[2 * i + 1]) << 16;
     }
-    typedef uint32_t Loose2 __attribute__((ext_vector_type(4), aligned(2)));
-    typedef uint32_t Loose4 __attribute__((ext_vector_type(4), aligned(4)));
-    const Loose4 y4 = {x.w[0], x.w[1], x.w[2], x.w[3]};
-    if constexpr (sizeof(T) == 4) __builtin_nontemporal_store(y4, reinterpret_cast<Loose4*>(g + (uint32_t)v * Words<T>::kElements));
-    else __builtin_nontemporal_store(y4, reinterpret_cast<Loose2*>(g + (uint32_t)v * Words<T>::kElements));
+    typedef uint32_t Loose2 __attribute__((ext_vector_type(kWords), aligned(2)));
+    typedef uint32_t Loose4 __attribute__((ext_vector_type(kWords), aligned(4)));
+    const Loose4 all = __builtin_bit_cast(Loose4, x);
+    T* const to = g + (uint32_t)v * Words<T, kWords>::kElements;
+    if constexpr (!kPast) *reinterpret_cast<Loose2*>(to) = all;
+    else if constexpr (sizeof(T) == 4) __builtin_nontemporal_store(all, reinterpret_cast<Loose4*>(to));
+    else __builtin_nontemporal_store(all, reinterpret_cast<Loose2*>(to));
 }
 
 // A stretch of `length` logits at z: `lead` elements up to the first address that is a multiple of 16, then `vecs` vectors, then

@@ -30,6 +30,7 @@ struct LogProbsArgs {
     float* chosen;   // may be null
     float* entropy;  // may be null
     float* stats;    // may be null: m, s, H
+    bool backward;   // stats are read, only the gradient is written
     int32_t top;
     int32_t* top_ids;
     float* top_logs;
@@ -351,7 +352,7 @@ __device__ inline float entropy_of(RowSums q) { return q.s == 0.0f ? 0.0f : logf
 __device__ inline int32_t id_of(const LogProbsArgs& a, int64_t row) { return a.ids != nullptr ? a.ids[row] : -1; }
 
 // A row's given label and its logit, two loads of which the second waits for the first. Groups of 8 and 16 lanes ask for them
-// beside the row (307200 x 150 with the gradient 58 us, 62 at the row's end), larger ones, whose other waves go on meanwhile, at
+// beside the row (307200 x 150 with the gradient 58 us, 62 at the row's end, before vectors of four), larger ones, whose other waves go on meanwhile, at
 // its end (100000 x 1000 in bf16 65 us, beside the row 71).
 struct GivenLabel {
     int32_t id;
@@ -413,13 +414,15 @@ __device__ inline RowGrad grad_of(const LogProbsArgs& a, int64_t row, int32_t id
     return g;
 }
 
-// Rows that fit the registers of a group: kGroup threads hold kVecs times 16 bytes each. Groups of 8 lanes take their vectors from the
-// row's start on, at whatever address that is, and at most one logit a thread behind the last vector.
+// Rows that fit the registers of a group: kGroup threads hold kVecs vectors of 16 bytes each. Groups of 8 lanes take vectors of four
+// logits, so that fewer lanes stand idle at the row's end (307200 x 150 with the gradient and three alternatives: in bf16 62 us, 70
+// with eight logits; in float32 88, 106 by groups of 16), from the row's start on, at whatever address that is, and at most one
+// logit a thread behind the last vector.
 template <typename T, int kGroup, int kVecs>
 struct HeldRow {
-    static constexpr int kElements = Words<T>::kElements;
+    static constexpr int kWords = kGroup == 8 ? (int)sizeof(T) : 4, kElements = Words<T, kWords>::kElements;
     static constexpr bool kKeeps = kGroup == 8;  // what sums() computes, for a gradient of the same pass
-    Words<T> x[kVecs];
+    Words<T, kWords> x[kVecs];
     float e[kKeeps ? kVecs * kElements : 1];
     float last;
     Stretch st;
@@ -433,7 +436,8 @@ struct HeldRow {
             st = stretch_of<T>(z, length, tid);
         }
 #pragma unroll
-        for (int u = 0; u < kVecs; ++u) x[u] = load_words<T>(z + st.lead + u * kGroup * kElements, tid, st.vecs - u * kGroup);
+        for (int u = 0; u < kVecs; ++u)
+            x[u] = load_words<T, kWords>(z + st.lead + u * kGroup * kElements, tid, st.vecs - u * kGroup);
         last = st.loose >= 0 ? to_float(z[st.loose]) : -INFINITY;
     }
     __device__ inline float largest() const {
@@ -554,13 +558,14 @@ __device__ inline uint32_t positive_nans(uint32_t w) {
 template <typename T, int kGroup, int kVecs, typename Emit>
 __device__ inline void top_of_lanes(HeldRow<T, kGroup, kVecs>& x, bool special, int top, int tid, Emit emit) {
     typedef typename RowKey<T>::Type Key;
-    constexpr int kElements = Words<T>::kElements, kKeys = kVecs * kElements + 1;
+    constexpr int kWords = HeldRow<T, kGroup, kVecs>::kWords, kElements = HeldRow<T, kGroup, kVecs>::kElements;
+    constexpr int kKeys = kVecs * kElements + 1;
     Key keys[kKeys];
     if (special) {
 #pragma unroll
         for (int u = 0; u < kVecs; ++u)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x.x[u].w[i] = positive_nans<T>(x.x[u].w[i]);
+            for (int i = 0; i < kWords; ++i) x.x[u].w[i] = positive_nans<T>(x.x[u].w[i]);
         if (x.last != x.last) x.last = __builtin_nanf("");
     }
 #pragma unroll
@@ -587,14 +592,14 @@ __device__ inline void top_of_lanes(HeldRow<T, kGroup, kVecs>& x, bool special, 
 
 // A row is read once: its largest logit, both sums, the gradient and the alternatives come from registers. Long rows are bound by
 // memory (4096 x 65537 in bf16: sums 111 us, 4.8 TB/s; with the gradient 224, 4.8; 8 alternatives more 24 and 17). Short ones are
-// bound by the vector units, never idle (307200 x 150 in bf16: sums 25 us, 3.6 TB/s; with the gradient 55, 3.3; three alternatives
-// more 18 and 12). Four waves a SIMD at least: 128 registers, of which a row has 64.
+// bound by the vector units, never idle (307200 x 150 in bf16: sums 27 us, 3.4 TB/s; with the gradient 45, 4.1; three alternatives
+// more 14 and 17). Four waves a SIMD at least: 128 registers, of which a row has 64.
 template <typename T, int kGroup, int kVecs>
 __global__ __launch_bounds__(kGroup < 256 ? 256 : kGroup, 4) void logprobs_held_kernel(LogProbsArgs a,
                                                                                        const T* __restrict__ logits,
                                                                                        T* __restrict__ grad) {
     constexpr int kGroups = kGroup < 256 ? 256 / kGroup : 1;  // rows of a workgroup
-    constexpr int kElements = Words<T>::kElements;
+    constexpr int kWords = HeldRow<T, kGroup, kVecs>::kWords, kElements = HeldRow<T, kGroup, kVecs>::kElements;
     __shared__ TopScratch<kGroups == 1 ? kGroup : 1> s_top[1];
     __shared__ typename RowKey<T>::Type s_keys[kGroup == 64 ? kGroups : 1][kWaveCandidates<T>];
     __shared__ float2 s_wave2[16];
@@ -608,18 +613,27 @@ __global__ __launch_bounds__(kGroup < 256 ? 256 : kGroup, 4) void logprobs_held_
         if (kGroup < 64) given = given_label(a, row, z);
         const float mine = x.largest();
         RowSums q;
-        q.m = largest_of_group<kGroup>(mine, s_wave);
-        const float base = q.m == -INFINITY ? 0.0f : q.m;
-        const float2 sums = sums_of_group<kGroup>(x.sums(base, a.scale2), s_wave2);
-        q.s = sums.x;
-        q.w = sums.y;
-        if (tid == 0) {
+        float h;
+        if (kGroup == 8 && a.backward) {
+            q.m = a.stats[3 * row];
+            q.s = a.stats[3 * row + 1];
+            h = a.stats[3 * row + 2];
+            x.sums(q.m == -INFINITY ? 0.0f : q.m, a.scale2);
+        } else {
+            q.m = largest_of_group<kGroup>(mine, s_wave);
+            const float base = q.m == -INFINITY ? 0.0f : q.m;
+            const float2 sums = sums_of_group<kGroup>(x.sums(base, a.scale2), s_wave2);
+            q.s = sums.x;
+            q.w = sums.y;
+            h = entropy_of(q);
+        }
+        if (tid == 0 && !(kGroup == 8 && a.backward)) {
             if (kGroup >= 64) given = given_label(a, row, z);
             write_row(a, row, given, q);
         }
         if (grad != nullptr) {
             T* const g = grad + row * a.grad_stride;
-            const RowGrad d = grad_of(a, row, kGroup < 64 ? given.id : id_of(a, row), q.m, q.s, entropy_of(q));
+            const RowGrad d = grad_of(a, row, kGroup < 64 ? given.id : id_of(a, row), q.m, q.s, h);
             const bool sloped = d.slope != 0.0f;
 #pragma unroll
             for (int u = 0; u < kVecs; ++u) {
@@ -638,7 +652,7 @@ __global__ __launch_bounds__(kGroup < 256 ? 256 : kGroup, 4) void logprobs_held_
 #pragma unroll
                     for (int i = 0; i < kElements; ++i) y[i] += i == own ? d.own : 0.0f;
                 }
-                store_words<T>(g + x.st.lead + u * kGroup * kElements, tid, x.st.vecs - u * kGroup, y);
+                store_words<T, kWords, kWords == 4>(g + x.st.lead + u * kGroup * kElements, tid, x.st.vecs - u * kGroup, y);
             }
             if (x.st.loose >= 0)
                 g[x.st.loose] =
@@ -761,7 +775,7 @@ __global__ __launch_bounds__(kSliceGroup) void logprobs_join_kernel(LogProbsArgs
 }
 
 // The gradient from a forward's statistics: kGroup threads take a stretch of a row. Bound by memory (4096 x 65537 in bf16 184 us, 5.8
-// TB/s; 307200 x 150 54, 3.4: rows of 300 bytes begin and end between vectors).
+// TB/s; 307200 x 150 in float32 74, 5.0).
 template <typename T, int kGroup>
 __global__ __launch_bounds__(256) void logprobs_grad_kernel(LogProbsArgs a, const T* __restrict__ logits,
                                                             T* __restrict__ grad) {
@@ -817,8 +831,12 @@ struct LogProbsPlan {
 LogProbsPlan logprobs_plan(int64_t rows, int64_t vocab, int64_t bytes, int32_t top) {
     LogProbsPlan p = {};
     const int64_t vecs = vocab * bytes / 16;
-    if (vecs <= 8 * 4 && top <= 8) p.group = 8;
-    else if (vecs <= 16 * 4 && top <= 8) p.group = 16;
+    if (vocab / 4 <= 8 * (bytes == 4 ? 6 : 8) && top <= 8) {
+        p.group = 8;
+        p.vecs = vocab >= 4 ? (int)ceil_div(vocab / 4, 8) : 1;
+        return p;
+    }
+    if (vecs <= 16 * 4 && top <= 8) p.group = 16;
     else if (vecs <= 64 * 4) p.group = 64;
     else if (vecs <= 256 * 4 || (vecs <= 256 * 16 && rows >= 192)) p.group = 256;
     else if (vecs <= 512 * 16 && rows >= 192) p.group = 512;
@@ -847,8 +865,31 @@ gsx_hip_status launch_held(const LogProbsArgs& a, const T* logits, T* grad, hipS
     return fields_launched("log probabilities launch");
 }
 
+// Rows of 8 lanes.
+template <typename T>
+gsx_hip_status launch_short(int vecs, const LogProbsArgs& a, const T* logits, T* grad, hipStream_t stream) {
+    if (vecs <= 1) return launch_held<T, 8, 1>(a, logits, grad, stream);
+    if (vecs <= 2) return launch_held<T, 8, 2>(a, logits, grad, stream);
+    if (vecs <= 3) return launch_held<T, 8, 3>(a, logits, grad, stream);
+    if (vecs <= 4) return launch_held<T, 8, 4>(a, logits, grad, stream);
+    if (vecs <= 5) return launch_held<T, 8, 5>(a, logits, grad, stream);
+    if constexpr (sizeof(T) == 4) {
+        return launch_held<T, 8, 6>(a, logits, grad, stream);
+    } else {
+        if (vecs <= 6) return launch_held<T, 8, 6>(a, logits, grad, stream);
+        return launch_held<T, 8, 8>(a, logits, grad, stream);
+    }
+}
+
 template <typename T>
 gsx_hip_status launch_grad(LogProbsArgs a, const T* logits, T* grad, hipStream_t stream) {
+    // rows that 8 lanes hold, in 16 bits, as in the forward: 307200 x 150 43 us, through the other kernel 54; in float32 102 and 74
+    const LogProbsPlan p = logprobs_plan(a.rows, a.vocab, sizeof(T), 0);
+    if (sizeof(T) == 2 && p.group == 8) {
+        a.backward = true;
+        a.top = 0;
+        return launch_short<T>(p.vecs, a, logits, grad, stream);
+    }
     const int64_t vecs = a.vocab * (int64_t)sizeof(T) / 16;
     const auto go = [&](auto kernel, int groups) {
         hipLaunchKernelGGL(kernel, logprobs_grid(ceil_div(a.rows * a.slices, groups)), dim3(256), 0, stream, a, logits, grad);
@@ -868,14 +909,10 @@ gsx_hip_status launch_grad(LogProbsArgs a, const T* logits, T* grad, hipStream_t
 template <typename T>
 gsx_hip_status launch_logprobs(const LogProbsPlan& p, LogProbsArgs a, const T* logits, T* grad, void* temp,
                                hipStream_t stream) {
-    if (p.group == 8) {
-        if (p.vecs <= 1) return launch_held<T, 8, 1>(a, logits, grad, stream);
-        if (p.vecs <= 2) return launch_held<T, 8, 2>(a, logits, grad, stream);
-        if (p.vecs <= 3) return launch_held<T, 8, 3>(a, logits, grad, stream);
-        return launch_held<T, 8, 4>(a, logits, grad, stream);
-    }
+    if (p.group == 8) return launch_short<T>(p.vecs, a, logits, grad, stream);
     if (p.group == 16) {
-        if (p.vecs <= 3) return launch_held<T, 16, 3>(a, logits, grad, stream);
+        if constexpr (sizeof(T) == 2)
+            if (p.vecs <= 3) return launch_held<T, 16, 3>(a, logits, grad, stream);
         return launch_held<T, 16, 4>(a, logits, grad, stream);
     }
     if (p.group == 64) {

@@ -5,10 +5,14 @@ def _ways(t, wide):
     k = 1 if wide else 2  # elements of 4 bytes
     return [
         (5, 3, 2, f"held_kernelI{t}Li8ELi1E"),
-        (33, 40 * k, 3, f"held_kernelI{t}Li8ELi2E"),
-        (300, 76 * k - 1, 8, f"held_kernelI{t}Li8ELi3E"),
-        (9, 120 * k, 8, f"held_kernelI{t}Li8ELi4E"),
-        (37, 180 * k + 1, 5, f"held_kernelI{t}Li16ELi3E"),
+        (33, 41, 3, f"held_kernelI{t}Li8ELi2E"),
+        (300, 75, 8, f"held_kernelI{t}Li8ELi3E"),
+        (33, 80, 3, f"held_kernelI{t}Li8ELi3E"),
+        (9, 120, 8, f"held_kernelI{t}Li8ELi4E"),
+        (301, 150, 3, f"held_kernelI{t}Li8ELi5E"),
+        (40, 191, 6, f"held_kernelI{t}Li8ELi6E"),
+        *([(9, 256, 8, f"held_kernelI{t}Li8ELi8E"), (30, 201, 8, f"held_kernelI{t}Li8ELi8E"),
+           (37, 361, 5, f"held_kernelI{t}Li16ELi3E")] if not wide else [(37, 201, 5, f"held_kernelI{t}Li16ELi4E")]),
         (21, 250 * k + 1, 5, f"held_kernelI{t}Li16ELi4E"),
         (6, 150, 9, f"held_kernelI{t}Li64ELi1E"),
         (6, 150, 64, f"held_kernelI{t}Li64ELi1E"),
