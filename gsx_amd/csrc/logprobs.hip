@@ -553,7 +553,8 @@ __device__ inline uint32_t positive_nans(uint32_t w) {
 }
 
 // One alternative after the other, from keys in the registers of 8 or 16 lanes: of the keys up to a bound, the nearest. How far a
-// key lies below it wraps around for those that do not. Lane p keeps the one at place p (top <= kGroup). special: there is NaN in
+// key lies below it wraps around for those that do not. Lane p keeps the one at place p until there
+// is one for each lane. special: there is NaN in
 // the wave's rows.
 template <typename T, int kGroup, int kVecs, typename Emit>
 __device__ inline void top_of_lanes(HeldRow<T, kGroup, kVecs>& x, bool special, int top, int tid, Emit emit) {
@@ -578,16 +579,19 @@ __device__ inline void top_of_lanes(HeldRow<T, kGroup, kVecs>& x, bool special, 
     }
     keys[kKeys - 1] = RowKey<T>::of_number(x.last, max((int)x.st.loose, 0));
     Key most = ~(Key)0, mine = 0;
-    for (int place = 0; place < top; ++place) {
-        Key apart = most - keys[0];
+    for (int first = 0; first < top; first += kGroup) {
+        const int count = min(top - first, kGroup);
+        for (int place = 0; place < count; ++place) {
+            Key apart = most - keys[0];
 #pragma unroll
-        for (int i = 1; i < kKeys; ++i) apart = smaller_key(apart, most - keys[i]);
-        apart = smallest_of_lanes<kGroup>(apart);
-        const Key best = most - apart;  // above the bound where none is left
-        if (place == tid) mine = best <= most ? best : 0;
-        if (best <= most) most = best - 1;
+            for (int i = 1; i < kKeys; ++i) apart = smaller_key(apart, most - keys[i]);
+            apart = smallest_of_lanes<kGroup>(apart);
+            const Key best = most - apart;  // above the bound where none is left
+            if (place == tid) mine = best <= most ? best : 0;
+            if (best <= most) most = best - 1;
+        }
+        if (tid < count) emit(first + tid, RowKey<T>::wide(mine));
     }
-    if (tid < top) emit(tid, RowKey<T>::wide(mine));
 }
 
 // A row is read once: its largest logit, both sums, the gradient and the alternatives come from registers. Long rows are bound by
@@ -821,8 +825,9 @@ namespace {
 
 // How a forward goes: by groups that hold whole rows (group > 0), or by slices. The smallest group that holds a row in 4 vectors a
 // thread, or 16 above 16 KB, where there are rows enough for the GPU's 256 CUs (4096 x 65537 with 8 alternatives 135 us, in slices
-// 189 to 213; one row of 131072 15 us in slices). More than 8 alternatives of a short row are a wave's: one after the other they
-// would cost what the row does, each.
+// 189 to 213; one row of 131072 15 us in slices). Rows of 8 lanes whatever the alternatives are (307200 x 150 in bf16 with 20 of them
+// 95 us, a wave a row 290; 100000 x 180 in float32 with 64, the worst, 206), of 16 lanes up to 16 of them, in float32 8: one after the
+// other each costs as much as the row's sums.
 struct LogProbsPlan {
     int group, vecs;
     int64_t slice, slices;
@@ -831,12 +836,12 @@ struct LogProbsPlan {
 LogProbsPlan logprobs_plan(int64_t rows, int64_t vocab, int64_t bytes, int32_t top) {
     LogProbsPlan p = {};
     const int64_t vecs = vocab * bytes / 16;
-    if (vocab / 4 <= 8 * (bytes == 4 ? 6 : 8) && top <= 8) {
+    if (vocab / 4 <= 8 * (bytes == 4 ? 6 : 8)) {
         p.group = 8;
         p.vecs = vocab >= 4 ? (int)ceil_div(vocab / 4, 8) : 1;
         return p;
     }
-    if (vecs <= 16 * 4 && top <= 8) p.group = 16;
+    if (vecs <= 16 * 4 && top <= (bytes == 4 ? 8 : 16)) p.group = 16;
     else if (vecs <= 64 * 4) p.group = 64;
     else if (vecs <= 256 * 4 || (vecs <= 256 * 16 && rows >= 192)) p.group = 256;
     else if (vecs <= 512 * 16 && rows >= 192) p.group = 512;

@@ -14,8 +14,11 @@ def _ways(t, wide):
         *([(9, 256, 8, f"held_kernelI{t}Li8ELi8E"), (30, 201, 8, f"held_kernelI{t}Li8ELi8E"),
            (37, 361, 5, f"held_kernelI{t}Li16ELi3E")] if not wide else [(37, 201, 5, f"held_kernelI{t}Li16ELi4E")]),
         (21, 250 * k + 1, 5, f"held_kernelI{t}Li16ELi4E"),
-        (6, 150, 9, f"held_kernelI{t}Li64ELi1E"),
-        (6, 150, 64, f"held_kernelI{t}Li64ELi1E"),
+        (6, 150, 9, f"held_kernelI{t}Li8ELi5E"),
+        (70, 150, 64, f"held_kernelI{t}Li8ELi5E"),
+        (11, 14, 14, f"held_kernelI{t}Li8ELi1E"),
+        (37, 251 * k, 16 // (3 - k), f"held_kernelI{t}Li16ELi4E"),
+        (6, 255 * k, 17, f"held_kernelI{t}Li64ELi1E"),
         (70, 250 * k, 40, f"held_kernelI{t}Li64ELi1E"),
         (5, 1021 * k, 64, f"held_kernelI{t}Li64ELi4E"),
         (66, 700 * k, 5, f"held_kernelI{t}Li64ELi4E"),
