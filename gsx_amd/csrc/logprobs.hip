@@ -826,8 +826,9 @@ namespace {
 // How a forward goes: by groups that hold whole rows (group > 0), or by slices. The smallest group that holds a row in 4 vectors a
 // thread, or 16 above 16 KB, where there are rows enough for the GPU's 256 CUs (4096 x 65537 with 8 alternatives 135 us, in slices
 // 189 to 213; one row of 131072 15 us in slices). Rows of 8 lanes whatever the alternatives are (307200 x 150 in bf16 with 20 of them
-// 95 us, a wave a row 290; 100000 x 180 in float32 with 64, the worst, 206), of 16 lanes up to 16 of them, in float32 8: one after the
-// other each costs as much as the row's sums.
+// 95 us, a wave a row 290; 100000 x 180 in float32 with 64, the worst, 206), of 16 lanes up to 16 of them, or 8
+// in float32 and of more than 64 vectors (100000 x 1000 with 5 of them 87 us, 16 130; a wave a row 105 and 118; 252716 x 565 with 3 104
+// and 238).
 struct LogProbsPlan {
     int group, vecs;
     int64_t slice, slices;
@@ -841,7 +842,7 @@ LogProbsPlan logprobs_plan(int64_t rows, int64_t vocab, int64_t bytes, int32_t t
         p.vecs = vocab >= 4 ? (int)ceil_div(vocab / 4, 8) : 1;
         return p;
     }
-    if (vecs <= 16 * 4 && top <= (bytes == 4 ? 8 : 16)) p.group = 16;
+    if (vecs <= 16 * (bytes == 4 ? 6 : 8) && top <= (bytes == 4 || vecs > 64 ? 8 : 16)) p.group = 16;
     else if (vecs <= 64 * 4) p.group = 64;
     else if (vecs <= 256 * 4 || (vecs <= 256 * 16 && rows >= 192)) p.group = 256;
     else if (vecs <= 512 * 16 && rows >= 192) p.group = 512;
@@ -901,7 +902,7 @@ gsx_hip_status launch_grad(LogProbsArgs a, const T* logits, T* grad, hipStream_t
     };
     a.slice = a.vocab;
     a.slices = 1;
-    if (vecs <= 64) go(logprobs_grad_kernel<T, 16>, 16);
+    if (vecs <= 96) go(logprobs_grad_kernel<T, 16>, 16);  // 252716 x 565 in bf16 140 us, by 64 lanes 196; 100000 x 1000 78 and 74
     else if (vecs <= 256) go(logprobs_grad_kernel<T, 64>, 4);
     else {
         a.slice = 16384 / (int64_t)sizeof(T);
@@ -918,7 +919,14 @@ gsx_hip_status launch_logprobs(const LogProbsPlan& p, LogProbsArgs a, const T* l
     if (p.group == 16) {
         if constexpr (sizeof(T) == 2)
             if (p.vecs <= 3) return launch_held<T, 16, 3>(a, logits, grad, stream);
-        return launch_held<T, 16, 4>(a, logits, grad, stream);
+        if (p.vecs <= 4) return launch_held<T, 16, 4>(a, logits, grad, stream);
+        if (p.vecs <= 5) return launch_held<T, 16, 5>(a, logits, grad, stream);
+        if constexpr (sizeof(T) == 4) {
+            return launch_held<T, 16, 6>(a, logits, grad, stream);
+        } else {
+            if (p.vecs <= 6) return launch_held<T, 16, 6>(a, logits, grad, stream);
+            return launch_held<T, 16, 8>(a, logits, grad, stream);
+        }
     }
     if (p.group == 64) {
         if (p.vecs <= 1) return launch_held<T, 64, 1>(a, logits, grad, stream);

@@ -18,6 +18,9 @@ def _ways(t, wide):
         (70, 150, 64, f"held_kernelI{t}Li8ELi5E"),
         (11, 14, 14, f"held_kernelI{t}Li8ELi1E"),
         (37, 251 * k, 16 // (3 - k), f"held_kernelI{t}Li16ELi4E"),
+        (37, 300 * k, 3, f"held_kernelI{t}Li16ELi5E"),
+        (19, 383 * k, 8, f"held_kernelI{t}Li16ELi6E"),
+        *([(19, 1024, 8, f"held_kernelI{t}Li16ELi8E"), (40, 801, 5, f"held_kernelI{t}Li16ELi8E")] if not wide else []),
         (6, 255 * k, 17, f"held_kernelI{t}Li64ELi1E"),
         (70, 250 * k, 40, f"held_kernelI{t}Li64ELi1E"),
         (5, 1021 * k, 64, f"held_kernelI{t}Li64ELi4E"),
