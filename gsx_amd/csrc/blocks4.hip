@@ -531,7 +531,8 @@ gsx_hip_status gsx_hip_blocks4_expand(const uint8_t* values, int64_t values_stri
         return fields_fail(GSX_HIP_ERROR_INVALID_ARGUMENT, "4-bit blocks: values must be non-null and aligned to their elements");
     return with_type(out_type, [&](auto t) {
         using O = decltype(t);
-        hipLaunchKernelGGL((expand4_kernel<O>), dim3(blocks_grid(ceil_div(rows * ceil_div(cols, 16 / (int64_t)sizeof(O)), kQuant4Threads * kExpand4Unroll))),
+        const int64_t pieces = rows * ceil_div(cols, 16 / (int64_t)sizeof(O));
+        hipLaunchKernelGGL((expand4_kernel<O>), dim3(blocks_grid(ceil_div(pieces, kQuant4Threads * kExpand4Unroll))),
                            dim3(kQuant4Threads), 0, stream, values, values_stride, exponents, exponents_stride, rows, cols,
                            static_cast<O*>(out), out_stride);
         return fields_launched("4-bit blocks expand launch");

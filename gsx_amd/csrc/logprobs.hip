@@ -220,10 +220,11 @@ struct TopScratch {
     int count, counts[2];
 };
 
-// A row's (or slice's) alternatives by a workgroup. `mine` is the thread's largest logit: what k of them reach is reached by at least k
-// logits, so only threads whose own reach it have candidates. Their logits are read again, by their waves. For up to 16 alternatives
-// the largest of four threads stand for them, which every wave searches for itself; for more one wave searches all. special: there
-// are NaN or +inf.
+// A row's (or slice's) alternatives by a workgroup. `mine` is the thread's largest logit: what k of them reach is reached by at least
+// k logits, so only threads whose own reach it have candidates. Their logits are read again, by their waves. For up to 16
+// alternatives the largest of four threads stand for them, which every wave searches for itself (4096 x 65537 with 8: 135 us; each
+// wave's own k-th largest, the highest of which bounds the row, let in more: 194); for more one wave searches all. special: there are
+// NaN or +inf.
 template <typename T, int kGroup, int kVecs, typename Emit>
 __device__ inline void top_of_workgroup(const T* __restrict__ z, int64_t length, int64_t from, const Stretch& st, float mine,
                                         float last, bool special, int top, TopScratch<kGroup>& s, Emit emit) {
@@ -352,8 +353,8 @@ __device__ inline float entropy_of(RowSums q) { return q.s == 0.0f ? 0.0f : logf
 __device__ inline int32_t id_of(const LogProbsArgs& a, int64_t row) { return a.ids != nullptr ? a.ids[row] : -1; }
 
 // A row's given label and its logit, two loads of which the second waits for the first. Groups of 8 and 16 lanes ask for them
-// beside the row (307200 x 150 with the gradient 58 us, 62 at the row's end, before vectors of four), larger ones, whose other waves go on meanwhile, at
-// its end (100000 x 1000 in bf16 65 us, beside the row 71).
+// beside the row (307200 x 150 with the gradient 58 us, 62 at the row's end, with vectors of eight logits), larger ones, whose other
+// waves go on meanwhile, at its end (100000 x 1000 in bf16 by a wave a row 65 us, beside the row 71).
 struct GivenLabel {
     int32_t id;
     bool known;
@@ -823,12 +824,12 @@ using namespace gsx_amd;
 
 namespace {
 
-// How a forward goes: by groups that hold whole rows (group > 0), or by slices. The smallest group that holds a row in 4 vectors a
-// thread, or 16 above 16 KB, where there are rows enough for the GPU's 256 CUs (4096 x 65537 with 8 alternatives 135 us, in slices
-// 189 to 213; one row of 131072 15 us in slices). Rows of 8 lanes whatever the alternatives are (307200 x 150 in bf16 with 20 of them
-// 95 us, a wave a row 290; 100000 x 180 in float32 with 64, the worst, 206), of 16 lanes up to 16 of them, or 8
-// in float32 and of more than 64 vectors (100000 x 1000 with 5 of them 87 us, 16 130; a wave a row 105 and 118; 252716 x 565 with 3 104
-// and 238).
+// How a forward goes: by groups that hold whole rows (group > 0), or by slices. The smallest group that holds a row, in vectors as
+// many as its kernels have, or 16 above 16 KB, where there are rows enough for the GPU's 256 CUs (4096 x 65537 with 8 alternatives
+// 135 us, in slices 189 to 213; one row of 131072 15 us in slices). Rows of 8 lanes whatever the alternatives are (307200 x 150 in
+// bf16 with 20 of them 88 us, a wave a row 290; 100000 x 180 in float32 with 64, the worst, 197); of 16 lanes up to 16 of them, or 8
+// in float32 and of more than 64 vectors (100000 x 1000 with 5 of them 87 us, with 16 130; a wave a row 105 and 118; 252716 x 565
+// with 3 104 and 238).
 struct LogProbsPlan {
     int group, vecs;
     int64_t slice, slices;
