@@ -211,6 +211,10 @@ __device__ inline int keep_first(Key* s_keys, int count, int top, int lane) {
     const Key least = reached_by<kMost / 64>(v, top);
     return collect_keys<kMost / 64, kMost>(v, least, s_keys, lane);
 }
+template <typename Key>
+__device__ inline int keep_first_of_any(Key* s_keys, int count, int top, int lane) {
+    return count <= 256 ? keep_first<256>(s_keys, count, top, lane) : keep_first<kCandidates>(s_keys, count, top, lane);
+}
 
 template <int kGroup>
 struct TopScratch {
@@ -270,15 +274,21 @@ __device__ inline void top_of_workgroup(const T* __restrict__ z, int64_t length,
             const int at = atomicAdd(&s.count, 1);
             if (at < kCandidates) s.keys[at] = key_of(x, from + index);
         };
-        for (uint64_t hits = __builtin_amdgcn_ballot_w64(most >= least); hits != 0; hits &= hits - 1) {
-            const int owner = (tid & ~63) + __builtin_ctzll(hits);
-            constexpr int kSteps = (kVecs * kElements + 63) / 64;
+        // the logits of as many owners together as a wave has lanes for
+        constexpr int kHeld = kVecs * kElements, kOwners = kHeld >= 64 ? 1 : 64 / kHeld, kSteps = kHeld >= 64 ? kHeld / 64 : 1;
+        for (uint64_t hits = __builtin_amdgcn_ballot_w64(most >= least); hits != 0;) {
+            int owner = -1;
+#pragma unroll
+            for (int o = 0; o < kOwners; ++o) {
+                if (hits != 0 && lane / (64 / kOwners) == o) owner = (tid & ~63) + __builtin_ctzll(hits);
+                hits &= hits - 1;
+            }
             float x[kSteps];
             int64_t at[kSteps];
 #pragma unroll
             for (int u = 0; u < kSteps; ++u) {
-                const int i = u * 64 + lane, vec = i / kElements * kGroup + owner;
-                const bool some = i < kVecs * kElements && vec < st.vecs;
+                const int i = u * 64 + lane % (64 / kOwners), vec = i / kElements * kGroup + owner;
+                const bool some = owner >= 0 && vec < st.vecs;
                 at[u] = some ? st.lead + (int64_t)vec * kElements + i % kElements : -1;
                 x[u] = some ? to_float(z[at[u]]) : -INFINITY;  // which is no alternative
             }
@@ -291,7 +301,7 @@ __device__ inline void top_of_workgroup(const T* __restrict__ z, int64_t length,
         if (count <= kCandidates) {
             if (count > kManyCandidates) {
                 if (tid < 64) {
-                    const int left = keep_first<kCandidates>(s.keys, count, top, lane);
+                    const int left = keep_first_of_any(s.keys, count, top, lane);
                     if (tid == 0) s.count = left;
                 }
                 __syncthreads();
@@ -767,7 +777,7 @@ __global__ __launch_bounds__(kSliceGroup) void logprobs_join_kernel(LogProbsArgs
             __syncthreads();  // everybody has read it
             if (count + kSliceGroup > kCandidates || (i0 + kSliceGroup >= all && count > kManyCandidates)) {
                 if (tid < 64) {
-                    const int left = keep_first<kCandidates>(s_keys, count, a.top, tid);
+                    const int left = keep_first_of_any(s_keys, count, a.top, tid);
                     if (tid == 0) s_count = left;
                 }
                 __syncthreads();
