@@ -300,6 +300,7 @@ __device__ inline void top_of_workgroup(const T* __restrict__ z, int64_t length,
         int count = s.count;
         if (count <= kCandidates) {
             if (count > kManyCandidates) {
+                __syncthreads();  // everybody has read s.count
                 if (tid < 64) {
                     const int left = keep_first_of_any(s.keys, count, top, lane);
                     if (tid == 0) s.count = left;

@@ -308,3 +308,26 @@ def test_nan_of_either_sign_comes_first(kind, vocab, top):
     for i, row in enumerate(z.float().cpu().numpy()):
         assert np.array_equal(ids[i], plain.order(row, top)), i
     assert r.entropy[:5].isnan().all() and r.entropy[5].isfinite()
+
+
+@pytest.mark.parametrize("kind", list(DTYPES))
+@pytest.mark.parametrize("rows,vocab,stretch", [(200, 3001, 3001), (200, 5003, 5003), (200, 16_001, 16_001), (200, 29_999, 29_999),
+                                                (200, 61_001, 61_001), (3, 40_003, 4096), (300, 150_001, 16_384)])
+@pytest.mark.parametrize("top", [5, 64])
+def test_hundreds_of_logits_at_the_last_alternatives_value(kind, rows, vocab, stretch, top):
+    """A workgroup thins its candidates out where there are more than 160 of them, up to 1024: `stretch` logits are what one has at
+    least. A row in 8 has 150 equal ones in each such stretch, the others 170 to 1000, and three larger ones."""
+    print(f"[case] {rows} x {vocab} {kind}, {top} alternatives", flush=True)
+    from gsx_amd import fields
+    rng = np.random.default_rng(vocab + top)
+    x = (rng.standard_normal((8, vocab)) - 6).astype(np.float32).clip(-12, -1)
+    for i, each in enumerate((150, 170, 250, 300, 500, 700, 900, 1000)):
+        for start in range(0, vocab, stretch):
+            span = min(stretch, vocab - start)
+            x[i, start + rng.choice(span, min(each, span), replace=False)] = 0.75
+        x[i, rng.choice(vocab, 3, replace=False)] = (1.0, 2.0, 1.5)
+    want = np.stack([plain.order(x[i], top) for i in range(8)])[np.arange(rows) % 8]
+    z = _put(x, kind).repeat(-(-rows // 8), 1)[:rows]
+    got = fields.log_probs(z, top=top)
+    assert np.array_equal(got.top_ids.cpu().numpy(), want)
+    assert (got.top_log_probs.diff(dim=1) <= 0).all()
