@@ -564,10 +564,17 @@ __device__ inline uint32_t positive_nans(uint32_t w) {
     }
 }
 
+// What a NaN is then as a number, also one that is not in a vector: equal ones go by their indices.
+template <typename T>
+__device__ inline float positive_nan() {
+    Words<T, 1> x;
+    x.w[0] = sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu;
+    return element_of(x, 0);
+}
+
 // One alternative after the other, from keys in the registers of 8 or 16 lanes: of the keys up to a bound, the nearest. How far a
-// key lies below it wraps around for those that do not. Lane p keeps the one at place p until there
-// is one for each lane. special: there is NaN in
-// the wave's rows.
+// key lies below it wraps around for those that do not. Lane p keeps the one at place p until there is one for each lane. special:
+// there is NaN in the wave's rows.
 template <typename T, int kGroup, int kVecs, typename Emit>
 __device__ inline void top_of_lanes(HeldRow<T, kGroup, kVecs>& x, bool special, int top, int tid, Emit emit) {
     typedef typename RowKey<T>::Type Key;
@@ -579,7 +586,7 @@ __device__ inline void top_of_lanes(HeldRow<T, kGroup, kVecs>& x, bool special, 
         for (int u = 0; u < kVecs; ++u)
 #pragma unroll
             for (int i = 0; i < kWords; ++i) x.x[u].w[i] = positive_nans<T>(x.x[u].w[i]);
-        if (x.last != x.last) x.last = __builtin_nanf("");
+        if (x.last != x.last) x.last = positive_nan<T>();
     }
 #pragma unroll
     for (int u = 0; u < kVecs; ++u) {

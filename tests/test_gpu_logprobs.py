@@ -331,3 +331,25 @@ def test_hundreds_of_logits_at_the_last_alternatives_value(kind, rows, vocab, st
     got = fields.log_probs(z, top=top)
     assert np.array_equal(got.top_ids.cpu().numpy(), want)
     assert (got.top_log_probs.diff(dim=1) <= 0).all()
+
+
+@pytest.mark.parametrize("kind", list(DTYPES))
+@pytest.mark.parametrize("vocab,top", [(149, 3), (301, 1), (301, 8), (383, 3), (901, 5), (1023, 8), (1501, 20), (5001, 9), (40_001, 9)])
+def test_nan_keeps_its_order_in_rows_that_begin_anywhere(kind, vocab, top):
+    """Rows of an odd length begin at every place between two multiples of 16 bytes: NaN of different bits before the first whole
+    vector, in vectors and behind the last one are equal, and come by their indices."""
+    from gsx_amd import fields
+    rows, bits = 16, {"f32": torch.int32, "bf16": torch.int16, "f16": torch.int16}[kind]
+    quiet = {"f32": 0x7FC00000, "bf16": 0x7FC0, "f16": 0x7E00}[kind]
+    full = {"f32": 0x7FFFFFFF, "bf16": 0x7FFF, "f16": 0x7FFF}[kind]
+    minus = -(2**31) if kind == "f32" else -(2**15)
+    z = torch.zeros(rows, vocab, device="cuda", dtype=DTYPES[kind])
+    z[:, 2] = float("inf")
+    for i, at in enumerate(((0, 100), (0, 1, 100), (3, 100), (0, vocab - 1), (100, vocab - 1), (1, vocab // 2, vocab - 2))):
+        for j, k in enumerate(at):
+            z.view(bits)[i::6, k] = (quiet, full, minus + quiet, minus + full)[(i + j) % 4]
+    r = fields.log_probs(z, None, top)
+    ids = r.top_ids.cpu().numpy()
+    for i, row in enumerate(z.float().cpu().numpy()):
+        assert np.array_equal(ids[i], plain.order(row, top)), (i, ids[i])
+    assert r.entropy.isnan().all()
