@@ -165,20 +165,33 @@ def _padded(stride: int, to: int, rows: int) -> int:
     return stride if rows > 1 else -(-stride // to) * to  # a single row's stride is never used
 
 
-def quantize(x: torch.Tensor, transpose: bool = False, stream=None) -> Blocks:
-    """x, or its transpose, in 8-bit blocks along the result's rows."""
+def _blocks_room(kind, block: int, size: int, rows: int, cols: int, out, device):
+    """`out`, or new blocks, as `kind` of a matrix [rows, cols] whose rows have room for whole blocks of `size` bytes and whole
+    words of exponents, and its arguments."""
+    n = -(-cols // block)
+    wide, words = n * size, -(-n // 4) * 4
+    if out is None:
+        values = torch.empty((rows, wide), dtype=torch.uint8, device=device)
+        exponents = torch.empty((rows, words), dtype=torch.uint8, device=device)
+        return kind(values, exponents, cols), (values.data_ptr(), wide, exponents.data_ptr(), words)
+    if not isinstance(out, kind) or out.rows != rows or out.cols != cols or out.values.shape[1] < wide or \
+            out.exponents.shape[1] < words:
+        raise GsxHipError(f"out must be {kind.__name__} of a matrix [{rows}, {cols}] with {wide} values and {words} exponents a row")
+    return out, out.arguments()
+
+
+def quantize(x: torch.Tensor, transpose: bool = False, stream=None, out: Blocks | None = None) -> Blocks:
+    """x, or its transpose, in 8-bit blocks along the result's rows. `out`: blocks of a matrix of the same sizes, as an earlier call
+    gave them, that are written instead of new ones; what reads their memory, a replayed graph too, finds x there from then on."""
     lib = _lib.load(require_device=False)
     base, stride = _rows(x, "x")
     code = _type(x.dtype)
     rows, cols = (x.shape[1], x.shape[0]) if transpose else x.shape
 
     def call(handle):
-        n = -(-cols // BLOCK)
-        values = torch.empty((rows, n * BLOCK), dtype=torch.uint8, device=x.device)
-        exponents = torch.empty((rows, -(-n // 4) * 4), dtype=torch.uint8, device=x.device)
-        check(lib.gsx_hip_blocks_quantize(base, code, x.shape[0], x.shape[1], stride, int(transpose), values.data_ptr(),
-                                          n * BLOCK, exponents.data_ptr(), -(-n // 4) * 4, handle), "quantize")
-        return Blocks(values, exponents, cols)
+        result, args = _blocks_room(Blocks, BLOCK, BLOCK, rows, cols, out, x.device)
+        check(lib.gsx_hip_blocks_quantize(base, code, x.shape[0], x.shape[1], stride, int(transpose), *args, handle), "quantize")
+        return result
 
     return _run(stream, call)
 

@@ -26,7 +26,10 @@ from .backend import Adam, AdamW
 class LabelField:
     """codes: rows of the table; features: columns of table and head; labels: rows of the head. Rows travel in `dtype`, table,
     head, their gradients and Adam's moments are float32. moments: None for Adam, 32 or 8 for AdamW with moments of as many bits and
-    with weight_decay."""
+    with weight_decay.
+
+    A step writes table, head and the head's blocks where they are: one with AdamW may be captured into a graph, whose replays go on
+    from whatever step was the last, and calls on other streams are the caller's to order against it."""
 
     def __init__(self, codes: int, features: int, labels: int, temperature: float = 2.0, learning_rate: float = 1e-2,
                  dtype=torch.bfloat16, seed: int = 0, moments: int | None = None, weight_decay: float = 0.0):
@@ -46,12 +49,13 @@ class LabelField:
         else:
             self.optimizer = AdamW([dict(parameters=[self.table, self.head], gradients=[self.table_grad, self.head_grad],
                                          learning_rate=learning_rate, weight_decay=weight_decay)], bits=moments)
+        self.blocks = self.blocks_t = None
         self._lay_out()
 
     def _lay_out(self):
         """The head's blocks, along features for the product and along labels for its gradient."""
-        self.blocks = fields.quantize(self.head)
-        self.blocks_t = fields.quantize(self.head, transpose=True)
+        self.blocks = fields.quantize(self.head, out=self.blocks)
+        self.blocks_t = fields.quantize(self.head, transpose=True, out=self.blocks_t)
         self._blocks4 = None  # laid out when the first answer after a step is asked for
 
     def head_blocks4(self) -> fields.Blocks4:
@@ -75,12 +79,18 @@ class LabelField:
         rows = fields.lookup(self.table, codes, self.scale, out_dtype=self.dtype)
         return fields.log_probs(fields.linear(rows, self.head_blocks4(), out_dtype=torch.float32), labels, top)
 
+    def _check_step(self, codes):
+        if codes.numel() == 0:
+            raise GsxHipError("a step needs at least one row")
+        if isinstance(self.optimizer, Adam) and torch.cuda.is_current_stream_capturing():
+            raise GsxHipError("a step that is captured needs AdamW (moments of 32 or 8 bits): Adam counts its steps on the host, "
+                              "replays would all be the same one")
+
     def step_labels(self, codes: torch.Tensor, labels: torch.Tensor, row_weight: torch.Tensor | None = None,
                     entropy_weight: float = 0.0) -> torch.Tensor:
         """One training step against given int32 labels (a row whose label lies outside of the field's has none); the rows'
         losses, -log p(label) times the row's weight less entropy_weight times the entropy. The gradient is that of their mean."""
-        if codes.numel() == 0:
-            raise GsxHipError("a step needs at least one row")
+        self._check_step(codes)
         rows = fields.lookup(self.table, codes, self.scale, out_dtype=self.dtype)
         logits = fields.linear(rows, self.blocks)
         mean = 1.0 / codes.numel()
@@ -92,8 +102,7 @@ class LabelField:
     def step(self, codes: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor,
              row_weight: torch.Tensor | None = None) -> torch.Tensor:
         """One training step; the rows' losses. The gradient is that of their mean."""
-        if codes.numel() == 0:
-            raise GsxHipError("a step needs at least one row")
+        self._check_step(codes)
         rows = fields.lookup(self.table, codes, self.scale, out_dtype=self.dtype)
         logits = fields.linear(rows, self.blocks)
         loss, _, grad = fields.distill(logits, teacher_ids, teacher_logits, self.temperature, row_weight,
