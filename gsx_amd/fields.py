@@ -232,20 +232,17 @@ class Blocks4:
         return _run(stream, call)
 
 
-def quantize4(x: torch.Tensor, stream=None) -> Blocks4:
-    """x in microscaled 4-bit blocks along its rows."""
+def quantize4(x: torch.Tensor, stream=None, out: Blocks4 | None = None) -> Blocks4:
+    """x in microscaled 4-bit blocks along its rows, written into `out` as `quantize` does if that is given."""
     lib = _lib.load(require_device=False)
     base, stride = _rows(x, "x")
     code = _type(x.dtype)
     rows, cols = x.shape
 
     def call(handle):
-        n = -(-cols // BLOCK4)
-        values = torch.empty((rows, n * BLOCK4 // 2), dtype=torch.uint8, device=x.device)
-        exponents = torch.empty((rows, -(-n // 4) * 4), dtype=torch.uint8, device=x.device)
-        check(lib.gsx_hip_blocks4_quantize(base, code, rows, cols, stride, values.data_ptr(), n * BLOCK4 // 2,
-                                           exponents.data_ptr(), -(-n // 4) * 4, handle), "quantize4")
-        return Blocks4(values, exponents, cols)
+        result, args = _blocks_room(Blocks4, BLOCK4, BLOCK4 // 2, rows, cols, out, x.device)
+        check(lib.gsx_hip_blocks4_quantize(base, code, rows, cols, stride, *args, handle), "quantize4")
+        return result
 
     return _run(stream, call)
 

@@ -29,7 +29,8 @@ class LabelField:
     with weight_decay.
 
     A step writes table, head and the head's blocks where they are: one with AdamW may be captured into a graph, whose replays go on
-    from whatever step was the last, and calls on other streams are the caller's to order against it."""
+    from whatever step was the last, and calls on other streams are the caller's to order against it. Logits and answers may be asked
+    for on several streams at once."""
 
     def __init__(self, codes: int, features: int, labels: int, temperature: float = 2.0, learning_rate: float = 1e-2,
                  dtype=torch.bfloat16, seed: int = 0, moments: int | None = None, weight_decay: float = 0.0):
@@ -50,20 +51,31 @@ class LabelField:
             self.optimizer = AdamW([dict(parameters=[self.table, self.head], gradients=[self.table_grad, self.head_grad],
                                          learning_rate=learning_rate, weight_decay=weight_decay)], bits=moments)
         self.blocks = self.blocks_t = None
+        self._blocks4 = fields.quantize4(self.head)  # their memory: _stream4 says whether they are the head's
+        self._ready4 = torch.cuda.Event()            # after they were laid out for an answer
         self._lay_out()
 
     def _lay_out(self):
         """The head's blocks, along features for the product and along labels for its gradient."""
         self.blocks = fields.quantize(self.head, out=self.blocks)
         self.blocks_t = fields.quantize(self.head, transpose=True, out=self.blocks_t)
-        self._blocks4 = None  # laid out when the first answer after a step is asked for
+        if torch.cuda.is_current_stream_capturing():
+            fields.quantize4(self.head, out=self._blocks4)  # a replay runs nothing that could ask for it
+        else:
+            self._stream4 = None  # laid out, and on which stream, when the first answer after a step is asked for
 
     def head_blocks4(self) -> fields.Blocks4:
-        """The head in 4-bit blocks. A graph that is captured lays them out at each replay, from the head as it is then."""
+        """The head in 4-bit blocks, for calls on the current stream. A graph that is captured lays out blocks of its own at each
+        replay, from the head as it is then."""
         if torch.cuda.is_current_stream_capturing():
             return fields.quantize4(self.head)
-        if self._blocks4 is None:
-            self._blocks4 = fields.quantize4(self.head)
+        handle = fields._current_stream(self.head.device.index)
+        if self._stream4 is None:
+            fields.quantize4(self.head, out=self._blocks4)
+            self._ready4.record()
+            self._stream4 = handle
+        elif self._stream4 != handle:
+            self._ready4.wait()
         return self._blocks4
 
     def logits(self, codes: torch.Tensor) -> torch.Tensor:

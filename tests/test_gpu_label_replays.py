@@ -137,3 +137,93 @@ def test_quantize_into_blocks(rows, cols, dtype, transpose):
     out.values.fill_(7)
     out.exponents.fill_(9)
     assert (room == 7).all() and (exponents == 9).all()
+
+
+def same_answers(got, want):
+    return all(torch.equal(a, b) for a, b in zip(got[:5], want[:5]))
+
+
+@pytest.mark.parametrize("asked_before", [False, True])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_answers_follow_replayed_steps(bits, asked_before):
+    """Eager answers, captured ones and the head's 4-bit blocks between replays of a step and eager steps, beside an eager twin."""
+    from gsx_amd import fields
+    from gsx_amd.label_field import LabelField
+    field, twin = (LabelField(CODES, FEATURES, LABELS, moments=bits, learning_rate=0.05) for _ in range(2))
+    codes, labels, weight, _, _ = data(9)
+    if asked_before:
+        assert same_answers(field.answers(codes, 5, labels), twin.answers(codes, 5, labels))
+    graph, _ = capture(lambda: field.step_labels(codes, labels, weight))
+    asking, captured = capture(lambda: field.answers(codes, 5, labels))
+    seen = []
+    for k in range(5):
+        if k == 2:
+            field.step_labels(codes, labels, weight)
+        else:
+            graph.replay()
+        twin.step_labels(codes, labels, weight)
+        want = twin.answers(codes, 5, labels)
+        asking.replay()
+        got = field.answers(codes, 5, labels)
+        torch.cuda.synchronize()
+        assert same_answers(got, want), k
+        assert same_answers(captured, want), k
+        assert torch.equal(field.head_blocks4().float(), fields.quantize4(field.head).float())
+        seen.append(want.chosen.clone())
+    assert not torch.equal(seen[0], seen[1])
+
+
+def test_answers_on_several_streams_wait_for_the_blocks():
+    """The first answer after a step lays the head's 4-bit blocks out behind long work of its stream; answers on other streams, asked
+    for at once, read them no earlier."""
+    from gsx_amd.label_field import LabelField
+    field, twin = (LabelField(CODES, FEATURES, LABELS, moments=32, learning_rate=0.2) for _ in range(2))
+    codes, labels, weight, _, _ = data(11)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for k in range(4):
+        field.step_labels(codes, labels, weight)
+        twin.step_labels(codes, labels, weight)
+        want = twin.answers(codes, 5, labels)
+        torch.cuda.synchronize()
+        got = []
+        for at in range(3):
+            with torch.cuda.stream(streams[(at + k) % 3]):
+                if at == 0:
+                    torch.cuda._sleep(20_000_000)
+                got.append(field.answers(codes, 5, labels))
+        torch.cuda.synchronize()
+        assert all(same_answers(a, want) for a in got), k
+
+
+def test_answers_of_a_head_that_was_read_in():
+    """A head written over before the first answer is the one that answers."""
+    from gsx_amd.label_field import LabelField
+    field, other = LabelField(CODES, FEATURES, LABELS, seed=1), LabelField(CODES, FEATURES, LABELS, seed=2)
+    codes = data(13)[0]
+    field.table.copy_(other.table)
+    field.head.copy_(other.head)
+    assert same_answers(field.answers(codes, 5), other.answers(codes, 5))
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 1), (33, 70), (70, 130), (5, 1000)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_quantize4_into_blocks(rows, cols, dtype):
+    from gsx_amd import fields
+    from gsx_amd._lib import GsxHipError
+    g = torch.Generator("cuda").manual_seed(rows + cols)
+    x = torch.randn(rows, cols, device="cuda", generator=g).to(dtype)
+    want = fields.quantize4(x)
+    wide, words, blocks = want.values.shape[1], want.exponents.shape[1], -(-cols // 32)
+    room = torch.full((rows + 2, wide + 32), 7, dtype=torch.uint8, device="cuda")
+    exponents = torch.full((rows + 2, words + 8), 9, dtype=torch.uint8, device="cuda")
+    out = fields.Blocks4(room[1: rows + 1, 16: 16 + wide], exponents[1: rows + 1, 4: 4 + words], cols)
+    assert fields.quantize4(x, out=out) is out
+    assert torch.equal(out.values, want.values) and torch.equal(out.exponents[:, :blocks], want.exponents[:, :blocks])
+    assert torch.equal(out.float(), want.float())
+    out.values.fill_(7)
+    out.exponents.fill_(9)
+    assert (room == 7).all() and (exponents == 9).all()
+    for bad in (fields.Blocks4(want.values, want.exponents, cols + 1), want.values,
+                fields.Blocks4(want.values[:, : wide - 16], want.exponents, cols)):
+        with pytest.raises(GsxHipError):
+            fields.quantize4(x, out=bad)
