@@ -258,7 +258,7 @@ class Adam:
 
 class AdamW:
     """AdamW over any number of tensors in one launch, with moments in 32 bits or in 8 (include/gsx_hip.h has the formulas and
-    the format).
+    the format). `Adam` is gsx's: up to 16 float32 tensors, steps counted on the host, so that it cannot be replayed.
 
     groups: up to 16 dicts of `parameters` and `gradients` (lists of contiguous tensors of the same sizes, float32, bfloat16 or
     float16, whose memory stays in use by this optimizer) and of learning_rate, beta1, beta2, weight_decay and epsilon, which may

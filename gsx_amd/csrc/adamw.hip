@@ -193,8 +193,9 @@ __device__ inline uint2 hold_second(const float (&v)[8], float& scale) {
 
 // A workgroup takes 2048 elements of one tensor, found in the table, so that tensors of any sizes fill the GPU in one launch; a thread
 // eight of them, whose moments in 8 bits are one load each, and 16 threads a block, whose largest value four lane exchanges find.
-// Bound by memory: 102M elements in 48 tensors, gradients of 16 bits and moments of 8, 263 us (5.5 TB/s; the vector units are busy
-// for 93% of it), 4.7M in 61 tensors of 16 bits 21 us (4.9 TB/s), 576000 in two tensors 6 us, its latency.
+// Bound by memory: 105M elements in 48 tensors, gradients of 16 bits and moments of 8, 267 to 279 us one step after another (5.3 to
+// 5.6 TB/s; the vector units are never idle either), 256 between calls that read the moments; 4.7M in 61 tensors of 16 bits 21 us
+// (4.9 TB/s), 576000 in two tensors 6 us, its latency.
 __global__ __launch_bounds__(kAdamwThreads) void adamw_kernel(const AdamwTable* __restrict__ table, AdamwLaunch launch,
                                                               int32_t group_count,
                                                               const AdamwFactors* __restrict__ factors) {
@@ -259,7 +260,8 @@ __global__ __launch_bounds__(kAdamwThreads) void adamw_kernel(const AdamwTable* 
 }
 
 // Whole blocks of moments from float32, 16 threads a block, and back: 16 bytes a thread and store, which pass the caches by. Bound by
-// memory: 102M moments read 146 us, 7 TB/s, 259 with 32 bytes a thread in two stores through the caches.
+// memory. 105M pairs of moments: held 182 us, 5.6 TB/s; read 145, 7.1 TB/s, call after call (259 with 32 bytes a thread in two stores
+// through the caches), and 208 to 213, 4.9 TB/s, right behind a step, where programs read them.
 constexpr int kReadEach = 4;  // fours of a thread
 constexpr int kReadFours = kAdamwThreads * kReadEach;
 

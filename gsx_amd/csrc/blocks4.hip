@@ -129,17 +129,19 @@ __global__ __launch_bounds__(kQuant4Threads) void expand4_kernel(const uint8_t* 
 // A workgroup of WM x WN waves forms a tile of c: BM rows (of a) by BN columns (rows of b), a wave TM x TN times 16 x 16 of it.
 // Eight blocks, 256 k, of both operands' tiles lie in LDS, two such steps at a time: while one is multiplied the next is on its way
 // there, straight from memory. A row is eight chunks of 16 bytes, one block each; chunk c lies at place c ^ swizzle(row), and a lane
-// of group g = lane / 16 reads chunks g and g + 4: no two lanes of a read meet in a bank. A row's eight exponents lie behind one
-// another, as in memory.
+// of group g = lane / 16 reads chunks g and g + 4: no two lanes of a read of values meet in a bank. A row's exponents of two steps lie
+// behind one another, as in memory, 16 bytes a row: those of rows 16 apart share a bank, which b's reads for 16-bit results meet
+// (conflicts in 13% of the cycles of 8192^3 to bf16; 5% in a product to float32, whose reads take 16 rows in a row).
 //
 // The matrix instructions take b as their first operand: a lane then holds four consecutive columns of one row of c. Which
 // row of b a lane brings for instruction j is chosen so that it has 16 bytes of columns together and that the four lanes of a row
 // store 64 bytes in a piece: 32 columns by a pair of instructions in 16-bit types, 16 by one in float32.
 //
 // 8192^3 to bf16: 285 to 300 us by the card, 3.7 to 3.85 PFLOP/s, 471 before the loads of the next step were in flight beside the
-// instructions, exponents came two steps at a time and rows left in pieces of 64 bytes. The matrix units are busy for 41% of it, at a
-// clock that falls under this load: four rows of tiles read ahead instead of two, a higher priority for the instructions or 4 waves
-// of 128 x 128 made it no faster (0, 0 and -7%).
+// instructions, exponents came two steps at a time and rows left in pieces of 64 bytes. The matrix units are busy for 41% of the
+// cycles; the waves spend 35% of their lives in waits and 36% waiting for issue. Every step waits for all of its loads, so that no
+// more than one step of 256 k is on its way. Four rows of tiles read ahead instead of two, a higher priority for the instructions or 4
+// waves of 128 x 128 made it no faster (0, 0 and -7%); shorter steps, more of them on their way, have not been tried.
 constexpr int kStep4 = 8;  // blocks
 
 template <typename O>

@@ -312,8 +312,10 @@ __device__ inline void top_of_workgroup(const T* __restrict__ z, int64_t length,
             return;
         }
     }
-    // Many equal logits, or some that are not finite: the value of the last alternative is found bit by bit, then the last index that
-    // has it. Each count is one more look at the row.
+    // More than kCandidates logits at the bound (rows of equal logits, as of a head of zeros, or saturated ones), or some that are not
+    // finite: the value of the last alternative is found bit by bit, then the last index that has it. Each count is one more look at
+    // the row, 65 in all, one logit a load: all logits equal, in bf16, one row of 131072 with 20 alternatives 268 us (37 of a call
+    // otherwise), 200 x 20000 with 8 773 (26), 20000 x 5000 with 20 3400 (110), 4096 x 65537 with 8 22100 (133).
     int turn = 0;
     const auto counted = [&](auto belongs) {
         int n = 0;
