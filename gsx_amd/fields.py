@@ -174,8 +174,8 @@ def _blocks_room(kind, block: int, size: int, rows: int, cols: int, out, device)
         values = torch.empty((rows, wide), dtype=torch.uint8, device=device)
         exponents = torch.empty((rows, words), dtype=torch.uint8, device=device)
         return kind(values, exponents, cols), (values.data_ptr(), wide, exponents.data_ptr(), words)
-    if not isinstance(out, kind) or out.rows != rows or out.cols != cols or out.values.shape[1] < wide or \
-            out.exponents.shape[1] < words:
+    if not isinstance(out, kind) or out.values.dim() != 2 or out.exponents.dim() != 2 or out.rows != rows or \
+            out.cols != cols or out.values.shape[1] < wide or out.exponents.shape[1] < words:
         raise GsxHipError(f"out must be {kind.__name__} of a matrix [{rows}, {cols}] with {wide} values and {words} exponents a row")
     return out, out.arguments()
 

@@ -33,6 +33,7 @@ def test_refused(rows, wide, words, cols):
 
 def test_refused_kinds():
     four = fields.Blocks4(torch.zeros(3, 256, dtype=torch.uint8), torch.zeros(3, 8, dtype=torch.uint8), 130)
-    for out in (four, four.values):
+    flat = fields.Blocks(torch.zeros(3, dtype=torch.uint8), torch.zeros(3, dtype=torch.uint8), 130)
+    for out in (four, four.values, flat):
         with pytest.raises(GsxHipError):
             _room(out)
